@@ -1,0 +1,652 @@
+// Attention of the newest tokens of a batch over a paged cache (single tokens, or a few drafted ones), with the keys that
+// a group of sequences shares read once for all of them.
+//
+// Bound by memory: a key and a value are used by the few query rows of one sequence (own units), so the kernel is a
+// stream of pages through shared memory: one warp asks for tiles of 64 keys by TMA several tiles ahead, four warps
+// consume them.  Scores and values go through mma.sync m16n8k16: with 4 to 16 query rows a tcgen05 tile of 128 rows would
+// be empty for the most part, and the 16-row form already computes a tile in a quarter of the time its bytes take.
+#include "attn_paged.cuh"
+
+#include <type_traits>
+
+namespace fa4b {
+
+constexpr int kPagedThreads = 160;
+constexpr int kPagedStageBytes = 96 * 1024;  // shared memory for tiles in flight; two CTAs per SM
+
+// ---- numbers ----------------------------------------------------------------------------------------------------------
+struct TagBf16 {};
+struct TagF16 {};
+
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, TagBf16) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, TagF16) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack16(float lo, float hi, TagBf16) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack16(float lo, float hi, TagF16) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ float2 unpack16(uint32_t x, TagBf16) { return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u)); }
+__device__ __forceinline__ float2 unpack16(uint32_t x, TagF16) { return __half22float2(*reinterpret_cast<const __half2*>(&x)); }
+// two E4M3 codes -> f16 pair (exact)
+__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two) {
+  uint32_t r;
+  asm("{ .reg .b16 lo, hi; mov.b32 {lo, hi}, %1; cvt.rn.f16x2.e4m3x2 %0, lo; }" : "=r"(r) : "r"(two));
+  return r;
+}
+__device__ __forceinline__ float paged_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w, int u, uint64_t* bar) {
+  asm volatile("cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(dst),
+               "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(u)
+               : "memory");
+}
+
+// ---- plan -------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ int paged_scan(int v, int* warp_sums, int& total) {  // exclusive, 1024 threads
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  if (lane == 31) warp_sums[warp] = x;
+  __syncthreads();
+  int w = warp_sums[lane];
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, w, o);
+    if (lane >= o) w += y;
+  }
+  total = __shfl_sync(0xffffffffu, w, 31);
+  const int before = __shfl_sync(0xffffffffu, w, (warp + 31) & 31);
+  __syncthreads();
+  return x - v + (warp ? before : 0);
+}
+
+// One CTA: lengths, groups, and the lines of tiles.  The shared part of a group is what the caller says, cut to what every
+// query row of every member sees (so that no row of a prefix unit needs a mask) and to whole 16 keys; a group of one
+// member has none.
+__global__ void __launch_bounds__(1024) paged_plan_kernel(const PagedParams p) {
+  __shared__ int warp_sums[32];
+  extern __shared__ int dyn[];
+  int* g_min = dyn;              // [groups] shortest member's length - T
+  int* g_first = dyn + p.groups;
+  int* g_count = dyn + 2 * p.groups;
+  pdl_trigger();
+  for (int g = threadIdx.x; g < p.groups; g += 1024) g_min[g] = INT_MAX, g_first[g] = INT_MAX, g_count[g] = 0;
+  __syncthreads();
+  pdl_wait();
+  if (threadIdx.x < 4) p.status[threadIdx.x] = 0u;
+  for (int i = threadIdx.x; i < p.n; i += 1024) {
+    const int slot = p.seqs ? p.seqs[i] : i;
+    int len = 0, g = p.groups > 0 ? -1 : 0;
+    if (slot >= 0 && slot < p.c.max_seqs) len = (int)min((int64_t)max(p.c.lens[slot], 0), (int64_t)p.c.width << p.c.page_shift);
+    if (p.groups > 0) {
+      int lo = 0, hi = p.groups;  // the last group that begins at or before i
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (p.offsets[mid] <= i) lo = mid; else hi = mid - 1;
+      }
+      if (lo < p.groups && p.offsets[lo] <= i && i < p.offsets[lo + 1]) g = lo;
+    }
+    p.plan.slot[i] = slot, p.plan.len[i] = len, p.plan.group[i] = g;
+    if (p.groups > 0 && g >= 0 && len > 0) {
+      atomicMin(g_min + g, max(len - p.T, 0));
+      atomicMin(g_first + g, i);
+      atomicAdd(g_count + g, 1);
+    }
+  }
+  __syncthreads();
+  int tiles = 0, units = 0;
+  for (int base = 0; base < p.groups; base += 1024) {
+    const int g = base + threadIdx.x;
+    int own_t = 0, own_u = 0;
+    if (g < p.groups) {
+      const int lo = max(p.offsets[g], 0), hi = min(p.offsets[g + 1], p.n);
+      int shared = g_count[g] > 1 ? min(max(p.shared[g], 0), g_min[g]) / kPagedAlign * kPagedAlign : 0;
+      if (hi <= lo) shared = 0;
+      own_u = hi > lo ? p.c.heads * ceil_div((hi - lo) * p.R, p.prefix_rows) : 0;
+      own_t = own_u * ceil_div(shared, p.prefix_tile);
+      p.plan.g_shared[g] = shared;
+      p.plan.g_first[g] = shared ? g_first[g] : 0;
+      g_min[g] = shared;
+    }
+    int t_total, u_total;
+    const int t_before = paged_scan(own_t, warp_sums, t_total), u_before = paged_scan(own_u, warp_sums, u_total);
+    if (g < p.groups) p.plan.g_cum[g] = tiles + t_before, p.plan.g_unit[g] = units + u_before;
+    tiles += t_total, units += u_total;
+  }
+  if (threadIdx.x == 0) p.plan.g_cum[p.groups] = tiles, p.plan.g_unit[p.groups] = units;
+  __syncthreads();
+  tiles = 0;
+  for (int base = 0; base < p.n; base += 1024) {
+    const int i = base + threadIdx.x;
+    int t = 0;
+    if (i < p.n) {
+      const int g = p.plan.group[i];
+      if (g >= 0) t = own_tiles(p.groups > 0 ? g_min[g] : 0, p.plan.len[i]);
+    }
+    int total;
+    const int before = paged_scan(t, warp_sums, total);
+    if (i < p.n) p.plan.own_cum[i] = tiles + before;
+    tiles += total;
+  }
+  if (threadIdx.x == 0) p.plan.own_cum[p.n] = tiles;
+}
+
+// ---- the units --------------------------------------------------------------------------------------------------------
+// Where a CTA stands on the line of tiles.
+struct PagedUnit {
+  int index;        // names the slot, together with the CTA
+  int head, row0, rows;   // rows row0 .. row0 + rows of the unit's sequence or group
+  int first_row;    // batch row of the sequence, or the group's first
+  int table_slot;   // whose row of the table names the pages
+  int key_lo, key_hi;     // keys that are this unit's
+  int key_all;      // own units: keys from here on are hidden from some rows
+  int tile, tile_end;     // tiles (64 keys, counted from key 0) that this CTA takes
+};
+
+template <bool kPrefix>
+__device__ __forceinline__ int64_t line_total(const PagedParams& p) {
+  return kPrefix ? (int64_t)p.plan.g_cum[p.groups] : (int64_t)p.plan.own_cum[p.n] * p.c.heads * p.own_blocks;
+}
+
+// the unit at position `at` of the line, cut at `end`
+template <bool kPrefix>
+__device__ __forceinline__ PagedUnit unit_at(const PagedParams& p, int64_t at, int64_t end) {
+  PagedUnit u;
+  if constexpr (kPrefix) {
+    const int g = last_at_or_before(p.plan.g_cum, p.groups, at, 1);
+    u.key_lo = 0, u.key_hi = u.key_all = p.plan.g_shared[g];
+    const int tiles = ceil_div(u.key_hi, p.prefix_tile);
+    const int lo = max(p.offsets[g], 0), hi = min(p.offsets[g + 1], p.n);
+    const int blocks = ceil_div((hi - lo) * p.R, p.prefix_rows);
+    const int64_t off = at - p.plan.g_cum[g];
+    const int which = (int)(off / tiles);
+    u.tile = (int)(off % tiles);
+    u.tile_end = (int)min((int64_t)tiles, u.tile + (end - at));
+    u.index = p.plan.g_unit[g] + which;
+    u.head = which / blocks;
+    u.row0 = (which % blocks) * p.prefix_rows;
+    u.rows = min(p.prefix_rows, (hi - lo) * p.R - u.row0);
+    u.first_row = lo;
+    u.table_slot = p.plan.slot[p.plan.g_first[g]];
+  } else {
+    const int per = p.c.heads * p.own_blocks;
+    const int i = last_at_or_before(p.plan.own_cum, p.n, at, per);
+    u.key_lo = own_first_key(p, i), u.key_hi = p.plan.len[i];
+    u.key_all = max(u.key_lo, u.key_hi - (p.T - 1));
+    const int tiles = own_tiles(u.key_lo, u.key_hi), skip = u.key_lo / kPagedTile;
+    const int64_t off = at - (int64_t)p.plan.own_cum[i] * per;
+    const int which = (int)(off / tiles);
+    const int t = (int)(off % tiles);
+    u.tile = skip + t;
+    u.tile_end = skip + (int)min((int64_t)tiles, t + (end - at));
+    u.index = i * per + which;
+    u.head = which / p.own_blocks;
+    u.row0 = (which % p.own_blocks) * p.own_rows;
+    u.rows = min(p.own_rows, p.R - u.row0);
+    u.first_row = i;
+    u.table_slot = p.plan.slot[i];
+  }
+  return u;
+}
+
+// a row of a unit: batch row, token and query head
+struct PagedRow {
+  int i, t, h;
+};
+__device__ __forceinline__ PagedRow paged_row(const PagedParams& p, const PagedUnit& u, int row) {
+  const int r = u.row0 + row, in_seq = r % p.R;
+  return {u.first_row + r / p.R, in_seq / p.G, u.head * p.G + in_seq % p.G};
+}
+
+template <int D, int kBytes>
+struct PagedSmem {
+  static constexpr int kTileBytes = kPagedTile * D * kBytes;  // K or V of one tile
+  static constexpr int kStages = kPagedStageBytes / (2 * kTileBytes) > 8 ? 8 : kPagedStageBytes / (2 * kTileBytes);
+  alignas(1024) uint8_t k[kStages][kTileBytes];
+  uint8_t v[kStages][kTileBytes];
+  float merge[2][16][D];
+  float2 ml[4][16];
+  uint64_t full[kStages], empty[kStages];
+  uint32_t valid[kStages];  // a bit per 16 keys: the table names a page of the pool
+  volatile uint32_t abort_flag;
+};
+
+// kWM warps side by side over rows (16 each), 4 / kWM over the keys of a tile.  Compute type: the cache's own 16-bit type, or
+// f16 for an E4M3 cache (every E4M3 value is exact in f16; bf16 queries are brought into its range by a power of two per
+// row, so they are exact as well down to 2^-38 of the row's largest).
+template <int D, typename CacheT, typename QT, int kWM, bool kPrefix>
+__global__ void __launch_bounds__(kPagedThreads, 2) attn_paged_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_k,
+                                                                      const __grid_constant__ CUtensorMap map_v) {
+  constexpr bool kE4M3 = std::is_same<CacheT, uint8_t>::value;
+  constexpr int kBytes = kE4M3 ? 1 : 2;
+  constexpr int kRowBytes = D * kBytes, kBoxBytes = kRowBytes < 128 ? kRowBytes : 128;  // a box: 64 or 128 bytes of a row
+  constexpr int kBoxes = kRowBytes / kBoxBytes;
+  constexpr int kWK = 4 / kWM, kKeys = kPagedTile / kWK;  // keys of a tile that one warp takes
+  using Smem = PagedSmem<D, kBytes>;
+  constexpr int kStages = Smem::kStages;
+  using Mma = typename std::conditional<kE4M3, TagF16, QT>::type;
+  extern __shared__ __align__(1024) uint8_t raw[];
+  Smem& s = *reinterpret_cast<Smem*>(raw);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const bool aligned = (smem_u32(raw) & 1023u) == 0u;  // the swizzle of the tiles goes by the address
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; ++i) mbar_init(&s.full[i], 1), mbar_init(&s.empty[i], 4);
+    s.abort_flag = 0u;
+    fence_barrier_init();
+    fence_async_smem();
+    tma_prefetch_desc(&map_k);
+    tma_prefetch_desc(&map_v);
+  }
+  __syncthreads();
+  pdl_trigger();
+  pdl_wait();
+  if (!aligned) {
+    if (threadIdx.x == 0) p.status[1] = 99u, p.status[0] = 1u;
+    return;
+  }
+  const int64_t total = line_total<kPrefix>(p), per_cta = piece_tiles(total, kPrefix ? p.prefix_ctas : p.own_ctas);
+  const int64_t begin = blockIdx.x * per_cta, end = min(total, begin + per_cta);
+  if (begin >= end) return;
+
+  if (warp == 4) {  // ---- producer: lane b of a tile's boxes asks for its own part of the pages
+    const int box_tokens = min(p.c.page_tokens, kPagedTile), boxes = kPagedTile / box_tokens;
+    int stage = 0, issued = 0;
+    uint32_t parity = 1u;
+    for (int64_t at = begin; at < end;) {
+      const PagedUnit u = unit_at<kPrefix>(p, at, end);
+      const int32_t* row = p.c.table + u.table_slot * p.c.table_stride;
+      for (int tile = u.tile; tile < u.tile_end; ++tile, ++at) {
+        const int token = tile * kPagedTile + lane * box_tokens;
+        const bool wanted = lane < boxes && token < u.key_hi && token + box_tokens > u.key_lo;
+        int page = -1;
+        if (wanted) page = row[token >> p.c.page_shift];
+        const bool load = wanted && page >= 0 && page < p.c.pages;
+        const uint32_t loads = __ballot_sync(0xffffffffu, load);
+        const bool go = mbar_wait_warp(&s.empty[stage], parity, &s.abort_flag, p.status, 1);
+        if (lane == 0) {
+          uint32_t valid = 0u;  // per 16 keys
+          for (int b = 0; b < boxes; ++b)
+            if (loads >> b & 1u) valid |= ((1u << (box_tokens / 16)) - 1u) << (b * (box_tokens / 16));
+          s.valid[stage] = valid;
+          mbar_expect_tx(&s.full[stage], go ? __popc(loads) * box_tokens * kRowBytes * 2 : 0);
+        }
+        __syncwarp();
+        if (go && load) {
+          const uint32_t in_page = (uint32_t)token & (uint32_t)(p.c.page_tokens - 1);
+#pragma unroll
+          for (int x = 0; x < kBoxes; ++x) {
+            const uint32_t off = x * (kPagedTile * kBoxBytes) + lane * box_tokens * kBoxBytes;
+            tma_load_5d(smem_u32(s.k[stage]) + off, &map_k, x * (kBoxBytes / kBytes), (int)in_page, u.head, page, p.layer, &s.full[stage]);
+            tma_load_5d(smem_u32(s.v[stage]) + off, &map_v, x * (kBoxBytes / kBytes), (int)in_page, u.head, page, p.layer, &s.full[stage]);
+          }
+        }
+        ++issued;
+        if (++stage == kStages) stage = 0, parity ^= 1u;
+      }
+    }
+    if (s.abort_flag) {  // copies in flight land before the CTA leaves
+      for (int k = max(0, issued - kStages); k < issued; ++k) mbar_wait_teardown(&s.full[k % kStages], (uint32_t)(k / kStages) & 1u);
+    }
+    return;
+  }
+
+  // ---- consumers
+  const int wm = warp % kWM, wk = warp / kWM, quad = lane >> 2, c4 = lane & 3;
+  int stage = 0;
+  uint32_t parity = 0u;
+  for (int64_t at = begin; at < end;) {
+    const PagedUnit u = unit_at<kPrefix>(p, at, end);
+    // query rows quad and quad + 8 of this warp's sixteen, as A fragments; row r of them sees keys below `limit`
+    uint32_t q[D / 16][4];
+    float scale[2];
+    int limit[2];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int row = wm * 16 + half * 8 + quad;
+      const bool there = row < u.rows;
+      const PagedRow r = paged_row(p, u, there ? row : 0);
+      const uint8_t* src = p.q + 2 * (r.i * p.q_sb + r.h * p.q_sh + r.t * p.q_st);
+      limit[half] = kPrefix ? u.key_hi : u.key_hi - (p.T - 1 - r.t);
+      scale[half] = p.scale_log2 * (p.k_scale ? p.k_scale[u.head] : 1.f);
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) {
+        if constexpr (kE4M3) {  // four neighbours: a thread's K codes are four neighbours too (see the scores below)
+          const uint2 x = there ? *reinterpret_cast<const uint2*>(src + 2 * (k * 16 + c4 * 4)) : make_uint2(0u, 0u);
+          q[k][half] = x.x, q[k][half + 2] = x.y;
+        } else {
+          q[k][half] = there ? *reinterpret_cast<const uint32_t*>(src + 2 * (k * 16 + c4 * 2)) : 0u;
+          q[k][half + 2] = there ? *reinterpret_cast<const uint32_t*>(src + 2 * (k * 16 + 8 + c4 * 2)) : 0u;
+        }
+      }
+      if constexpr (kE4M3 && std::is_same<QT, TagBf16>::value) {
+        float top = 0.f;
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+          for (int e = 0; e < 4; e += 2) {
+            const float2 f = unpack16(q[k][half + e], TagBf16{});
+            top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
+          }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // the largest becomes 2^14..2^15; a row of zeros, subnormals or infinities stays as it is
+        const int e = (int)(__float_as_uint(top) >> 23);
+        const int shift = (e == 0 || e == 255) ? 0 : 127 + 14 - e;
+        const float a = __uint_as_float((uint32_t)(127 + max(min(shift / 2, 126), -126)) << 23);
+        const float b = __uint_as_float((uint32_t)(127 + max(min(shift - shift / 2, 126), -126)) << 23);
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+          for (int x = 0; x < 4; x += 2) {
+            const float2 f = unpack16(q[k][half + x], TagBf16{});
+            q[k][half + x] = pack16(f.x * a * b, f.y * a * b, TagF16{});
+          }
+        scale[half] = scale[half] / a / b;
+      }
+    }
+    float acc[D / 8][4];
+#pragma unroll
+    for (int j = 0; j < D / 8; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+
+    for (int tile = u.tile; tile < u.tile_end; ++tile, ++at) {
+      mbar_wait_warp(&s.full[stage], parity, &s.abort_flag, p.status, 2);
+      const uint32_t kbase = smem_u32(s.k[stage]), vbase = smem_u32(s.v[stage]);
+      const int key0 = tile * kPagedTile + wk * kKeys;  // this warp's keys: key0 .. key0 + kKeys
+      const uint32_t valid = s.valid[stage] >> (wk * kKeys / 16);
+      constexpr uint32_t kAllValid = (1u << (kKeys / 16)) - 1u;
+      // not every key of these is there for every row
+      const bool special = key0 < u.key_lo || key0 + kKeys > u.key_all || (valid & kAllValid) != kAllValid;
+      float sc[kKeys / 8][4];
+#pragma unroll
+      for (int j = 0; j < kKeys / 8; ++j) {
+        sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.f;
+        const uint32_t row = wk * kKeys + j * 8 + (lane & 7);
+        if constexpr (kE4M3) {
+          // a matrix of ldmatrix is 8 keys x 16 codes, four neighbours to a thread: they stand in for k = 2c, 2c+1, 2c+8, 2c+9 of
+          // the fragment, and the query fragments above hold the same four neighbours there
+#pragma unroll
+          for (int x = 0; x < D / 64; ++x) {
+            uint32_t b[4];
+            ldmatrix4(b, kbase + swizzled_offset(row, x * 64 + (lane >> 3) * 16, kBoxBytes));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mma16816(sc[j], q[x * 4 + e], e4m3x2_to_f16x2(b[e]), e4m3x2_to_f16x2(b[e] >> 16), Mma{});
+          }
+        } else {
+#pragma unroll
+          for (int x = 0; x < D / 32; ++x) {
+            uint32_t b[4];
+            const uint32_t col = x * 64 + (lane >> 3) * 16;  // bytes of the row
+            ldmatrix4(b, kbase + (col >> 7) * (kPagedTile * 128) + swizzled_offset(row, col & 127u, 128));
+            mma16816(sc[j], q[2 * x], b[0], b[1], Mma{});
+            mma16816(sc[j], q[2 * x + 1], b[2], b[3], Mma{});
+          }
+        }
+      }
+      float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int j = 0; j < kKeys / 8; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float x = sc[j][e] * scale[e >> 1];
+          if (special) {
+            const int key = key0 + j * 8 + c4 * 2 + (e & 1);
+            if (key < u.key_lo || key >= limit[e >> 1] || !(valid >> (j >> 1) & 1u)) x = -INFINITY;
+          }
+          sc[j][e] = x;
+          top[e >> 1] = fmaxf(top[e >> 1], x);
+        }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
+        top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
+      }
+      // The reference point of a row moves only when its maximum has grown by more than 2^8 (probabilities then stay below
+      // 2^8, which costs 16-bit ones no precision): most tiles leave the accumulators alone.
+      if (__any_sync(0xffffffffu, top[0] > m[0] + 8.f || top[1] > m[1] + 8.f)) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float next = fmaxf(m[h], top[h]);
+          const float f = next == -INFINITY ? 1.f : paged_ex2(m[h] - next);
+          m[h] = next;
+          l[h] *= f;
+#pragma unroll
+          for (int j = 0; j < D / 8; ++j) acc[j][2 * h] *= f, acc[j][2 * h + 1] *= f;
+        }
+      }
+      const float m0 = m[0] == -INFINITY ? 0.f : m[0], m1 = m[1] == -INFINITY ? 0.f : m[1];
+#pragma unroll
+      for (int j = 0; j < kKeys / 8; ++j) {
+        sc[j][0] = paged_ex2(sc[j][0] - m0), sc[j][1] = paged_ex2(sc[j][1] - m0);
+        sc[j][2] = paged_ex2(sc[j][2] - m1), sc[j][3] = paged_ex2(sc[j][3] - m1);
+        l[0] += sc[j][0] + sc[j][1], l[1] += sc[j][2] + sc[j][3];
+      }
+      // Values.  A key that is not there, or that some row must not see, has probability 0 for those rows, and 0 times what its
+      // value may hold (anything, beyond the length) need not be 0: such keys are taken out of the product on both sides,
+      // and those that some rows do see (the newest T - 1) are added row by row behind it.
+#pragma unroll
+      for (int kk = 0; kk < kKeys / 16; ++kk) {
+        uint32_t a[4] = {pack16(sc[2 * kk][0], sc[2 * kk][1], Mma{}), pack16(sc[2 * kk][2], sc[2 * kk][3], Mma{}),
+                         pack16(sc[2 * kk + 1][0], sc[2 * kk + 1][1], Mma{}), pack16(sc[2 * kk + 1][2], sc[2 * kk + 1][3], Mma{})};
+        uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
+        if (special) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int key = key0 + kk * 16 + h * 8 + c4 * 2;
+            const bool ok = valid >> kk & 1u;
+            keep[h] = (ok && key >= u.key_lo && key < u.key_all ? 0x0000ffffu : 0u) | (ok && key + 1 >= u.key_lo && key + 1 < u.key_all ? 0xffff0000u : 0u);
+            a[2 * h] &= keep[h], a[2 * h + 1] &= keep[h];
+          }
+        }
+        if constexpr (kE4M3) {
+#pragma unroll
+          for (int x = 0; x < D / 32; ++x) {  // matrices: keys 0-7 and 8-15 of 16 codes, then of the next 16
+            uint32_t b[4];
+            ldmatrix4_trans(b, vbase + swizzled_offset(wk * kKeys + kk * 16 + ((lane >> 3) & 1) * 8 + (lane & 7), x * 32 + (lane >> 4) * 16, kBoxBytes));
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              // a register holds (key, key + 1) x (d, d + 1): even and odd d go to accumulators of their own
+              uint32_t lo0 = e4m3x2_to_f16x2(__byte_perm(b[2 * e], 0, 0x4420)), lo1 = e4m3x2_to_f16x2(__byte_perm(b[2 * e + 1], 0, 0x4420));
+              uint32_t hi0 = e4m3x2_to_f16x2(__byte_perm(b[2 * e], 0, 0x4431)), hi1 = e4m3x2_to_f16x2(__byte_perm(b[2 * e + 1], 0, 0x4431));
+              if (special) lo0 &= keep[0], lo1 &= keep[1], hi0 &= keep[0], hi1 &= keep[1];
+              mma16816(acc[4 * x + 2 * e], a, lo0, lo1, Mma{});
+              mma16816(acc[4 * x + 2 * e + 1], a, hi0, hi1, Mma{});
+            }
+          }
+        } else {
+#pragma unroll
+          for (int x = 0; x < D / 16; ++x) {
+            uint32_t b[4];
+            const uint32_t col = x * 32 + (lane >> 4) * 16;
+            ldmatrix4_trans(b, vbase + (col >> 7) * (kPagedTile * 128) +
+                                   swizzled_offset(wk * kKeys + kk * 16 + ((lane >> 3) & 1) * 8 + (lane & 7), col & 127u, 128));
+            if (special) b[0] &= keep[0], b[1] &= keep[1], b[2] &= keep[0], b[3] &= keep[1];
+            mma16816(acc[2 * x], a, b[0], b[1], Mma{});
+            mma16816(acc[2 * x + 1], a, b[2], b[3], Mma{});
+          }
+        }
+      }
+      if (!kPrefix && key0 + kKeys > u.key_all) {
+#pragma unroll 1
+        for (int kk = max(0, u.key_all - key0); kk < min(kKeys, u.key_hi - key0); ++kk) {
+          if (!(valid >> (kk >> 4) & 1u)) continue;
+          const int from = (lane & ~3) | ((kk & 7) >> 1);
+          float mine[2] = {0.f, 0.f};
+#pragma unroll
+          for (int j = 0; j < kKeys / 8; ++j)
+            if (j == kk >> 3) mine[0] = kk & 1 ? sc[j][1] : sc[j][0], mine[1] = kk & 1 ? sc[j][3] : sc[j][2];
+          const float p0 = __shfl_sync(0xffffffffu, mine[0], from), p1 = __shfl_sync(0xffffffffu, mine[1], from);
+          const bool see0 = key0 + kk < limit[0], see1 = key0 + kk < limit[1];
+          const uint32_t row = wk * kKeys + kk;
+#pragma unroll
+          for (int j = 0; j < D / 8; ++j) {
+            float2 f;
+            if constexpr (kE4M3) {  // accumulators 2x and 2x + 1: d = 16 x + 4 c + {0, 2} and {1, 3}
+              const uint32_t four = *reinterpret_cast<const uint32_t*>(s.v[stage] + swizzled_offset(row, (j >> 1) * 16 + c4 * 4, kBoxBytes));
+              f = unpack16(e4m3x2_to_f16x2(__byte_perm(four, 0, j & 1 ? 0x4431 : 0x4420)), TagF16{});
+            } else {
+              const uint32_t col = j * 16 + c4 * 4;
+              f = unpack16(*reinterpret_cast<const uint32_t*>(s.v[stage] + (col >> 7) * (kPagedTile * 128) + swizzled_offset(row, col & 127u, 128)), Mma{});
+            }
+            if (see0) acc[j][0] = fmaf(p0, f.x, acc[j][0]), acc[j][1] = fmaf(p0, f.y, acc[j][1]);
+            if (see1) acc[j][2] = fmaf(p1, f.x, acc[j][2]), acc[j][3] = fmaf(p1, f.y, acc[j][3]);
+          }
+        }
+      }
+      mbar_arrive_warp(&s.empty[stage]);
+      if (++stage == kStages) stage = 0, parity ^= 1u;
+    }
+
+    // ---- the unit's share of this CTA: warps over keys meet, then rows and statistics go to the slot
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+    }
+    if constexpr (kWK > 1) {
+      if (c4 == 0) s.ml[warp][quad] = make_float2(m[0], l[0]), s.ml[warp][quad + 8] = make_float2(m[1], l[1]);
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWK; ++w) top = fmaxf(top, s.ml[w * kWM + wm][quad + 8 * h].x);
+        const float f = m[h] == -INFINITY ? 0.f : paged_ex2(m[h] - top);
+        float sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWK; ++w) {
+          const float2 x = s.ml[w * kWM + wm][quad + 8 * h];
+          sum += x.x == -INFINITY ? 0.f : x.y * paged_ex2(x.x - top);
+        }
+        m[h] = top, l[h] = sum;
+#pragma unroll
+        for (int j = 0; j < D / 8; ++j) acc[j][2 * h] *= f, acc[j][2 * h + 1] *= f;
+      }
+      // the upper half of the warps hands its sums to the lower half, until one row of warps is left
+#pragma unroll
+      for (int half = kWK / 2; half >= 1; half /= 2) {
+        const bool gives = wk >= half && wk < 2 * half;
+        float* buf = &s.merge[kWK == 4 ? (wk & (half - 1)) : wm][0][0];
+        if (kWK == 4 && half == 1) buf = &s.merge[1][0][0];  // warp 1 reads and then writes there, warp 0 still reads the other
+        if (gives) {
+#pragma unroll
+          for (int j = 0; j < D / 8; ++j) {
+            *reinterpret_cast<float2*>(buf + quad * D + j * 8 + c4 * 2) = make_float2(acc[j][0], acc[j][1]);
+            *reinterpret_cast<float2*>(buf + (quad + 8) * D + j * 8 + c4 * 2) = make_float2(acc[j][2], acc[j][3]);
+          }
+        }
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        if (wk < half) {
+#pragma unroll
+          for (int j = 0; j < D / 8; ++j) {
+            const float2 x = *reinterpret_cast<const float2*>(buf + quad * D + j * 8 + c4 * 2);
+            const float2 y = *reinterpret_cast<const float2*>(buf + (quad + 8) * D + j * 8 + c4 * 2);
+            acc[j][0] += x.x, acc[j][1] += x.y, acc[j][2] += y.x, acc[j][3] += y.y;
+          }
+        }
+      }
+    }
+    if (wk == 0) {
+      const int64_t slot = (int64_t)u.index + blockIdx.x;
+      float* out = kPrefix ? p.prefix_acc + slot * p.prefix_rows * D : p.own_acc + slot * p.own_rows * D;
+      float2* ml = kPrefix ? p.prefix_ml + slot * p.prefix_rows : p.own_ml + slot * p.own_rows;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int row = wm * 16 + h * 8 + quad;
+        if (row >= u.rows) continue;
+        if (c4 == 0) ml[row] = make_float2(m[h], l[h]);
+        if constexpr (kE4M3) {
+#pragma unroll
+          for (int x = 0; x < D / 16; ++x)
+            *reinterpret_cast<float4*>(out + row * D + x * 16 + c4 * 4) =
+                make_float4(acc[2 * x][2 * h], acc[2 * x + 1][2 * h], acc[2 * x][2 * h + 1], acc[2 * x + 1][2 * h + 1]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < D / 8; ++j) *reinterpret_cast<float2*>(out + row * D + j * 8 + c4 * 2) = make_float2(acc[j][2 * h], acc[j][2 * h + 1]);
+        }
+      }
+    }
+  }
+}
+
+// ---- join -------------------------------------------------------------------------------------------------------------
+// One warp per output row; a lane holds D / 32 neighbours.
+template <int D, typename QT>
+__global__ void __launch_bounds__(256) paged_join_kernel(const PagedParams p) {
+  constexpr int kPer = D / 32;
+  pdl_trigger();
+  pdl_wait();
+  const int64_t w = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (w >= (int64_t)p.n * p.Hq * p.T) return;
+  const int t = (int)(w % p.T), h = (int)(w / p.T % p.Hq), i = (int)(w / p.T / p.Hq);
+  const int g = p.plan.group[i];
+  if (g < 0) return;  // behind the last group: left as it was
+  const int head = h / p.G, r = t * p.G + h % p.G, len = p.plan.len[i];
+  float acc[kPer], m = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) acc[e] = 0.f;
+  auto add = [&](const float* rows, const float2* ml, int64_t row) {
+    const float2 x = ml[row];
+    if (x.x == -INFINITY) return;
+    const float next = fmaxf(m, x.x), f = m == -INFINITY ? 0.f : paged_ex2(m - next), y = paged_ex2(x.x - next);
+    m = next;
+    l = l * f + x.y * y;
+    if constexpr (kPer == 4) {
+      const float4 v = reinterpret_cast<const float4*>(rows + row * D)[lane];
+      acc[0] = acc[0] * f + v.x * y, acc[1] = acc[1] * f + v.y * y, acc[2] = acc[2] * f + v.z * y, acc[3] = acc[3] * f + v.w * y;
+    } else {
+      const float2 v = reinterpret_cast<const float2*>(rows + row * D)[lane];
+      acc[0] = acc[0] * f + v.x * y, acc[1] = acc[1] * f + v.y * y;
+    }
+  };
+  if (len - (p.T - 1 - t) > 0) {
+    const int first = own_first_key(p, i), tiles = own_tiles(first, len);
+    if (first > 0) {
+      const int64_t per_cta = piece_tiles(line_total<true>(p), p.prefix_ctas);
+      const int lo = max(p.offsets[g], 0), hi = min(p.offsets[g + 1], p.n);
+      const int row = (i - lo) * p.R + r, block = row / p.prefix_rows, blocks = ceil_div((hi - lo) * p.R, p.prefix_rows);
+      const int which = head * blocks + block, ptiles = ceil_div(first, p.prefix_tile);
+      const int64_t from = p.plan.g_cum[g] + (int64_t)which * ptiles;
+      for (int64_t cta = from / per_cta; cta <= (from + ptiles - 1) / per_cta; ++cta)
+        add(p.prefix_acc, p.prefix_ml, (p.plan.g_unit[g] + which + cta) * p.prefix_rows + row % p.prefix_rows);
+    }
+    const int per = p.c.heads * p.own_blocks, which = head * p.own_blocks + r / p.own_rows;
+    const int64_t per_cta = piece_tiles(line_total<false>(p), p.own_ctas), from = (int64_t)p.plan.own_cum[i] * per + (int64_t)which * tiles;
+    for (int64_t cta = from / per_cta; cta <= (from + tiles - 1) / per_cta; ++cta)
+      add(p.own_acc, p.own_ml, ((int64_t)i * per + which + cta) * p.own_rows + r % p.own_rows);
+  }
+  const float inv = l == 0.f ? 0.f : (p.v_scale ? p.v_scale[head] : 1.f) / l;  // a row that sees nothing: zeros, -inf
+  uint8_t* out = p.o + 2 * (i * p.o_sb + h * p.o_sh + t * p.o_st + lane * kPer);
+  if constexpr (kPer == 4) *reinterpret_cast<uint2*>(out) = make_uint2(pack16(acc[0] * inv, acc[1] * inv, QT{}), pack16(acc[2] * inv, acc[3] * inv, QT{}));
+  else *reinterpret_cast<uint32_t*>(out) = pack16(acc[0] * inv, acc[1] * inv, QT{});
+  if (lane == 0) p.lse[((int64_t)i * p.Hq + h) * p.T + t] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+}
+
+}  // namespace fa4b

@@ -1,0 +1,732 @@
+// Pages of a key / value cache: claim, write, fork, copy, compact, free.  Everything here moves bytes; what decides the
+// time is how many launches a call needs while it is small and how close the copies come to the memory's rate when it
+// is large.  Claiming is deterministic (the lowest free pages, in the order of the request), so two runs of a program
+// hold the same pages.
+#include "kv_cache.cuh"
+
+namespace fa4b {
+
+// `work` in 32-bit words: status, header of a compaction, the pages a fork claims, flags of a copy, then the lists of a
+// compaction: used pages of each block of kBlockPages, holes, movers by the used pages before them, and those per page
+constexpr int kWorkStatus = 0, kWorkHead = 8, kWorkFresh = 16, kWorkFlags = kWorkFresh + FA4B_KV_MAX_LIST,
+              kWorkLists = kWorkFlags + FA4B_KV_MAX_LIST;
+constexpr int kBlockPages = 4096;
+constexpr int kPieceBytes = 32768;  // what one CTA of the copy kernels moves: 256 threads x 8 x 16 bytes, all loads in flight at once
+constexpr int kWarpBytes = 4096;    // the same per warp
+constexpr int kCheckInline = 512;   // copy lists up to this length are checked for collisions by the copying CTAs themselves
+
+enum KvFinding { kOk = 0, kNoPages = 1, kBadSlot = 2, kSlotTwice = 3, kChildInUse = 4, kRowTooShort = 5, kBadPage = 6, kBadCount = 7, kCollision = 8 };
+
+__device__ __forceinline__ void kv_report(const KvView& c, int what, int index, int detail) {
+  if (atomicCAS(c.work + kWorkStatus, 0, what) == 0) {
+    c.work[kWorkStatus + 1] = index;
+    c.work[kWorkStatus + 2] = detail;
+  }
+}
+
+__device__ __forceinline__ int pages_of(const KvView& c, int len) { return (int)(((int64_t)len + c.page_tokens - 1) >> c.page_shift); }
+
+// exclusive prefix sum over a block of 1024 threads; `total` gets the sum
+__device__ __forceinline__ int block_scan1024(int v, int* warp_sums, int& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  if (lane == 31) warp_sums[warp] = x;
+  __syncthreads();
+  if (warp == 0) {
+    int w = warp_sums[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, w, o);
+      if (lane >= o) w += y;
+    }
+    warp_sums[lane] = w;
+  }
+  __syncthreads();
+  const int before = x - v + (warp ? warp_sums[warp - 1] : 0);
+  total = warp_sums[31];
+  __syncthreads();
+  return before;
+}
+
+// sixteen counts from page `p` on as a mask of the pages in use (or, with `want_free`, of the free ones)
+__device__ __forceinline__ uint32_t page_mask16(const KvView& c, int64_t p, bool want_free) {
+  int r[16];
+  if (p + 16 <= c.pages) {
+    const int4* q = reinterpret_cast<const int4*>(c.refs + p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int4 x = __ldcg(q + i);
+      r[4 * i] = x.x, r[4 * i + 1] = x.y, r[4 * i + 2] = x.z, r[4 * i + 3] = x.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) r[i] = p + i < c.pages ? __ldcg(c.refs + p + i) : (want_free ? 1 : 0);
+  }
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) m |= (uint32_t)((r[i] > 0) != want_free) << i;
+  return m;
+}
+
+// The first `want` free pages in ascending order into out[]; a block of 1024 threads looks at 16384 pages per step and
+// stops as soon as it has enough.  Returns how many there are (at least `want`, when it stopped early).
+__device__ int find_free(const KvView& c, int want, int32_t* out, int* warp_sums) {
+  int have = 0;
+  for (int64_t base = 0; base < c.pages && have < want; base += 16384) {
+    const int64_t p = base + threadIdx.x * 16;
+    uint32_t m = p < c.pages ? page_mask16(c, p, true) : 0u;
+    int total;
+    int rank = have + block_scan1024(__popc(m), warp_sums, total);
+    while (m != 0u && rank < want) {
+      out[rank++] = (int32_t)(p + __ffs(m) - 1);
+      m &= m - 1;
+    }
+    have += total;
+  }
+  __syncthreads();
+  return have;
+}
+
+// ---- free -------------------------------------------------------------------------------------------------------------
+// One CTA per slot.  The exchange of the length decides who frees a slot that the list names twice.
+__global__ void __launch_bounds__(128) kv_free_kernel(const KvView c, const int32_t* __restrict__ seqs) {
+  pdl_trigger();
+  pdl_wait();
+  __shared__ int held;
+  const int slot = seqs[blockIdx.x];
+  if (slot < 0 || slot >= c.max_seqs) {
+    if (threadIdx.x == 0) kv_report(c, kBadSlot, blockIdx.x, slot);
+    return;
+  }
+  if (threadIdx.x == 0) held = min(pages_of(c, max(atomicExch(c.lens + slot, 0), 0)), c.width);
+  __syncthreads();
+  int32_t* row = c.table + slot * c.table_stride;
+  for (int j = threadIdx.x; j < held; j += 128) {
+    const int p = row[j];
+    if (p >= 0 && p < c.pages) atomicSub(c.refs + p, 1);
+    row[j] = -1;
+  }
+}
+
+// ---- extend -----------------------------------------------------------------------------------------------------------
+// Checks a list of distinct slots against a bitmap in shared memory; true where slot i is new and in range.
+__device__ __forceinline__ int check_slot(const KvView& c, int slot, uint32_t* seen) {
+  if (slot < 0 || slot >= c.max_seqs) return kBadSlot;
+  const uint32_t bit = 1u << (slot & 31);
+  return (atomicOr(seen + (slot >> 5), bit) & bit) ? kSlotTwice : kOk;
+}
+
+// One CTA: what is claimed in one call is a few thousand pages at most, and the order of the claims is a prefix sum over
+// requests and one over free pages.
+__global__ void __launch_bounds__(1024) kv_extend_kernel(const KvView c, const int32_t* __restrict__ seqs, const int32_t* __restrict__ n_new,
+                                                         int n, int32_t* __restrict__ fresh) {
+  extern __shared__ int dyn[];
+  __shared__ int warp_sums[32];
+  int* first = dyn;                                          // [n + 1]: claims before request i
+  uint32_t* seen = reinterpret_cast<uint32_t*>(dyn + n + 1);  // [max_seqs / 32]
+  pdl_trigger();
+  for (int i = threadIdx.x; i < (c.max_seqs + 31) / 32; i += 1024) seen[i] = 0u;
+  __syncthreads();
+  pdl_wait();
+  bool bad = false;
+  int want = 0;
+  for (int base = 0; base < n; base += 1024) {
+    const int i = base + threadIdx.x;
+    int need = 0;
+    if (i < n) {
+      const int slot = seqs[i], add = n_new[i];
+      int e = check_slot(c, slot, seen);
+      if (e == kOk) {
+        const int len = c.lens[slot];
+        if (add < 0) e = kBadCount;
+        else if ((int64_t)len + add > (int64_t)c.width << c.page_shift || len < 0) e = kRowTooShort;
+        else need = pages_of(c, len + add) - pages_of(c, len);
+      }
+      if (e != kOk) {
+        kv_report(c, e, i, slot);
+        bad = true;
+      }
+    }
+    int total;
+    const int before = block_scan1024(need, warp_sums, total);
+    if (i < n) first[i] = want + before;
+    want += total;  // at most 4096 x 2^18
+  }
+  if (threadIdx.x == 0) first[n] = want;
+  if (__syncthreads_or(bad)) return;
+  const int have = want ? find_free(c, want, fresh, warp_sums) : 0;
+  if (have < want) {
+    if (threadIdx.x == 0) kv_report(c, kNoPages, want, have);
+    return;
+  }
+  for (int r = threadIdx.x; r < want; r += 1024) {
+    int lo = 0, hi = n - 1;  // the last request whose claims begin at or before r
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (first[mid] <= r) lo = mid; else hi = mid - 1;
+    }
+    const int slot = seqs[lo], p = fresh[r];
+    c.table[slot * c.table_stride + pages_of(c, c.lens[slot]) + (r - first[lo])] = p;
+    c.refs[p] = 1;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += 1024) c.lens[seqs[i]] += n_new[i];
+}
+
+// ---- write ------------------------------------------------------------------------------------------------------------
+struct WriteParams {
+  const uint8_t* src[2];
+  int64_t sb[2], sh[2], st[2];  // byte strides: batch, head, token
+  const float* scale[2];        // this layer's, or NULL
+  uint8_t* dst[2];              // this layer's pool
+  const int32_t* seqs;
+  const int32_t* n_new;
+  int T, D, tile_tokens;
+};
+
+template <typename Src>
+__device__ __forceinline__ uint2 quantise8(uint4 x, float scale) {
+  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+  float f[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float2 p;
+    if constexpr (sizeof(Src) == 2 && std::is_same<Src, __half>::value) p = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    else p = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[i]));
+    f[2 * i] = __fdiv_rn(p.x, scale);  // the definition's quotient: one rounding to 32 bits, one to E4M3
+    f[2 * i + 1] = __fdiv_rn(p.y, scale);
+  }
+  return make_uint2(cvt_e4m3x4(f[0], f[1], f[2], f[3]), cvt_e4m3x4(f[4], f[5], f[6], f[7]));
+}
+
+// grid (row of the batch x kv head, tile of tokens); a thread takes 16 bytes of K and of V of one token at a time, so a
+// warp reads 512 contiguous bytes and writes whole rows.  Bound by memory: 2 x 2 bytes read, 2 x (1 or 2) written a value.
+template <bool kE4M3, typename Src>
+__global__ void __launch_bounds__(256) kv_write_kernel(const KvView c, const WriteParams w) {
+  pdl_trigger();
+  pdl_wait();
+  const int i = blockIdx.x / c.heads, h = blockIdx.x % c.heads;
+  const int slot = w.seqs[i];
+  if (slot < 0 || slot >= c.max_seqs) {
+    if (threadIdx.x == 0 && h == 0 && blockIdx.y == 0) kv_report(c, kBadSlot, i, slot);
+    return;
+  }
+  const int add = w.n_new ? min(w.n_new[i], w.T) : w.T;
+  const int64_t start = (int64_t)c.lens[slot] - (w.n_new ? w.n_new[i] : w.T);
+  const int chunks = w.D / 8, chunk = threadIdx.x & (chunks - 1), step = 256 / chunks;
+  const int32_t* row = c.table + slot * c.table_stride;
+  const float sk = kE4M3 ? w.scale[0][h] : 1.f, sv = kE4M3 ? w.scale[1][h] : 1.f;
+  const int t_end = min(add, (int)(blockIdx.y + 1) * w.tile_tokens);
+#pragma unroll 4
+  for (int t = blockIdx.y * w.tile_tokens + (int)(threadIdx.x / chunks); t < t_end; t += step) {
+    const int64_t pos = start + t;
+    if (pos < 0 || (pos >> c.page_shift) >= c.width) continue;
+    const int p = row[pos >> c.page_shift];
+    if (p < 0 || p >= c.pages) continue;
+    const uint4 xk = __ldcs(reinterpret_cast<const uint4*>(w.src[0] + i * w.sb[0] + h * w.sh[0] + t * w.st[0]) + chunk);
+    const uint4 xv = __ldcs(reinterpret_cast<const uint4*>(w.src[1] + i * w.sb[1] + h * w.sh[1] + t * w.st[1]) + chunk);
+    const int64_t in_page = ((int64_t)h * c.page_tokens + (pos & (c.page_tokens - 1))) * c.row_bytes;
+    uint8_t* dk = w.dst[0] + p * c.k_page + in_page;
+    uint8_t* dv = w.dst[1] + p * c.v_page + in_page;
+    if constexpr (kE4M3) {
+      reinterpret_cast<uint2*>(dk)[chunk] = quantise8<Src>(xk, sk);
+      reinterpret_cast<uint2*>(dv)[chunk] = quantise8<Src>(xv, sv);
+    } else {
+      reinterpret_cast<uint4*>(dk)[chunk] = xk;
+      reinterpret_cast<uint4*>(dv)[chunk] = xv;
+    }
+  }
+}
+
+// ---- fork -------------------------------------------------------------------------------------------------------------
+// First launch, one CTA: checks the lists, claims the tail pages.  fresh[i]: child i's tail page, -1: none; head[0]: 1
+// when the second launch may go on.
+__global__ void __launch_bounds__(1024) kv_fork_plan_kernel(const KvView c, const int32_t* __restrict__ parents, const int32_t* __restrict__ children,
+                                                            int n, int32_t* __restrict__ list) {
+  extern __shared__ uint32_t seen[];  // [max_seqs / 32]
+  __shared__ int warp_sums[32];
+  int32_t* fresh = c.work + kWorkFresh;
+  pdl_trigger();
+  for (int i = threadIdx.x; i < (c.max_seqs + 31) / 32; i += 1024) seen[i] = 0u;
+  __syncthreads();
+  pdl_wait();
+  if (threadIdx.x == 0) c.work[kWorkHead] = 0;
+  bool bad = false;
+  int want = 0;
+  for (int base = 0; base < n; base += 1024) {
+    const int i = base + threadIdx.x;
+    int need = 0;
+    if (i < n) {
+      const int parent = parents[i], child = children[i];
+      int e = check_slot(c, child, seen), named = child;
+      if (e == kOk && (parent < 0 || parent >= c.max_seqs)) e = kBadSlot, named = parent;
+      if (e == kOk && c.lens[child] != 0) e = kChildInUse;
+      if (e == kOk) {
+        const int len = c.lens[parent];
+        if (len < 0 || len > (int64_t)c.width << c.page_shift) e = kRowTooShort, named = parent;
+        else need = (len & (c.page_tokens - 1)) != 0;
+      }
+      if (e != kOk) {
+        kv_report(c, e, i, named);
+        bad = true;
+      }
+    }
+    int total;
+    const int before = block_scan1024(need, warp_sums, total);
+    if (i < n) fresh[i] = need ? want + before : -1;
+    want += total;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < n && !bad; i += 1024) {  // an empty slot that is forked from and into at once
+    const int parent = parents[i];
+    if (seen[parent >> 5] >> (parent & 31) & 1u) {
+      kv_report(c, kSlotTwice, i, parent);
+      bad = true;
+    }
+  }
+  if (__syncthreads_or(bad)) return;
+  const int have = want ? find_free(c, want, list, warp_sums) : 0;
+  if (have < want) {
+    if (threadIdx.x == 0) kv_report(c, kNoPages, want, have);
+    return;
+  }
+  for (int i = threadIdx.x; i < n; i += 1024) {
+    const int rank = fresh[i];
+    if (rank >= 0) {
+      const int p = list[rank];
+      fresh[i] = p;
+      c.refs[p] = 1;
+    }
+    c.lens[children[i]] = c.lens[parents[i]];
+  }
+  if (threadIdx.x == 0) c.work[kWorkHead] = 1;
+}
+
+// Second launch.  CTAs 0..n-1: the child's row of the table and the counts of the pages it shares.  The others: one warp
+// per 4 KB of a tail page's rows of one kv head, K or V, one layer.
+__global__ void __launch_bounds__(256) kv_fork_move_kernel(const KvView c, const int32_t* __restrict__ parents, const int32_t* __restrict__ children,
+                                                           int n, int pieces, int64_t units) {
+  pdl_trigger();
+  pdl_wait();
+  if (c.work[kWorkHead] == 0) return;
+  const int32_t* fresh = c.work + kWorkFresh;
+  if ((int)blockIdx.x < n) {
+    const int i = blockIdx.x, len = c.lens[parents[i]], full = len >> c.page_shift;
+    const int32_t* from = c.table + parents[i] * c.table_stride;
+    int32_t* to = c.table + children[i] * c.table_stride;
+    for (int j = threadIdx.x; j < full; j += 256) {
+      const int p = from[j];
+      to[j] = p;
+      if (p >= 0 && p < c.pages) atomicAdd(c.refs + p, 1);
+    }
+    if (threadIdx.x == 0 && fresh[i] >= 0) to[full] = fresh[i];
+    return;
+  }
+  int64_t u = (int64_t)(blockIdx.x - n) * 8 + (threadIdx.x >> 5);
+  if (u >= units) return;
+  const int piece = (int)(u % pieces);
+  u /= pieces;
+  const int h = (int)(u % c.heads);
+  u /= c.heads;
+  const bool is_v = u & 1;
+  u >>= 1;
+  const int layer = (int)(u % c.layers), i = (int)(u / c.layers);
+  const int dst = fresh[i];
+  if (dst < 0) return;
+  const int len = c.lens[parents[i]];
+  const int bytes = (len & (c.page_tokens - 1)) * c.row_bytes - piece * kWarpBytes;  // of this head's rows, from this piece on
+  if (bytes <= 0) return;
+  const int src = c.table[parents[i] * c.table_stride + (len >> c.page_shift)];
+  if (src < 0 || src >= c.pages) return;
+  uint8_t* base = (is_v ? c.v : c.k) + layer * (is_v ? c.v_layer : c.k_layer) + (int64_t)h * c.page_tokens * c.row_bytes + piece * kWarpBytes;
+  const int64_t page = is_v ? c.v_page : c.k_page;
+  const uint4* from = reinterpret_cast<const uint4*>(base + src * page);
+  uint4* to = reinterpret_cast<uint4*>(base + dst * page);
+  uint4 r[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if ((j * 32 + (int)(threadIdx.x & 31)) * 16 < bytes) r[j] = from[j * 32 + (threadIdx.x & 31)];
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if ((j * 32 + (int)(threadIdx.x & 31)) * 16 < bytes) to[j * 32 + (threadIdx.x & 31)] = r[j];
+}
+
+// ---- whole pages ------------------------------------------------------------------------------------------------------
+struct PieceRegs {
+  uint4 r[8];
+};
+__device__ __forceinline__ void piece_load(PieceRegs& x, const uint8_t* from, int bytes) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if ((j * 256 + (int)threadIdx.x) * 16 < bytes) x.r[j] = __ldcs(reinterpret_cast<const uint4*>(from) + j * 256 + threadIdx.x);
+}
+__device__ __forceinline__ void piece_store(const PieceRegs& x, uint8_t* to, int bytes) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if ((j * 256 + (int)threadIdx.x) * 16 < bytes) __stcs(reinterpret_cast<uint4*>(to) + j * 256 + threadIdx.x, x.r[j]);
+}
+
+__device__ __forceinline__ bool collides(int i, int j, int s, int d, int sj, int dj) { return (j != i && dj == d) || sj == d || dj == s; }
+
+// one warp per pair
+__global__ void __launch_bounds__(256) kv_copy_check_kernel(const KvView c, const int32_t* __restrict__ src, const int32_t* __restrict__ dst, int n) {
+  pdl_trigger();
+  pdl_wait();
+  const int i = blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (i >= n) return;
+  const int s = src[i], d = dst[i];
+  bool bad = false;
+  if (s >= 0 && d >= 0)
+    for (int j = threadIdx.x & 31; j < n; j += 32) bad |= collides(i, j, s, d, src[j], dst[j]);
+  bad = __any_sync(0xffffffffu, bad);
+  if ((threadIdx.x & 31) == 0) c.work[kWorkFlags + i] = bad;
+}
+
+// One CTA per 32 KB of a page of one layer, K or V: every thread has eight 16-byte loads in flight before its first store.
+// Below kCheckInline pairs each CTA checks its own pair (two words per thread while the loads are on their way), above it a
+// launch of its own does, which then costs less than the lists read by every CTA.
+__global__ void __launch_bounds__(256) kv_copy_kernel(const KvView c, const int32_t* __restrict__ src, const int32_t* __restrict__ dst, int n,
+                                                      int pieces) {
+  pdl_trigger();
+  pdl_wait();
+  int64_t u = blockIdx.x;
+  const int piece = (int)(u % pieces);
+  u /= pieces;
+  const bool is_v = u & 1;
+  u >>= 1;
+  const int layer = (int)(u % c.layers), i = (int)(u / c.layers);
+  const int s = src[i], d = dst[i];
+  if (s < 0 || d < 0) return;
+  const bool reports = threadIdx.x == 0 && layer == 0 && !is_v && piece == 0;
+  if (s >= c.pages || d >= c.pages) {
+    if (reports) kv_report(c, kBadPage, i, s >= c.pages ? s : d);
+    return;
+  }
+  uint8_t* base = (is_v ? c.v : c.k) + layer * (is_v ? c.v_layer : c.k_layer) + (int64_t)piece * kPieceBytes;
+  const int64_t page = is_v ? c.v_page : c.k_page;
+  const int bytes = min(kPieceBytes, c.block_bytes - piece * kPieceBytes);
+  PieceRegs x;
+  piece_load(x, base + s * page, bytes);
+  bool bad = false;
+  if (n <= kCheckInline) {
+    for (int j = threadIdx.x; j < n; j += 256) bad |= collides(i, j, s, d, src[j], dst[j]);
+    bad = __syncthreads_or(bad);
+  } else {
+    bad = c.work[kWorkFlags + i] != 0;
+  }
+  if (bad) {
+    if (reports) kv_report(c, kCollision, i, d);
+    return;
+  }
+  piece_store(x, base + d * page, bytes);
+}
+
+// ---- compact ----------------------------------------------------------------------------------------------------------
+struct CompactLists {
+  int32_t *counts, *holes, *movers, *rank;
+};
+__host__ __device__ inline int compact_blocks(int pages) { return (pages + kBlockPages - 1) / kBlockPages; }
+__device__ __forceinline__ CompactLists compact_lists(const KvView& c) {
+  CompactLists l;
+  l.counts = c.work + kWorkLists;
+  l.holes = l.counts + compact_blocks(c.pages);
+  l.movers = l.holes + c.pages;
+  l.rank = l.movers + c.pages;
+  return l;
+}
+
+// used pages of each block of 4096
+__global__ void __launch_bounds__(256) kv_compact_count_kernel(const KvView c) {
+  pdl_trigger();
+  pdl_wait();
+  const int64_t p = (int64_t)blockIdx.x * kBlockPages + threadIdx.x * 16;
+  int v = p < c.pages ? __popc(page_mask16(c, p, false)) : 0;
+  __shared__ int sum;
+  if (threadIdx.x == 0) sum = 0;
+  __syncthreads();
+  v = __reduce_add_sync(0xffffffffu, v);
+  if ((threadIdx.x & 31) == 0) atomicAdd(&sum, v);
+  __syncthreads();
+  if (threadIdx.x == 0) compact_lists(c).counts[blockIdx.x] = sum;
+}
+
+// With U used pages in all and b(p) used pages below p: a free page p < U is hole p - b(p); a used page p >= U is the
+// mover after the b(p) - b(U) movers before it.  Movers are kept at b(p); head = {U, b(U)} lets the last launch pair them.
+__global__ void __launch_bounds__(256) kv_compact_plan_kernel(const KvView c) {
+  pdl_trigger();
+  pdl_wait();
+  const CompactLists l = compact_lists(c);
+  __shared__ int warp_sums[8], all_before, all_used;
+  if (threadIdx.x == 0) all_before = all_used = 0;
+  __syncthreads();
+  int before = 0, used = 0;
+  for (int j = threadIdx.x; j < (int)gridDim.x; j += 256) {
+    const int v = l.counts[j];
+    used += v;
+    before += j < (int)blockIdx.x ? v : 0;
+  }
+  used = __reduce_add_sync(0xffffffffu, used);
+  before = __reduce_add_sync(0xffffffffu, before);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (lane == 0) atomicAdd(&all_used, used), atomicAdd(&all_before, before);
+  const int64_t p0 = (int64_t)blockIdx.x * kBlockPages + threadIdx.x * 16;
+  const uint32_t m = p0 < c.pages ? page_mask16(c, p0, false) : 0u;
+  int x = __popc(m);
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  if (lane == 31) warp_sums[warp] = x;
+  __syncthreads();
+  int b = all_before + x - __popc(m);
+  for (int w = 0; w < warp; ++w) b += warp_sums[w];
+  const int n_used = all_used;
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    const int64_t p = p0 + j;
+    if (p >= c.pages) break;
+    if (p == n_used) c.work[kWorkHead] = n_used, c.work[kWorkHead + 1] = b;
+    if (m >> j & 1u) {
+      if (p >= n_used) l.movers[b] = (int32_t)p, l.rank[p] = b;
+      ++b;
+    } else if (p < n_used) {
+      l.holes[p - b] = (int32_t)p;
+    }
+  }
+  if (n_used >= c.pages && blockIdx.x == 0 && threadIdx.x == 0) c.work[kWorkHead] = c.work[kWorkHead + 1] = n_used;
+}
+
+// The moves (destinations lie below U, sources at or above it, so no order matters), counts and tables.  How many there are
+// only the device knows: a fixed grid walks them.
+__global__ void __launch_bounds__(256) kv_compact_move_kernel(const KvView c, int pieces) {
+  pdl_trigger();
+  pdl_wait();
+  const CompactLists l = compact_lists(c);
+  const int n_used = c.work[kWorkHead], b_used = c.work[kWorkHead + 1], moves = n_used - b_used;
+  const int64_t units = (int64_t)moves * c.layers * 2 * pieces;
+  for (int64_t unit = blockIdx.x; unit < units; unit += gridDim.x) {
+    int64_t u = unit;
+    const int piece = (int)(u % pieces);
+    u /= pieces;
+    const bool is_v = u & 1;
+    u >>= 1;
+    const int layer = (int)(u % c.layers), i = (int)(u / c.layers);
+    uint8_t* base = (is_v ? c.v : c.k) + layer * (is_v ? c.v_layer : c.k_layer) + (int64_t)piece * kPieceBytes;
+    const int64_t page = is_v ? c.v_page : c.k_page;
+    const int bytes = min(kPieceBytes, c.block_bytes - piece * kPieceBytes);
+    PieceRegs x;
+    piece_load(x, base + l.movers[b_used + i] * page, bytes);
+    piece_store(x, base + l.holes[i] * page, bytes);
+  }
+  const int64_t tid = (int64_t)blockIdx.x * 256 + threadIdx.x, threads = (int64_t)gridDim.x * 256;
+  for (int64_t i = tid; i < moves; i += threads) {
+    const int from = l.movers[b_used + i];
+    c.refs[l.holes[i]] = c.refs[from];
+    c.refs[from] = 0;
+  }
+  if (moves == 0) return;
+  // a warp per slot's row, entries of the slot's length only
+  for (int64_t s = tid >> 5; s < c.max_seqs; s += threads >> 5) {
+    const int held = min(pages_of(c, max(c.lens[s], 0)), c.width);
+    int32_t* row = c.table + s * c.table_stride;
+    for (int j = threadIdx.x & 31; j < held; j += 32) {
+      const int p = row[j];
+      if (p < n_used || p >= c.pages) continue;
+      const int i = l.rank[p] - b_used;  // of a page that no count covers this is what some earlier call left: not followed
+      if (i >= 0 && i < moves && l.movers[b_used + i] == p) row[j] = l.holes[i];
+    }
+  }
+}
+
+// ---- host -------------------------------------------------------------------------------------------------------------
+static bool misaligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) != 0; }
+
+static int kv_view(const fa4b_kv_cache* c, KvView* out) {
+  FA4B_REQUIRE(c != nullptr, FA4B_BAD_ARG, "cache is NULL");
+  FA4B_REQUIRE(c->dtype == FA4B_KV_BF16 || c->dtype == FA4B_KV_F16 || c->dtype == FA4B_KV_E4M3, FA4B_UNSUPPORTED, "unknown cache dtype %d", c->dtype);
+  FA4B_REQUIRE(c->D == 64 || c->D == 128, FA4B_BAD_SHAPE, "head dim %d: only 64 and 128 are built", c->D);
+  FA4B_REQUIRE(c->page_tokens == 16 || c->page_tokens == 32 || c->page_tokens == 64 || c->page_tokens == 128, FA4B_BAD_SHAPE,
+               "pages of %d tokens: 16, 32, 64 or 128 are built", c->page_tokens);
+  FA4B_REQUIRE(c->layers > 0 && c->num_pages > 0 && c->Hkv > 0 && c->max_seqs > 0 && c->table_width > 0, FA4B_BAD_SHAPE,
+               "layers, num_pages, Hkv, max_seqs and table_width must be positive");
+  FA4B_REQUIRE(c->max_seqs <= FA4B_KV_MAX_SEQS, FA4B_BAD_SHAPE, "max_seqs=%d is above %d", c->max_seqs, (int)FA4B_KV_MAX_SEQS);
+  FA4B_REQUIRE(c->table_width <= (1 << 18) && c->Hkv <= 1024 && c->layers <= 4096 && c->num_pages <= 1 << 30, FA4B_BAD_SHAPE,
+               "table_width <= 2^18, Hkv <= 1024, layers <= 4096 and num_pages <= 2^30 are built");
+  const int esz = c->dtype == FA4B_KV_E4M3 ? 1 : 2;
+  const int64_t block = (int64_t)c->Hkv * c->page_tokens * c->D;
+  FA4B_REQUIRE(c->k && c->v && c->page_table && c->seq_lens && c->ref_counts && c->work, FA4B_BAD_ARG, "NULL buffer in the cache");
+  FA4B_REQUIRE(c->dtype != FA4B_KV_E4M3 || (c->k_scale && c->v_scale), FA4B_BAD_ARG, "an E4M3 cache needs k_scale and v_scale");
+  FA4B_REQUIRE(!misaligned(c->k, 16) && !misaligned(c->v, 16) && !misaligned(c->ref_counts, 16) && !misaligned(c->work, 16), FA4B_BAD_ALIGN,
+               "k, v, ref_counts and work must be 16-byte aligned");
+  FA4B_REQUIRE(c->table_stride >= c->table_width || c->max_seqs == 1, FA4B_BAD_SHAPE, "rows of the page table overlap (stride %lld, width %d)",
+               (long long)c->table_stride, c->table_width);
+  const int64_t strides[4] = {c->k_layer_stride, c->k_page_stride, c->v_layer_stride, c->v_page_stride};
+  for (int64_t s : strides)
+    FA4B_REQUIRE(s >= 0 && s * esz % 16 == 0, FA4B_BAD_ALIGN, "layer and page strides must be multiples of 16 bytes");
+  FA4B_REQUIRE(c->num_pages == 1 || (c->k_page_stride >= block && c->v_page_stride >= block), FA4B_BAD_SHAPE, "pages overlap: the page stride is below %lld",
+               (long long)block);
+  KvView v{};
+  v.k = static_cast<uint8_t*>(c->k);
+  v.v = static_cast<uint8_t*>(c->v);
+  v.k_layer = c->k_layer_stride * esz, v.k_page = c->k_page_stride * esz;
+  v.v_layer = c->v_layer_stride * esz, v.v_page = c->v_page_stride * esz;
+  v.layers = c->layers, v.pages = c->num_pages, v.heads = c->Hkv, v.page_tokens = c->page_tokens;
+  v.page_shift = __builtin_ctz((unsigned)c->page_tokens);
+  v.row_bytes = c->D * esz;
+  v.block_bytes = (int)(block * esz);
+  v.table = c->page_table, v.table_stride = c->table_stride, v.max_seqs = c->max_seqs, v.width = c->table_width;
+  v.lens = c->seq_lens, v.refs = c->ref_counts, v.work = static_cast<int32_t*>(c->work);
+  *out = v;
+  return FA4B_OK;
+}
+
+static int check_list(const fa4b_kv_cache* c, const void* a, const void* b, int32_t n) {
+  FA4B_REQUIRE(n >= 0 && n <= FA4B_KV_MAX_LIST, FA4B_BAD_SHAPE, "lists of 0 to %d entries are built, got %d", (int)FA4B_KV_MAX_LIST, n);
+  FA4B_REQUIRE(n == 0 || (a && b), FA4B_BAD_ARG, "NULL list");
+  (void)c;
+  return FA4B_OK;
+}
+
+template <typename K>
+static int allow_smem(K kernel, size_t bytes) {
+  if (bytes > 48 * 1024) FA4B_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+  return FA4B_OK;
+}
+
+}  // namespace fa4b
+
+using namespace fa4b;
+
+extern "C" {
+
+size_t fa4b_kv_workspace_bytes(const fa4b_kv_cache* c) {
+  if (c == nullptr || c->num_pages <= 0) return 0;
+  return 4 * ((size_t)kWorkLists + compact_blocks(c->num_pages) + 3 * (size_t)c->num_pages);
+}
+
+int fa4b_kv_free(const fa4b_kv_cache* c, const int32_t* seqs, int32_t n, void* stream) {
+  KvView v;
+  if (int s = kv_view(c, &v)) return s;
+  if (int s = check_list(c, seqs, seqs, n)) return s;
+  if (n == 0) return FA4B_OK;
+  FA4B_CUDA(launch_overlapped(kv_free_kernel, n, 128, 0, static_cast<cudaStream_t>(stream), v, seqs));
+  return FA4B_OK;
+}
+
+int fa4b_kv_extend(const fa4b_kv_cache* c, const int32_t* seqs, const int32_t* n_new, int32_t n, void* stream) {
+  KvView v;
+  if (int s = kv_view(c, &v)) return s;
+  if (int s = check_list(c, seqs, n_new, n)) return s;
+  if (n == 0) return FA4B_OK;
+  const size_t smem = 4 * ((size_t)n + 1 + (v.max_seqs + 31) / 32);
+  if (int s = allow_smem(kv_extend_kernel, smem)) return s;
+  int32_t* fresh = v.work + kWorkLists;  // the lists of a compaction are at least num_pages long
+  FA4B_CUDA(launch_overlapped(kv_extend_kernel, 1, 1024, smem, static_cast<cudaStream_t>(stream), v, seqs, n_new, n, fresh));
+  return FA4B_OK;
+}
+
+int fa4b_kv_write(const fa4b_kv_cache* c, const fa4b_kv_write_args* a, void* stream) {
+  KvView v;
+  if (int s = kv_view(c, &v)) return s;
+  FA4B_REQUIRE(a != nullptr, FA4B_BAD_ARG, "args is NULL");
+  if (int s = check_list(c, a->seqs, a->seqs, a->n)) return s;
+  FA4B_REQUIRE(a->T >= 0, FA4B_BAD_SHAPE, "T=%d is negative", a->T);
+  FA4B_REQUIRE(a->layer >= 0 && a->layer < c->layers, FA4B_BAD_SHAPE, "layer %d of %d", a->layer, c->layers);
+  FA4B_REQUIRE(a->src_dtype == FA4B_KV_BF16 || a->src_dtype == FA4B_KV_F16, FA4B_UNSUPPORTED, "values are written from bf16 or f16");
+  FA4B_REQUIRE(c->dtype == FA4B_KV_E4M3 || a->src_dtype == c->dtype, FA4B_UNSUPPORTED, "a 16-bit cache takes values of its own type");
+  if (a->n == 0 || a->T == 0) return FA4B_OK;
+  FA4B_REQUIRE(a->k_new && a->v_new, FA4B_BAD_ARG, "k_new or v_new is NULL");
+  FA4B_REQUIRE(!misaligned(a->k_new, 16) && !misaligned(a->v_new, 16), FA4B_BAD_ALIGN, "k_new and v_new must be 16-byte aligned");
+  const fa4b_strides st[2] = {a->k_strides, a->v_strides};
+  WriteParams w{};
+  w.src[0] = static_cast<const uint8_t*>(a->k_new), w.src[1] = static_cast<const uint8_t*>(a->v_new);
+  for (int i = 0; i < 2; ++i) {
+    FA4B_REQUIRE(st[i].batch % 8 == 0 && st[i].head % 8 == 0 && st[i].seq % 8 == 0, FA4B_BAD_ALIGN, "strides must be multiples of 8 elements");
+    w.sb[i] = st[i].batch * 2, w.sh[i] = st[i].head * 2, w.st[i] = st[i].seq * 2;
+  }
+  if (c->dtype == FA4B_KV_E4M3) w.scale[0] = c->k_scale + (int64_t)a->layer * c->Hkv, w.scale[1] = c->v_scale + (int64_t)a->layer * c->Hkv;
+  w.dst[0] = v.k + a->layer * v.k_layer, w.dst[1] = v.v + a->layer * v.v_layer;
+  w.seqs = a->seqs, w.n_new = a->n_new, w.T = a->T, w.D = c->D;
+  w.tile_tokens = 4 * (256 / (c->D / 8));  // four tokens of K and V in flight per thread
+  const int64_t tiles = ((int64_t)a->T + w.tile_tokens - 1) / w.tile_tokens;
+  FA4B_REQUIRE(tiles <= 65535, FA4B_BAD_SHAPE, "T=%d: at most %d tokens in one call", a->T, 65535 * w.tile_tokens);
+  const dim3 grid((unsigned)(a->n * c->Hkv), (unsigned)tiles);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (c->dtype != FA4B_KV_E4M3) FA4B_CUDA(launch_overlapped(kv_write_kernel<false, __nv_bfloat16>, grid, 256, 0, s, v, w));
+  else if (a->src_dtype == FA4B_KV_F16) FA4B_CUDA(launch_overlapped(kv_write_kernel<true, __half>, grid, 256, 0, s, v, w));
+  else FA4B_CUDA(launch_overlapped(kv_write_kernel<true, __nv_bfloat16>, grid, 256, 0, s, v, w));
+  return FA4B_OK;
+}
+
+int fa4b_kv_fork(const fa4b_kv_cache* c, const int32_t* parents, const int32_t* children, int32_t n, void* stream) {
+  KvView v;
+  if (int s = kv_view(c, &v)) return s;
+  if (int s = check_list(c, parents, children, n)) return s;
+  if (n == 0) return FA4B_OK;
+  const int pieces = (v.page_tokens * v.row_bytes + kWarpBytes - 1) / kWarpBytes;
+  const int64_t units = (int64_t)n * v.layers * 2 * v.heads * pieces, ctas = n + (units + 7) / 8;
+  FA4B_REQUIRE(ctas < 1ll << 31, FA4B_BAD_SHAPE, "%d forks over %d layers and %d heads are too many for one call", n, v.layers, v.heads);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const size_t smem = 4 * (size_t)((v.max_seqs + 31) / 32);
+  FA4B_CUDA(launch_overlapped(kv_fork_plan_kernel, 1, 1024, smem, st, v, parents, children, n, v.work + kWorkFlags));
+  FA4B_CUDA(launch_overlapped(kv_fork_move_kernel, (unsigned)ctas, 256, 0, st, v, parents, children, n, pieces, units));
+  return FA4B_OK;
+}
+
+int fa4b_kv_copy_pages(const fa4b_kv_cache* c, const int32_t* src, const int32_t* dst, int32_t n, void* stream) {
+  KvView v;
+  if (int s = kv_view(c, &v)) return s;
+  if (int s = check_list(c, src, dst, n)) return s;
+  if (n == 0) return FA4B_OK;
+  const int pieces = (v.block_bytes + kPieceBytes - 1) / kPieceBytes;
+  const int64_t ctas = (int64_t)n * v.layers * 2 * pieces;
+  FA4B_REQUIRE(ctas < 1ll << 31, FA4B_BAD_SHAPE, "%d pages of %d layers are too many for one call", n, v.layers);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (n > kCheckInline) FA4B_CUDA(launch_overlapped(kv_copy_check_kernel, (n + 7) / 8, 256, 0, st, v, src, dst, n));
+  FA4B_CUDA(launch_overlapped(kv_copy_kernel, (unsigned)ctas, 256, 0, st, v, src, dst, n, pieces));
+  return FA4B_OK;
+}
+
+int fa4b_kv_compact(const fa4b_kv_cache* c, void* stream) {
+  KvView v;
+  if (int s = kv_view(c, &v)) return s;
+  const int pieces = (v.block_bytes + kPieceBytes - 1) / kPieceBytes;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  FA4B_CUDA(launch_overlapped(kv_compact_count_kernel, compact_blocks(v.pages), 256, 0, st, v));
+  FA4B_CUDA(launch_overlapped(kv_compact_plan_kernel, compact_blocks(v.pages), 256, 0, st, v));
+  const int64_t most = std::max<int64_t>((int64_t)(v.pages / 2) * v.layers * 2 * pieces, (v.max_seqs + 7) / 8);
+  const unsigned grid = (unsigned)std::min<int64_t>(std::max<int64_t>(most, 1), (int64_t)std::max(sm_count(), 1) * 6);
+  FA4B_CUDA(launch_overlapped(kv_compact_move_kernel, grid, 256, 0, st, v, pieces));
+  return FA4B_OK;
+}
+
+int fa4b_kv_check_status(const fa4b_kv_cache* c, void* stream) {
+  KvView v;
+  if (int s = kv_view(c, &v)) return s;
+  int32_t host[3] = {0, 0, 0};
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  FA4B_CUDA(cudaMemcpyAsync(host, v.work + kWorkStatus, sizeof(host), cudaMemcpyDeviceToHost, st));
+  FA4B_CUDA(cudaStreamSynchronize(st));
+  if (host[0] == kOk) return FA4B_OK;
+  FA4B_CUDA(cudaMemsetAsync(v.work + kWorkStatus, 0, sizeof(host), st));
+  switch (host[0]) {
+    case kNoPages: set_error("%d pages were asked for, %d are free", host[1], host[2]); return FA4B_NO_PAGES;
+    case kBadSlot: set_error("entry %d names slot %d of %d", host[1], host[2], v.max_seqs); break;
+    case kSlotTwice: set_error("entry %d names slot %d a second time", host[1], host[2]); break;
+    case kChildInUse: set_error("entry %d forks into slot %d, which is not empty", host[1], host[2]); break;
+    case kRowTooShort: set_error("entry %d: a row of the page table holds %d pages, too few for slot %d", host[1], v.width, host[2]); break;
+    case kBadPage: set_error("pair %d names page %d of %d", host[1], host[2], v.pages); break;
+    case kBadCount: set_error("entry %d: negative number of new tokens for slot %d", host[1], host[2]); break;
+    case kCollision: set_error("pair %d: page %d is also another pair's destination or source", host[1], host[2]); break;
+    default: set_error("finding %d (%d, %d)", host[0], host[1], host[2]); break;
+  }
+  return FA4B_BAD_ARG;
+}
+
+}  // extern "C"

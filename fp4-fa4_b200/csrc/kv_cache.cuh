@@ -1,0 +1,45 @@
+// The paged key / value cache as the kernels see it, and launches that overlap the end of the one before.
+#pragma once
+#include "common.cuh"
+
+#include <algorithm>
+#include <utility>
+
+namespace fa4b {
+
+// Strides and row sizes in bytes.
+struct KvView {
+  uint8_t* k;
+  uint8_t* v;
+  int64_t k_layer, k_page, v_layer, v_page;
+  int layers, pages, heads, page_tokens, page_shift, row_bytes, block_bytes;  // block: the dense [heads, tokens, D] of a page
+  int32_t* table;
+  int64_t table_stride;
+  int max_seqs, width;
+  int32_t* lens;
+  int32_t* refs;
+  int32_t* work;
+};
+
+// A launch that may begin while the kernel before it on the stream still runs: every kernel launched this way runs
+// pdl_wait() before it touches memory (which returns once the kernel before has ended and its writes are visible), so only
+// the launch itself overlaps.  pdl_trigger() lets the next such launch come up early.
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+template <typename... P, typename... A>
+cudaError_t launch_overlapped(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, A&&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(std::forward<A>(args))...);
+}
+
+}  // namespace fa4b

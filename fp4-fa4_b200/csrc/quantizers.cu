@@ -702,6 +702,7 @@ const char* fa4b_status_string(int s) {
     case FA4B_CUDA_ERROR: return "CUDA error";
     case FA4B_TIMEOUT: return "device wait timed out";
     case FA4B_BAD_ARG: return "bad argument";
+    case FA4B_NO_PAGES: return "no free pages";
     default: return "unknown status";
   }
 }

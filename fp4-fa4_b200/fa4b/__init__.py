@@ -5,6 +5,7 @@ include/fa4b.h; every operator runs hand-written CUDA and raises if the
 library is missing."""
 
 from . import _lib, parallel  # noqa: F401
+from .kv_cache import PagedKVCache  # noqa: F401
 from .quantizers import (  # noqa: F401
     amax,
     dequant_mxfp4,
@@ -24,5 +25,5 @@ from .quantizers import (  # noqa: F401
 
 __all__ = [
     "amax", "dequant_mxfp4", "dequant_nvfp4", "mxfp4_quantize_for_gemm", "prepare_nvfp4_projection_weight", "project_nvfp4", "project_qkv_publish", "project_dout_publish", "rope_pair_", "pack_qkv_grads", "prepare_nvfp4_projection_weight_dual", "rmsnorm_backward_bf16", "tk_fused_norm_quantize",
-    "tk_quantize_for_gemm",
+    "tk_quantize_for_gemm", "PagedKVCache",
 ]

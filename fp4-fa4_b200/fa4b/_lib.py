@@ -11,7 +11,7 @@ import pathlib
 
 _LIB_PATH = pathlib.Path(__file__).resolve().parents[1] / "lib" / "libfa4b.so"
 
-STATUS_EXC = {1: ValueError, 2: ValueError, 3: NotImplementedError, 4: RuntimeError, 5: TimeoutError, 6: ValueError}
+STATUS_EXC = {1: ValueError, 2: ValueError, 3: NotImplementedError, 4: RuntimeError, 5: TimeoutError, 6: ValueError, 7: RuntimeError}
 
 
 class Fa4bError(RuntimeError):
@@ -104,6 +104,19 @@ class BwdPlan(C.Structure):
                 ("grid", C.c_int64)]
 
 
+class KvCache(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_layer_stride", C.c_int64), ("k_page_stride", C.c_int64),
+                ("v_layer_stride", C.c_int64), ("v_page_stride", C.c_int64), ("layers", C.c_int32), ("num_pages", C.c_int32),
+                ("Hkv", C.c_int32), ("page_tokens", C.c_int32), ("D", C.c_int32), ("dtype", C.c_int32), ("k_scale", C.c_void_p),
+                ("v_scale", C.c_void_p), ("page_table", C.c_void_p), ("table_stride", C.c_int64), ("max_seqs", C.c_int32),
+                ("table_width", C.c_int32), ("seq_lens", C.c_void_p), ("ref_counts", C.c_void_p), ("work", C.c_void_p)]
+
+
+class KvWriteArgs(C.Structure):
+    _fields_ = [("k_new", C.c_void_p), ("v_new", C.c_void_p), ("k_strides", Strides), ("v_strides", Strides), ("T", C.c_int32),
+                ("src_dtype", C.c_int32), ("layer", C.c_int32), ("n", C.c_int32), ("seqs", C.c_void_p), ("n_new", C.c_void_p)]
+
+
 class Info(C.Structure):
     _fields_ = [(n, C.c_int) for n in (
         "abi_version", "build_sm", "fwd_threads", "fwd_smem_bytes", "fwd_tmem_columns", "fwd_kv_stages",
@@ -114,7 +127,8 @@ EXPORTS = (
     "fa4b_status_string", "fa4b_last_error", "fa4b_query", "fa4b_amax", "fa4b_quant_nvfp4", "fa4b_quant_check_status", "fa4b_quant_nvfp4_weight", "fa4b_project_nvfp4", "fa4b_project_qkv_publish", "fa4b_project_dout_publish", "fa4b_rope_pair", "fa4b_pack_qkv_grads",
     "fa4b_rmsnorm_quant_nvfp4", "fa4b_quant_mxfp4", "fa4b_dequant_nvfp4", "fa4b_dequant_mxfp4",
     "fa4b_attn_workspace_bytes", "fa4b_attn_ws_layout_query", "fa4b_attn_prepare", "fa4b_attn_fwd",
-    "fa4b_attn_fwd_static", "fa4b_attn_bwd_preprocess", "fa4b_attn_bwd", "fa4b_attn_bwd_plan", "fa4b_attn_bwd_plan_item", "fa4b_attn_check_status", "fa4b_attn_merge", "fa4b_attn_accumulate", "fa4b_rmsnorm_bwd", "fa4b_rmsnorm_bwd_workspace_bytes", "fa4b_microgate", "fa4b_tensor_peak", "fa4b_wait_selftest",
+    "fa4b_attn_fwd_static", "fa4b_attn_bwd_preprocess", "fa4b_attn_bwd", "fa4b_attn_bwd_plan", "fa4b_attn_bwd_plan_item", "fa4b_attn_check_status", "fa4b_attn_merge", "fa4b_attn_accumulate", "fa4b_rmsnorm_bwd", "fa4b_rmsnorm_bwd_workspace_bytes", "fa4b_kv_workspace_bytes", "fa4b_kv_free", "fa4b_kv_extend", "fa4b_kv_write", "fa4b_kv_fork", "fa4b_kv_copy_pages", "fa4b_kv_compact", "fa4b_kv_check_status",
+    "fa4b_microgate", "fa4b_tensor_peak", "fa4b_wait_selftest",
 )
 
 _lib = None
@@ -132,6 +146,11 @@ def lib() -> C.CDLL:
         handle.fa4b_attn_workspace_bytes.restype = C.c_size_t
         handle.fa4b_rmsnorm_bwd_workspace_bytes.restype = C.c_size_t
         handle.fa4b_rmsnorm_bwd_workspace_bytes.argtypes = [C.c_int64]
+        handle.fa4b_kv_workspace_bytes.restype = C.c_size_t
+        p, i = C.c_void_p, C.c_int32
+        for name, args in (("workspace_bytes", (p,)), ("free", (p, p, i, p)), ("extend", (p, p, p, i, p)), ("write", (p, p, p)), ("fork", (p, p, p, i, p)),
+                           ("copy_pages", (p, p, p, i, p)), ("compact", (p, p)), ("check_status", (p, p))):
+            getattr(handle, f"fa4b_kv_{name}").argtypes = args
         for name in EXPORTS:
             getattr(handle, name)  # AttributeError if the ABI is incomplete
         _lib = handle
@@ -155,3 +174,26 @@ def current_stream() -> int:
     import torch
 
     return torch.cuda.current_stream().cuda_stream
+
+
+class on_device:
+    """The device of a call's tensors as the current one, and its current stream's handle."""
+
+    __slots__ = ("index", "before")
+
+    def __init__(self, device):
+        self.index = device.index
+
+    def __enter__(self) -> int:
+        import torch
+
+        self.before = torch.cuda.current_device()
+        if self.before != self.index:
+            torch.cuda.set_device(self.index)
+        return torch.cuda.current_stream(self.index).cuda_stream
+
+    def __exit__(self, *_):
+        import torch
+
+        if self.before != self.index:
+            torch.cuda.set_device(self.before)

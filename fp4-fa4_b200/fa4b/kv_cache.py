@@ -1,0 +1,169 @@
+"""Paged key / value cache over the C ABI: claim, write, fork, copy, compact and free pages, and attention over them.
+
+K and V are pools ``[layers, pages, Hkv, page tokens, D]`` (bf16, f16, or E4M3 with one factor per layer and kv head).
+A slot is one sequence: its row of ``page_table`` names its pages in order (-1 behind them), ``seq_lens`` its tokens,
+``ref_counts`` how many slots hold a page.  Everything lives on the device and no call synchronises, so a serving step
+(extend, write, attend) can be captured into a graph; lists of slots and pages are int32 CUDA tensors.  Calls on one
+cache have to be ordered on the device, as they change it."""
+
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from . import _lib
+from ._lib import check, lib, on_device, ptr
+
+KV_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float8_e4m3fn: 2}
+
+
+def _pool(t, name: str):
+    if not isinstance(t, torch.Tensor) or t.ndim != 5:
+        raise ValueError(f"{name} must be a [layers, pages, Hkv, page tokens, D] tensor")
+    if t.dtype not in KV_DTYPES:
+        raise TypeError(f"{name} must be bfloat16, float16 or float8_e4m3fn, got {t.dtype}")
+    if not t.is_cuda:
+        raise RuntimeError(f"{name} must live on a CUDA device (there is no CPU path)")
+    _, _, heads, tokens, d = t.shape
+    if t.stride()[2:] != (tokens * d, d, 1):
+        raise ValueError(f"the inner three dimensions of {name} must be contiguous")
+
+
+def _ints(t, name: str, ndim: int, device) -> None:
+    if not isinstance(t, torch.Tensor) or t.ndim != ndim:
+        raise ValueError(f"{name} must be a {ndim}-D tensor")
+    if t.dtype != torch.int32:
+        raise TypeError(f"{name} must be int32, got {t.dtype}")
+    if t.device != device:
+        raise RuntimeError(f"{name} must live on {device}, got {t.device}")
+    if t.stride(ndim - 1) != 1 and t.shape[ndim - 1] > 1:
+        raise ValueError(f"{name} must have a contiguous last dimension")
+
+
+class PagedKVCache:
+    """A cache over tensors that the caller made (:meth:`empty` makes them).
+
+    ``k``, ``v`` ``[layers, pages, Hkv, page tokens, D]``: inner three dimensions contiguous, any layer and page strides
+    (two views of one ``[layers, pages, 2, Hkv, page tokens, D]`` tensor serve).  ``k_scale``, ``v_scale`` f32
+    ``[layers, Hkv]``: what an E4M3 code is multiplied with."""
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor, ref_counts: torch.Tensor, *,
+                 k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None):
+        _pool(k, "k")
+        _pool(v, "v")
+        if k.shape != v.shape or k.dtype != v.dtype or k.device != v.device:
+            raise ValueError(f"k and v must be alike, got {tuple(k.shape)} {k.dtype} and {tuple(v.shape)} {v.dtype}")
+        layers, pages, heads, tokens, d = k.shape
+        _ints(page_table, "page_table", 2, k.device)
+        _ints(seq_lens, "seq_lens", 1, k.device)
+        _ints(ref_counts, "ref_counts", 1, k.device)
+        if seq_lens.shape[0] != page_table.shape[0]:
+            raise ValueError(f"page_table has {page_table.shape[0]} rows, seq_lens {seq_lens.shape[0]} entries")
+        if ref_counts.shape[0] != pages:
+            raise ValueError(f"ref_counts must have {pages} entries, got {ref_counts.shape[0]}")
+        e4m3 = k.dtype == torch.float8_e4m3fn
+        for t, name in ((k_scale, "k_scale"), (v_scale, "v_scale")):
+            if (t is not None) != e4m3:
+                raise ValueError(f"{name} goes with a float8_e4m3fn cache, and with no other")
+            if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != (layers, heads) or not t.is_contiguous() or t.device != k.device):
+                raise ValueError(f"{name} must be a contiguous float32 [{layers}, {heads}] tensor on {k.device}")
+        self.k, self.v, self.page_table, self.seq_lens, self.ref_counts = k, v, page_table, seq_lens, ref_counts
+        self.k_scale, self.v_scale = k_scale, v_scale
+        self.device = k.device
+        self._c = _lib.KvCache(ptr(k), ptr(v), k.stride(0), k.stride(1), v.stride(0), v.stride(1), layers, pages, heads, tokens, d,
+                               KV_DTYPES[k.dtype], ptr(k_scale), ptr(v_scale), ptr(page_table), page_table.stride(0), page_table.shape[0],
+                               page_table.shape[1], ptr(seq_lens), ptr(ref_counts), 0)
+        with on_device(self.device):
+            self._work = torch.zeros((lib().fa4b_kv_workspace_bytes(C.byref(self._c)) + 3) // 4, dtype=torch.int32, device=self.device)
+            self._c.work = ptr(self._work)
+            self._at = C.addressof(self._c)
+            check(lib().fa4b_kv_free(self._at, 0, 0, 0), "PagedKVCache")  # an empty list: the checks of the C side
+
+    @classmethod
+    def empty(cls, num_pages: int, page_tokens: int, n_kv_heads: int, head_dim: int, max_seqs: int, max_pages_per_seq: int, *, n_layers: int = 1,
+              dtype: torch.dtype = torch.bfloat16, device="cuda", k_scale=None, v_scale=None) -> "PagedKVCache":
+        """A cache with every page free and every slot empty; the pools are not initialised (nothing reads a token that
+        was not written)."""
+        if dtype not in KV_DTYPES:
+            raise TypeError(f"dtype must be bfloat16, float16 or float8_e4m3fn, got {dtype}")
+        shape = (n_layers, num_pages, n_kv_heads, page_tokens, head_dim)
+        if min(shape) < 1 or max_seqs < 1 or max_pages_per_seq < 1:
+            raise ValueError("all sizes must be positive")
+        pools = [torch.empty(shape, dtype=dtype, device=device) for _ in range(2)]
+        return cls(*pools, torch.full((max_seqs, max_pages_per_seq), -1, dtype=torch.int32, device=device),
+                   torch.zeros(max_seqs, dtype=torch.int32, device=device), torch.zeros(num_pages, dtype=torch.int32, device=device),
+                   k_scale=k_scale, v_scale=v_scale)
+
+    # ------------------------------------------------------------------------------------------------ pages
+    def _list(self, t, name: str, like: torch.Tensor | None = None) -> int:
+        _ints(t, name, 1, self.device)
+        if like is not None and t.shape[0] != like.shape[0]:
+            raise ValueError(f"{name} has {t.shape[0]} entries, expected {like.shape[0]}")
+        return t.data_ptr()
+
+    def free(self, seqs: torch.Tensor) -> None:
+        """The slots ``seqs`` give their pages back and are empty then.  Empty slots and repeated ones do no harm."""
+        a = self._list(seqs, "seqs")
+        with on_device(self.device) as stream:
+            check(lib().fa4b_kv_free(self._at, a, seqs.shape[0], stream), "fa4b_kv_free")
+
+    def extend(self, seqs: torch.Tensor, n_new: torch.Tensor) -> None:
+        """Slot ``seqs[i]`` grows by ``n_new[i]`` tokens (:meth:`write` fills them) and claims pages for them: the lowest
+        free ones, in the order of the list.  All or nothing; :meth:`check_status` tells."""
+        a, b = self._list(seqs, "seqs"), self._list(n_new, "n_new", seqs)
+        with on_device(self.device) as stream:
+            check(lib().fa4b_kv_extend(self._at, a, b, seqs.shape[0], stream), "fa4b_kv_extend")
+
+    def write(self, k: torch.Tensor, v: torch.Tensor, seqs: torch.Tensor, *, n_new: torch.Tensor | None = None, layer: int = 0) -> None:
+        """Keys and values ``[n, Hkv, T, D]`` (any batch / head / token strides) of the newest tokens: token ``t < n_new[i]``
+        goes to position ``seq_lens[seqs[i]] - n_new[i] + t`` (``n_new`` None: T for every row).  A 16-bit cache takes its
+        own type, an E4M3 cache bf16 or f16, divided by the scale, clamped to +-448 and rounded."""
+        c = self._c
+        a = self._list(seqs, "seqs")
+        b = 0 if n_new is None else self._list(n_new, "n_new", seqs)
+        for t, name in ((k, "k"), (v, "v")):
+            if not isinstance(t, torch.Tensor) or t.ndim != 4 or t.shape[0] != seqs.shape[0] or t.shape[1] != c.Hkv or t.shape[3] != c.D:
+                raise ValueError(f"{name} must be a [{seqs.shape[0]}, {c.Hkv}, T, {c.D}] tensor")
+            if t.dtype not in (torch.bfloat16, torch.float16) or (c.dtype != 2 and t.dtype != self.k.dtype):
+                raise TypeError(f"{name} is {t.dtype}, the cache {self.k.dtype}")
+            if t.device != self.device:
+                raise RuntimeError(f"{name} must live on {self.device}, got {t.device}")
+            if t.stride(3) != 1:
+                raise ValueError(f"{name} must have a contiguous head dimension")
+        if k.shape != v.shape or k.dtype != v.dtype:
+            raise ValueError("k and v must be alike")
+        w = _lib.KvWriteArgs(k.data_ptr(), v.data_ptr(), _strides(k), _strides(v), k.shape[2], KV_DTYPES[k.dtype], layer, seqs.shape[0], a, b)
+        with on_device(self.device) as stream:
+            check(lib().fa4b_kv_write(self._at, C.addressof(w), stream), "fa4b_kv_write")
+
+    def fork(self, parents: torch.Tensor, children: torch.Tensor) -> None:
+        """Slot ``children[i]``, which is empty, becomes a copy of ``parents[i]``: full pages are shared, the page that is
+        still being filled is copied.  All or nothing; :meth:`check_status` tells."""
+        a, b = self._list(parents, "parents"), self._list(children, "children", parents)
+        with on_device(self.device) as stream:
+            check(lib().fa4b_kv_fork(self._at, a, b, parents.shape[0], stream), "fa4b_kv_fork")
+
+    def copy_pages(self, src: torch.Tensor, dst: torch.Tensor) -> None:
+        """Pages ``src[i]`` to pages ``dst[i]`` in every layer; tables and counts stay.  A pair with a negative entry is
+        skipped, and one whose pages another pair writes, or whose destination another reads, is left out and reported."""
+        a, b = self._list(src, "src"), self._list(dst, "dst", src)
+        with on_device(self.device) as stream:
+            check(lib().fa4b_kv_copy_pages(self._at, a, b, src.shape[0], stream), "fa4b_kv_copy_pages")
+
+    def compact(self) -> None:
+        """Moves the used pages behind the first ``n`` (``n``: pages in use) to the free ones among them, in order, so
+        that the pages in use are ``0..n-1``; tables and counts follow."""
+        with on_device(self.device) as stream:
+            check(lib().fa4b_kv_compact(self._at, stream), "fa4b_kv_compact")
+
+    def check_status(self) -> None:
+        """Synchronise and raise on what the calls since the last check found wrong on the device (slots out of range, too
+        few free pages, ...)."""
+        with on_device(self.device) as stream:
+            check(lib().fa4b_kv_check_status(self._at, stream), "fa4b_kv_check_status")
+
+
+def _strides(t: torch.Tensor) -> _lib.Strides:
+    # a dimension of one entry carries no stride of its own
+    return _lib.Strides(*(s if n > 1 else 0 for n, s in zip(t.shape[:3], t.stride()[:3])))

@@ -30,7 +30,8 @@ typedef enum fa4b_status {
   FA4B_UNSUPPORTED = 3, /* format / mode / device not supported               */
   FA4B_CUDA_ERROR = 4,  /* a CUDA runtime or driver call failed               */
   FA4B_TIMEOUT = 5,     /* a bounded device-side wait ran out                 */
-  FA4B_BAD_ARG = 6      /* NULL where a buffer is required, overlap, ...      */
+  FA4B_BAD_ARG = 6,     /* NULL where a buffer is required, overlap, ...      */
+  FA4B_NO_PAGES = 7     /* a paged cache has fewer free pages than were asked */
 } fa4b_status;
 
 const char* fa4b_status_string(int status);
@@ -480,6 +481,82 @@ int fa4b_attn_accumulate(float* acc, const void* part, int64_t n, void* out, voi
  * query has no counterpart there).  ws == NULL: the built-in operand cache of
  * fa4b_attn_fwd_static on the current device. */
 int fa4b_attn_check_status(const fa4b_attn_dims* d, const void* ws, void* stream);
+
+/* ---- paged key / value cache ---------------------------------------------
+ * (no reference counterpart: the reference trains and evaluates whole sequences only)
+ *
+ * K and V live in two pools [layers, num_pages, Hkv, page_tokens, D] whose inner three dimensions are dense; the
+ * layer and page strides are the caller's (16-byte multiples).  A slot (a sequence) names its pages in its row of
+ * page_table; token j of slot s is row j % page_tokens of page page_table[s][j / page_tokens].  Invariants that every
+ * call keeps: a slot of length len has exactly ceil(len / page_tokens) entries, the rest of its row is -1;
+ * ref_counts[p] is the number of slots that hold page p (0: free); a page that several slots hold is full, so nothing
+ * is ever written to a shared page.  All of it is device memory: no call synchronises, all may be captured into a
+ * graph, and calls on one cache have to be ordered (one stream, or events), as they change it.
+ *
+ * What a call finds wrong on the device (an index out of range, no free pages, ...) goes to the status words in
+ * `work`, first finding kept; fa4b_kv_check_status reads and clears them.  extend and fork are all or nothing; the
+ * other calls leave out the entries that are wrong.  n is at most FA4B_KV_MAX_LIST; n == 0 returns at once. */
+enum { FA4B_KV_BF16 = 0, FA4B_KV_F16 = 1, FA4B_KV_E4M3 = 2 };
+enum { FA4B_KV_MAX_LIST = 4096, FA4B_KV_MAX_SEQS = 262144 };
+typedef struct fa4b_kv_cache {
+  void* k;                          /* 16-byte aligned */
+  void* v;
+  int64_t k_layer_stride, k_page_stride, v_layer_stride, v_page_stride; /* elements */
+  int32_t layers, num_pages, Hkv;
+  int32_t page_tokens;              /* 16, 32, 64 or 128 */
+  int32_t D;                        /* 64 or 128 */
+  int32_t dtype;                    /* FA4B_KV_* */
+  const float* k_scale;             /* E4M3: [layers, Hkv], what a code is multiplied with; else NULL */
+  const float* v_scale;
+  int32_t* page_table;              /* [max_seqs, table_width], row stride table_stride (elements) */
+  int64_t table_stride;
+  int32_t max_seqs, table_width;
+  int32_t* seq_lens;                /* [max_seqs] */
+  int32_t* ref_counts;              /* [num_pages], 16-byte aligned */
+  void* work;                       /* fa4b_kv_workspace_bytes bytes, 16-byte aligned, zeroed once before the first call */
+} fa4b_kv_cache;
+size_t fa4b_kv_workspace_bytes(const fa4b_kv_cache* c);
+
+/* fa4b_kv_free: the slots seqs[0..n) (device) give their pages back; a slot that is empty or named twice is freed once. */
+int fa4b_kv_free(const fa4b_kv_cache* c, const int32_t* seqs, int32_t n, void* stream);
+
+/* fa4b_kv_extend: slot seqs[i] grows by n_new[i] >= 0 tokens and claims the pages for them: the lowest free pages, in
+ * the order of i.  Nothing changes when a slot is out of range or named twice, a row of the table is too short, or
+ * there are too few free pages. */
+int fa4b_kv_extend(const fa4b_kv_cache* c, const int32_t* seqs, const int32_t* n_new, int32_t n, void* stream);
+
+/* fa4b_kv_write: token t < n_new[i] of row i goes to position seq_lens[seqs[i]] - n_new[i] + t (n_new NULL: T for every
+ * row).  k_new, v_new: [n, Hkv, T, D] bf16 or f16, batch / head / token strides in elements (multiples of 8), pointers
+ * 16-byte aligned.  A 16-bit cache takes values of its own type; an E4M3 cache stores RN(clamp(x / scale, +-448)),
+ * NaN kept.  Positions below 0 and rows whose slot is out of range are left out. */
+typedef struct fa4b_kv_write_args {
+  const void* k_new;
+  const void* v_new;
+  fa4b_strides k_strides, v_strides;
+  int32_t T, src_dtype, layer, n;
+  const int32_t* seqs;
+  const int32_t* n_new;
+} fa4b_kv_write_args;
+int fa4b_kv_write(const fa4b_kv_cache* c, const fa4b_kv_write_args* a, void* stream);
+
+/* fa4b_kv_fork: slot children[i], which is empty, becomes a copy of slot parents[i] (a parent may be named many times):
+ * it shares the parent's full pages and gets a page of its own (the lowest free ones, in the order of i) for the tokens
+ * behind them, which are copied in every layer.  Nothing changes when a slot is out of range, a child is not empty,
+ * named twice or a parent as well, or there are too few free pages. */
+int fa4b_kv_fork(const fa4b_kv_cache* c, const int32_t* parents, const int32_t* children, int32_t n, void* stream);
+
+/* fa4b_kv_copy_pages: pages src[i] to pages dst[i], all layers, K and V; tables and counts stay as they are.  A pair
+ * with an entry below 0 is skipped.  A pair whose destination is also another pair's destination or any pair's source,
+ * or whose source is any pair's destination, is left out and reported: the pairs are copied in no particular order. */
+int fa4b_kv_copy_pages(const fa4b_kv_cache* c, const int32_t* src, const int32_t* dst, int32_t n, void* stream);
+
+/* fa4b_kv_compact: with n pages in use, the k-th used page at or above n moves to the k-th free page below n, in all
+ * layers; tables and counts follow, so the pages in use are 0..n-1 afterwards. */
+int fa4b_kv_compact(const fa4b_kv_cache* c, void* stream);
+
+/* fa4b_kv_check_status: synchronises `stream`, returns what the calls since the last check found wrong
+ * (FA4B_NO_PAGES, FA4B_BAD_ARG; FA4B_OK when nothing) and clears it. */
+int fa4b_kv_check_status(const fa4b_kv_cache* c, void* stream);
 
 /* ---- tensor-core self tests ("microgates") -------------------------------
  * One 128x128xK product per launch through the same tcgen05 instruction

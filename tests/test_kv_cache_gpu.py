@@ -1,0 +1,299 @@
+"""Paged cache on the device against a model on lists: every byte of pools, tables, lengths and counts."""
+
+import random
+
+import pytest
+import torch
+
+from fa4b import PagedKVCache
+from kv_model import ModelCache
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+DTYPES = [torch.bfloat16, torch.float16, torch.float8_e4m3fn]
+
+
+def ints(x, dev=DEV):
+    return torch.tensor(x, dtype=torch.int32, device=dev)
+
+
+def make(pages=40, page=16, heads=2, d=64, seqs=12, width=9, layers=2, dtype=torch.bfloat16, seed=0, joint=False, dev=DEV):
+    """A cache whose pools hold noise; with `joint`, K and V are views of one tensor (other strides)."""
+    gen = torch.Generator().manual_seed(seed)
+    scales = {}
+    if dtype == torch.float8_e4m3fn:
+        scales = {n: (0.01 + 0.02 * torch.rand(layers, heads, generator=gen)).to(dev) for n in ("k_scale", "v_scale")}
+    noise = torch.randn(layers, pages, 2, heads, page, d, generator=gen).to(dtype).to(dev)
+    k, v = noise[:, :, 0], noise[:, :, 1]
+    if not joint:
+        k, v = k.contiguous(), v.contiguous()
+    return PagedKVCache(k, v, torch.full((seqs, width), -1, dtype=torch.int32, device=dev), torch.zeros(seqs, dtype=torch.int32, device=dev),
+                        torch.zeros(pages, dtype=torch.int32, device=dev), **scales)
+
+
+def values(n, heads, t, d, dtype, seed, dev=DEV):
+    gen = torch.Generator().manual_seed(seed)
+    return [(3 * torch.randn(n, heads, t, d, generator=gen)).to(dtype).to(dev) for _ in range(2)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("page,d,heads,joint", [(16, 64, 2, False), (32, 128, 3, True), (128, 64, 1, True), (64, 128, 8, False)])
+def test_a_random_run_of_all_calls(dtype, page, d, heads, joint):
+    rng = random.Random(page * 7 + d)
+    c = make(pages=60, page=page, heads=heads, d=d, seqs=14, width=7, layers=2, dtype=dtype, seed=3, joint=joint)
+    m = ModelCache(c)
+    src = torch.float16 if dtype == torch.float16 else torch.bfloat16
+    for step in range(40):
+        what = rng.choice(["extend", "extend", "free", "fork", "fork", "compact", "copy"])
+        slots = rng.sample(range(14), rng.randint(1, 6))
+        if what == "extend":
+            new = [rng.choice([0, 1, 1, page - 1, page, page + 1, 2 * page + 5]) for _ in slots]
+            c.extend(ints(slots), ints(new))
+            if m.extend(slots, new):
+                t = max(new)
+                layer = rng.randrange(2)
+                k, v = values(len(slots), heads, max(t, 1), d, src, step)
+                c.write(k, v, ints(slots), n_new=ints(new), layer=layer)
+                m.write(k, v, slots, new, layer)
+        elif what == "free":
+            c.free(ints(slots))
+            m.free(slots)
+        elif what == "fork":
+            full = [s for s in range(14) if m.lens[s]]
+            empty = [s for s in range(14) if not m.lens[s]]
+            if full and empty:
+                children = rng.sample(empty, rng.randint(1, len(empty)))
+                parents = [rng.choice(full) for _ in children]
+                c.fork(ints(parents), ints(children))
+                m.fork(parents, children)
+        elif what == "compact":
+            c.compact()
+            m.compact()
+        else:
+            free = [p for p, r in enumerate(m.refs) if r == 0]
+            used = [p for p, r in enumerate(m.refs) if r > 0]
+            n = min(len(free), len(used), 5)
+            a, b = rng.sample(used, n), rng.sample(free, n)
+            c.copy_pages(ints(a), ints(b))
+            m.copy_pages(a, b)
+        m.check(c, f"step {step}: {what}")
+        m.invariants()
+
+
+def test_status_of_a_run_without_faults_is_clean():
+    c = make()
+    c.extend(ints([0, 3]), ints([17, 40]))
+    c.fork(ints([0, 0, 3]), ints([1, 2, 4]))
+    c.free(ints([0, 0, 5]))  # a slot named twice and an empty one
+    c.compact()
+    c.copy_pages(ints([0, -1]), ints([30, 31]))
+    c.check_status()
+
+
+@pytest.mark.parametrize("call,error,text", [
+    (lambda c: c.extend(ints([1, 12]), ints([5, 5])), ValueError, "slot 12 of 12"),
+    (lambda c: c.extend(ints([1, -1]), ints([5, 5])), ValueError, "slot -1"),
+    (lambda c: c.extend(ints([1, 2, 1]), ints([5, 5, 5])), ValueError, "second time"),
+    (lambda c: c.extend(ints([1, 2]), ints([5, -5])), ValueError, "negative"),
+    (lambda c: c.extend(ints([1, 2]), ints([5, 9 * 16 + 1])), ValueError, "too few"),
+    (lambda c: c.extend(ints([0]), ints([2 ** 31 - 1])), ValueError, "too few"),
+    (lambda c: c.extend(ints([1, 2, 3, 4, 5]), ints([140, 140, 140, 140, 140])), RuntimeError, "45 pages were asked for, 36 are free"),
+    (lambda c: c.fork(ints([0, 0]), ints([3, 3])), ValueError, "second time"),
+    (lambda c: c.fork(ints([0]), ints([0])), ValueError, "not empty"),
+    (lambda c: c.fork(ints([0, 5]), ints([5, 6])), ValueError, "second time"),
+    (lambda c: c.fork(ints([12]), ints([5])), ValueError, "slot 12"),
+    (lambda c: c.fork(ints([0]), ints([99])), ValueError, "slot"),
+    (lambda c: c.free(ints([50])), ValueError, "slot 50"),
+    (lambda c: c.copy_pages(ints([0]), ints([40])), ValueError, "page 40 of 40"),
+    (lambda c: c.copy_pages(ints([0, 1]), ints([9, 9])), ValueError, "page 9"),
+    (lambda c: c.copy_pages(ints([0, 9]), ints([9, 11])), ValueError, "another pair"),
+    (lambda c: c.copy_pages(ints([3]), ints([3])), ValueError, "page 3"),
+    (lambda c: c.write(*values(1, 2, 3, 64, torch.bfloat16, 0), ints([77])), ValueError, "slot 77"),
+])
+def test_what_is_wrong_changes_nothing_and_is_reported_once(call, error, text):
+    c = make()
+    c.extend(ints([0]), ints([50]))
+    m = ModelCache(c)
+    call(c)
+    m.check(c)
+    with pytest.raises(error, match=text):
+        c.check_status()
+    c.check_status()
+
+
+def test_free_leaves_out_what_is_wrong_and_frees_the_rest():
+    c = make()
+    c.extend(ints([0, 1]), ints([50, 20]))
+    m = ModelCache(c)
+    c.free(ints([1, -7, 1]))
+    m.free([1])
+    m.check(c)
+    with pytest.raises(ValueError, match="slot -7"):
+        c.check_status()
+
+
+@pytest.mark.parametrize("n", [3, 600])
+def test_copies_that_collide_are_left_out(n):
+    c = make(pages=2 * n + 9, heads=1, layers=1)
+    m = ModelCache(c)
+    src, dst = list(range(n)), list(range(n, 2 * n))
+    dst[1] = dst[0]
+    src[-1] = 2 * n + 5
+    c.copy_pages(ints(src), ints(dst))
+    m.copy_pages(src, dst)
+    m.check(c)
+    with pytest.raises(ValueError, match="another pair"):
+        c.check_status()
+
+
+@pytest.mark.parametrize("pages", [1, 15, 16, 17, 4095, 4097, 40001])
+@pytest.mark.parametrize("share", [0.0, 0.02, 0.5, 0.97, 1.0])
+def test_compaction_of_pools_of_any_size(pages, share):
+    rng = random.Random(pages)
+    c = make(pages=pages, heads=1, layers=1, seqs=7, width=pages)
+    used = rng.sample(range(pages), int(pages * share))
+    table, lens, refs = c.page_table.cpu(), c.seq_lens.cpu(), c.ref_counts.cpu()
+    for i in range(7):
+        mine = used[i::7]
+        table[i, :len(mine)] = torch.tensor(mine, dtype=torch.int32)
+        lens[i] = max(0, 16 * len(mine) - i)
+        refs[mine] = 1
+    c.page_table.copy_(table), c.seq_lens.copy_(lens), c.ref_counts.copy_(refs)
+    m = ModelCache(c)
+    for _ in range(2):  # the second time there is nothing left to do
+        c.compact()
+        m.compact()
+        m.check(c)
+        m.invariants()
+    c.check_status()
+
+
+def test_claims_reach_over_a_long_list_of_counts_and_take_the_last_page():
+    c = make(pages=40000, heads=1, layers=1, d=64, seqs=3000, width=40000)
+    refs = torch.ones(40000, dtype=torch.int32)
+    spare = [5, 16383, 16384, 20001, 39998, 39999]
+    refs[spare] = 0
+    c.ref_counts.copy_(refs)
+    c.extend(ints([2999, 7]), ints([16 * 4, 2 * 16 - 3]))
+    assert c.page_table[2999, :4].tolist() == spare[:4] and c.page_table[7, :2].tolist() == spare[4:]
+    c.check_status()
+    c.extend(ints([8]), ints([1]))
+    with pytest.raises(RuntimeError, match="1 pages were asked for, 0 are free"):
+        c.check_status()
+
+
+def test_a_list_of_thousands():
+    c = make(pages=5000, heads=1, layers=1, seqs=4500, width=3)
+    m = ModelCache(c)
+    order = random.Random(1).sample(range(4500), 4096)
+    new = [1 + i % 17 for i in range(4096)]
+    c.extend(ints(order[:2500]), ints(new[:2500]))
+    assert m.extend(order[:2500], new[:2500])
+    m.check(c)
+    c.fork(ints(order[:1500]), ints(order[2500:4000]))
+    assert m.fork(order[:1500], order[2500:4000])
+    m.check(c)
+    c.free(ints(order))
+    m.free(order)
+    m.check(c)
+    c.check_status()
+    with pytest.raises(ValueError, match="4096"):
+        c.free(ints(list(range(4097))))
+
+
+@pytest.mark.parametrize("src", [torch.bfloat16, torch.float16])
+def test_what_an_e4m3_cache_stores(src):
+    """Against the quotient in 64 bits: the 32-bit quotient is off by at most half a step (2^-24 relative), the code by half
+    an E4M3 step of it (2^-4 relative, 2^-10 below 2^-6); clamped at 448, NaN kept."""
+    c = make(pages=30, heads=3, d=128, layers=2, dtype=torch.float8_e4m3fn)
+    k, v = values(2, 3, 37, 128, src, 5)
+    k[0, 0, 0, :6] = torch.tensor([1e4, -1e4, float("inf"), -float("inf"), float("nan"), 0.0])
+    v[1, 2, 5, :64] = torch.linspace(-1e-4, 1e-4, 64)
+    c.extend(ints([4, 2]), ints([37, 37]))
+    c.write(k, v, ints([4, 2]), layer=1)
+    c.check_status()
+    for i, s in enumerate([4, 2]):
+        for pool, x, scale in ((c.k, k, c.k_scale), (c.v, v, c.v_scale)):
+            rows = pool[1, c.page_table[s, :3].long()].float().permute(1, 0, 2, 3).flatten(1, 2)[:, :37].double()
+            want = x[i].double() / scale[1].double()[:, None, None]
+            assert torch.equal(rows.isnan(), want.isnan())
+            want = want.clamp(-448, 448)
+            tol = torch.maximum(want.abs() * 2 ** -4 * (1 + 2 ** -20), torch.full_like(want, 2 ** -10)) + want.abs() * 2 ** -24
+            assert ((rows - want).abs() <= tol)[~want.isnan()].all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_write_takes_any_strides_and_leaves_other_tokens_alone(dtype):
+    c = make(dtype=dtype, heads=4, d=64)
+    src = torch.float16 if dtype == torch.float16 else torch.bfloat16
+    c.extend(ints([1, 2, 3]), ints([20, 33, 7]))
+    m = ModelCache(c)
+    flat = torch.randn(3, 9, 3 * 4 * 64, dtype=torch.float32).to(src).to(DEV)  # [n, T, (q k v) heads x d], as a projection leaves it
+    k, v = (flat[:, :, j * 256:(j + 1) * 256].view(3, 9, 4, 64).transpose(1, 2) for j in (1, 2))
+    assert not k.is_contiguous()
+    c.write(k, v, ints([1, 2, 3]), n_new=ints([9, 0, 12]), layer=0)  # 12 > T: the first 9 of 12; 12 > 7: positions below 0
+    m.write(k, v, [1, 2, 3], [9, 0, 12], 0)
+    m.check(c)
+    c.write(k[:, :, :1], v[:, :, :1], ints([3, 1, 2]), layer=1)
+    m.write(k[:, :, :1], v[:, :, :1], [3, 1, 2], None, 1)
+    m.check(c)
+    c.check_status()
+
+
+def test_empty_lists_and_no_tokens():
+    c = make()
+    m = ModelCache(c)
+    none = torch.empty(0, dtype=torch.int32, device=DEV)
+    c.free(none), c.extend(none, none), c.fork(none, none), c.copy_pages(none, none)
+    c.write(*values(0, 2, 3, 64, torch.bfloat16, 0), none)
+    c.write(*values(1, 2, 0, 64, torch.bfloat16, 0), ints([0]))
+    c.compact()
+    m.check(c)
+    c.check_status()
+
+
+def test_a_step_is_captured_and_replayed():
+    c = make(pages=50, width=8)
+    seqs, one = ints([0, 1]), ints([1, 1])
+    c.extend(ints([0, 1, 2]), ints([14, 30, 33]))
+    m = ModelCache(c)
+    k, v = values(2, 2, 1, 64, torch.bfloat16, 0)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            c.extend(seqs, one)
+            c.write(k, v, seqs)
+            c.free(ints_static := torch.zeros(1, dtype=torch.int32, device=DEV) + 5)
+            c.fork(seqs[:1], ints_static)
+            c.compact()
+    torch.cuda.current_stream().wait_stream(side)
+    m.check(c)  # capturing ran nothing
+    for step in range(5):
+        k.normal_(), v.normal_()
+        graph.replay()
+        assert m.extend([0, 1], [1, 1])
+        m.write(k, v, [0, 1], None, 0)
+        m.free([5])
+        assert m.fork([0], [5])
+        m.compact()
+        m.check(c, f"replay {step}")
+        m.invariants()
+    c.check_status()
+
+
+def test_calls_follow_the_current_stream():
+    c = make()
+    side = torch.cuda.Stream()
+    seqs, new = ints([0, 1]), ints([40, 16])
+    m = ModelCache(c)
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20_000_000)
+        c.extend(seqs, new)
+        c.fork(ints([0]), ints([3]))
+        c.check_status()
+    m.extend([0, 1], [40, 16])
+    m.fork([0], [3])
+    m.check(c)

@@ -1,0 +1,87 @@
+"""Refusals of the paged cache that need no device: the C entry points check before they launch, the Python side before it calls."""
+
+import ctypes as C
+
+import pytest
+import torch
+
+from fa4b import PagedKVCache, _lib
+
+
+def good(**change):
+    f = dict(k=0x10000, v=0x20000, k_layer_stride=100 * 8 * 16 * 128, k_page_stride=8 * 16 * 128, v_layer_stride=100 * 8 * 16 * 128,
+             v_page_stride=8 * 16 * 128, layers=2, num_pages=100, Hkv=8, page_tokens=16, D=128, dtype=0, k_scale=0, v_scale=0, page_table=0x30000,
+             table_stride=50, max_seqs=10, table_width=50, seq_lens=0x40000, ref_counts=0x50000, work=0x60000)
+    return _lib.KvCache(**(f | change))
+
+
+@pytest.mark.parametrize("change,status,text", [
+    (dict(D=96), 1, b"head dim"), (dict(page_tokens=24), 1, b"pages of 24"), (dict(page_tokens=0), 1, b"pages of 0"), (dict(dtype=3), 3, b"dtype"),
+    (dict(dtype=2), 6, b"k_scale"), (dict(k=0), 6, b"NULL"), (dict(k=0x10008), 2, b"16-byte"), (dict(work=0x60004), 2, b"16-byte"), (dict(work=0), 6, b"NULL"),
+    (dict(max_seqs=1 << 20), 1, b"max_seqs"), (dict(table_width=1 << 19, table_stride=1 << 19), 1, b"table_width"), (dict(layers=0), 1, b"positive"),
+    (dict(num_pages=-1), 1, b"positive"), (dict(table_stride=49), 1, b"overlap"), (dict(k_page_stride=8), 1, b"overlap"), (dict(v_layer_stride=12), 2, b"multiples"),
+])
+def test_every_call_refuses_a_bad_cache(change, status, text):
+    h = _lib.lib()
+    c = good(**change)
+    w = _lib.KvWriteArgs(0x1000, 0x1000, _lib.Strides(), _lib.Strides(), 1, 0, 0, 1, 0x1000, 0)
+    for got in (h.fa4b_kv_free(C.addressof(c), 0x1000, 1, 0), h.fa4b_kv_extend(C.addressof(c), 0x1000, 0x1000, 1, 0),
+                h.fa4b_kv_fork(C.addressof(c), 0x1000, 0x1000, 1, 0), h.fa4b_kv_copy_pages(C.addressof(c), 0x1000, 0x1000, 1, 0),
+                h.fa4b_kv_compact(C.addressof(c), 0), h.fa4b_kv_write(C.addressof(c), C.addressof(w), 0), h.fa4b_kv_check_status(C.addressof(c), 0)):
+        assert got == status and text in h.fa4b_last_error()
+
+
+def test_lists_and_arguments_are_checked():
+    h = _lib.lib()
+    c = good()
+    at = C.addressof(c)
+    assert h.fa4b_kv_free(None, 0x1000, 1, 0) == 6
+    assert h.fa4b_kv_free(at, 0x1000, -1, 0) == 1 and h.fa4b_kv_free(at, 0x1000, 4097, 0) == 1 and b"4096" in h.fa4b_last_error()
+    assert h.fa4b_kv_free(at, 0, 1, 0) == 6 and h.fa4b_kv_extend(at, 0x1000, 0, 1, 0) == 6 and h.fa4b_kv_fork(at, 0, 0x1000, 1, 0) == 6
+    assert h.fa4b_kv_free(at, 0, 0, 0) == 0 and h.fa4b_kv_copy_pages(at, 0, 0, 0, 0) == 0  # nothing to do
+    s = _lib.Strides(8, 8, 8)
+
+    def write(**change):
+        f = dict(k_new=0x1000, v_new=0x1000, k_strides=s, v_strides=s, T=1, src_dtype=0, layer=0, n=1, seqs=0x1000, n_new=0)
+        w = _lib.KvWriteArgs(**(f | change))
+        return h.fa4b_kv_write(at, C.addressof(w), 0)
+
+    assert write(layer=2) == 1 and write(layer=-1) == 1 and write(T=-1) == 1 and write(T=2 ** 31 - 1) == 1
+    assert write(src_dtype=1) == 3 and write(src_dtype=2) == 3
+    assert write(k_new=0) == 6 and write(seqs=0) == 6 and write(v_new=0x1008) == 2 and write(k_strides=_lib.Strides(4, 8, 8)) == 2
+    assert write(T=0) == 0 and write(n=0) == 0
+
+
+def test_workspace_bytes_cover_the_lists_of_a_compaction():
+    h = _lib.lib()
+    for pages in (1, 100, 4096, 4097, 1 << 20):
+        c = good(num_pages=pages)
+        assert h.fa4b_kv_workspace_bytes(C.addressof(c)) == 4 * (16 + 2 * 4096 + -(-pages // 4096) + 3 * pages)
+    assert h.fa4b_kv_workspace_bytes(None) == 0
+
+
+def test_constants_agree_between_the_header_and_the_python_side():
+    import pathlib
+    import re
+
+    from fa4b import kv_cache
+
+    header = (pathlib.Path(__file__).resolve().parents[1] / "include" / "fa4b.h").read_text()
+    got = {m.group(1): int(m.group(2)) for m in re.finditer(r"(FA4B_KV_(?:BF16|F16|E4M3)) = (\d+)", header)}
+    assert got == {"FA4B_KV_BF16": 0, "FA4B_KV_F16": 1, "FA4B_KV_E4M3": 2}
+    assert kv_cache.KV_DTYPES == {torch.bfloat16: 0, torch.float16: 1, torch.float8_e4m3fn: 2}
+
+
+def test_the_python_side_refuses_cpu_tensors_and_wrong_types():
+    k = torch.zeros(1, 4, 2, 16, 64, dtype=torch.bfloat16)
+    i = torch.zeros(4, dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        PagedKVCache(k, k.clone(), i[None], i[:1], i)
+    with pytest.raises(TypeError, match="float32"):
+        PagedKVCache(k.float(), k.float(), i[None], i[:1], i)
+    with pytest.raises(ValueError, match="layers"):
+        PagedKVCache(k[0], k[0], i[None], i[:1], i)
+    with pytest.raises(TypeError, match="dtype"):
+        PagedKVCache.empty(4, 16, 2, 64, 3, 3, dtype=torch.float32, device="cpu")
+    with pytest.raises(ValueError, match="positive"):
+        PagedKVCache.empty(4, 16, 2, 64, 0, 3, device="cpu")
