@@ -97,14 +97,16 @@ __global__ void __launch_bounds__(1024) paged_plan_kernel(const PagedParams p) {
   int* g_count = dyn + 2 * p.groups;
   pdl_trigger();
   for (int g = threadIdx.x; g < p.groups; g += 1024) g_min[g] = INT_MAX, g_first[g] = INT_MAX, g_count[g] = 0;
-  __syncthreads();
   pdl_wait();
-  if (threadIdx.x < 4) p.status[threadIdx.x] = 0u;
+  bool bad = false;  // groups have to lie behind one another: the slots of their units are counted on it
+  for (int g = threadIdx.x; g < p.groups; g += 1024) bad |= p.offsets[g] < 0 || p.offsets[g + 1] < p.offsets[g] || p.offsets[g + 1] > p.n;
+  bad = __syncthreads_or(bad);
+  if (bad && threadIdx.x == 0 && atomicCAS(p.status, 0u, 2u) == 0u) p.status[1] = (uint32_t)p.groups;
   for (int i = threadIdx.x; i < p.n; i += 1024) {
     const int slot = p.seqs ? p.seqs[i] : i;
-    int len = 0, g = p.groups > 0 ? -1 : 0;
+    int len = 0, g = p.groups > 0 || bad ? -1 : 0;
     if (slot >= 0 && slot < p.c.max_seqs) len = (int)min((int64_t)max(p.c.lens[slot], 0), (int64_t)p.c.width << p.c.page_shift);
-    if (p.groups > 0) {
+    if (p.groups > 0 && !bad) {
       int lo = 0, hi = p.groups;  // the last group that begins at or before i
       while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
@@ -127,8 +129,8 @@ __global__ void __launch_bounds__(1024) paged_plan_kernel(const PagedParams p) {
     if (g < p.groups) {
       const int lo = max(p.offsets[g], 0), hi = min(p.offsets[g + 1], p.n);
       int shared = g_count[g] > 1 ? min(max(p.shared[g], 0), g_min[g]) / kPagedAlign * kPagedAlign : 0;
-      if (hi <= lo) shared = 0;
-      own_u = hi > lo ? p.c.heads * ceil_div((hi - lo) * p.R, p.prefix_rows) : 0;
+      if (hi <= lo || bad) shared = 0;
+      own_u = hi > lo && !bad ? p.c.heads * ceil_div((hi - lo) * p.R, p.prefix_rows) : 0;
       own_t = own_u * ceil_div(shared, p.prefix_tile);
       p.plan.g_shared[g] = shared;
       p.plan.g_first[g] = shared ? g_first[g] : 0;
@@ -650,3 +652,135 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedParams p) {
 }
 
 }  // namespace fa4b
+
+// ---- host -------------------------------------------------------------------------------------------------------------
+namespace fa4b {
+
+template <int D, typename CacheT, typename QT, int kWM, bool kPrefix>
+static int launch_units(const PagedParams& p, const CUtensorMap& mk, const CUtensorMap& mv, int ctas, cudaStream_t st) {
+  auto kernel = attn_paged_kernel<D, CacheT, QT, kWM, kPrefix>;
+  constexpr int smem = (int)sizeof(PagedSmem<D, std::is_same<CacheT, uint8_t>::value ? 1 : 2>);
+  static_assert(smem <= 113 * 1024, "two CTAs per SM");
+  FA4B_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  FA4B_CUDA(launch_overlapped(kernel, ctas, kPagedThreads, smem, st, p, mk, mv));
+  return FA4B_OK;
+}
+
+template <int D, typename CacheT, typename QT>
+static int launch_paged(const PagedParams& p, const CUtensorMap& mk, const CUtensorMap& mv, cudaStream_t st) {
+  FA4B_CUDA(launch_overlapped(paged_plan_kernel, 1, 1024, 12 * (size_t)p.groups, st, p));
+  if (p.groups > 0)
+    if (int s = launch_units<D, CacheT, QT, 4, true>(p, mk, mv, p.prefix_ctas, st)) return s;
+  const int s = p.own_rows == 16   ? launch_units<D, CacheT, QT, 1, false>(p, mk, mv, p.own_ctas, st)
+                : p.own_rows == 32 ? launch_units<D, CacheT, QT, 2, false>(p, mk, mv, p.own_ctas, st)
+                                   : launch_units<D, CacheT, QT, 4, false>(p, mk, mv, p.own_ctas, st);
+  if (s) return s;
+  const int64_t rows = (int64_t)p.n * p.Hq * p.T;
+  FA4B_CUDA(launch_overlapped(paged_join_kernel<D, QT>, (unsigned)((rows + 7) / 8), 256, 0, st, p));
+  return FA4B_OK;
+}
+
+static bool off16(const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15) != 0; }
+
+// checks a call and lays its workspace out; `ws` may be NULL (a size query)
+static int paged_params(const fa4b_kv_cache* c, const fa4b_attn_paged_args* a, PagedParams* out, size_t* bytes) {
+  PagedParams p{};
+  if (int s = kv_view(c, &p.c)) return s;
+  FA4B_REQUIRE(a != nullptr, FA4B_BAD_ARG, "args is NULL");
+  FA4B_REQUIRE(a->n >= 0 && a->n <= kPagedMaxRows, FA4B_BAD_SHAPE, "n=%d: batches of 0 to %d rows are built", a->n, kPagedMaxRows);
+  FA4B_REQUIRE(a->T >= 1 && a->T <= kPagedMaxT, FA4B_BAD_SHAPE, "T=%d: 1 to %d query tokens per sequence are built", a->T, kPagedMaxT);
+  FA4B_REQUIRE(a->Hq > 0 && a->Hq % c->Hkv == 0, FA4B_BAD_SHAPE, "Hq=%d must be a multiple of Hkv=%d", a->Hq, c->Hkv);
+  FA4B_REQUIRE(a->Hq / c->Hkv <= 128, FA4B_BAD_SHAPE, "%d query heads per kv head: at most 128 are built", a->Hq / c->Hkv);
+  FA4B_REQUIRE(a->layer >= 0 && a->layer < c->layers, FA4B_BAD_SHAPE, "layer %d of %d", a->layer, c->layers);
+  FA4B_REQUIRE(a->q_dtype == FA4B_KV_BF16 || a->q_dtype == FA4B_KV_F16, FA4B_UNSUPPORTED, "queries are bf16 or f16");
+  FA4B_REQUIRE(c->dtype == FA4B_KV_E4M3 || a->q_dtype == c->dtype, FA4B_UNSUPPORTED, "a 16-bit cache takes queries of its own type");
+  FA4B_REQUIRE(a->groups >= 0 && a->groups <= std::max(a->n, 1), FA4B_BAD_SHAPE, "groups=%d: at most one for each of %d rows", a->groups, a->n);
+  FA4B_REQUIRE(a->groups == 0 || (a->group_offsets && a->shared_lens), FA4B_BAD_ARG, "groups need group_offsets and shared_lens");
+  FA4B_REQUIRE(a->seqs || a->n <= c->max_seqs, FA4B_BAD_SHAPE, "n=%d rows without a list of slots, and %d slots", a->n, c->max_seqs);
+  p.layer = a->layer, p.n = a->n, p.T = a->T, p.Hq = a->Hq, p.G = a->Hq / c->Hkv, p.R = p.T * p.G, p.groups = a->groups;
+  p.seqs = a->seqs, p.offsets = a->group_offsets, p.shared = a->shared_lens;
+  p.q = static_cast<const uint8_t*>(a->q), p.q_sb = a->q_strides.batch, p.q_sh = a->q_strides.head, p.q_st = a->q_strides.seq;
+  p.o = static_cast<uint8_t*>(a->o), p.o_sb = a->o_strides.batch, p.o_sh = a->o_strides.head, p.o_st = a->o_strides.seq;
+  p.lse = a->lse;
+  for (int64_t s : {p.q_sb, p.q_sh, p.q_st, p.o_sb, p.o_sh, p.o_st})
+    FA4B_REQUIRE(s % 8 == 0, FA4B_BAD_ALIGN, "strides of q and o must be multiples of 8 elements");
+  FA4B_REQUIRE(!off16(p.q) && !off16(p.o), FA4B_BAD_ALIGN, "q and o must be 16-byte aligned");
+  p.scale_log2 = (a->softmax_scale > 0.f ? a->softmax_scale : 1.0f / sqrtf((float)c->D)) * kLog2e;
+  if (c->dtype == FA4B_KV_E4M3) p.k_scale = c->k_scale + (int64_t)a->layer * c->Hkv, p.v_scale = c->v_scale + (int64_t)a->layer * c->Hkv;
+  const int n_sm = sm_count() > 0 ? sm_count() : 148;
+  p.own_rows = p.R <= 16 ? 16 : p.R <= 32 ? 32 : 64;
+  p.own_blocks = (p.R + p.own_rows - 1) / p.own_rows;
+  p.own_ctas = 2 * n_sm;
+  p.prefix_rows = 64, p.prefix_tile = 64, p.prefix_ctas = 2 * n_sm;
+  const int64_t row_tiles = ((int64_t)c->table_width * c->page_tokens + kPagedTile - 1) / kPagedTile + 1;
+  const int64_t prefix_units = p.groups ? (int64_t)c->Hkv * (((int64_t)p.n * p.R + p.prefix_rows - 1) / p.prefix_rows + p.groups) : 0;
+  const int64_t own_slots = (int64_t)p.n * c->Hkv * p.own_blocks + p.own_ctas, prefix_slots = p.groups ? prefix_units + p.prefix_ctas : 0;
+  // positions on the two lines are counted in 32 bits
+  FA4B_REQUIRE(p.n * row_tiles < INT32_MAX && prefix_units * row_tiles < INT32_MAX && own_slots < INT32_MAX, FA4B_BAD_SHAPE,
+               "%d rows over tables of %d pages of %d tokens are too many for one call", p.n, c->table_width, c->page_tokens);
+  size_t off = 0;
+  uint8_t* ws = static_cast<uint8_t*>(a->ws);
+  auto take = [&](size_t size) {
+    uint8_t* at = ws ? ws + off : nullptr;
+    off = align_up(off + size, 256);
+    return at;
+  };
+  const size_t n = p.n, g = p.groups;
+  p.plan.slot = reinterpret_cast<int*>(take(4 * n));
+  p.plan.len = reinterpret_cast<int*>(take(4 * n));
+  p.plan.group = reinterpret_cast<int*>(take(4 * n));
+  p.plan.own_cum = reinterpret_cast<int*>(take(4 * (n + 1)));
+  p.plan.g_first = reinterpret_cast<int*>(take(4 * g));
+  p.plan.g_shared = reinterpret_cast<int*>(take(4 * g));
+  p.plan.g_cum = reinterpret_cast<int*>(take(4 * (g + 1)));
+  p.plan.g_unit = reinterpret_cast<int*>(take(4 * (g + 1)));
+  p.own_ml = reinterpret_cast<float2*>(take((size_t)own_slots * p.own_rows * 8));
+  p.prefix_ml = reinterpret_cast<float2*>(take((size_t)prefix_slots * p.prefix_rows * 8));
+  p.own_acc = reinterpret_cast<float*>(take((size_t)own_slots * p.own_rows * c->D * 4));
+  p.prefix_acc = reinterpret_cast<float*>(take((size_t)prefix_slots * p.prefix_rows * c->D * 4));
+  p.status = reinterpret_cast<uint32_t*>(p.c.work + kKvAttnStatus);
+  *out = p;
+  *bytes = off;
+  return FA4B_OK;
+}
+
+}  // namespace fa4b
+
+using namespace fa4b;
+
+extern "C" {
+
+size_t fa4b_attn_paged_workspace_bytes(const fa4b_kv_cache* c, const fa4b_attn_paged_args* a) {
+  PagedParams p;
+  size_t bytes = 0;
+  return paged_params(c, a, &p, &bytes) == FA4B_OK ? bytes : 0;
+}
+
+int fa4b_attn_paged_fwd(const fa4b_kv_cache* c, const fa4b_attn_paged_args* a, void* stream) {
+  PagedParams p;
+  size_t bytes = 0;
+  if (int s = paged_params(c, a, &p, &bytes)) return s;
+  if (a->n == 0) return FA4B_OK;
+  FA4B_REQUIRE(a->q && a->o && a->lse && a->ws, FA4B_BAD_ARG, "q, o, lse or ws is NULL");
+  FA4B_REQUIRE((reinterpret_cast<uintptr_t>(a->ws) & 255) == 0, FA4B_BAD_ALIGN, "ws must be 256-byte aligned");
+  const bool e4m3 = c->dtype == FA4B_KV_E4M3;
+  CUtensorMap mk, mv;
+  const uint32_t box = c->D * (e4m3 ? 1 : 2) < 128 ? c->D : 128 / (e4m3 ? 1 : 2);
+  const int esz = e4m3 ? 1 : 2;
+  const uint64_t dims[5] = {(uint64_t)c->D, (uint64_t)c->page_tokens, (uint64_t)c->Hkv, (uint64_t)c->num_pages, (uint64_t)c->layers};
+  const uint32_t boxes[5] = {box, (uint32_t)std::min(c->page_tokens, kPagedTile), 1, 1, 1};
+  const uint64_t sk[4] = {(uint64_t)p.c.row_bytes, (uint64_t)p.c.row_bytes * c->page_tokens, (uint64_t)p.c.k_page, (uint64_t)p.c.k_layer};
+  const uint64_t sv[4] = {sk[0], sk[1], (uint64_t)p.c.v_page, (uint64_t)p.c.v_layer};
+  if (int s = make_tensor_map_5d(&mk, c->k, esz, dims, sk, boxes)) return s;
+  if (int s = make_tensor_map_5d(&mv, c->v, esz, dims, sv, boxes)) return s;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool q16 = a->q_dtype == FA4B_KV_F16;
+  if (c->D == 128) {
+    if (e4m3) return q16 ? launch_paged<128, uint8_t, TagF16>(p, mk, mv, st) : launch_paged<128, uint8_t, TagBf16>(p, mk, mv, st);
+    return q16 ? launch_paged<128, uint16_t, TagF16>(p, mk, mv, st) : launch_paged<128, uint16_t, TagBf16>(p, mk, mv, st);
+  }
+  if (e4m3) return q16 ? launch_paged<64, uint8_t, TagF16>(p, mk, mv, st) : launch_paged<64, uint8_t, TagBf16>(p, mk, mv, st);
+  return q16 ? launch_paged<64, uint16_t, TagF16>(p, mk, mv, st) : launch_paged<64, uint16_t, TagBf16>(p, mk, mv, st);
+}
+
+}  // extern "C"

@@ -6,9 +6,9 @@
 
 namespace fa4b {
 
-// `work` in 32-bit words: status, header of a compaction, the pages a fork claims, flags of a copy, then the lists of a
-// compaction: used pages of each block of kBlockPages, holes, movers by the used pages before them, and those per page
-constexpr int kWorkStatus = 0, kWorkHead = 8, kWorkFresh = 16, kWorkFlags = kWorkFresh + FA4B_KV_MAX_LIST,
+// `work` behind the status words: header of a fork or compaction, the pages a fork claims, flags of a copy, then the lists
+// of a compaction: used pages of each block of kBlockPages, holes, movers by the used pages before them, and those per page
+constexpr int kWorkStatus = kKvStatus, kWorkHead = kKvHead, kWorkFresh = 16, kWorkFlags = kWorkFresh + FA4B_KV_MAX_LIST,
               kWorkLists = kWorkFlags + FA4B_KV_MAX_LIST;
 constexpr int kBlockPages = 4096;
 constexpr int kPieceBytes = 32768;  // what one CTA of the copy kernels moves: 256 threads x 8 x 16 bytes, all loads in flight at once
@@ -547,7 +547,7 @@ __global__ void __launch_bounds__(256) kv_compact_move_kernel(const KvView c, in
 // ---- host -------------------------------------------------------------------------------------------------------------
 static bool misaligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) != 0; }
 
-static int kv_view(const fa4b_kv_cache* c, KvView* out) {
+int kv_view(const fa4b_kv_cache* c, KvView* out) {
   FA4B_REQUIRE(c != nullptr, FA4B_BAD_ARG, "cache is NULL");
   FA4B_REQUIRE(c->dtype == FA4B_KV_BF16 || c->dtype == FA4B_KV_F16 || c->dtype == FA4B_KV_E4M3, FA4B_UNSUPPORTED, "unknown cache dtype %d", c->dtype);
   FA4B_REQUIRE(c->D == 64 || c->D == 128, FA4B_BAD_SHAPE, "head dim %d: only 64 and 128 are built", c->D);
@@ -709,12 +709,18 @@ int fa4b_kv_compact(const fa4b_kv_cache* c, void* stream) {
 int fa4b_kv_check_status(const fa4b_kv_cache* c, void* stream) {
   KvView v;
   if (int s = kv_view(c, &v)) return s;
-  int32_t host[3] = {0, 0, 0};
+  int32_t host[kKvStatusWords] = {};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   FA4B_CUDA(cudaMemcpyAsync(host, v.work + kWorkStatus, sizeof(host), cudaMemcpyDeviceToHost, st));
   FA4B_CUDA(cudaStreamSynchronize(st));
-  if (host[0] == kOk) return FA4B_OK;
+  if (host[0] == kOk && host[kKvAttnStatus] == 0) return FA4B_OK;
   FA4B_CUDA(cudaMemsetAsync(v.work + kWorkStatus, 0, sizeof(host), st));
+  const int32_t* attn = host + kKvAttnStatus;
+  FA4B_REQUIRE(attn[0] != 1, FA4B_TIMEOUT, "a device-side wait of the attention over the cache ran out (site %d, block %d)", attn[1], attn[2]);
+  if (host[0] == kOk) {
+    set_error("the offsets of %d groups do not rise from 0 to at most the number of rows", attn[1]);
+    return FA4B_BAD_ARG;
+  }
   switch (host[0]) {
     case kNoPages: set_error("%d pages were asked for, %d are free", host[1], host[2]); return FA4B_NO_PAGES;
     case kBadSlot: set_error("entry %d names slot %d of %d", host[1], host[2], v.max_seqs); break;

@@ -65,6 +65,21 @@ int make_tensor_map_4d_bf16(CUtensorMap* out, const void* base, uint64_t inner, 
   return r == CUDA_SUCCESS ? FA4B_OK : FA4B_CUDA_ERROR;
 }
 
+int make_tensor_map_5d(CUtensorMap* out, const void* base, int elem_bytes, const uint64_t (&dims)[5], const uint64_t (&strides)[4],
+                       const uint32_t (&box)[5]) {
+  EncodeTiledFn fn = encode_fn();
+  FA4B_REQUIRE(fn != nullptr, FA4B_CUDA_ERROR, "cuTensorMapEncodeTiled is not available from this driver");
+  cuuint64_t d[5], s[4];
+  cuuint32_t b[5], one[5] = {1, 1, 1, 1, 1};
+  for (int i = 0; i < 5; ++i) d[i] = dims[i], b[i] = box[i];
+  for (int i = 0; i < 4; ++i) s[i] = dims[i + 1] > 1 && strides[i] ? strides[i] : dims[0] * elem_bytes;  // of one entry: none of its own
+  CUresult r = fn(out, elem_bytes == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<void*>(base), d, s, b, one,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, box[0] * elem_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  FA4B_REQUIRE(r == CUDA_SUCCESS, FA4B_CUDA_ERROR, "cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
+  return FA4B_OK;
+}
+
 struct GateSmem {
   alignas(1024) uint8_t a[128 * 128];
   alignas(1024) uint8_t b[128 * 128];

@@ -340,4 +340,9 @@ int make_tensor_map_4d_bf16(CUtensorMap* out, const void* base, uint64_t inner, 
                             uint64_t row_stride_bytes, uint64_t d2_stride_bytes, uint64_t d3_stride_bytes, uint32_t box_inner,
                             uint32_t box_rows);
 
+// 5-D tensor of 1- or 2-byte elements, inner dimension first; the inner box is 64 or 128 bytes wide and swizzled to match.
+// The stride of a dimension of one entry is not looked at.
+int make_tensor_map_5d(CUtensorMap* out, const void* base, int elem_bytes, const uint64_t (&dims)[5], const uint64_t (&strides)[4],
+                       const uint32_t (&box)[5]);
+
 }  // namespace fa4b

@@ -117,6 +117,13 @@ class KvWriteArgs(C.Structure):
                 ("src_dtype", C.c_int32), ("layer", C.c_int32), ("n", C.c_int32), ("seqs", C.c_void_p), ("n_new", C.c_void_p)]
 
 
+class AttnPagedArgs(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("q_strides", Strides), ("o", C.c_void_p), ("o_strides", Strides), ("lse", C.c_void_p),
+                ("n", C.c_int32), ("T", C.c_int32), ("Hq", C.c_int32), ("layer", C.c_int32), ("q_dtype", C.c_int32),
+                ("softmax_scale", C.c_float), ("seqs", C.c_void_p), ("groups", C.c_int32), ("group_offsets", C.c_void_p),
+                ("shared_lens", C.c_void_p), ("ws", C.c_void_p)]
+
+
 class Info(C.Structure):
     _fields_ = [(n, C.c_int) for n in (
         "abi_version", "build_sm", "fwd_threads", "fwd_smem_bytes", "fwd_tmem_columns", "fwd_kv_stages",
@@ -127,7 +134,7 @@ EXPORTS = (
     "fa4b_status_string", "fa4b_last_error", "fa4b_query", "fa4b_amax", "fa4b_quant_nvfp4", "fa4b_quant_check_status", "fa4b_quant_nvfp4_weight", "fa4b_project_nvfp4", "fa4b_project_qkv_publish", "fa4b_project_dout_publish", "fa4b_rope_pair", "fa4b_pack_qkv_grads",
     "fa4b_rmsnorm_quant_nvfp4", "fa4b_quant_mxfp4", "fa4b_dequant_nvfp4", "fa4b_dequant_mxfp4",
     "fa4b_attn_workspace_bytes", "fa4b_attn_ws_layout_query", "fa4b_attn_prepare", "fa4b_attn_fwd",
-    "fa4b_attn_fwd_static", "fa4b_attn_bwd_preprocess", "fa4b_attn_bwd", "fa4b_attn_bwd_plan", "fa4b_attn_bwd_plan_item", "fa4b_attn_check_status", "fa4b_attn_merge", "fa4b_attn_accumulate", "fa4b_rmsnorm_bwd", "fa4b_rmsnorm_bwd_workspace_bytes", "fa4b_kv_workspace_bytes", "fa4b_kv_free", "fa4b_kv_extend", "fa4b_kv_write", "fa4b_kv_fork", "fa4b_kv_copy_pages", "fa4b_kv_compact", "fa4b_kv_check_status",
+    "fa4b_attn_fwd_static", "fa4b_attn_bwd_preprocess", "fa4b_attn_bwd", "fa4b_attn_bwd_plan", "fa4b_attn_bwd_plan_item", "fa4b_attn_check_status", "fa4b_attn_merge", "fa4b_attn_accumulate", "fa4b_rmsnorm_bwd", "fa4b_rmsnorm_bwd_workspace_bytes", "fa4b_kv_workspace_bytes", "fa4b_kv_free", "fa4b_kv_extend", "fa4b_kv_write", "fa4b_kv_fork", "fa4b_kv_copy_pages", "fa4b_kv_compact", "fa4b_kv_check_status", "fa4b_attn_paged_workspace_bytes", "fa4b_attn_paged_fwd",
     "fa4b_microgate", "fa4b_tensor_peak", "fa4b_wait_selftest",
 )
 
@@ -147,7 +154,9 @@ def lib() -> C.CDLL:
         handle.fa4b_rmsnorm_bwd_workspace_bytes.restype = C.c_size_t
         handle.fa4b_rmsnorm_bwd_workspace_bytes.argtypes = [C.c_int64]
         handle.fa4b_kv_workspace_bytes.restype = C.c_size_t
+        handle.fa4b_attn_paged_workspace_bytes.restype = C.c_size_t
         p, i = C.c_void_p, C.c_int32
+        handle.fa4b_attn_paged_workspace_bytes.argtypes, handle.fa4b_attn_paged_fwd.argtypes = (p, p), (p, p, p)
         for name, args in (("workspace_bytes", (p,)), ("free", (p, p, i, p)), ("extend", (p, p, p, i, p)), ("write", (p, p, p)), ("fork", (p, p, p, i, p)),
                            ("copy_pages", (p, p, p, i, p)), ("compact", (p, p)), ("check_status", (p, p))):
             getattr(handle, f"fa4b_kv_{name}").argtypes = args

@@ -157,6 +157,51 @@ class PagedKVCache:
         with on_device(self.device) as stream:
             check(lib().fa4b_kv_compact(self._at, stream), "fa4b_kv_compact")
 
+    # ------------------------------------------------------------------------------------------------ attention
+    def attend(self, q: torch.Tensor, seqs: torch.Tensor | None = None, *, layer: int = 0, group_offsets: torch.Tensor | None = None,
+               shared_lens: torch.Tensor | None = None, softmax_scale: float | None = None, out: torch.Tensor | None = None):
+        """O ``[n, Hq, T, D]`` and LSE ``[n, Hq, T]`` f32 of the newest ``T <= 16`` tokens of ``n`` sequences: ``q [n, Hq, T, D]``
+        (any batch / head / token strides) over the pages of slots ``seqs`` (None: slot ``i`` for row ``i``).  Query ``t``
+        sees keys ``j < len - (T - 1 - t)``; a row that sees none, or whose slot is out of range (padding), is 0 with LSE -inf.
+
+        ``group_offsets [groups + 1]``, ``shared_lens [groups]``: rows ``group_offsets[g]`` up to ``group_offsets[g + 1]`` hold
+        the same pages for their first ``shared_lens[g]`` tokens (as :meth:`fork` leaves them), which are read once for
+        the group; rows in no group are left as they were.  ``out`` receives O when given (any strides)."""
+        c = self._c
+        if not isinstance(q, torch.Tensor) or q.ndim != 4 or q.shape[3] != c.D:
+            raise ValueError(f"q must be a [n, Hq, T, {c.D}] tensor")
+        if q.dtype not in (torch.bfloat16, torch.float16) or (c.dtype != 2 and q.dtype != self.k.dtype):
+            raise TypeError(f"q is {q.dtype}, the cache {self.k.dtype}")
+        if q.device != self.device:
+            raise RuntimeError(f"q must live on {self.device}, got {q.device}")
+        n, hq, t, d = q.shape
+        if q.stride(3) != 1:
+            raise ValueError("q must have a contiguous head dimension")
+        if (group_offsets is None) != (shared_lens is None):
+            raise ValueError("group_offsets and shared_lens go together")
+        slots = 0 if seqs is None else self._list(seqs, "seqs")
+        if seqs is not None and seqs.shape[0] != n:
+            raise ValueError(f"seqs has {seqs.shape[0]} entries, q {n} rows")
+        groups = offsets = shared = 0
+        if group_offsets is not None:
+            offsets, shared, groups = self._list(group_offsets, "group_offsets"), self._list(shared_lens, "shared_lens"), shared_lens.shape[0]
+            if group_offsets.shape[0] != groups + 1:
+                raise ValueError(f"group_offsets must have {groups + 1} entries, got {group_offsets.shape[0]}")
+        with on_device(self.device) as stream:
+            if out is None:
+                out = torch.empty(n, hq, t, d, dtype=q.dtype, device=self.device)
+            elif tuple(out.shape) != (n, hq, t, d) or out.dtype != q.dtype or out.device != self.device or out.stride(3) != 1:
+                raise ValueError(f"out must be a {tuple(q.shape)} tensor like q with a contiguous head dimension")
+            lse = torch.empty(n, hq, t, dtype=torch.float32, device=self.device)
+            a = _lib.AttnPagedArgs(q.data_ptr(), _strides(q), out.data_ptr(), _strides(out), lse.data_ptr(), n, t, hq, layer, KV_DTYPES[q.dtype],
+                                   softmax_scale or 0.0, slots, groups, offsets, shared, 0)
+            at = C.addressof(a)
+            need = lib().fa4b_attn_paged_workspace_bytes(self._at, at)
+            ws = torch.empty(need + 256, dtype=torch.uint8, device=self.device)
+            a.ws = (ws.data_ptr() + 255) & ~255
+            check(lib().fa4b_attn_paged_fwd(self._at, at, stream), "fa4b_attn_paged_fwd")
+        return out, lse
+
     def check_status(self) -> None:
         """Synchronise and raise on what the calls since the last check found wrong on the device (slots out of range, too
         few free pages, ...)."""

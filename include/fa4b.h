@@ -554,8 +554,34 @@ int fa4b_kv_copy_pages(const fa4b_kv_cache* c, const int32_t* src, const int32_t
  * layers; tables and counts follow, so the pages in use are 0..n-1 afterwards. */
 int fa4b_kv_compact(const fa4b_kv_cache* c, void* stream);
 
-/* fa4b_kv_check_status: synchronises `stream`, returns what the calls since the last check found wrong
- * (FA4B_NO_PAGES, FA4B_BAD_ARG; FA4B_OK when nothing) and clears it. */
+/* fa4b_attn_paged_fwd: attention of the newest T tokens of n sequences over their pages in one layer,
+ *   o[i, h, t] = sum_j softmax_j(softmax_scale q[i, h, t] . k_j) v_j  over keys j < len - (T - 1 - t) of slot seqs[i]
+ * (seqs NULL: slot i), and lse, the logarithm of the sum; query head h reads kv head h / (Hq / Hkv).  A row that sees
+ * no key (len 0, a slot out of range as padding, T > len) gets o = 0 and lse = -inf; keys of a page that the table does not name
+ * (entry out of range) do not exist.
+ *
+ * Groups: rows group_offsets[g] .. group_offsets[g + 1] - 1 hold the same pages for their first shared_lens[g] tokens
+ * (what fa4b_kv_fork makes); those are then read and multiplied once for the group instead of once per row.  The result is
+ * the same whatever is said to be shared, as long as it is; the table row of one member names the shared pages.  Offsets
+ * rise from 0 or more to n or less; rows in no group are left as they were.  groups == 0: every row by itself. */
+typedef struct fa4b_attn_paged_args {
+  const void* q; fa4b_strides q_strides;  /* [n, Hq, T, D] bf16 or f16 (16-bit caches: the cache's type); any strides, multiples of 8 */
+  void* o; fa4b_strides o_strides;        /* [n, Hq, T, D], q's type */
+  float* lse;                             /* [n, Hq, T] dense */
+  int32_t n, T, Hq, layer;                /* n <= 4096, T <= 16 */
+  int32_t q_dtype;                        /* FA4B_KV_BF16 or FA4B_KV_F16 */
+  float softmax_scale;                    /* <= 0: 1 / sqrt(D) */
+  const int32_t* seqs;                    /* [n] or NULL */
+  int32_t groups;
+  const int32_t* group_offsets;           /* [groups + 1] */
+  const int32_t* shared_lens;             /* [groups] */
+  void* ws;                               /* fa4b_attn_paged_workspace_bytes bytes, 256-byte aligned; not shared by calls that may overlap */
+} fa4b_attn_paged_args;
+size_t fa4b_attn_paged_workspace_bytes(const fa4b_kv_cache* c, const fa4b_attn_paged_args* a); /* 0: refused */
+int fa4b_attn_paged_fwd(const fa4b_kv_cache* c, const fa4b_attn_paged_args* a, void* stream);
+
+/* fa4b_kv_check_status: synchronises `stream`, returns what the calls since the last check found wrong (FA4B_NO_PAGES,
+ * FA4B_BAD_ARG; FA4B_TIMEOUT when a bounded wait of the attention ran out; FA4B_OK when nothing) and clears it. */
 int fa4b_kv_check_status(const fa4b_kv_cache* c, void* stream);
 
 /* ---- tensor-core self tests ("microgates") -------------------------------

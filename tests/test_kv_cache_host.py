@@ -85,3 +85,26 @@ def test_the_python_side_refuses_cpu_tensors_and_wrong_types():
         PagedKVCache.empty(4, 16, 2, 64, 3, 3, dtype=torch.float32, device="cpu")
     with pytest.raises(ValueError, match="positive"):
         PagedKVCache.empty(4, 16, 2, 64, 0, 3, device="cpu")
+
+
+def test_attention_over_the_cache_is_refused_before_a_launch():
+    h = _lib.lib()
+    z = _lib.Strides(1024, 128, 128)
+
+    def call(cache=None, **change):
+        f = dict(q=0x1000, q_strides=z, o=0x2000, o_strides=z, lse=0x3000, n=2, T=1, Hq=32, layer=0, q_dtype=0, softmax_scale=0.0, seqs=0x4000, groups=0,
+                 group_offsets=0, shared_lens=0, ws=0x10000)
+        a = _lib.AttnPagedArgs(**(f | change))
+        c = cache or good()
+        return h.fa4b_attn_paged_fwd(C.addressof(c), C.addressof(a), 0), h.fa4b_attn_paged_workspace_bytes(C.addressof(c), C.addressof(a)), h.fa4b_last_error()
+
+    for change, status, text in ((dict(n=-1), 1, b"n=-1"), (dict(n=5000), 1, b"n=5000"), (dict(T=0), 1, b"T=0"), (dict(T=17), 1, b"T=17"),
+                                 (dict(Hq=12), 1, b"multiple"), (dict(Hq=8 * 129), 1, b"at most 128"), (dict(layer=2), 1, b"layer 2"), (dict(q_dtype=1), 3, b"own type"),
+                                 (dict(q_dtype=2), 3, b"bf16 or f16"), (dict(groups=3), 1, b"groups=3"), (dict(groups=1), 6, b"group_offsets"),
+                                 (dict(seqs=0, n=11), 1, b"list of slots"), (dict(q=0x1008), 2, b"16-byte"), (dict(o_strides=_lib.Strides(4, 8, 8)), 2, b"multiples of 8")):
+        got, size, error = call(**change)
+        assert got == status and size == 0 and text in error, change
+    assert call(ws=0)[0] == 6 and call(lse=0)[0] == 6 and call(ws=0x10010)[0] == 2 and call(n=0, q=0, o=0, lse=0, ws=0)[0] == 0
+    got, size, error = call(cache=good(table_width=1 << 18, table_stride=1 << 18, page_tokens=128, k_page_stride=1 << 17, v_page_stride=1 << 17, max_seqs=5000), n=4096)
+    assert got == 1 and size == 0 and b"too many" in error
+    assert call(cache=good(D=96))[0] == 1
