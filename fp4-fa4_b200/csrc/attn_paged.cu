@@ -14,55 +14,6 @@ namespace fa4b {
 constexpr int kPagedThreads = 160;
 constexpr int kPagedStageBytes = 96 * 1024;  // shared memory for tiles in flight; two CTAs per SM
 
-// ---- numbers ----------------------------------------------------------------------------------------------------------
-struct TagBf16 {};
-struct TagF16 {};
-
-__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, TagBf16) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, TagF16) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ uint32_t pack16(float lo, float hi, TagBf16) {
-  uint32_t r;
-  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-__device__ __forceinline__ uint32_t pack16(float lo, float hi, TagF16) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-__device__ __forceinline__ float2 unpack16(uint32_t x, TagBf16) { return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u)); }
-__device__ __forceinline__ float2 unpack16(uint32_t x, TagF16) { return __half22float2(*reinterpret_cast<const __half2*>(&x)); }
-// two E4M3 codes -> f16 pair (exact)
-__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two) {
-  uint32_t r;
-  asm("{ .reg .b16 lo, hi; mov.b32 {lo, hi}, %1; cvt.rn.f16x2.e4m3x2 %0, lo; }" : "=r"(r) : "r"(two));
-  return r;
-}
-__device__ __forceinline__ float paged_ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
-__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
-__device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w, int u, uint64_t* bar) {
-  asm volatile("cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(dst),
-               "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(u)
-               : "memory");
-}
-
 // ---- plan -------------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ int paged_scan(int v, int* warp_sums, int& total) {  // exclusive, 1024 threads
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -122,14 +73,28 @@ __global__ void __launch_bounds__(1024) paged_plan_kernel(const PagedParams p) {
     }
   }
   __syncthreads();
+  for (int g = threadIdx.x; g < p.groups; g += 1024) {
+    g_min[g] = g_count[g] > 1 ? min(max(p.shared[g], 0), g_min[g]) / kPagedAlign * kPagedAlign : 0;
+    g_count[g] = 0;
+  }
+  __syncthreads();
+  // A shared page that the table does not name: the group goes without, the own units know how to leave such a page out.
+  const int per_group = 1024 >> (32 - __clz(min(max(p.groups, 1), 32) - 1));  // threads: a warp at least
+  for (int g = threadIdx.x / per_group; g < p.groups; g += 1024 / per_group) {
+    const int pages = (g_min[g] + p.c.page_tokens - 1) >> p.c.page_shift;
+    const int32_t* row = p.c.table + (pages ? (int64_t)p.plan.slot[g_first[g]] * p.c.table_stride : 0);
+    bool missing = false;
+    for (int j = threadIdx.x % per_group; j < pages; j += per_group) missing |= (uint32_t)row[j] >= (uint32_t)p.c.pages;
+    if (missing) g_count[g] = 1;
+  }
+  __syncthreads();
   int tiles = 0, units = 0;
   for (int base = 0; base < p.groups; base += 1024) {
     const int g = base + threadIdx.x;
     int own_t = 0, own_u = 0;
     if (g < p.groups) {
       const int lo = max(p.offsets[g], 0), hi = min(p.offsets[g + 1], p.n);
-      int shared = g_count[g] > 1 ? min(max(p.shared[g], 0), g_min[g]) / kPagedAlign * kPagedAlign : 0;
-      if (hi <= lo || bad) shared = 0;
+      const int shared = hi <= lo || bad || g_count[g] ? 0 : g_min[g];
       own_u = hi > lo && !bad ? p.c.heads * ceil_div((hi - lo) * p.R, p.prefix_rows) : 0;
       own_t = own_u * ceil_div(shared, p.prefix_tile);
       p.plan.g_shared[g] = shared;
@@ -159,73 +124,7 @@ __global__ void __launch_bounds__(1024) paged_plan_kernel(const PagedParams p) {
   if (threadIdx.x == 0) p.plan.own_cum[p.n] = tiles;
 }
 
-// ---- the units --------------------------------------------------------------------------------------------------------
-// Where a CTA stands on the line of tiles.
-struct PagedUnit {
-  int index;        // names the slot, together with the CTA
-  int head, row0, rows;   // rows row0 .. row0 + rows of the unit's sequence or group
-  int first_row;    // batch row of the sequence, or the group's first
-  int table_slot;   // whose row of the table names the pages
-  int key_lo, key_hi;     // keys that are this unit's
-  int key_all;      // own units: keys from here on are hidden from some rows
-  int tile, tile_end;     // tiles (64 keys, counted from key 0) that this CTA takes
-};
-
-template <bool kPrefix>
-__device__ __forceinline__ int64_t line_total(const PagedParams& p) {
-  return kPrefix ? (int64_t)p.plan.g_cum[p.groups] : (int64_t)p.plan.own_cum[p.n] * p.c.heads * p.own_blocks;
-}
-
-// the unit at position `at` of the line, cut at `end`
-template <bool kPrefix>
-__device__ __forceinline__ PagedUnit unit_at(const PagedParams& p, int64_t at, int64_t end) {
-  PagedUnit u;
-  if constexpr (kPrefix) {
-    const int g = last_at_or_before(p.plan.g_cum, p.groups, at, 1);
-    u.key_lo = 0, u.key_hi = u.key_all = p.plan.g_shared[g];
-    const int tiles = ceil_div(u.key_hi, p.prefix_tile);
-    const int lo = max(p.offsets[g], 0), hi = min(p.offsets[g + 1], p.n);
-    const int blocks = ceil_div((hi - lo) * p.R, p.prefix_rows);
-    const int64_t off = at - p.plan.g_cum[g];
-    const int which = (int)(off / tiles);
-    u.tile = (int)(off % tiles);
-    u.tile_end = (int)min((int64_t)tiles, u.tile + (end - at));
-    u.index = p.plan.g_unit[g] + which;
-    u.head = which / blocks;
-    u.row0 = (which % blocks) * p.prefix_rows;
-    u.rows = min(p.prefix_rows, (hi - lo) * p.R - u.row0);
-    u.first_row = lo;
-    u.table_slot = p.plan.slot[p.plan.g_first[g]];
-  } else {
-    const int per = p.c.heads * p.own_blocks;
-    const int i = last_at_or_before(p.plan.own_cum, p.n, at, per);
-    u.key_lo = own_first_key(p, i), u.key_hi = p.plan.len[i];
-    u.key_all = max(u.key_lo, u.key_hi - (p.T - 1));
-    const int tiles = own_tiles(u.key_lo, u.key_hi), skip = u.key_lo / kPagedTile;
-    const int64_t off = at - (int64_t)p.plan.own_cum[i] * per;
-    const int which = (int)(off / tiles);
-    const int t = (int)(off % tiles);
-    u.tile = skip + t;
-    u.tile_end = skip + (int)min((int64_t)tiles, t + (end - at));
-    u.index = i * per + which;
-    u.head = which / p.own_blocks;
-    u.row0 = (which % p.own_blocks) * p.own_rows;
-    u.rows = min(p.own_rows, p.R - u.row0);
-    u.first_row = i;
-    u.table_slot = p.plan.slot[i];
-  }
-  return u;
-}
-
-// a row of a unit: batch row, token and query head
-struct PagedRow {
-  int i, t, h;
-};
-__device__ __forceinline__ PagedRow paged_row(const PagedParams& p, const PagedUnit& u, int row) {
-  const int r = u.row0 + row, in_seq = r % p.R;
-  return {u.first_row + r / p.R, in_seq / p.G, u.head * p.G + in_seq % p.G};
-}
-
+// ---- the units over keys of one sequence ----------------------------------------------------------------------------------
 template <int D, int kBytes>
 struct PagedSmem {
   static constexpr int kTileBytes = kPagedTile * D * kBytes;  // K or V of one tile
@@ -242,7 +141,7 @@ struct PagedSmem {
 // kWM warps side by side over rows (16 each), 4 / kWM over the keys of a tile.  Compute type: the cache's own 16-bit type, or
 // f16 for an E4M3 cache (every E4M3 value is exact in f16; bf16 queries are brought into its range by a power of two per
 // row, so they are exact as well down to 2^-38 of the row's largest).
-template <int D, typename CacheT, typename QT, int kWM, bool kPrefix>
+template <int D, typename CacheT, typename QT, int kWM>
 __global__ void __launch_bounds__(kPagedThreads, 2) attn_paged_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_k,
                                                                       const __grid_constant__ CUtensorMap map_v) {
   constexpr bool kE4M3 = std::is_same<CacheT, uint8_t>::value;
@@ -272,7 +171,7 @@ __global__ void __launch_bounds__(kPagedThreads, 2) attn_paged_kernel(const Page
     if (threadIdx.x == 0) p.status[1] = 99u, p.status[0] = 1u;
     return;
   }
-  const int64_t total = line_total<kPrefix>(p), per_cta = piece_tiles(total, kPrefix ? p.prefix_ctas : p.own_ctas);
+  const int64_t total = line_total<false>(p), per_cta = piece_tiles(total, p.own_ctas);
   const int64_t begin = blockIdx.x * per_cta, end = min(total, begin + per_cta);
   if (begin >= end) return;
 
@@ -281,7 +180,7 @@ __global__ void __launch_bounds__(kPagedThreads, 2) attn_paged_kernel(const Page
     int stage = 0, issued = 0;
     uint32_t parity = 1u;
     for (int64_t at = begin; at < end;) {
-      const PagedUnit u = unit_at<kPrefix>(p, at, end);
+      const PagedUnit u = unit_at<false>(p, at, end);
       const int32_t* row = p.c.table + u.table_slot * p.c.table_stride;
       for (int tile = u.tile; tile < u.tile_end; ++tile, ++at) {
         const int token = tile * kPagedTile + lane * box_tokens;
@@ -323,7 +222,7 @@ __global__ void __launch_bounds__(kPagedThreads, 2) attn_paged_kernel(const Page
   int stage = 0;
   uint32_t parity = 0u;
   for (int64_t at = begin; at < end;) {
-    const PagedUnit u = unit_at<kPrefix>(p, at, end);
+    const PagedUnit u = unit_at<false>(p, at, end);
     // query rows quad and quad + 8 of this warp's sixteen, as A fragments; row r of them sees keys below `limit`
     uint32_t q[D / 16][4];
     float scale[2];
@@ -334,7 +233,7 @@ __global__ void __launch_bounds__(kPagedThreads, 2) attn_paged_kernel(const Page
       const bool there = row < u.rows;
       const PagedRow r = paged_row(p, u, there ? row : 0);
       const uint8_t* src = p.q + 2 * (r.i * p.q_sb + r.h * p.q_sh + r.t * p.q_st);
-      limit[half] = kPrefix ? u.key_hi : u.key_hi - (p.T - 1 - r.t);
+      limit[half] = u.key_hi - (p.T - 1 - r.t);
       scale[half] = p.scale_log2 * (p.k_scale ? p.k_scale[u.head] : 1.f);
 #pragma unroll
       for (int k = 0; k < D / 16; ++k) {
@@ -357,19 +256,15 @@ __global__ void __launch_bounds__(kPagedThreads, 2) attn_paged_kernel(const Page
           }
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // the largest becomes 2^14..2^15; a row of zeros, subnormals or infinities stays as it is
-        const int e = (int)(__float_as_uint(top) >> 23);
-        const int shift = (e == 0 || e == 255) ? 0 : 127 + 14 - e;
-        const float a = __uint_as_float((uint32_t)(127 + max(min(shift / 2, 126), -126)) << 23);
-        const float b = __uint_as_float((uint32_t)(127 + max(min(shift - shift / 2, 126), -126)) << 23);
+        const RowShift to_f16 = row_shift(top);
 #pragma unroll
         for (int k = 0; k < D / 16; ++k)
 #pragma unroll
           for (int x = 0; x < 4; x += 2) {
             const float2 f = unpack16(q[k][half + x], TagBf16{});
-            q[k][half + x] = pack16(f.x * a * b, f.y * a * b, TagF16{});
+            q[k][half + x] = pack16(f.x * to_f16.a * to_f16.b, f.y * to_f16.a * to_f16.b, TagF16{});
           }
-        scale[half] = scale[half] / a / b;
+        scale[half] = scale[half] / to_f16.a / to_f16.b;
       }
     }
     float acc[D / 8][4];
@@ -494,7 +389,7 @@ __global__ void __launch_bounds__(kPagedThreads, 2) attn_paged_kernel(const Page
           }
         }
       }
-      if (!kPrefix && key0 + kKeys > u.key_all) {
+      if (key0 + kKeys > u.key_all) {
 #pragma unroll 1
         for (int kk = max(0, u.key_all - key0); kk < min(kKeys, u.key_hi - key0); ++kk) {
           if (!(valid >> (kk >> 4) & 1u)) continue;
@@ -544,7 +439,7 @@ __global__ void __launch_bounds__(kPagedThreads, 2) attn_paged_kernel(const Page
 #pragma unroll
         for (int w = 0; w < kWK; ++w) {
           const float2 x = s.ml[w * kWM + wm][quad + 8 * h];
-          sum += x.x == -INFINITY ? 0.f : x.y * paged_ex2(x.x - top);
+          sum += x.y * (x.x == -INFINITY ? 0.f : paged_ex2(x.x - top));
         }
         m[h] = top, l[h] = sum;
 #pragma unroll
@@ -576,8 +471,8 @@ __global__ void __launch_bounds__(kPagedThreads, 2) attn_paged_kernel(const Page
     }
     if (wk == 0) {
       const int64_t slot = (int64_t)u.index + blockIdx.x;
-      float* out = kPrefix ? p.prefix_acc + slot * p.prefix_rows * D : p.own_acc + slot * p.own_rows * D;
-      float2* ml = kPrefix ? p.prefix_ml + slot * p.prefix_rows : p.own_ml + slot * p.own_rows;
+      float* out = p.own_acc + slot * p.own_rows * D;
+      float2* ml = p.own_ml + slot * p.own_rows;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int row = wm * 16 + h * 8 + quad;
@@ -598,7 +493,8 @@ __global__ void __launch_bounds__(kPagedThreads, 2) attn_paged_kernel(const Page
 }
 
 // ---- join -------------------------------------------------------------------------------------------------------------
-// One warp per output row; a lane holds D / 32 neighbours.
+// One warp per output row.  The pieces' statistics come to the lanes at once, so that what is left to wait for is one
+// round of loads: a lane holds D / 32 neighbours of eight pieces at a time.
 template <int D, typename QT>
 __global__ void __launch_bounds__(256) paged_join_kernel(const PagedParams p) {
   constexpr int kPer = D / 32;
@@ -614,35 +510,70 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedParams p) {
   float acc[kPer], m = -INFINITY, l = 0.f;
 #pragma unroll
   for (int e = 0; e < kPer; ++e) acc[e] = 0.f;
-  auto add = [&](const float* rows, const float2* ml, int64_t row) {
-    const float2 x = ml[row];
-    if (x.x == -INFINITY) return;
-    const float next = fmaxf(m, x.x), f = m == -INFINITY ? 0.f : paged_ex2(m - next), y = paged_ex2(x.x - next);
-    m = next;
-    l = l * f + x.y * y;
-    if constexpr (kPer == 4) {
-      const float4 v = reinterpret_cast<const float4*>(rows + row * D)[lane];
-      acc[0] = acc[0] * f + v.x * y, acc[1] = acc[1] * f + v.y * y, acc[2] = acc[2] * f + v.z * y, acc[3] = acc[3] * f + v.w * y;
-    } else {
-      const float2 v = reinterpret_cast<const float2*>(rows + row * D)[lane];
-      acc[0] = acc[0] * f + v.x * y, acc[1] = acc[1] * f + v.y * y;
-    }
-  };
   if (len - (p.T - 1 - t) > 0) {
     const int first = own_first_key(p, i), tiles = own_tiles(first, len);
+    // rows of the row's pieces: piece k of the prefix, then of the own keys, `rows` apart
+    int n_prefix = 0, prefix_row = 0;
+    int64_t prefix_slot = 0;
     if (first > 0) {
       const int64_t per_cta = piece_tiles(line_total<true>(p), p.prefix_ctas);
       const int lo = max(p.offsets[g], 0), hi = min(p.offsets[g + 1], p.n);
-      const int row = (i - lo) * p.R + r, block = row / p.prefix_rows, blocks = ceil_div((hi - lo) * p.R, p.prefix_rows);
-      const int which = head * blocks + block, ptiles = ceil_div(first, p.prefix_tile);
-      const int64_t from = p.plan.g_cum[g] + (int64_t)which * ptiles;
-      for (int64_t cta = from / per_cta; cta <= (from + ptiles - 1) / per_cta; ++cta)
-        add(p.prefix_acc, p.prefix_ml, (p.plan.g_unit[g] + which + cta) * p.prefix_rows + row % p.prefix_rows);
+      const int row = (i - lo) * p.R + r, blocks = ceil_div((hi - lo) * p.R, p.prefix_rows);
+      const int which = head * blocks + row / p.prefix_rows, ptiles = ceil_div(first, p.prefix_tile);
+      const int64_t from = p.plan.g_cum[g] + (int64_t)which * ptiles, cta = from / per_cta;
+      n_prefix = (int)((from + ptiles - 1) / per_cta - cta) + 1;
+      prefix_slot = p.plan.g_unit[g] + which + cta;
+      prefix_row = row % p.prefix_rows;
     }
     const int per = p.c.heads * p.own_blocks, which = head * p.own_blocks + r / p.own_rows;
     const int64_t per_cta = piece_tiles(line_total<false>(p), p.own_ctas), from = (int64_t)p.plan.own_cum[i] * per + (int64_t)which * tiles;
-    for (int64_t cta = from / per_cta; cta <= (from + tiles - 1) / per_cta; ++cta)
-      add(p.own_acc, p.own_ml, ((int64_t)i * per + which + cta) * p.own_rows + r % p.own_rows);
+    const int64_t cta = from / per_cta, own_slot = (int64_t)i * per + which + cta;
+    const int n_own = (int)((from + tiles - 1) / per_cta - cta) + 1, own_row = r % p.own_rows;
+    for (int base = 0; base < n_prefix + n_own; base += 32) {
+      const int k = base + lane;
+      const bool is_prefix = k < n_prefix;
+      const int64_t row = is_prefix ? (prefix_slot + k) * p.prefix_rows + prefix_row : (own_slot + (k - n_prefix)) * p.own_rows + own_row;
+      float2 x = make_float2(-INFINITY, 0.f);
+      if (k < n_prefix + n_own) x = is_prefix ? p.prefix_ml[row] : p.own_ml[row];
+      float top = x.x;
+#pragma unroll
+      for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const float next = fmaxf(m, top), f = m == -INFINITY ? 0.f : paged_ex2(m - next);
+      const float y = x.x == -INFINITY ? 0.f : paged_ex2(x.x - next);
+      float sum = x.y * y;
+#pragma unroll
+      for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      m = next, l = l * f + sum;
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) acc[e] *= f;
+      const float* at = (is_prefix ? p.prefix_acc : p.own_acc) + row * D;
+      const int count = min(32, n_prefix + n_own - base);
+      for (int k0 = 0; k0 < count; k0 += 8) {
+        float v[8][kPer], weight[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          weight[j] = __shfl_sync(0xffffffffu, y, (k0 + j) & 31);
+          const float* from_row = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, (unsigned long long)at, (k0 + j) & 31));
+#pragma unroll
+          for (int e = 0; e < kPer; ++e) v[j][e] = 0.f;
+          if (k0 + j < count) {
+            if constexpr (kPer == 4) {
+              const float4 q = __ldcg(reinterpret_cast<const float4*>(from_row) + lane);
+              v[j][0] = q.x, v[j][1] = q.y, v[j][2] = q.z, v[j][3] = q.w;
+            } else {
+              const float2 q = __ldcg(reinterpret_cast<const float2*>(from_row) + lane);
+              v[j][0] = q.x, v[j][1] = q.y;
+            }
+          } else {
+            weight[j] = 0.f;
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+          for (int e = 0; e < kPer; ++e) acc[e] = fmaf(v[j][e], weight[j], acc[e]);
+      }
+    }
   }
   const float inv = l == 0.f ? 0.f : (p.v_scale ? p.v_scale[head] : 1.f) / l;  // a row that sees nothing: zeros, -inf
   uint8_t* out = p.o + 2 * (i * p.o_sb + h * p.o_sh + t * p.o_st + lane * kPer);
@@ -656,9 +587,9 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedParams p) {
 // ---- host -------------------------------------------------------------------------------------------------------------
 namespace fa4b {
 
-template <int D, typename CacheT, typename QT, int kWM, bool kPrefix>
+template <int D, typename CacheT, typename QT, int kWM>
 static int launch_units(const PagedParams& p, const CUtensorMap& mk, const CUtensorMap& mv, int ctas, cudaStream_t st) {
-  auto kernel = attn_paged_kernel<D, CacheT, QT, kWM, kPrefix>;
+  auto kernel = attn_paged_kernel<D, CacheT, QT, kWM>;
   constexpr int smem = (int)sizeof(PagedSmem<D, std::is_same<CacheT, uint8_t>::value ? 1 : 2>);
   static_assert(smem <= 113 * 1024, "two CTAs per SM");
   FA4B_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
@@ -670,10 +601,10 @@ template <int D, typename CacheT, typename QT>
 static int launch_paged(const PagedParams& p, const CUtensorMap& mk, const CUtensorMap& mv, cudaStream_t st) {
   FA4B_CUDA(launch_overlapped(paged_plan_kernel, 1, 1024, 12 * (size_t)p.groups, st, p));
   if (p.groups > 0)
-    if (int s = launch_units<D, CacheT, QT, 4, true>(p, mk, mv, p.prefix_ctas, st)) return s;
-  const int s = p.own_rows == 16   ? launch_units<D, CacheT, QT, 1, false>(p, mk, mv, p.own_ctas, st)
-                : p.own_rows == 32 ? launch_units<D, CacheT, QT, 2, false>(p, mk, mv, p.own_ctas, st)
-                                   : launch_units<D, CacheT, QT, 4, false>(p, mk, mv, p.own_ctas, st);
+    if (int s = launch_prefix(p, D, std::is_same<CacheT, uint8_t>::value, std::is_same<QT, TagF16>::value, mk, mv, st)) return s;
+  const int s = p.own_rows == 16   ? launch_units<D, CacheT, QT, 1>(p, mk, mv, p.own_ctas, st)
+                : p.own_rows == 32 ? launch_units<D, CacheT, QT, 2>(p, mk, mv, p.own_ctas, st)
+                                   : launch_units<D, CacheT, QT, 4>(p, mk, mv, p.own_ctas, st);
   if (s) return s;
   const int64_t rows = (int64_t)p.n * p.Hq * p.T;
   FA4B_CUDA(launch_overlapped(paged_join_kernel<D, QT>, (unsigned)((rows + 7) / 8), 256, 0, st, p));
@@ -711,7 +642,10 @@ static int paged_params(const fa4b_kv_cache* c, const fa4b_attn_paged_args* a, P
   p.own_rows = p.R <= 16 ? 16 : p.R <= 32 ? 32 : 64;
   p.own_blocks = (p.R + p.own_rows - 1) / p.own_rows;
   p.own_ctas = 2 * n_sm;
-  p.prefix_rows = 64, p.prefix_tile = 64, p.prefix_ctas = 2 * n_sm;
+  // two blocks of 128 rows over the same keys where the groups have the rows for it: each tile then comes from memory half
+  // as often; otherwise the two halves of a CTA take the keys in turn
+  p.prefix_rows = p.groups > 0 && (int64_t)p.n * p.R > 128ll * p.groups ? 256 : 128;
+  p.prefix_tile = 128, p.prefix_ctas = n_sm;
   const int64_t row_tiles = ((int64_t)c->table_width * c->page_tokens + kPagedTile - 1) / kPagedTile + 1;
   const int64_t prefix_units = p.groups ? (int64_t)c->Hkv * (((int64_t)p.n * p.R + p.prefix_rows - 1) / p.prefix_rows + p.groups) : 0;
   const int64_t own_slots = (int64_t)p.n * c->Hkv * p.own_blocks + p.own_ctas, prefix_slots = p.groups ? prefix_units + p.prefix_ctas : 0;
