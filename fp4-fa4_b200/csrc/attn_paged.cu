@@ -2,17 +2,13 @@
 // a group of sequences shares read once for all of them.
 //
 // Bound by memory: a key and a value are used by the few query rows of one sequence (own units), so the kernel is a
-// stream of pages through shared memory: one warp asks for tiles of 64 keys by TMA several tiles ahead, four warps
-// consume them.  Scores and values go through mma.sync m16n8k16: with 4 to 16 query rows a tcgen05 tile of 128 rows would
+// stream of pages through shared memory: tiles are asked for by TMA several tiles ahead.  Scores and values go through mma.sync m16n8k16: with 4 to 16 query rows a tcgen05 tile of 128 rows would
 // be empty for the most part, and the 16-row form already computes a tile in a quarter of the time its bytes take.
 #include "attn_paged.cuh"
 
 #include <type_traits>
 
 namespace fa4b {
-
-constexpr int kPagedThreads = 160;
-constexpr int kPagedStageBytes = 96 * 1024;  // shared memory for tiles in flight; two CTAs per SM
 
 // ---- plan -------------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ int paged_scan(int v, int* warp_sums, int& total) {  // exclusive, 1024 threads
@@ -40,201 +36,171 @@ __device__ __forceinline__ int paged_scan(int v, int* warp_sums, int& total) {  
 // One CTA: lengths, groups, and the lines of tiles.  The shared part of a group is what the caller says, cut to what every
 // query row of every member sees (so that no row of a prefix unit needs a mask) and to whole 16 keys; a group of one
 // member has none.
+// The last i in [0, n) whose part of the line begins at or before x; cum counts one `factor`-th of it.
+__device__ __forceinline__ int paged_find(const int* cum, int n, int64_t x, int64_t factor) {
+  int lo = 0, hi = n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (cum[mid] * factor <= x) lo = mid; else hi = mid - 1;
+  }
+  return lo;
+}
+
+// dynamic shared memory of the plan, in words
+__host__ __device__ inline size_t paged_plan_words(int n, int groups) { return 4 * (size_t)n + 6 * (size_t)groups + 1; }
+
 __global__ void __launch_bounds__(1024) paged_plan_kernel(const PagedParams p) {
   __shared__ int warp_sums[32];
   extern __shared__ int dyn[];
-  int* g_min = dyn;              // [groups] shortest member's length - T
-  int* g_first = dyn + p.groups;
-  int* g_count = dyn + 2 * p.groups;
+  int* own_cum = dyn;                  // [n]
+  int* s_slot = own_cum + p.n;         // [n]
+  int* s_len = s_slot + p.n;           // [n]
+  int* s_group = s_len + p.n;          // [n] -1: none
+  int* offsets = s_group + p.n;        // [groups + 1]
+  int* g_shared = offsets + p.groups + 1;  // [groups] shortest member's length - T, then the shared keys
+  int* g_first = g_shared + p.groups;  // [groups] a member with keys
+  int* g_count = g_first + p.groups;   // [groups] members with keys, then whether a shared page is missing
+  int* g_cum = g_count + p.groups;     // [groups]
+  int* g_unit = g_cum + p.groups;      // [groups]
   pdl_trigger();
-  for (int g = threadIdx.x; g < p.groups; g += 1024) g_min[g] = INT_MAX, g_first[g] = INT_MAX, g_count[g] = 0;
   pdl_wait();
-  bool bad = false;  // groups have to lie behind one another: the slots of their units are counted on it
-  for (int g = threadIdx.x; g < p.groups; g += 1024) bad |= p.offsets[g] < 0 || p.offsets[g + 1] < p.offsets[g] || p.offsets[g + 1] > p.n;
-  bad = __syncthreads_or(bad);
-  if (bad && threadIdx.x == 0 && atomicCAS(p.status, 0u, 2u) == 0u) p.status[1] = (uint32_t)p.groups;
+  for (int g = threadIdx.x; g < p.groups; g += 1024) offsets[g] = p.offsets[g], g_shared[g] = INT_MAX, g_first[g] = INT_MAX, g_count[g] = 0;
+  if (threadIdx.x == 0 && p.groups > 0) offsets[p.groups] = p.offsets[p.groups];
   for (int i = threadIdx.x; i < p.n; i += 1024) {
     const int slot = p.seqs ? p.seqs[i] : i;
-    int len = 0, g = p.groups > 0 || bad ? -1 : 0;
+    int len = 0;
     if (slot >= 0 && slot < p.c.max_seqs) len = (int)min((int64_t)max(p.c.lens[slot], 0), (int64_t)p.c.width << p.c.page_shift);
-    if (p.groups > 0 && !bad) {
-      int lo = 0, hi = p.groups;  // the last group that begins at or before i
-      while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (p.offsets[mid] <= i) lo = mid; else hi = mid - 1;
+    s_slot[i] = slot, s_len[i] = len, s_group[i] = p.groups > 0 ? -1 : 0;
+  }
+  __syncthreads();
+  int prefix_total = 0;
+  if (p.groups > 0) {
+    bool bad = false;  // groups have to lie behind one another: the slots of their units are counted on it
+    for (int g = threadIdx.x; g < p.groups; g += 1024) bad |= offsets[g] < 0 || offsets[g + 1] < offsets[g] || offsets[g + 1] > p.n;
+    bad = __syncthreads_or(bad);
+    if (bad && threadIdx.x == 0 && atomicCAS(p.status, 0u, 2u) == 0u) p.status[1] = (uint32_t)p.groups;
+    if (!bad)
+      for (int i = threadIdx.x; i < p.n; i += 1024) {
+        int lo = 0, hi = p.groups - 1;  // the last group that begins at or before i
+        while (lo < hi) {
+          const int mid = (lo + hi + 1) >> 1;
+          if (offsets[mid] <= i) lo = mid; else hi = mid - 1;
+        }
+        if (i < offsets[lo] || i >= offsets[lo + 1]) continue;
+        s_group[i] = lo;
+        if (s_len[i] > 0) {
+          atomicMin(g_shared + lo, max(s_len[i] - p.T, 0));
+          atomicMin(g_first + lo, i);
+          atomicAdd(g_count + lo, 1);
+        }
       }
-      if (lo < p.groups && p.offsets[lo] <= i && i < p.offsets[lo + 1]) g = lo;
+    __syncthreads();
+    for (int g = threadIdx.x; g < p.groups; g += 1024) {
+      g_shared[g] = g_count[g] > 1 ? min(max(p.shared[g], 0), g_shared[g]) / kPagedAlign * kPagedAlign : 0;
+      g_count[g] = 0;
     }
-    p.plan.slot[i] = slot, p.plan.len[i] = len, p.plan.group[i] = g;
-    if (p.groups > 0 && g >= 0 && len > 0) {
-      atomicMin(g_min + g, max(len - p.T, 0));
-      atomicMin(g_first + g, i);
-      atomicAdd(g_count + g, 1);
+    __syncthreads();
+    // A shared page that the table does not name: the group goes without, the own units know how to leave such a page out.
+    const int per_group = 1024 >> (32 - __clz(min(p.groups, 32) - 1));  // threads: a warp at least
+    for (int g = threadIdx.x / per_group; g < p.groups; g += 1024 / per_group) {
+      const int pages = (g_shared[g] + p.c.page_tokens - 1) >> p.c.page_shift;
+      const int32_t* row = p.c.table + (pages ? (int64_t)s_slot[g_first[g]] * p.c.table_stride : 0);
+      bool missing = false;
+#pragma unroll 4
+      for (int j = threadIdx.x % per_group; j < pages; j += per_group) missing |= (uint32_t)row[j] >= (uint32_t)p.c.pages;
+      if (missing) g_count[g] = 1;
     }
-  }
-  __syncthreads();
-  for (int g = threadIdx.x; g < p.groups; g += 1024) {
-    g_min[g] = g_count[g] > 1 ? min(max(p.shared[g], 0), g_min[g]) / kPagedAlign * kPagedAlign : 0;
-    g_count[g] = 0;
-  }
-  __syncthreads();
-  // A shared page that the table does not name: the group goes without, the own units know how to leave such a page out.
-  const int per_group = 1024 >> (32 - __clz(min(max(p.groups, 1), 32) - 1));  // threads: a warp at least
-  for (int g = threadIdx.x / per_group; g < p.groups; g += 1024 / per_group) {
-    const int pages = (g_min[g] + p.c.page_tokens - 1) >> p.c.page_shift;
-    const int32_t* row = p.c.table + (pages ? (int64_t)p.plan.slot[g_first[g]] * p.c.table_stride : 0);
-    bool missing = false;
-    for (int j = threadIdx.x % per_group; j < pages; j += per_group) missing |= (uint32_t)row[j] >= (uint32_t)p.c.pages;
-    if (missing) g_count[g] = 1;
-  }
-  __syncthreads();
-  int tiles = 0, units = 0;
-  for (int base = 0; base < p.groups; base += 1024) {
-    const int g = base + threadIdx.x;
-    int own_t = 0, own_u = 0;
-    if (g < p.groups) {
-      const int lo = max(p.offsets[g], 0), hi = min(p.offsets[g + 1], p.n);
-      const int shared = hi <= lo || bad || g_count[g] ? 0 : g_min[g];
-      own_u = hi > lo && !bad ? p.c.heads * ceil_div((hi - lo) * p.R, p.prefix_rows) : 0;
-      own_t = own_u * ceil_div(shared, p.prefix_tile);
-      p.plan.g_shared[g] = shared;
-      p.plan.g_first[g] = shared ? g_first[g] : 0;
-      g_min[g] = shared;
+    __syncthreads();
+    int units = 0;
+    for (int base = 0; base < p.groups; base += 1024) {
+      const int g = base + threadIdx.x;
+      int length = 0, own_u = 0;
+      PagedGroup r{};
+      if (g < p.groups) {
+        r.shared = g_count[g] ? 0 : g_shared[g];
+        g_shared[g] = r.shared;
+        if (r.shared > 0) {
+          r.row = offsets[g], r.rows = (offsets[g + 1] - r.row) * p.R;
+          r.slot = s_slot[g_first[g]];
+          r.blocks = ceil_div(r.rows, p.prefix_rows);
+          own_u = p.c.heads * r.blocks;
+          length = own_u * (ceil_div(r.shared, p.prefix_tile) + p.prefix_extra);
+        }
+      }
+      int t_total, u_total;
+      r.cum = prefix_total + paged_scan(length, warp_sums, t_total), r.unit = units + paged_scan(own_u, warp_sums, u_total);
+      if (g < p.groups) p.group[g] = r, g_cum[g] = r.cum, g_unit[g] = r.unit;
+      prefix_total += t_total, units += u_total;
     }
-    int t_total, u_total;
-    const int t_before = paged_scan(own_t, warp_sums, t_total), u_before = paged_scan(own_u, warp_sums, u_total);
-    if (g < p.groups) p.plan.g_cum[g] = tiles + t_before, p.plan.g_unit[g] = units + u_before;
-    tiles += t_total, units += u_total;
+    __syncthreads();
   }
-  if (threadIdx.x == 0) p.plan.g_cum[p.groups] = tiles, p.plan.g_unit[p.groups] = units;
-  __syncthreads();
-  tiles = 0;
+  int own_total = 0;
   for (int base = 0; base < p.n; base += 1024) {
     const int i = base + threadIdx.x;
-    int t = 0;
+    int length = 0;
+    PagedSeq s{};
     if (i < p.n) {
-      const int g = p.plan.group[i];
-      if (g >= 0) t = own_tiles(p.groups > 0 ? g_min[g] : 0, p.plan.len[i]);
-    }
-    int total;
-    const int before = paged_scan(t, warp_sums, total);
-    if (i < p.n) p.plan.own_cum[i] = tiles + before;
-    tiles += total;
-  }
-  if (threadIdx.x == 0) p.plan.own_cum[p.n] = tiles;
-}
-
-// ---- the units over keys of one sequence ----------------------------------------------------------------------------------
-template <int D, int kBytes>
-struct PagedSmem {
-  static constexpr int kTileBytes = kPagedTile * D * kBytes;  // K or V of one tile
-  static constexpr int kStages = kPagedStageBytes / (2 * kTileBytes) > 8 ? 8 : kPagedStageBytes / (2 * kTileBytes);
-  alignas(1024) uint8_t k[kStages][kTileBytes];
-  uint8_t v[kStages][kTileBytes];
-  float merge[2][16][D];
-  float2 ml[4][16];
-  uint64_t full[kStages], empty[kStages];
-  uint32_t valid[kStages];  // a bit per 16 keys: the table names a page of the pool
-  volatile uint32_t abort_flag;
-};
-
-// kWM warps side by side over rows (16 each), 4 / kWM over the keys of a tile.  Compute type: the cache's own 16-bit type, or
-// f16 for an E4M3 cache (every E4M3 value is exact in f16; bf16 queries are brought into its range by a power of two per
-// row, so they are exact as well down to 2^-38 of the row's largest).
-template <int D, typename CacheT, typename QT, int kWM>
-__global__ void __launch_bounds__(kPagedThreads, 2) attn_paged_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_k,
-                                                                      const __grid_constant__ CUtensorMap map_v) {
-  constexpr bool kE4M3 = std::is_same<CacheT, uint8_t>::value;
-  constexpr int kBytes = kE4M3 ? 1 : 2;
-  constexpr int kRowBytes = D * kBytes, kBoxBytes = kRowBytes < 128 ? kRowBytes : 128;  // a box: 64 or 128 bytes of a row
-  constexpr int kBoxes = kRowBytes / kBoxBytes;
-  constexpr int kWK = 4 / kWM, kKeys = kPagedTile / kWK;  // keys of a tile that one warp takes
-  using Smem = PagedSmem<D, kBytes>;
-  constexpr int kStages = Smem::kStages;
-  using Mma = typename std::conditional<kE4M3, TagF16, QT>::type;
-  extern __shared__ __align__(1024) uint8_t raw[];
-  Smem& s = *reinterpret_cast<Smem*>(raw);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const bool aligned = (smem_u32(raw) & 1023u) == 0u;  // the swizzle of the tiles goes by the address
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < kStages; ++i) mbar_init(&s.full[i], 1), mbar_init(&s.empty[i], 4);
-    s.abort_flag = 0u;
-    fence_barrier_init();
-    fence_async_smem();
-    tma_prefetch_desc(&map_k);
-    tma_prefetch_desc(&map_v);
-  }
-  __syncthreads();
-  pdl_trigger();
-  pdl_wait();
-  if (!aligned) {
-    if (threadIdx.x == 0) p.status[1] = 99u, p.status[0] = 1u;
-    return;
-  }
-  const int64_t total = line_total<false>(p), per_cta = piece_tiles(total, p.own_ctas);
-  const int64_t begin = blockIdx.x * per_cta, end = min(total, begin + per_cta);
-  if (begin >= end) return;
-
-  if (warp == 4) {  // ---- producer: lane b of a tile's boxes asks for its own part of the pages
-    const int box_tokens = min(p.c.page_tokens, kPagedTile), boxes = kPagedTile / box_tokens;
-    int stage = 0, issued = 0;
-    uint32_t parity = 1u;
-    for (int64_t at = begin; at < end;) {
-      const PagedUnit u = unit_at<false>(p, at, end);
-      const int32_t* row = p.c.table + u.table_slot * p.c.table_stride;
-      for (int tile = u.tile; tile < u.tile_end; ++tile, ++at) {
-        const int token = tile * kPagedTile + lane * box_tokens;
-        const bool wanted = lane < boxes && token < u.key_hi && token + box_tokens > u.key_lo;
-        int page = -1;
-        if (wanted) page = row[token >> p.c.page_shift];
-        const bool load = wanted && page >= 0 && page < p.c.pages;
-        const uint32_t loads = __ballot_sync(0xffffffffu, load);
-        const bool go = mbar_wait_warp(&s.empty[stage], parity, &s.abort_flag, p.status, 1);
-        if (lane == 0) {
-          uint32_t valid = 0u;  // per 16 keys
-          for (int b = 0; b < boxes; ++b)
-            if (loads >> b & 1u) valid |= ((1u << (box_tokens / 16)) - 1u) << (b * (box_tokens / 16));
-          s.valid[stage] = valid;
-          mbar_expect_tx(&s.full[stage], go ? __popc(loads) * box_tokens * kRowBytes * 2 : 0);
-        }
-        __syncwarp();
-        if (go && load) {
-          const uint32_t in_page = (uint32_t)token & (uint32_t)(p.c.page_tokens - 1);
-#pragma unroll
-          for (int x = 0; x < kBoxes; ++x) {
-            const uint32_t off = x * (kPagedTile * kBoxBytes) + lane * box_tokens * kBoxBytes;
-            tma_load_5d(smem_u32(s.k[stage]) + off, &map_k, x * (kBoxBytes / kBytes), (int)in_page, u.head, page, p.layer, &s.full[stage]);
-            tma_load_5d(smem_u32(s.v[stage]) + off, &map_v, x * (kBoxBytes / kBytes), (int)in_page, u.head, page, p.layer, &s.full[stage]);
-          }
-        }
-        ++issued;
-        if (++stage == kStages) stage = 0, parity ^= 1u;
+      const int g = s_group[i];
+      s.slot = s_slot[i], s.len = s_len[i], s.left_alone = g < 0;
+      if (g >= 0) {
+        if (p.groups > 0 && g_shared[g] > 0 && s.len > 0)
+          s.first = g_shared[g], s.g_row = offsets[g], s.g_blocks = ceil_div((offsets[g + 1] - offsets[g]) * p.R, p.prefix_rows), s.g_unit = g_unit[g], s.g_cum = g_cum[g];
+        length = own_tiles(p, s.first, s.len);
+        length += length ? p.own_extra : 0;
       }
     }
-    if (s.abort_flag) {  // copies in flight land before the CTA leaves
-      for (int k = max(0, issued - kStages); k < issued; ++k) mbar_wait_teardown(&s.full[k % kStages], (uint32_t)(k / kStages) & 1u);
-    }
-    return;
+    int total;
+    s.cum = own_total + paged_scan(length, warp_sums, total);
+    if (i < p.n) p.seq[i] = s, own_cum[i] = s.cum;
+    own_total += total;
   }
+  __syncthreads();
+  const int per = p.c.heads * p.own_blocks;
+  const int64_t line = (int64_t)own_total * per;
+  const int64_t own_per = max((line + p.own_workers - 1) / p.own_workers, (int64_t)p.own_min);
+  const int64_t prefix_per = max((prefix_total + p.prefix_workers - 1) / p.prefix_workers, 1);
+  if (threadIdx.x == 0) *p.head = {line, own_per, prefix_total, prefix_per};
+  for (int w = threadIdx.x; w < p.own_workers; w += 1024) {
+    const int64_t at = w * own_per;
+    if (at >= line) break;
+    const int i = paged_find(own_cum, p.n, at, per);
+    const int length = (i + 1 < p.n ? own_cum[i + 1] : own_total) - own_cum[i];
+    const int64_t off = at - (int64_t)own_cum[i] * per;
+    const int which = (int)(off / length);
+    p.own_start[w] = {i, which, (int)(off - (int64_t)which * length), 0};
+  }
+  if (prefix_total == 0) return;
+  for (int w = threadIdx.x; w < p.prefix_workers; w += 1024) {
+    const int64_t at = w * prefix_per;
+    if (at >= prefix_total) break;
+    const int g = paged_find(g_cum, p.groups, at, 1);
+    const int length = ceil_div(g_shared[g], p.prefix_tile) + p.prefix_extra, off = (int)at - g_cum[g];
+    p.prefix_start[w] = {g, off / length, off % length, 0};
+  }
+}
 
-  // ---- consumers
-  const int wm = warp % kWM, wk = warp / kWM, quad = lane >> 2, c4 = lane & 3;
-  int stage = 0;
-  uint32_t parity = 0u;
-  for (int64_t at = begin; at < end;) {
-    const PagedUnit u = unit_at<false>(p, at, end);
-    // query rows quad and quad + 8 of this warp's sixteen, as A fragments; row r of them sees keys below `limit`
-    uint32_t q[D / 16][4];
-    float scale[2];
-    int limit[2];
+// ---- the units over keys of one sequence ------------------------------------------------------------------------------
+// Sixteen query rows of a unit as one warp holds them: rows quad and quad + 8 of the fragments, accumulators over D, running
+// maximum and sum.  Compute type: the cache's own 16-bit type, or f16 for an E4M3 cache (every E4M3 value is exact in f16;
+// bf16 queries are brought into its range by a power of two per row, exact down to 2^-38 of the row's largest).
+template <int D, bool kE4M3, typename QT>
+struct PagedRows {
+  using Mma = typename std::conditional<kE4M3, TagF16, QT>::type;
+  static constexpr int kBoxBytes = D * (kE4M3 ? 1 : 2) < 128 ? D : 128;  // of a row, side by side in one box of shared memory
+  uint32_t q[D / 16][4];
+  float acc[D / 8][4], scale[2], m[2], l[2];
+  int limit[2];  // the row sees keys below
+
+  __device__ __forceinline__ void start(const PagedParams& p, const PagedUnit& u, int row0) {
+    const int lane = threadIdx.x & 31, quad = lane >> 2, c4 = lane & 3;
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-      const int row = wm * 16 + half * 8 + quad;
+      const int row = row0 + half * 8 + quad;
       const bool there = row < u.rows;
       const PagedRow r = paged_row(p, u, there ? row : 0);
       const uint8_t* src = p.q + 2 * (r.i * p.q_sb + r.h * p.q_sh + r.t * p.q_st);
       limit[half] = u.key_hi - (p.T - 1 - r.t);
-      scale[half] = p.scale_log2 * (p.k_scale ? p.k_scale[u.head] : 1.f);
+      scale[half] = p.scale_log2 * (kE4M3 ? p.k_scale[u.head] : 1.f);
 #pragma unroll
       for (int k = 0; k < D / 16; ++k) {
         if constexpr (kE4M3) {  // four neighbours: a thread's K codes are four neighbours too (see the scores below)
@@ -266,269 +232,504 @@ __global__ void __launch_bounds__(kPagedThreads, 2) attn_paged_kernel(const Page
           }
         scale[half] = scale[half] / to_f16.a / to_f16.b;
       }
+      m[half] = -INFINITY, l[half] = 0.f;
     }
-    float acc[D / 8][4];
 #pragma unroll
     for (int j = 0; j < D / 8; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  }
 
-    for (int tile = u.tile; tile < u.tile_end; ++tile, ++at) {
-      mbar_wait_warp(&s.full[stage], parity, &s.abort_flag, p.status, 2);
-      const uint32_t kbase = smem_u32(s.k[stage]), vbase = smem_u32(s.v[stage]);
-      const int key0 = tile * kPagedTile + wk * kKeys;  // this warp's keys: key0 .. key0 + kKeys
-      const uint32_t valid = s.valid[stage] >> (wk * kKeys / 16);
-      constexpr uint32_t kAllValid = (1u << (kKeys / 16)) - 1u;
-      // not every key of these is there for every row
-      const bool special = key0 < u.key_lo || key0 + kKeys > u.key_all || (valid & kAllValid) != kAllValid;
-      float sc[kKeys / 8][4];
+  // kKeys keys from key0 on, at row `at` of a tile of kTileRows keys in shared memory; `valid`: a bit per 16 of them, the
+  // table names a page of the pool
+  template <int kKeys, int kTileRows>
+  __device__ __forceinline__ void tile(const PagedUnit& u, const uint8_t* ktile, const uint8_t* vtile, int at, int key0, uint32_t valid) {
+    const int lane = threadIdx.x & 31, c4 = lane & 3;
+    const uint32_t kbase = smem_u32(ktile), vbase = smem_u32(vtile);
+    constexpr uint32_t kAllValid = (1u << (kKeys / 16)) - 1u;
+    // not every key of these is there for every row
+    const bool special = key0 < u.key_lo || key0 + kKeys > u.key_all || (valid & kAllValid) != kAllValid;
+    float sc[kKeys / 8][4];
 #pragma unroll
-      for (int j = 0; j < kKeys / 8; ++j) {
-        sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.f;
-        const uint32_t row = wk * kKeys + j * 8 + (lane & 7);
-        if constexpr (kE4M3) {
-          // a matrix of ldmatrix is 8 keys x 16 codes, four neighbours to a thread: they stand in for k = 2c, 2c+1, 2c+8, 2c+9 of
-          // the fragment, and the query fragments above hold the same four neighbours there
+    for (int j = 0; j < kKeys / 8; ++j) {
+      sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.f;
+      const uint32_t row = at + j * 8 + (lane & 7);
+      if constexpr (kE4M3) {
+        // a matrix of ldmatrix is 8 keys x 16 codes, four neighbours to a thread: they stand in for k = 2c, 2c+1, 2c+8, 2c+9 of
+        // the fragment, and the query fragments hold the same four neighbours there
 #pragma unroll
-          for (int x = 0; x < D / 64; ++x) {
-            uint32_t b[4];
-            ldmatrix4(b, kbase + swizzled_offset(row, x * 64 + (lane >> 3) * 16, kBoxBytes));
+        for (int x = 0; x < D / 64; ++x) {
+          uint32_t b[4];
+          ldmatrix4(b, kbase + swizzled_offset(row, x * 64 + (lane >> 3) * 16, kBoxBytes));
 #pragma unroll
-            for (int e = 0; e < 4; ++e) mma16816(sc[j], q[x * 4 + e], e4m3x2_to_f16x2(b[e]), e4m3x2_to_f16x2(b[e] >> 16), Mma{});
-          }
-        } else {
+          for (int e = 0; e < 4; ++e) mma16816(sc[j], q[x * 4 + e], e4m3x2_to_f16x2(b[e]), e4m3x2_to_f16x2(b[e] >> 16), Mma{});
+        }
+      } else {
 #pragma unroll
-          for (int x = 0; x < D / 32; ++x) {
-            uint32_t b[4];
-            const uint32_t col = x * 64 + (lane >> 3) * 16;  // bytes of the row
-            ldmatrix4(b, kbase + (col >> 7) * (kPagedTile * 128) + swizzled_offset(row, col & 127u, 128));
-            mma16816(sc[j], q[2 * x], b[0], b[1], Mma{});
-            mma16816(sc[j], q[2 * x + 1], b[2], b[3], Mma{});
-          }
+        for (int x = 0; x < D / 32; ++x) {
+          uint32_t b[4];
+          const uint32_t col = x * 64 + (lane >> 3) * 16;  // bytes of the row
+          ldmatrix4(b, kbase + (col >> 7) * (kTileRows * 128) + swizzled_offset(row, col & 127u, 128));
+          mma16816(sc[j], q[2 * x], b[0], b[1], Mma{});
+          mma16816(sc[j], q[2 * x + 1], b[2], b[3], Mma{});
         }
       }
-      float top[2] = {-INFINITY, -INFINITY};
+    }
+    float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-      for (int j = 0; j < kKeys / 8; ++j)
+    for (int j = 0; j < kKeys / 8; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float x = sc[j][e] * scale[e >> 1];
-          if (special) {
-            const int key = key0 + j * 8 + c4 * 2 + (e & 1);
-            if (key < u.key_lo || key >= limit[e >> 1] || !(valid >> (j >> 1) & 1u)) x = -INFINITY;
-          }
-          sc[j][e] = x;
-          top[e >> 1] = fmaxf(top[e >> 1], x);
+      for (int e = 0; e < 4; ++e) {
+        float x = sc[j][e] * scale[e >> 1];
+        if (special) {
+          const int key = key0 + j * 8 + c4 * 2 + (e & 1);
+          if (key < u.key_lo || key >= limit[e >> 1] || !(valid >> (j >> 1) & 1u)) x = -INFINITY;
         }
+        sc[j][e] = x;
+        top[e >> 1] = fmaxf(top[e >> 1], x);
+      }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
+      top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
+    }
+    // The reference point of a row moves only when its maximum has grown by more than 2^8 (probabilities then stay below
+    // 2^8, which costs 16-bit ones no precision): most tiles leave the accumulators alone.
+    if (__any_sync(0xffffffffu, top[0] > m[0] + 8.f || top[1] > m[1] + 8.f)) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
-        top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
+        const float next = fmaxf(m[h], top[h]);
+        const float f = next == -INFINITY ? 1.f : paged_ex2(m[h] - next);
+        m[h] = next;
+        l[h] *= f;
+#pragma unroll
+        for (int j = 0; j < D / 8; ++j) acc[j][2 * h] *= f, acc[j][2 * h + 1] *= f;
       }
-      // The reference point of a row moves only when its maximum has grown by more than 2^8 (probabilities then stay below
-      // 2^8, which costs 16-bit ones no precision): most tiles leave the accumulators alone.
-      if (__any_sync(0xffffffffu, top[0] > m[0] + 8.f || top[1] > m[1] + 8.f)) {
+    }
+    const float m0 = m[0] == -INFINITY ? 0.f : m[0], m1 = m[1] == -INFINITY ? 0.f : m[1];
+#pragma unroll
+    for (int j = 0; j < kKeys / 8; ++j) {
+      sc[j][0] = paged_ex2(sc[j][0] - m0), sc[j][1] = paged_ex2(sc[j][1] - m0);
+      sc[j][2] = paged_ex2(sc[j][2] - m1), sc[j][3] = paged_ex2(sc[j][3] - m1);
+      l[0] += sc[j][0] + sc[j][1], l[1] += sc[j][2] + sc[j][3];
+    }
+    // Values.  A key that is not there, or that some row must not see, has probability 0 for those rows, and 0 times what its
+    // value may hold (anything, beyond the length) need not be 0: such keys are taken out of the product on both sides,
+    // and those that some rows do see (the newest T - 1) are added row by row behind it.
+#pragma unroll
+    for (int kk = 0; kk < kKeys / 16; ++kk) {
+      uint32_t a[4] = {pack16(sc[2 * kk][0], sc[2 * kk][1], Mma{}), pack16(sc[2 * kk][2], sc[2 * kk][3], Mma{}),
+                       pack16(sc[2 * kk + 1][0], sc[2 * kk + 1][1], Mma{}), pack16(sc[2 * kk + 1][2], sc[2 * kk + 1][3], Mma{})};
+      uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
+      if (special) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const float next = fmaxf(m[h], top[h]);
-          const float f = next == -INFINITY ? 1.f : paged_ex2(m[h] - next);
-          m[h] = next;
-          l[h] *= f;
-#pragma unroll
-          for (int j = 0; j < D / 8; ++j) acc[j][2 * h] *= f, acc[j][2 * h + 1] *= f;
+          const int key = key0 + kk * 16 + h * 8 + c4 * 2;
+          const bool ok = valid >> kk & 1u;
+          keep[h] = (ok && key >= u.key_lo && key < u.key_all ? 0x0000ffffu : 0u) | (ok && key + 1 >= u.key_lo && key + 1 < u.key_all ? 0xffff0000u : 0u);
+          a[2 * h] &= keep[h], a[2 * h + 1] &= keep[h];
         }
       }
-      const float m0 = m[0] == -INFINITY ? 0.f : m[0], m1 = m[1] == -INFINITY ? 0.f : m[1];
+      const uint32_t row = at + kk * 16 + ((lane >> 3) & 1) * 8 + (lane & 7);
+      if constexpr (kE4M3) {
 #pragma unroll
-      for (int j = 0; j < kKeys / 8; ++j) {
-        sc[j][0] = paged_ex2(sc[j][0] - m0), sc[j][1] = paged_ex2(sc[j][1] - m0);
-        sc[j][2] = paged_ex2(sc[j][2] - m1), sc[j][3] = paged_ex2(sc[j][3] - m1);
-        l[0] += sc[j][0] + sc[j][1], l[1] += sc[j][2] + sc[j][3];
-      }
-      // Values.  A key that is not there, or that some row must not see, has probability 0 for those rows, and 0 times what its
-      // value may hold (anything, beyond the length) need not be 0: such keys are taken out of the product on both sides,
-      // and those that some rows do see (the newest T - 1) are added row by row behind it.
+        for (int x = 0; x < D / 32; ++x) {  // matrices: keys 0-7 and 8-15 of 16 codes, then of the next 16
+          uint32_t b[4];
+          ldmatrix4_trans(b, vbase + swizzled_offset(row, x * 32 + (lane >> 4) * 16, kBoxBytes));
 #pragma unroll
-      for (int kk = 0; kk < kKeys / 16; ++kk) {
-        uint32_t a[4] = {pack16(sc[2 * kk][0], sc[2 * kk][1], Mma{}), pack16(sc[2 * kk][2], sc[2 * kk][3], Mma{}),
-                         pack16(sc[2 * kk + 1][0], sc[2 * kk + 1][1], Mma{}), pack16(sc[2 * kk + 1][2], sc[2 * kk + 1][3], Mma{})};
-        uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
-        if (special) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int key = key0 + kk * 16 + h * 8 + c4 * 2;
-            const bool ok = valid >> kk & 1u;
-            keep[h] = (ok && key >= u.key_lo && key < u.key_all ? 0x0000ffffu : 0u) | (ok && key + 1 >= u.key_lo && key + 1 < u.key_all ? 0xffff0000u : 0u);
-            a[2 * h] &= keep[h], a[2 * h + 1] &= keep[h];
+          for (int e = 0; e < 2; ++e) {
+            // a register holds (key, key + 1) x (d, d + 1): even and odd d go to accumulators of their own
+            uint32_t lo0 = e4m3x2_to_f16x2(__byte_perm(b[2 * e], 0, 0x4420)), lo1 = e4m3x2_to_f16x2(__byte_perm(b[2 * e + 1], 0, 0x4420));
+            uint32_t hi0 = e4m3x2_to_f16x2(__byte_perm(b[2 * e], 0, 0x4431)), hi1 = e4m3x2_to_f16x2(__byte_perm(b[2 * e + 1], 0, 0x4431));
+            if (special) lo0 &= keep[0], lo1 &= keep[1], hi0 &= keep[0], hi1 &= keep[1];
+            mma16816(acc[4 * x + 2 * e], a, lo0, lo1, Mma{});
+            mma16816(acc[4 * x + 2 * e + 1], a, hi0, hi1, Mma{});
           }
         }
-        if constexpr (kE4M3) {
+      } else {
 #pragma unroll
-          for (int x = 0; x < D / 32; ++x) {  // matrices: keys 0-7 and 8-15 of 16 codes, then of the next 16
-            uint32_t b[4];
-            ldmatrix4_trans(b, vbase + swizzled_offset(wk * kKeys + kk * 16 + ((lane >> 3) & 1) * 8 + (lane & 7), x * 32 + (lane >> 4) * 16, kBoxBytes));
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              // a register holds (key, key + 1) x (d, d + 1): even and odd d go to accumulators of their own
-              uint32_t lo0 = e4m3x2_to_f16x2(__byte_perm(b[2 * e], 0, 0x4420)), lo1 = e4m3x2_to_f16x2(__byte_perm(b[2 * e + 1], 0, 0x4420));
-              uint32_t hi0 = e4m3x2_to_f16x2(__byte_perm(b[2 * e], 0, 0x4431)), hi1 = e4m3x2_to_f16x2(__byte_perm(b[2 * e + 1], 0, 0x4431));
-              if (special) lo0 &= keep[0], lo1 &= keep[1], hi0 &= keep[0], hi1 &= keep[1];
-              mma16816(acc[4 * x + 2 * e], a, lo0, lo1, Mma{});
-              mma16816(acc[4 * x + 2 * e + 1], a, hi0, hi1, Mma{});
-            }
-          }
-        } else {
-#pragma unroll
-          for (int x = 0; x < D / 16; ++x) {
-            uint32_t b[4];
-            const uint32_t col = x * 32 + (lane >> 4) * 16;
-            ldmatrix4_trans(b, vbase + (col >> 7) * (kPagedTile * 128) +
-                                   swizzled_offset(wk * kKeys + kk * 16 + ((lane >> 3) & 1) * 8 + (lane & 7), col & 127u, 128));
-            if (special) b[0] &= keep[0], b[1] &= keep[1], b[2] &= keep[0], b[3] &= keep[1];
-            mma16816(acc[2 * x], a, b[0], b[1], Mma{});
-            mma16816(acc[2 * x + 1], a, b[2], b[3], Mma{});
-          }
+        for (int x = 0; x < D / 16; ++x) {
+          uint32_t b[4];
+          const uint32_t col = x * 32 + (lane >> 4) * 16;
+          ldmatrix4_trans(b, vbase + (col >> 7) * (kTileRows * 128) + swizzled_offset(row, col & 127u, 128));
+          if (special) b[0] &= keep[0], b[1] &= keep[1], b[2] &= keep[0], b[3] &= keep[1];
+          mma16816(acc[2 * x], a, b[0], b[1], Mma{});
+          mma16816(acc[2 * x + 1], a, b[2], b[3], Mma{});
         }
       }
-      if (key0 + kKeys > u.key_all) {
-#pragma unroll 1
-        for (int kk = max(0, u.key_all - key0); kk < min(kKeys, u.key_hi - key0); ++kk) {
-          if (!(valid >> (kk >> 4) & 1u)) continue;
-          const int from = (lane & ~3) | ((kk & 7) >> 1);
-          float mine[2] = {0.f, 0.f};
-#pragma unroll
-          for (int j = 0; j < kKeys / 8; ++j)
-            if (j == kk >> 3) mine[0] = kk & 1 ? sc[j][1] : sc[j][0], mine[1] = kk & 1 ? sc[j][3] : sc[j][2];
-          const float p0 = __shfl_sync(0xffffffffu, mine[0], from), p1 = __shfl_sync(0xffffffffu, mine[1], from);
-          const bool see0 = key0 + kk < limit[0], see1 = key0 + kk < limit[1];
-          const uint32_t row = wk * kKeys + kk;
-#pragma unroll
-          for (int j = 0; j < D / 8; ++j) {
-            float2 f;
-            if constexpr (kE4M3) {  // accumulators 2x and 2x + 1: d = 16 x + 4 c + {0, 2} and {1, 3}
-              const uint32_t four = *reinterpret_cast<const uint32_t*>(s.v[stage] + swizzled_offset(row, (j >> 1) * 16 + c4 * 4, kBoxBytes));
-              f = unpack16(e4m3x2_to_f16x2(__byte_perm(four, 0, j & 1 ? 0x4431 : 0x4420)), TagF16{});
-            } else {
-              const uint32_t col = j * 16 + c4 * 4;
-              f = unpack16(*reinterpret_cast<const uint32_t*>(s.v[stage] + (col >> 7) * (kPagedTile * 128) + swizzled_offset(row, col & 127u, 128)), Mma{});
-            }
-            if (see0) acc[j][0] = fmaf(p0, f.x, acc[j][0]), acc[j][1] = fmaf(p0, f.y, acc[j][1]);
-            if (see1) acc[j][2] = fmaf(p1, f.x, acc[j][2]), acc[j][3] = fmaf(p1, f.y, acc[j][3]);
-          }
-        }
-      }
-      mbar_arrive_warp(&s.empty[stage]);
-      if (++stage == kStages) stage = 0, parity ^= 1u;
     }
+    if (key0 + kKeys > u.key_all) {
+#pragma unroll 1
+      for (int kk = max(0, u.key_all - key0); kk < min(kKeys, u.key_hi - key0); ++kk) {
+        if (!(valid >> (kk >> 4) & 1u)) continue;
+        const int from = (lane & ~3) | ((kk & 7) >> 1);
+        float mine[2] = {0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < kKeys / 8; ++j)
+          if (j == kk >> 3) mine[0] = kk & 1 ? sc[j][1] : sc[j][0], mine[1] = kk & 1 ? sc[j][3] : sc[j][2];
+        const float p0 = __shfl_sync(0xffffffffu, mine[0], from), p1 = __shfl_sync(0xffffffffu, mine[1], from);
+        const bool see0 = key0 + kk < limit[0], see1 = key0 + kk < limit[1];
+        const uint32_t row = at + kk;
+#pragma unroll
+        for (int j = 0; j < D / 8; ++j) {
+          float2 f;
+          if constexpr (kE4M3) {  // accumulators 2x and 2x + 1: d = 16 x + 4 c + {0, 2} and {1, 3}
+            const uint32_t four = *reinterpret_cast<const uint32_t*>(vtile + swizzled_offset(row, (j >> 1) * 16 + c4 * 4, kBoxBytes));
+            f = unpack16(e4m3x2_to_f16x2(__byte_perm(four, 0, j & 1 ? 0x4431 : 0x4420)), TagF16{});
+          } else {
+            const uint32_t col = j * 16 + c4 * 4;
+            f = unpack16(*reinterpret_cast<const uint32_t*>(vtile + (col >> 7) * (kTileRows * 128) + swizzled_offset(row, col & 127u, 128)), Mma{});
+          }
+          if (see0) acc[j][0] = fmaf(p0, f.x, acc[j][0]), acc[j][1] = fmaf(p0, f.y, acc[j][1]);
+          if (see1) acc[j][2] = fmaf(p1, f.x, acc[j][2]), acc[j][3] = fmaf(p1, f.y, acc[j][3]);
+        }
+      }
+    }
+  }
 
-    // ---- the unit's share of this CTA: warps over keys meet, then rows and statistics go to the slot
+  __device__ __forceinline__ void sum_up() {  // the four lanes of a row meet
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
       l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
     }
-    if constexpr (kWK > 1) {
-      if (c4 == 0) s.ml[warp][quad] = make_float2(m[0], l[0]), s.ml[warp][quad + 8] = make_float2(m[1], l[1]);
+  }
+
+  __device__ __forceinline__ void store(const PagedParams& p, const PagedUnit& u, int row0, int worker) const {
+    const int lane = threadIdx.x & 31, quad = lane >> 2, c4 = lane & 3;
+    const int64_t slot = (int64_t)u.index + worker;
+    float* out = p.own_acc + slot * p.own_rows * D;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int row = row0 + h * 8 + quad;
+      if (row >= u.rows) continue;
+      if (c4 == 0) p.own_ml[slot * p.own_rows + row] = make_float2(m[h], l[h]);
+      if constexpr (kE4M3) {
+#pragma unroll
+        for (int x = 0; x < D / 16; ++x)
+          *reinterpret_cast<float4*>(out + row * D + x * 16 + c4 * 4) =
+              make_float4(acc[2 * x][2 * h], acc[2 * x + 1][2 * h], acc[2 * x][2 * h + 1], acc[2 * x + 1][2 * h + 1]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < D / 8; ++j) *reinterpret_cast<float2*>(out + row * D + j * 8 + c4 * 2) = make_float2(acc[j][2 * h], acc[j][2 * h + 1]);
+      }
+    }
+  }
+};
+
+// One box of tokens as a producing lane sees it: which of them a copy is asked for, and what the consumers may look at.
+struct PagedBoxes {
+  int tokens, per_tile;  // of a box; boxes of a tile
+  __device__ __forceinline__ uint32_t valid_bits(uint32_t loads) const {  // a bit per box -> a bit per 16 keys
+    const int per = tokens / 16;
+    uint32_t v = 0u;
+    for (int b = 0; b < per_tile; ++b)
+      if (loads >> b & 1u) v |= ((1u << per) - 1u) << (b * per);
+    return v;
+  }
+};
+
+// How a launch of own units stands to the ones before it.  Behind a plan it waits for it.  Behind prefix units it comes up
+// once all of those have seen the plan end (they trigger behind their own wait) and needs nothing of what they compute: it
+// runs beside them, and waits for them when it is done, so that the join, which waits for this launch, finds both.
+struct OwnOrder {
+  const bool beside;
+  __device__ __forceinline__ explicit OwnOrder(const PagedParams& p) : beside(p.groups > 0) {
+    if (!beside) pdl_wait();
+    pdl_trigger();
+  }
+  __device__ __forceinline__ ~OwnOrder() {
+    if (beside) pdl_wait();
+  }
+};
+
+// Up to sixteen query rows per unit (a single token, or a few drafted ones, of a group of query heads): every warp is a worker
+// with a line piece, a ring of tiles and copies of its own, and nothing in the loop waits for another warp.
+template <int D, bool kE4M3>
+struct SoloSmem {
+  static constexpr int kRowBytes = D * (kE4M3 ? 1 : 2);
+  static constexpr int kKeys = kRowBytes == 256 ? 16 : 32;            // of a tile
+  static constexpr int kTileBytes = kKeys * kRowBytes;               // K or V: 4 KB, 2 KB for E4M3 with D = 64
+  static constexpr int kStages = 24 * 1024 / (2 * kTileBytes);       // 24 KB in flight per warp, 192 KB per SM
+  alignas(1024) uint8_t ring[4][kStages][2][kTileBytes];
+  uint64_t full[4][kStages];
+  volatile uint32_t abort_flag;
+};
+
+template <int D, bool kE4M3, typename QT>
+__global__ void __launch_bounds__(128, 2) attn_solo_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_k,
+                                                           const __grid_constant__ CUtensorMap map_v) {
+  using Smem = SoloSmem<D, kE4M3>;
+  constexpr int kBytes = kE4M3 ? 1 : 2, kRowBytes = Smem::kRowBytes, kBoxBytes = kRowBytes < 128 ? kRowBytes : 128, kSubs = kRowBytes / kBoxBytes;
+  constexpr int kKeys = Smem::kKeys, kStages = Smem::kStages;
+  extern __shared__ __align__(1024) uint8_t raw[];
+  Smem& s = *reinterpret_cast<Smem*>(raw);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, worker = blockIdx.x * 4 + warp;
+  const bool aligned = (smem_u32(raw) & 1023u) == 0u;  // the swizzle of the tiles goes by the address
+  if (threadIdx.x == 0) {
+    for (int w = 0; w < 4; ++w)
+      for (int i = 0; i < kStages; ++i) mbar_init(&s.full[w][i], 1);
+    s.abort_flag = 0u;
+    fence_barrier_init();
+    fence_async_smem();
+    tma_prefetch_desc(&map_k);
+    tma_prefetch_desc(&map_v);
+  }
+  __syncthreads();
+  OwnOrder order(p);
+  if (!aligned) {
+    if (threadIdx.x == 0) p.status[1] = 99u, p.status[0] = 1u;
+    return;
+  }
+  PagedWalk<false> ahead, walk;  // of the copies, and of the products
+  ahead.start(p, worker);
+  walk = ahead;
+  if (walk.done()) return;
+
+  const PagedBoxes box{min(p.c.page_tokens, kKeys), kKeys / min(p.c.page_tokens, kKeys)};
+  PagedUnit next{};
+  int next_tile = 0, page_base = 0, pages = 0;  // `pages`: entry page_base + lane of the table row
+  bool more = true, fresh = true;
+  int issued = 0;
+  uint32_t valid_ring = 0u;  // two bits per stage
+  auto issue = [&]() {       // asks for the tile behind the last one that was asked for
+    if (!more) return;
+    while (fresh || next_tile == next.tile_end) {
+      if (!fresh && ahead.done()) {
+        more = false;
+        return;
+      }
+      next = ahead.next(p);
+      next_tile = next.tile;
+      fresh = next_tile == next.tile_end;
+      if (fresh && ahead.done()) {
+        more = false;
+        return;
+      }
+      page_base = INT_MIN;
+      if (!fresh) break;
+    }
+    const int stage = issued % kStages;
+    const int first = (next_tile * kKeys) >> p.c.page_shift;
+    if (page_base == INT_MIN || first + box.per_tile > page_base + 32) {
+      page_base = first;
+      const int at = first + lane;
+      pages = at < p.c.width ? p.c.table[(int64_t)next.table_slot * p.c.table_stride + at] : -1;
+    }
+    // lane = box + boxes x (sub-tile + sub-tiles x (K, V))
+    const int b = lane % box.per_tile, which = lane / box.per_tile;
+    const int token = next_tile * kKeys + b * box.tokens;
+    const int page = __shfl_sync(0xffffffffu, pages, (token >> p.c.page_shift) - page_base);
+    const bool wanted = token < next.key_hi && token + box.tokens > next.key_lo && page >= 0 && page < p.c.pages;
+    const uint32_t loads = __ballot_sync(0xffffffffu, wanted && which == 0);
+    valid_ring = (valid_ring & ~(3u << (2 * stage))) | box.valid_bits(loads) << (2 * stage);
+    if (lane == 0) mbar_expect_tx(&s.full[warp][stage], __popc(loads) * box.tokens * kRowBytes * 2);
+    __syncwarp();
+    if (wanted && which < 2 * kSubs) {
+      const int sub = which % kSubs;
+      uint8_t* dst = s.ring[warp][stage][which / kSubs] + sub * (kKeys * kBoxBytes) + b * box.tokens * kBoxBytes;
+      tma_load_5d(smem_u32(dst), which / kSubs ? &map_v : &map_k, sub * (kBoxBytes / kBytes), token & (p.c.page_tokens - 1), next.head, page, p.layer,
+                  &s.full[warp][stage]);
+    }
+    ++issued;
+    ++next_tile;
+  };
+#pragma unroll 1
+  for (int i = 0; i < kStages; ++i) issue();
+
+  int done = 0;
+  PagedRows<D, kE4M3, QT> rows;
+  while (!walk.done()) {
+    const PagedUnit u = walk.next(p);
+    if (u.tile == u.tile_end) continue;
+    rows.start(p, u, 0);
+#pragma unroll 1
+    for (int tile = u.tile; tile < u.tile_end; ++tile) {
+      const int stage = done % kStages;
+      if (!mbar_wait_warp(&s.full[warp][stage], (uint32_t)(done / kStages) & 1u, &s.abort_flag, p.status, 1)) {
+        for (int k = done; k < issued; ++k) mbar_wait_teardown(&s.full[warp][k % kStages], (uint32_t)(k / kStages) & 1u);
+        return;
+      }
+      rows.template tile<kKeys, kKeys>(u, s.ring[warp][stage][0], s.ring[warp][stage][1], 0, tile * kKeys, valid_ring >> (2 * stage) & 3u);
+      ++done;
+      __syncwarp();
+      issue();
+    }
+    rows.sum_up();
+    rows.store(p, u, 0, worker);
+  }
+}
+
+// More rows than that: kWM warps side by side over rows (16 each), 4 / kWM over the keys of a tile of 64; a fifth warp asks for
+// the tiles.
+template <int D, bool kE4M3>
+struct TeamSmem {
+  static constexpr int kKeys = 64;
+  static constexpr int kTileBytes = kKeys * D * (kE4M3 ? 1 : 2);  // K or V of one tile
+  static constexpr int kFit = 96 * 1024 / (2 * kTileBytes), kStages = kFit > 8 ? 8 : kFit;
+  alignas(1024) uint8_t k[kStages][kTileBytes];
+  uint8_t v[kStages][kTileBytes];
+  float merge[2][16][D];
+  float2 ml[4][16];
+  uint64_t full[kStages], empty[kStages];
+  uint32_t valid[kStages];  // a bit per 16 keys: the table names a page of the pool
+  volatile uint32_t abort_flag;
+};
+
+template <int D, bool kE4M3, typename QT, int kWM>
+__global__ void __launch_bounds__(160, 2) attn_team_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_k,
+                                                           const __grid_constant__ CUtensorMap map_v) {
+  using Smem = TeamSmem<D, kE4M3>;
+  constexpr int kBytes = kE4M3 ? 1 : 2, kRowBytes = D * kBytes, kBoxBytes = kRowBytes < 128 ? kRowBytes : 128, kSubs = kRowBytes / kBoxBytes;
+  constexpr int kTile = Smem::kKeys, kWK = 4 / kWM, kKeys = kTile / kWK;  // keys of a tile that one warp takes
+  constexpr int kStages = Smem::kStages;
+  extern __shared__ __align__(1024) uint8_t raw[];
+  Smem& s = *reinterpret_cast<Smem*>(raw);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const bool aligned = (smem_u32(raw) & 1023u) == 0u;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; ++i) mbar_init(&s.full[i], 1), mbar_init(&s.empty[i], 4);
+    s.abort_flag = 0u;
+    fence_barrier_init();
+    fence_async_smem();
+    tma_prefetch_desc(&map_k);
+    tma_prefetch_desc(&map_v);
+  }
+  __syncthreads();
+  OwnOrder order(p);
+  if (!aligned) {
+    if (threadIdx.x == 0) p.status[1] = 99u, p.status[0] = 1u;
+    return;
+  }
+  PagedWalk<false> walk;
+  walk.start(p, blockIdx.x);
+
+  if (warp == 4) {  // ---- producer: lane b of a tile's boxes asks for its own part of the pages
+    const PagedBoxes box{min(p.c.page_tokens, kTile), kTile / min(p.c.page_tokens, kTile)};
+    int stage = 0, issued = 0;
+    uint32_t parity = 1u;
+    while (!walk.done()) {
+      const PagedUnit u = walk.next(p);
+      const int32_t* row = p.c.table + (int64_t)u.table_slot * p.c.table_stride;
+      for (int tile = u.tile; tile < u.tile_end; ++tile) {
+        const int token = tile * kTile + lane * box.tokens;
+        const bool wanted = lane < box.per_tile && token < u.key_hi && token + box.tokens > u.key_lo;
+        int page = -1;
+        if (wanted) page = row[token >> p.c.page_shift];
+        const bool load = wanted && page >= 0 && page < p.c.pages;
+        const uint32_t loads = __ballot_sync(0xffffffffu, load);
+        const bool go = mbar_wait_warp(&s.empty[stage], parity, &s.abort_flag, p.status, 1);
+        if (lane == 0) {
+          s.valid[stage] = box.valid_bits(loads);
+          mbar_expect_tx(&s.full[stage], go ? __popc(loads) * box.tokens * kRowBytes * 2 : 0);
+        }
+        __syncwarp();
+        if (go && load) {
+          const int in_page = token & (p.c.page_tokens - 1);
+#pragma unroll
+          for (int x = 0; x < kSubs; ++x) {
+            const uint32_t off = x * (kTile * kBoxBytes) + lane * box.tokens * kBoxBytes;
+            tma_load_5d(smem_u32(s.k[stage]) + off, &map_k, x * (kBoxBytes / kBytes), in_page, u.head, page, p.layer, &s.full[stage]);
+            tma_load_5d(smem_u32(s.v[stage]) + off, &map_v, x * (kBoxBytes / kBytes), in_page, u.head, page, p.layer, &s.full[stage]);
+          }
+        }
+        ++issued;
+        if (++stage == kStages) stage = 0, parity ^= 1u;
+      }
+    }
+    if (s.abort_flag)  // copies in flight land before the CTA leaves
+      for (int k = max(0, issued - kStages); k < issued; ++k) mbar_wait_teardown(&s.full[k % kStages], (uint32_t)(k / kStages) & 1u);
+    return;
+  }
+
+  // ---- consumers
+  const int wm = warp % kWM, wk = warp / kWM, quad = lane >> 2, c4 = lane & 3;
+  int stage = 0;
+  uint32_t parity = 0u;
+  PagedRows<D, kE4M3, QT> rows;
+  while (!walk.done()) {
+    const PagedUnit u = walk.next(p);
+    if (u.tile == u.tile_end) continue;
+    rows.start(p, u, wm * 16);
+    for (int tile = u.tile; tile < u.tile_end; ++tile) {
+      mbar_wait_warp(&s.full[stage], parity, &s.abort_flag, p.status, 2);
+      rows.template tile<kKeys, kTile>(u, s.k[stage], s.v[stage], wk * kKeys, tile * kTile + wk * kKeys, s.valid[stage] >> (wk * kKeys / 16));
+      mbar_arrive_warp(&s.empty[stage]);
+      if (++stage == kStages) stage = 0, parity ^= 1u;
+    }
+    rows.sum_up();
+    if constexpr (kWK > 1) {  // the warps over keys meet: the upper half of them hands its sums to the lower half
+      if (c4 == 0) s.ml[warp][quad] = make_float2(rows.m[0], rows.l[0]), s.ml[warp][quad + 8] = make_float2(rows.m[1], rows.l[1]);
       asm volatile("bar.sync 1, 128;" ::: "memory");
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        float top = -INFINITY;
+        const float2 x = s.ml[warp][quad + 8 * h], y = s.ml[(wk ^ 1) * kWM + wm][quad + 8 * h];
+        const float top = fmaxf(x.x, y.x);
+        const float f = x.x == -INFINITY ? 0.f : paged_ex2(x.x - top), g = y.x == -INFINITY ? 0.f : paged_ex2(y.x - top);
+        rows.m[h] = top, rows.l[h] = x.y * f + y.y * g;
 #pragma unroll
-        for (int w = 0; w < kWK; ++w) top = fmaxf(top, s.ml[w * kWM + wm][quad + 8 * h].x);
-        const float f = m[h] == -INFINITY ? 0.f : paged_ex2(m[h] - top);
-        float sum = 0.f;
-#pragma unroll
-        for (int w = 0; w < kWK; ++w) {
-          const float2 x = s.ml[w * kWM + wm][quad + 8 * h];
-          sum += x.y * (x.x == -INFINITY ? 0.f : paged_ex2(x.x - top));
-        }
-        m[h] = top, l[h] = sum;
-#pragma unroll
-        for (int j = 0; j < D / 8; ++j) acc[j][2 * h] *= f, acc[j][2 * h + 1] *= f;
+        for (int j = 0; j < D / 8; ++j) rows.acc[j][2 * h] *= f, rows.acc[j][2 * h + 1] *= f;
       }
-      // the upper half of the warps hands its sums to the lower half, until one row of warps is left
+      float* buf = &s.merge[wm][0][0];
+      if (wk == 1) {
 #pragma unroll
-      for (int half = kWK / 2; half >= 1; half /= 2) {
-        const bool gives = wk >= half && wk < 2 * half;
-        float* buf = &s.merge[kWK == 4 ? (wk & (half - 1)) : wm][0][0];
-        if (kWK == 4 && half == 1) buf = &s.merge[1][0][0];  // warp 1 reads and then writes there, warp 0 still reads the other
-        if (gives) {
-#pragma unroll
-          for (int j = 0; j < D / 8; ++j) {
-            *reinterpret_cast<float2*>(buf + quad * D + j * 8 + c4 * 2) = make_float2(acc[j][0], acc[j][1]);
-            *reinterpret_cast<float2*>(buf + (quad + 8) * D + j * 8 + c4 * 2) = make_float2(acc[j][2], acc[j][3]);
-          }
+        for (int j = 0; j < D / 8; ++j) {
+          *reinterpret_cast<float2*>(buf + quad * D + j * 8 + c4 * 2) = make_float2(rows.acc[j][0], rows.acc[j][1]);
+          *reinterpret_cast<float2*>(buf + (quad + 8) * D + j * 8 + c4 * 2) = make_float2(rows.acc[j][2], rows.acc[j][3]);
         }
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-        if (wk < half) {
+      }
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      if (wk == 0) {
 #pragma unroll
-          for (int j = 0; j < D / 8; ++j) {
-            const float2 x = *reinterpret_cast<const float2*>(buf + quad * D + j * 8 + c4 * 2);
-            const float2 y = *reinterpret_cast<const float2*>(buf + (quad + 8) * D + j * 8 + c4 * 2);
-            acc[j][0] += x.x, acc[j][1] += x.y, acc[j][2] += y.x, acc[j][3] += y.y;
-          }
+        for (int j = 0; j < D / 8; ++j) {
+          const float2 x = *reinterpret_cast<const float2*>(buf + quad * D + j * 8 + c4 * 2);
+          const float2 y = *reinterpret_cast<const float2*>(buf + (quad + 8) * D + j * 8 + c4 * 2);
+          rows.acc[j][0] += x.x, rows.acc[j][1] += x.y, rows.acc[j][2] += y.x, rows.acc[j][3] += y.y;
         }
       }
     }
-    if (wk == 0) {
-      const int64_t slot = (int64_t)u.index + blockIdx.x;
-      float* out = p.own_acc + slot * p.own_rows * D;
-      float2* ml = p.own_ml + slot * p.own_rows;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int row = wm * 16 + h * 8 + quad;
-        if (row >= u.rows) continue;
-        if (c4 == 0) ml[row] = make_float2(m[h], l[h]);
-        if constexpr (kE4M3) {
-#pragma unroll
-          for (int x = 0; x < D / 16; ++x)
-            *reinterpret_cast<float4*>(out + row * D + x * 16 + c4 * 4) =
-                make_float4(acc[2 * x][2 * h], acc[2 * x + 1][2 * h], acc[2 * x][2 * h + 1], acc[2 * x + 1][2 * h + 1]);
-        } else {
-#pragma unroll
-          for (int j = 0; j < D / 8; ++j) *reinterpret_cast<float2*>(out + row * D + j * 8 + c4 * 2) = make_float2(acc[j][2 * h], acc[j][2 * h + 1]);
-        }
-      }
-    }
+    if (wk == 0) rows.store(p, u, wm * 16, blockIdx.x);
   }
 }
 
 // ---- join -------------------------------------------------------------------------------------------------------------
 // One warp per output row.  The pieces' statistics come to the lanes at once, so that what is left to wait for is one
-// round of loads: a lane holds D / 32 neighbours of eight pieces at a time.
+// round of loads: a lane holds D / 32 neighbours of eight pieces at a time.  Which pieces there are follows from the
+// plan, which is complete when this launch comes up (the own units trigger behind it), so it is looked up before the wait.
 template <int D, typename QT>
-__global__ void __launch_bounds__(256) paged_join_kernel(const PagedParams p) {
+__global__ void __launch_bounds__(128) paged_join_kernel(const PagedParams p) {
   constexpr int kPer = D / 32;
-  pdl_trigger();
-  pdl_wait();
-  const int64_t w = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
-  if (w >= (int64_t)p.n * p.Hq * p.T) return;
-  const int t = (int)(w % p.T), h = (int)(w / p.T % p.Hq), i = (int)(w / p.T / p.Hq);
-  const int g = p.plan.group[i];
-  if (g < 0) return;  // behind the last group: left as it was
-  const int head = h / p.G, r = t * p.G + h % p.G, len = p.plan.len[i];
+  pdl_trigger();
+  const bool there = w < (int64_t)p.n * p.Hq * p.T;
+  const uint32_t row_id = there ? (uint32_t)w : 0u;
+  const uint32_t t = row_id % (uint32_t)p.T, ih = row_id / (uint32_t)p.T, h = ih % (uint32_t)p.Hq, i = ih / (uint32_t)p.Hq;
+  const PagedSeq s = p.seq[i];
+  const PagedHead line = *p.head;
+  const int head = h / p.G, r = t * p.G + h % p.G, len = s.len;
   float acc[kPer], m = -INFINITY, l = 0.f;
 #pragma unroll
   for (int e = 0; e < kPer; ++e) acc[e] = 0.f;
-  if (len - (p.T - 1 - t) > 0) {
-    const int first = own_first_key(p, i), tiles = own_tiles(first, len);
-    // rows of the row's pieces: piece k of the prefix, then of the own keys, `rows` apart
-    int n_prefix = 0, prefix_row = 0;
-    int64_t prefix_slot = 0;
-    if (first > 0) {
-      const int64_t per_cta = piece_tiles(line_total<true>(p), p.prefix_ctas);
-      const int lo = max(p.offsets[g], 0), hi = min(p.offsets[g + 1], p.n);
-      const int row = (i - lo) * p.R + r, blocks = ceil_div((hi - lo) * p.R, p.prefix_rows);
-      const int which = head * blocks + row / p.prefix_rows, ptiles = ceil_div(first, p.prefix_tile);
-      const int64_t from = p.plan.g_cum[g] + (int64_t)which * ptiles, cta = from / per_cta;
-      n_prefix = (int)((from + ptiles - 1) / per_cta - cta) + 1;
-      prefix_slot = p.plan.g_unit[g] + which + cta;
-      prefix_row = row % p.prefix_rows;
+  // the workers that have a part of the unit's tiles: from the one where the first tile lies to the one where the last does
+  int n_prefix = 0, prefix_row = 0, n_own = 0, own_row = 0;
+  int64_t prefix_slot = 0, own_slot = 0;
+  if (len - (p.T - 1 - (int)t) > 0) {
+    if (s.first > 0) {
+      const int row = ((int)i - s.g_row) * p.R + r, block = row / p.prefix_rows, which = head * s.g_blocks + block;
+      const int tiles = ceil_div(s.first, p.prefix_tile);
+      const uint32_t per = (uint32_t)line.prefix_per, from = (uint32_t)(s.g_cum + which * (tiles + p.prefix_extra) + p.prefix_extra), worker = from / per;
+      n_prefix = (int)((from + tiles - 1) / per - worker) + 1;
+      prefix_slot = s.g_unit + which + (int64_t)worker;
+      prefix_row = row - block * p.prefix_rows;
     }
-    const int per = p.c.heads * p.own_blocks, which = head * p.own_blocks + r / p.own_rows;
-    const int64_t per_cta = piece_tiles(line_total<false>(p), p.own_ctas), from = (int64_t)p.plan.own_cum[i] * per + (int64_t)which * tiles;
-    const int64_t cta = from / per_cta, own_slot = (int64_t)i * per + which + cta;
-    const int n_own = (int)((from + tiles - 1) / per_cta - cta) + 1, own_row = r % p.own_rows;
+    const int per = p.c.heads * p.own_blocks, block = r / p.own_rows, which = head * p.own_blocks + block, tiles = own_tiles(p, s.first, len);
+    const int64_t from = (int64_t)s.cum * per + (int64_t)which * (tiles + p.own_extra) + p.own_extra, worker = from / line.own_per;
+    own_slot = (int64_t)i * per + which + worker;
+    n_own = (int)((from + tiles - 1) / line.own_per - worker) + 1;
+    own_row = r - block * p.own_rows;
+  }
+  pdl_wait();
+  if (!there || s.left_alone) return;  // or behind the last group
+  {
     for (int base = 0; base < n_prefix + n_own; base += 32) {
       const int k = base + lane;
       const bool is_prefix = k < n_prefix;
@@ -576,7 +777,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedParams p) {
     }
   }
   const float inv = l == 0.f ? 0.f : (p.v_scale ? p.v_scale[head] : 1.f) / l;  // a row that sees nothing: zeros, -inf
-  uint8_t* out = p.o + 2 * (i * p.o_sb + h * p.o_sh + t * p.o_st + lane * kPer);
+  uint8_t* out = p.o + 2 * ((int64_t)i * p.o_sb + (int64_t)h * p.o_sh + (int64_t)t * p.o_st + lane * kPer);
   if constexpr (kPer == 4) *reinterpret_cast<uint2*>(out) = make_uint2(pack16(acc[0] * inv, acc[1] * inv, QT{}), pack16(acc[2] * inv, acc[3] * inv, QT{}));
   else *reinterpret_cast<uint32_t*>(out) = pack16(acc[0] * inv, acc[1] * inv, QT{});
   if (lane == 0) p.lse[((int64_t)i * p.Hq + h) * p.T + t] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
@@ -587,27 +788,35 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedParams p) {
 // ---- host -------------------------------------------------------------------------------------------------------------
 namespace fa4b {
 
-template <int D, typename CacheT, typename QT, int kWM>
-static int launch_units(const PagedParams& p, const CUtensorMap& mk, const CUtensorMap& mv, int ctas, cudaStream_t st) {
-  auto kernel = attn_paged_kernel<D, CacheT, QT, kWM>;
-  constexpr int smem = (int)sizeof(PagedSmem<D, std::is_same<CacheT, uint8_t>::value ? 1 : 2>);
+struct PagedMaps {
+  CUtensorMap own_k, own_v, prefix_k, prefix_v;
+};
+
+template <typename Smem, typename K>
+static int launch_units(K kernel, const PagedParams& p, const CUtensorMap& mk, const CUtensorMap& mv, int ctas, int threads, cudaStream_t st,
+                        std::atomic<uint64_t>& allowed) {
+  constexpr int smem = (int)sizeof(Smem);
   static_assert(smem <= 113 * 1024, "two CTAs per SM");
-  FA4B_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  FA4B_CUDA(launch_overlapped(kernel, ctas, kPagedThreads, smem, st, p, mk, mv));
+  if (int s = allow_smem(kernel, smem, allowed)) return s;
+  FA4B_CUDA(launch_overlapped(kernel, ctas, threads, smem, st, p, mk, mv));
   return FA4B_OK;
 }
 
-template <int D, typename CacheT, typename QT>
-static int launch_paged(const PagedParams& p, const CUtensorMap& mk, const CUtensorMap& mv, cudaStream_t st) {
-  FA4B_CUDA(launch_overlapped(paged_plan_kernel, 1, 1024, 12 * (size_t)p.groups, st, p));
+template <int D, bool kE4M3, typename QT>
+static int launch_paged(const PagedParams& p, const PagedMaps& m, cudaStream_t st) {
+  const size_t smem = 4 * paged_plan_words(p.n, p.groups);
+  static std::atomic<uint64_t> allowed[4];
+  if (smem > 48 * 1024)
+    if (int s = allow_smem(paged_plan_kernel, 4 * (int)paged_plan_words(kPagedMaxRows, kPagedMaxRows), allowed[3])) return s;
+  FA4B_CUDA(launch_overlapped(paged_plan_kernel, 1, 1024, smem, st, p));
   if (p.groups > 0)
-    if (int s = launch_prefix(p, D, std::is_same<CacheT, uint8_t>::value, std::is_same<QT, TagF16>::value, mk, mv, st)) return s;
-  const int s = p.own_rows == 16   ? launch_units<D, CacheT, QT, 1>(p, mk, mv, p.own_ctas, st)
-                : p.own_rows == 32 ? launch_units<D, CacheT, QT, 2>(p, mk, mv, p.own_ctas, st)
-                                   : launch_units<D, CacheT, QT, 4>(p, mk, mv, p.own_ctas, st);
+    if (int s = launch_prefix(p, D, kE4M3, std::is_same<QT, TagF16>::value, m.prefix_k, m.prefix_v, st)) return s;
+  const int s = p.own_rows == 16   ? launch_units<SoloSmem<D, kE4M3>>(attn_solo_kernel<D, kE4M3, QT>, p, m.own_k, m.own_v, p.own_workers / 4, 128, st, allowed[0])
+                : p.own_rows == 32 ? launch_units<TeamSmem<D, kE4M3>>(attn_team_kernel<D, kE4M3, QT, 2>, p, m.own_k, m.own_v, p.own_workers, 160, st, allowed[1])
+                                   : launch_units<TeamSmem<D, kE4M3>>(attn_team_kernel<D, kE4M3, QT, 4>, p, m.own_k, m.own_v, p.own_workers, 160, st, allowed[2]);
   if (s) return s;
   const int64_t rows = (int64_t)p.n * p.Hq * p.T;
-  FA4B_CUDA(launch_overlapped(paged_join_kernel<D, QT>, (unsigned)((rows + 7) / 8), 256, 0, st, p));
+  FA4B_CUDA(launch_overlapped(paged_join_kernel<D, QT>, (unsigned)((rows + 3) / 4), 128, 0, st, p));
   return FA4B_OK;
 }
 
@@ -621,6 +830,7 @@ static int paged_params(const fa4b_kv_cache* c, const fa4b_attn_paged_args* a, P
   FA4B_REQUIRE(a->n >= 0 && a->n <= kPagedMaxRows, FA4B_BAD_SHAPE, "n=%d: batches of 0 to %d rows are built", a->n, kPagedMaxRows);
   FA4B_REQUIRE(a->T >= 1 && a->T <= kPagedMaxT, FA4B_BAD_SHAPE, "T=%d: 1 to %d query tokens per sequence are built", a->T, kPagedMaxT);
   FA4B_REQUIRE(a->Hq > 0 && a->Hq % c->Hkv == 0, FA4B_BAD_SHAPE, "Hq=%d must be a multiple of Hkv=%d", a->Hq, c->Hkv);
+  FA4B_REQUIRE((int64_t)a->n * a->Hq * a->T < INT32_MAX, FA4B_BAD_SHAPE, "n Hq T must be below 2^31");
   FA4B_REQUIRE(a->Hq / c->Hkv <= 128, FA4B_BAD_SHAPE, "%d query heads per kv head: at most 128 are built", a->Hq / c->Hkv);
   FA4B_REQUIRE(a->layer >= 0 && a->layer < c->layers, FA4B_BAD_SHAPE, "layer %d of %d", a->layer, c->layers);
   FA4B_REQUIRE(a->q_dtype == FA4B_KV_BF16 || a->q_dtype == FA4B_KV_F16, FA4B_UNSUPPORTED, "queries are bf16 or f16");
@@ -641,16 +851,20 @@ static int paged_params(const fa4b_kv_cache* c, const fa4b_attn_paged_args* a, P
   const int n_sm = sm_count() > 0 ? sm_count() : 148;
   p.own_rows = p.R <= 16 ? 16 : p.R <= 32 ? 32 : 64;
   p.own_blocks = (p.R + p.own_rows - 1) / p.own_rows;
-  p.own_ctas = 2 * n_sm;
+  const bool solo = p.own_rows == 16, short_rows = c->D * (c->dtype == FA4B_KV_E4M3 ? 1 : 2) < 256;
+  p.own_tile = !solo ? TeamSmem<64, true>::kKeys : short_rows ? 32 : 16;
+  p.own_workers = (solo ? 8 : 2) * n_sm;
+  p.own_extra = solo ? 2 : 1;
+  p.own_min = p.own_extra + (solo ? 64 / p.own_tile : 1);  // a piece shorter than 64 keys is mostly its beginning
   // two blocks of 128 rows over the same keys where the groups have the rows for it: each tile then comes from memory half
   // as often; otherwise the two halves of a CTA take the keys in turn
   p.prefix_rows = p.groups > 0 && (int64_t)p.n * p.R > 128ll * p.groups ? 256 : 128;
-  p.prefix_tile = 128, p.prefix_ctas = n_sm;
-  const int64_t row_tiles = ((int64_t)c->table_width * c->page_tokens + kPagedTile - 1) / kPagedTile + 1;
+  p.prefix_tile = 128, p.prefix_workers = n_sm, p.prefix_extra = 1;
+  const int64_t keys = (int64_t)c->table_width * c->page_tokens, own_length = keys / p.own_tile + 2 + p.own_extra;
   const int64_t prefix_units = p.groups ? (int64_t)c->Hkv * (((int64_t)p.n * p.R + p.prefix_rows - 1) / p.prefix_rows + p.groups) : 0;
-  const int64_t own_slots = (int64_t)p.n * c->Hkv * p.own_blocks + p.own_ctas, prefix_slots = p.groups ? prefix_units + p.prefix_ctas : 0;
-  // positions on the two lines are counted in 32 bits
-  FA4B_REQUIRE(p.n * row_tiles < INT32_MAX && prefix_units * row_tiles < INT32_MAX && own_slots < INT32_MAX, FA4B_BAD_SHAPE,
+  const int64_t own_slots = (int64_t)p.n * c->Hkv * p.own_blocks + p.own_workers, prefix_slots = p.groups ? prefix_units + p.prefix_workers : 0;
+  // positions on the lines (of one head and row block, and of all) are counted in 32 bits
+  FA4B_REQUIRE(p.n * own_length < INT32_MAX && prefix_units * (keys / p.prefix_tile + 2 + p.prefix_extra) < INT32_MAX && own_slots < INT32_MAX, FA4B_BAD_SHAPE,
                "%d rows over tables of %d pages of %d tokens are too many for one call", p.n, c->table_width, c->page_tokens);
   size_t off = 0;
   uint8_t* ws = static_cast<uint8_t*>(a->ws);
@@ -660,14 +874,11 @@ static int paged_params(const fa4b_kv_cache* c, const fa4b_attn_paged_args* a, P
     return at;
   };
   const size_t n = p.n, g = p.groups;
-  p.plan.slot = reinterpret_cast<int*>(take(4 * n));
-  p.plan.len = reinterpret_cast<int*>(take(4 * n));
-  p.plan.group = reinterpret_cast<int*>(take(4 * n));
-  p.plan.own_cum = reinterpret_cast<int*>(take(4 * (n + 1)));
-  p.plan.g_first = reinterpret_cast<int*>(take(4 * g));
-  p.plan.g_shared = reinterpret_cast<int*>(take(4 * g));
-  p.plan.g_cum = reinterpret_cast<int*>(take(4 * (g + 1)));
-  p.plan.g_unit = reinterpret_cast<int*>(take(4 * (g + 1)));
+  p.head = reinterpret_cast<PagedHead*>(take(sizeof(PagedHead)));
+  p.seq = reinterpret_cast<PagedSeq*>(take(sizeof(PagedSeq) * n));
+  p.group = reinterpret_cast<PagedGroup*>(take(sizeof(PagedGroup) * g));
+  p.own_start = reinterpret_cast<PagedStart*>(take(sizeof(PagedStart) * p.own_workers));
+  p.prefix_start = reinterpret_cast<PagedStart*>(take(sizeof(PagedStart) * p.prefix_workers));
   p.own_ml = reinterpret_cast<float2*>(take((size_t)own_slots * p.own_rows * 8));
   p.prefix_ml = reinterpret_cast<float2*>(take((size_t)prefix_slots * p.prefix_rows * 8));
   p.own_acc = reinterpret_cast<float*>(take((size_t)own_slots * p.own_rows * c->D * 4));
@@ -698,23 +909,29 @@ int fa4b_attn_paged_fwd(const fa4b_kv_cache* c, const fa4b_attn_paged_args* a, v
   FA4B_REQUIRE(a->q && a->o && a->lse && a->ws, FA4B_BAD_ARG, "q, o, lse or ws is NULL");
   FA4B_REQUIRE((reinterpret_cast<uintptr_t>(a->ws) & 255) == 0, FA4B_BAD_ALIGN, "ws must be 256-byte aligned");
   const bool e4m3 = c->dtype == FA4B_KV_E4M3;
-  CUtensorMap mk, mv;
-  const uint32_t box = c->D * (e4m3 ? 1 : 2) < 128 ? c->D : 128 / (e4m3 ? 1 : 2);
+  // one map per pool and width of a copy: the units take what a tile of theirs holds of a page
   const int esz = e4m3 ? 1 : 2;
   const uint64_t dims[5] = {(uint64_t)c->D, (uint64_t)c->page_tokens, (uint64_t)c->Hkv, (uint64_t)c->num_pages, (uint64_t)c->layers};
-  const uint32_t boxes[5] = {box, (uint32_t)std::min(c->page_tokens, kPagedTile), 1, 1, 1};
   const uint64_t sk[4] = {(uint64_t)p.c.row_bytes, (uint64_t)p.c.row_bytes * c->page_tokens, (uint64_t)p.c.k_page, (uint64_t)p.c.k_layer};
   const uint64_t sv[4] = {sk[0], sk[1], (uint64_t)p.c.v_page, (uint64_t)p.c.v_layer};
-  if (int s = make_tensor_map_5d(&mk, c->k, esz, dims, sk, boxes)) return s;
-  if (int s = make_tensor_map_5d(&mv, c->v, esz, dims, sv, boxes)) return s;
+  uint32_t box[5] = {(uint32_t)std::min(c->D, 128 / esz), (uint32_t)std::min(c->page_tokens, p.own_tile), 1, 1, 1};
+  PagedMaps m;
+  if (int s = make_tensor_map_5d(&m.own_k, c->k, esz, dims, sk, box)) return s;
+  if (int s = make_tensor_map_5d(&m.own_v, c->v, esz, dims, sv, box)) return s;
+  m.prefix_k = m.own_k, m.prefix_v = m.own_v;
+  if (p.groups > 0 && (int)box[1] != std::min(c->page_tokens, kPagedBox)) {
+    box[1] = (uint32_t)std::min(c->page_tokens, kPagedBox);
+    if (int s = make_tensor_map_5d(&m.prefix_k, c->k, esz, dims, sk, box)) return s;
+    if (int s = make_tensor_map_5d(&m.prefix_v, c->v, esz, dims, sv, box)) return s;
+  }
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool q16 = a->q_dtype == FA4B_KV_F16;
   if (c->D == 128) {
-    if (e4m3) return q16 ? launch_paged<128, uint8_t, TagF16>(p, mk, mv, st) : launch_paged<128, uint8_t, TagBf16>(p, mk, mv, st);
-    return q16 ? launch_paged<128, uint16_t, TagF16>(p, mk, mv, st) : launch_paged<128, uint16_t, TagBf16>(p, mk, mv, st);
+    if (e4m3) return q16 ? launch_paged<128, true, TagF16>(p, m, st) : launch_paged<128, true, TagBf16>(p, m, st);
+    return q16 ? launch_paged<128, false, TagF16>(p, m, st) : launch_paged<128, false, TagBf16>(p, m, st);
   }
-  if (e4m3) return q16 ? launch_paged<64, uint8_t, TagF16>(p, mk, mv, st) : launch_paged<64, uint8_t, TagBf16>(p, mk, mv, st);
-  return q16 ? launch_paged<64, uint16_t, TagF16>(p, mk, mv, st) : launch_paged<64, uint16_t, TagBf16>(p, mk, mv, st);
+  if (e4m3) return q16 ? launch_paged<64, true, TagF16>(p, m, st) : launch_paged<64, true, TagBf16>(p, m, st);
+  return q16 ? launch_paged<64, false, TagF16>(p, m, st) : launch_paged<64, false, TagBf16>(p, m, st);
 }
 
 }  // extern "C"

@@ -3,9 +3,10 @@
 // A call has two kinds of work.  "Own" units: one sequence, one kv head, up to own_rows of its T x (Hq / Hkv) query rows,
 // over the keys that are the sequence's own.  "Prefix" units: one group, one kv head, up to prefix_rows of the group's
 // rows, over the keys that its members share, so that those are read once for all of them.  Either kind's units are
-// laid end to end as one line of key tiles which is cut into equal pieces, one per CTA: long and short sequences load every
-// SM alike, and what a CTA keeps of a unit goes to a slot of its own (unit + CTA: either grows along the line, so the sum
-// names the pair).  The last launch joins the slots of a row: out = sum 2^(m_i - M) acc_i / sum 2^(m_i - M) l_i.
+// laid end to end as one line, each as long as its tiles of keys plus what starting a unit costs, and the line is cut into
+// equal pieces, one per worker (a warp, or a CTA): long and short sequences load every SM alike.  What a worker has of a
+// unit goes to a slot of its own (unit + worker: either grows along the line, so the sum names the pair).  The last launch
+// joins the slots of a row: out = sum 2^(m_i - M) acc_i / sum 2^(m_i - M) l_i.
 #pragma once
 #include "attn.cuh"
 #include "kv_cache.cuh"
@@ -14,20 +15,26 @@
 
 namespace fa4b {
 
-constexpr int kPagedTile = 64;        // keys of a tile of the own units
+constexpr int kPagedBox = 64;         // tokens of a page that one copy brings at most
 constexpr int kPagedAlign = 16;       // the shared part of a group ends on a multiple of this
 constexpr int kPagedMaxRows = 4096;   // sequences of one call
 constexpr int kPagedMaxT = 16;
 
-struct PagedPlan {  // device arrays in the workspace
-  int* slot;        // [n] -1: none
-  int* len;         // [n] keys (0: nothing to do)
-  int* group;       // [n] -1: the row belongs to no group and is left alone
-  int* own_cum;     // [n + 1] tiles of one (kv head, row block) before sequence i
-  int* g_first;     // [groups] a member whose row of the table names the shared pages
-  int* g_shared;    // [groups] shared keys that every row of the group sees
-  int* g_cum;       // [groups + 1] tiles before group g, all heads and row blocks
-  int* g_unit;      // [groups + 1] units before group g
+// What the plan writes down, so that a worker knows all about its first unit after one round of loads.
+struct PagedSeq {    // one row of the batch
+  int slot, len, first, cum;             // first key that is its own; length of the line before it, of one (kv head, row block)
+  int g_row, g_blocks, g_unit, g_cum;  // its group's first row, row blocks, first unit, length of the line before it
+  int left_alone, pad[3];               // 1: in no group
+};
+struct PagedGroup {
+  int shared, slot, row, rows;           // keys; whose row of the table names the pages; first row of the batch, query rows per kv head
+  int cum, unit, blocks, pad;
+};
+struct PagedStart {  // where a worker begins
+  int item, which, off, pad;             // sequence or group, its unit, position in the unit
+};
+struct PagedHead {
+  int64_t own_total, own_per, prefix_total, prefix_per;  // lengths of the lines and of their pieces
 };
 
 struct PagedParams {
@@ -46,35 +53,24 @@ struct PagedParams {
   float scale_log2;
   const float* k_scale;  // this layer's [Hkv], or NULL
   const float* v_scale;
-  PagedPlan plan;
+  PagedHead* head;       // the plan
+  PagedSeq* seq;         // [n]
+  PagedGroup* group;     // [groups]
+  PagedStart* own_start; // [own_workers]
+  PagedStart* prefix_start;
   float* own_acc;        // [slots][own_rows][D]
   float2* own_ml;        // [slots][own_rows]: running maximum (log2 domain), sum
   float* prefix_acc;
   float2* prefix_ml;
-  int own_rows, own_blocks, own_ctas;  // rows of a unit, units per (sequence, kv head), CTAs
-  int prefix_rows, prefix_tile, prefix_ctas;
+  int own_rows, own_blocks, own_tile, own_extra, own_min, own_workers;  // rows of a unit, units per (sequence, kv head), keys of
+                         // a tile, what a unit costs beside its tiles, the shortest piece, pieces
+  int prefix_rows, prefix_tile, prefix_extra, prefix_workers;
   uint32_t* status;
 };
 
 __device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
-__device__ __forceinline__ int64_t piece_tiles(int64_t total, int ctas) { return total <= 0 ? 1 : (total + ctas - 1) / ctas; }
-
-// the last i in [0, n) with cum[i] <= x (cum ascending, cum[0] = 0)
-__device__ __forceinline__ int last_at_or_before(const int* cum, int n, int64_t x, int64_t factor) {
-  int lo = 0, hi = n - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if ((int64_t)cum[mid] * factor <= x) lo = mid; else hi = mid - 1;
-  }
-  return lo;
-}
-
-__device__ __forceinline__ int own_first_key(const PagedParams& p, int i) {
-  const int g = p.plan.group[i];
-  return p.groups > 0 && g >= 0 ? p.plan.g_shared[g] : 0;
-}
-__device__ __forceinline__ int own_tiles(int first, int len) {
-  return len > first ? (len + kPagedTile - 1) / kPagedTile - first / kPagedTile : 0;
+__device__ __forceinline__ int own_tiles(const PagedParams& p, int first, int len) {
+  return len > first ? ceil_div(len, p.own_tile) - first / p.own_tile : 0;
 }
 
 // ---- numbers ----------------------------------------------------------------------------------------------------------
@@ -177,62 +173,84 @@ __device__ __forceinline__ void store8(float* to, const uint32_t* x) {
 }
 
 // ---- the units --------------------------------------------------------------------------------------------------------
-// Where a CTA stands on the line of tiles.
+// A worker's walk along its line.
 struct PagedUnit {
-  int index;        // names the slot, together with the CTA
+  int index;        // names the slot, together with the worker
   int head, row0, rows;   // rows row0 .. row0 + rows of the unit's sequence or group
   int first_row;    // batch row of the sequence, or the group's first
   int table_slot;   // whose row of the table names the pages
   int key_lo, key_hi;     // keys that are this unit's
   int key_all;      // own units: keys from here on are hidden from some rows
-  int tile, tile_end;     // tiles (64 keys, counted from key 0) that this CTA takes
+  int tile, tile_end;     // tiles (counted from key 0) that this worker takes; none, when its piece only has the unit's beginning
 };
 
 template <bool kPrefix>
-__device__ __forceinline__ int64_t line_total(const PagedParams& p) {
-  return kPrefix ? (int64_t)p.plan.g_cum[p.groups] : (int64_t)p.plan.own_cum[p.n] * p.c.heads * p.own_blocks;
-}
+struct PagedWalk {
+  int64_t left;     // positions of the line to go
+  int item, which, off;
+  int a0, a1, a2, a3, b0, b1, b2;  // the item's record
 
-// the unit at position `at` of the line, cut at `end`
-template <bool kPrefix>
-__device__ __forceinline__ PagedUnit unit_at(const PagedParams& p, int64_t at, int64_t end) {
-  PagedUnit u;
-  if constexpr (kPrefix) {
-    const int g = last_at_or_before(p.plan.g_cum, p.groups, at, 1);
-    u.key_lo = 0, u.key_hi = u.key_all = p.plan.g_shared[g];
-    const int tiles = ceil_div(u.key_hi, p.prefix_tile);
-    const int lo = max(p.offsets[g], 0), hi = min(p.offsets[g + 1], p.n);
-    const int blocks = ceil_div((hi - lo) * p.R, p.prefix_rows);
-    const int64_t off = at - p.plan.g_cum[g];
-    const int which = (int)(off / tiles);
-    u.tile = (int)(off % tiles);
-    u.tile_end = (int)min((int64_t)tiles, u.tile + (end - at));
-    u.index = p.plan.g_unit[g] + which;
-    u.head = which / blocks;
-    u.row0 = (which % blocks) * p.prefix_rows;
-    u.rows = min(p.prefix_rows, (hi - lo) * p.R - u.row0);
-    u.first_row = lo;
-    u.table_slot = p.plan.slot[p.plan.g_first[g]];
-  } else {
-    const int per = p.c.heads * p.own_blocks;
-    const int i = last_at_or_before(p.plan.own_cum, p.n, at, per);
-    u.key_lo = own_first_key(p, i), u.key_hi = p.plan.len[i];
-    u.key_all = max(u.key_lo, u.key_hi - (p.T - 1));
-    const int tiles = own_tiles(u.key_lo, u.key_hi), skip = u.key_lo / kPagedTile;
-    const int64_t off = at - (int64_t)p.plan.own_cum[i] * per;
-    const int which = (int)(off / tiles);
-    const int t = (int)(off % tiles);
-    u.tile = skip + t;
-    u.tile_end = skip + (int)min((int64_t)tiles, t + (end - at));
-    u.index = i * per + which;
-    u.head = which / p.own_blocks;
-    u.row0 = (which % p.own_blocks) * p.own_rows;
-    u.rows = min(p.own_rows, p.R - u.row0);
-    u.first_row = i;
-    u.table_slot = p.plan.slot[i];
+  __device__ __forceinline__ void load(const PagedParams& p) {
+    const int4* r = kPrefix ? reinterpret_cast<const int4*>(p.group + item) : reinterpret_cast<const int4*>(p.seq + item);
+    const int4 a = r[0];
+    a0 = a.x, a1 = a.y, a2 = a.z, a3 = a.w;
+    if constexpr (kPrefix) {
+      const int4 b = r[1];
+      b0 = b.x, b1 = b.y, b2 = b.z;
+    }
   }
-  return u;
-}
+  __device__ __forceinline__ void start(const PagedParams& p, int worker) {
+    const int64_t total = kPrefix ? p.head->prefix_total : p.head->own_total, per = kPrefix ? p.head->prefix_per : p.head->own_per;
+    const int4 s = *reinterpret_cast<const int4*>((kPrefix ? p.prefix_start : p.own_start) + worker);
+    left = min(per, total - worker * per);
+    item = s.x, which = s.y, off = s.z;
+    if (left > 0) load(p);
+  }
+  __device__ __forceinline__ int tiles(const PagedParams& p) const { return kPrefix ? ceil_div(a0, p.prefix_tile) : own_tiles(p, a2, a1); }
+  __device__ __forceinline__ bool done() const { return left <= 0; }
+
+  // the unit at hand; then the walk stands at the next one
+  __device__ __forceinline__ PagedUnit next(const PagedParams& p) {
+    PagedUnit u;
+    const int n_tiles = tiles(p), extra = kPrefix ? p.prefix_extra : p.own_extra, length = n_tiles + extra;
+    const int upto = (int)min((int64_t)length, off + left);
+    u.tile = max(off - extra, 0);
+    u.tile_end = max(upto - extra, 0);
+    int units;
+    if constexpr (kPrefix) {
+      units = p.c.heads * b2;
+      u.key_lo = 0, u.key_hi = u.key_all = a0;
+      u.index = b1 + which;
+      u.head = which / b2;
+      u.row0 = (which - u.head * b2) * p.prefix_rows;
+      u.rows = min(p.prefix_rows, a3 - u.row0);
+      u.first_row = a2;
+      u.table_slot = a1;
+    } else {
+      units = p.c.heads * p.own_blocks;
+      u.key_lo = a2, u.key_hi = a1;
+      u.key_all = max(a2, a1 - (p.T - 1));
+      const int skip = a2 / p.own_tile;
+      u.tile += skip, u.tile_end += skip;
+      u.index = item * units + which;
+      u.head = which / p.own_blocks;
+      u.row0 = (which - u.head * p.own_blocks) * p.own_rows;
+      u.rows = min(p.own_rows, p.R - u.row0);
+      u.first_row = item;
+      u.table_slot = a0;
+    }
+    left -= upto - off;
+    off = 0;
+    if (left > 0 && ++which == units) {
+      which = 0;
+      do {  // the line goes on, so there is another item with tiles
+        ++item;
+        load(p);
+      } while (tiles(p) == 0);
+    }
+    return u;
+  }
+};
 
 // a row of a unit: batch row, token and query head
 struct PagedRow {

@@ -45,13 +45,14 @@ struct PrefixSmem {
   static constexpr int kSub = 128 * 128;                 // 128 rows of 64 values
   static constexpr int kTile = D / 64 * kSub;            // K or V of 128 keys, or 128 query rows
   static constexpr int kRawTile = 128 * D;
-  static constexpr int kRoom = 224 * 1024 - (kWide ? 2 : 1) * kTile;
+  // without E4M3 tiles to turn, a narrow CTA leaves room for one of the own units beside it
+  static constexpr int kRoom = (kWide || kE4M3 ? 224 : 128) * 1024 - (kWide ? 2 : 1) * kTile;
   static constexpr int kRaw = kE4M3 ? 4 : 0;
   static constexpr int kRing = (kRoom - kRaw * kRawTile) / kTile > 8 ? 8 : (kRoom - kRaw * kRawTile) / kTile;
   alignas(1024) uint8_t q[kWide ? 2 : 1][kTile];
   uint8_t ring[kRing][kTile];
   uint8_t raw[kRaw ? kRaw : 1][kRaw ? kRawTile : 16];
-  float2 ml[2][128];
+  float2 ml[kWide ? 1 : 128];
   uint64_t q_full, q_free, full[kRing], empty[kRing], raw_full[kRaw ? kRaw : 1], raw_empty[kRaw ? kRaw : 1], s_full[2], p_ready[2], o_done[2], drained;
   uint32_t tmem_base;
   volatile uint32_t abort_flag;
@@ -68,8 +69,80 @@ __device__ __forceinline__ int v_at(int t, int nt) {
   return kWide ? 2 * t + 1 : (t == nt - 1 ? 2 * nt - 1 : 2 * t + 2);
 }
 
+// Threads of a CTA: eight warps of softmax, one for pages, one for products, four that turn E4M3 codes.  A narrow 16-bit CTA
+// is held to 96 registers (the bound of 576 threads), so that a CTA of own units with up to 224 fits beside it in
+// each quarter of the SM (3 x 96 + 224 = 512).
+__host__ __device__ constexpr int prefix_threads(bool e4m3) { return e4m3 ? 448 : 320; }
+__host__ __device__ constexpr int prefix_bound(bool e4m3, bool wide) { return e4m3 || wide ? prefix_threads(e4m3) : 576; }
+
+// The accumulator of a row scaled where it lies, behind the product that last added to it.
+template <int D, typename Smem>
+__device__ __forceinline__ void rescale_o(uint32_t to, float f, Smem& s, int w, int steps, uint32_t* status) {
+  mbar_wait_warp(&s.o_done[w], (uint32_t)(steps - 1) & 1u, &s.abort_flag, status, 19);
+  tc_fence_after();
+#pragma unroll 1
+  for (int c = 0; c < D; c += 32) {
+    uint32_t o[32];
+    tmem_ld32(to + c, o);
+    tmem_ld_wait(o);
+#pragma unroll
+    for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+    tmem_st32(to + c, o);
+  }
+  tmem_st_wait();
+}
+
+// A tile of 128 keys that are all there.  Two passes over the scores in TMEM, 32 columns at a time, the next 32 on their way
+// while these are worked on (all 128 in registers at once do not fit beside the rest of the row's state).
+template <int D, typename Mma, typename Smem>
+__device__ __forceinline__ void softmax_tile(uint32_t ts, uint32_t to, float scale, float& m, float& l, bool first, Smem& s, int w, int steps,
+                                             uint32_t* status) {
+  uint32_t a[2][32];
+  tmem_ld32(ts, a[0]);
+  float t0 = -INFINITY, t1 = -INFINITY;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    tmem_ld_wait(a[c & 1]);
+    tmem_ld32(ts + ((c + 1) & 3) * 32, a[(c + 1) & 1]);  // the last one: the first of the second pass
+#pragma unroll
+    for (int j = 0; j < 32; j += 4) {
+      t0 = max3(t0, __uint_as_float(a[c & 1][j]), __uint_as_float(a[c & 1][j + 1]));
+      t1 = max3(t1, __uint_as_float(a[c & 1][j + 2]), __uint_as_float(a[c & 1][j + 3]));
+    }
+  }
+  const float top = fmaxf(t0, t1) * scale;
+  if (__any_sync(0xffffffffu, top > m + 8.f)) {
+    const float next = fmaxf(m, top), f = next == -INFINITY ? 1.f : paged_ex2(m - next);
+    m = next;
+    l *= f;
+    if (!first) rescale_o<D>(to, f, s, w, steps, status);
+  }
+  const float shift = m == -INFINITY ? 0.f : -m;
+  const uint64_t scale2 = pack2(scale, scale), shift2 = pack2(shift, shift);
+  uint64_t sum0 = pack2(0.f, 0.f), sum1 = sum0;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    uint32_t out[16];
+    tmem_ld_wait(a[c & 1]);
+    if (c < 3) tmem_ld32(ts + (c + 1) * 32, a[(c + 1) & 1]);
+#pragma unroll
+    for (int j = 0; j < 32; j += 2) {
+      float e0, e1;
+      unpack2(fma2(pack2u(a[c & 1][j], a[c & 1][j + 1]), scale2, shift2), e0, e1);
+      e0 = paged_ex2(e0), e1 = paged_ex2(e1);
+      if (j & 2) sum1 = add2(sum1, pack2(e0, e1)); else sum0 = add2(sum0, pack2(e0, e1));
+      out[j / 2] = pack16(e0, e1, Mma{});
+    }
+    tmem_st16(ts + c * 16, out);  // over scores that have been read: chunk c lies at or below column 16 (c + 1)
+  }
+  tmem_st_wait();
+  float s0, s1;
+  unpack2(add2(sum0, sum1), s0, s1);
+  l += s0 + s1;
+}
+
 template <int D, bool kE4M3, typename QT, bool kWide>
-__global__ void __launch_bounds__(kE4M3 ? 448 : 320, 1) attn_prefix_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_k,
+__global__ void __launch_bounds__(prefix_bound(kE4M3, kWide), 1) attn_prefix_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_k,
                                                                            const __grid_constant__ CUtensorMap map_v) {
   using Smem = PrefixSmem<D, kE4M3, kWide>;
   using Mma = typename std::conditional<kE4M3, TagF16, QT>::type;
@@ -100,22 +173,24 @@ __global__ void __launch_bounds__(kE4M3 ? 448 : 320, 1) attn_prefix_kernel(const
   const uint32_t tmem = s.tmem_base;
   pdl_wait();
   pdl_trigger();
-  const int64_t total = line_total<true>(p), per_cta = piece_tiles(total, p.prefix_ctas);
-  const int64_t begin = blockIdx.x * per_cta, end = aligned ? min(total, begin + per_cta) : begin;
+  PagedWalk<true> walk;
+  walk.start(p, blockIdx.x);
+  if (!aligned) walk.left = 0;
   if (!aligned && threadIdx.x == 0) p.status[1] = 98u, p.status[0] = 1u;
 
   if (warp == 8) {  // ---- pages
-    const int box_tokens = min(p.c.page_tokens, kPagedTile), boxes = kPrefixTile / box_tokens;
+    const int box_tokens = min(p.c.page_tokens, kPagedBox), boxes = kPrefixTile / box_tokens;
     constexpr int kBytes = kE4M3 ? 1 : 2, kBoxBytes = D * kBytes < 128 ? D * kBytes : 128, kBoxes = D * kBytes / kBoxBytes;
     constexpr int kSlots = kE4M3 ? kRaw : kRing;
     uint64_t* full = kE4M3 ? s.raw_full : s.full;
     uint64_t* empty = kE4M3 ? s.raw_empty : s.empty;
     int slot = 0, issued = 0;
     uint32_t parity = 1u;
-    for (int64_t at = begin; at < end;) {
-      const PagedUnit u = unit_at<true>(p, at, end);
+    while (!walk.done()) {
+      const PagedUnit u = walk.next(p);
       const int32_t* row = p.c.table + u.table_slot * p.c.table_stride;
       const int nt = u.tile_end - u.tile;
+      if (nt == 0) continue;
       for (int x = 0; x < 2 * nt; ++x) {
         bool is_v;
         int t;
@@ -141,7 +216,6 @@ __global__ void __launch_bounds__(kE4M3 ? 448 : 320, 1) attn_prefix_kernel(const
         ++issued;
         if (++slot == kSlots) slot = 0, parity ^= 1u;
       }
-      at += nt;
     }
     if (s.abort_flag)  // copies in flight land before the CTA leaves
       for (int k = max(0, issued - kSlots); k < issued; ++k) mbar_wait_teardown(&full[k % kSlots], (uint32_t)(k / kSlots) & 1u);
@@ -150,9 +224,10 @@ __global__ void __launch_bounds__(kE4M3 ? 448 : 320, 1) attn_prefix_kernel(const
       int base = 0, units = 0, steps[2] = {0, 0};
       bool ok = true;
       auto wait_full = [&](int x) { ok = mbar_wait(&s.full[(base + x) % kRing], (uint32_t)((base + x) / kRing) & 1u, &s.abort_flag, p.status, 12) && ok; };
-      for (int64_t at = begin; at < end;) {
-        const PagedUnit u = unit_at<true>(p, at, end);
+      while (!walk.done()) {
+        const PagedUnit u = walk.next(p);
         const int nt = u.tile_end - u.tile;
+        if (nt == 0) continue;
         const int halves = kWide ? (u.rows > 128 ? 2 : 1) : (nt > 1 ? 2 : 1);
         auto keys_of = [&](int t) { return min(kPrefixTile, u.key_hi - (u.tile + t) * kPrefixTile); };
         auto scores = [&](int w, int t) {  // S of half w = Q . K(t)
@@ -214,7 +289,6 @@ __global__ void __launch_bounds__(kE4M3 ? 448 : 320, 1) attn_prefix_kernel(const
           }
         }
         base += 2 * nt;
-        at += nt;
       }
       mma_commit(&s.drained);
       mbar_wait_teardown(&s.drained, 0u);
@@ -224,21 +298,28 @@ __global__ void __launch_bounds__(kE4M3 ? 448 : 320, 1) attn_prefix_kernel(const
     const int w = warp - 10, tid = w * 32 + lane;
     constexpr int kChunks = D / 16, kRawRow = D;  // 16 codes each
     int n = 0;
-    for (int64_t at = begin; at < end;) {
-      const PagedUnit u = unit_at<true>(p, at, end);
+    while (!walk.done()) {
+      const PagedUnit u = walk.next(p);
       const int nt = u.tile_end - u.tile;
+      if (nt == 0) continue;
       for (int x = 0; x < 2 * nt; ++x, ++n) {
         const int raw = n % kRaw, slot = n % kRing;
         mbar_wait_warp(&s.raw_full[raw], (uint32_t)(n / kRaw) & 1u, &s.abort_flag, p.status, 15);
         mbar_wait_warp(&s.empty[slot], ((uint32_t)(n / kRing) & 1u) ^ 1u, &s.abort_flag, p.status, 16);
-#pragma unroll 4
-        for (int i = tid; i < 128 * kChunks; i += 128) {
-          const uint32_t row = i / kChunks, c = i % kChunks;
-          const uint4 x16 = *reinterpret_cast<const uint4*>(s.raw[raw] + swizzled_offset(row, c * 16, kRawRow));
-          const uint32_t in[4] = {x16.x, x16.y, x16.z, x16.w};
+        // eight chunks per thread (four for D = 64), all read before the first is written
+        uint4 in[kChunks];
+#pragma unroll
+        for (int i = 0; i < kChunks; ++i) {
+          const uint32_t at = tid + i * 128;
+          in[i] = *reinterpret_cast<const uint4*>(s.raw[raw] + swizzled_offset(at / kChunks, (at % kChunks) * 16, kRawRow));
+        }
+#pragma unroll
+        for (int i = 0; i < kChunks; ++i) {
+          const uint32_t at = tid + i * 128, row = at / kChunks, c = at % kChunks;
+          const uint32_t x[4] = {in[i].x, in[i].y, in[i].z, in[i].w};
           uint32_t out[8];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) out[2 * e] = e4m3x2_to_f16x2(in[e]), out[2 * e + 1] = e4m3x2_to_f16x2(in[e] >> 16);
+          for (int e = 0; e < 4; ++e) out[2 * e] = e4m3x2_to_f16x2(x[e]), out[2 * e + 1] = e4m3x2_to_f16x2(x[e] >> 16);
           uint8_t* sub = s.ring[slot] + (c >> 2) * kSub;
           *reinterpret_cast<uint4*>(sub + swizzled_offset(row, (c & 3) * 32, 128)) = make_uint4(out[0], out[1], out[2], out[3]);
           *reinterpret_cast<uint4*>(sub + swizzled_offset(row, (c & 3) * 32 + 16, 128)) = make_uint4(out[4], out[5], out[6], out[7]);
@@ -247,16 +328,16 @@ __global__ void __launch_bounds__(kE4M3 ? 448 : 320, 1) attn_prefix_kernel(const
         mbar_arrive_warp(&s.full[slot]);
         mbar_arrive_warp(&s.raw_empty[raw]);
       }
-      at += nt;
     }
   } else if (warp < 8) {  // ---- softmax: thread = row
     const int w = warp >> 2, r = threadIdx.x & 127;
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // this warp's quarter of the lanes
     const uint32_t ts = tmem + lanes + w * 128, to = tmem + lanes + kColO + w * 128;
     int units = 0, steps = 0, other_steps = 0;  // tiles that this half, and the other, have done
-    for (int64_t at = begin; at < end;) {
-      const PagedUnit u = unit_at<true>(p, at, end);
+    while (!walk.done()) {
+      const PagedUnit u = walk.next(p);
       const int nt = u.tile_end - u.tile;
+      if (nt == 0) continue;
       const int row = (kWide ? w * 128 : 0) + r;
       const bool there = row < u.rows, active = (kWide ? w * 128 : 0) + (warp & 3) * 32 < u.rows;
       const bool half_there = kWide ? w * 128 < u.rows : w < nt;
@@ -286,6 +367,13 @@ __global__ void __launch_bounds__(kE4M3 ? 448 : 320, 1) attn_prefix_kernel(const
           mbar_wait_warp(&s.s_full[w], (uint32_t)steps & 1u, &s.abort_flag, p.status, 18);
           tc_fence_after();
           if (active) {
+            if (keys == kPrefixTile) {
+              softmax_tile<D, Mma>(ts, to, scale, m, l, t < (kWide ? 1 : 2), s, w, steps, p.status);
+              tc_fence_before();
+              mbar_arrive_warp(&s.p_ready[w]);
+              ++steps;
+              continue;
+            }
             float top = -INFINITY;
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
@@ -318,20 +406,7 @@ __global__ void __launch_bounds__(kE4M3 ? 448 : 320, 1) attn_prefix_kernel(const
               const bool first = t < (kWide ? 1 : 2);
               m = next;
               l *= f;
-              if (!first) {
-                mbar_wait_warp(&s.o_done[w], (uint32_t)(steps - 1) & 1u, &s.abort_flag, p.status, 19);
-                tc_fence_after();
-#pragma unroll 1
-                for (int c = 0; c < D; c += 32) {
-                  uint32_t o[32];
-                  tmem_ld32(to + c, o);
-                  tmem_ld_wait(o);
-#pragma unroll
-                  for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
-                  tmem_st32(to + c, o);
-                }
-                tmem_st_wait();
-              }
+              if (!first) rescale_o<D>(to, f, s, w, steps, p.status);
             }
             const float shift = m == -INFINITY ? 0.f : -m;
             const uint64_t scale2 = pack2(scale, scale), shift2 = pack2(shift, shift);
@@ -389,10 +464,13 @@ __global__ void __launch_bounds__(kE4M3 ? 448 : 320, 1) attn_prefix_kernel(const
         }
       } else {
         // both halves hold sums of the same rows: each joins one half of the columns
-        s.ml[w][r] = make_float2(m, l);
         other_steps += w == 0 ? nt / 2 : (nt + 1) / 2;
+        if (w == 0) s.ml[r] = make_float2(m, l);
         asm volatile("bar.sync 1, 256;" ::: "memory");
-        const float2 x = s.ml[w ^ 1][r];
+        float2 x;
+        if (w == 1) x = s.ml[r], s.ml[r] = make_float2(m, l);
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        if (w == 0) x = s.ml[r];
         const bool both = nt > 1;
         if (w < nt) mbar_wait_warp(&s.o_done[w], (uint32_t)(steps - 1) & 1u, &s.abort_flag, p.status, 21);
         if (w != 0 || both) mbar_wait_warp(&s.o_done[w ^ 1], (uint32_t)(other_steps - 1) & 1u, &s.abort_flag, p.status, 22);
@@ -403,24 +481,21 @@ __global__ void __launch_bounds__(kE4M3 ? 448 : 320, 1) attn_prefix_kernel(const
           const float f0 = w == 0 ? mine : theirs, f1 = w == 0 ? theirs : mine;
           const uint32_t t0 = tmem + lanes + kColO;
 #pragma unroll 1
-          for (int c = w * (D / 2); c < (w + 1) * (D / 2); c += 32) {
-            uint32_t a[32], b[32];
-            tmem_ld32(t0 + c, a);
-            if (both) tmem_ld32(t0 + 128 + c, b);
-            tmem_ld_wait(a);
-            if (both) tmem_ld_wait(b);
+          for (int c = w * (D / 2); c < (w + 1) * (D / 2); c += 16) {
+            uint32_t a[16], b[16];
+            tmem_ld16(t0 + c, a);
+            if (both) tmem_ld16(t0 + 128 + c, b);
+            tmem_ld_wait16(a);
+            if (both) tmem_ld_wait16(b);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) a[j] = __float_as_uint(__uint_as_float(a[j]) * f0 + (both ? __uint_as_float(b[j]) * f1 : 0.f));
-            if (there)
-#pragma unroll
-              for (int j = 0; j < 32; j += 8) store8(out + c + j, a + j);
+            for (int j = 0; j < 16; ++j) a[j] = __float_as_uint(__uint_as_float(a[j]) * f0 + (both ? __uint_as_float(b[j]) * f1 : 0.f));
+            if (there) store8(out + c, a), store8(out + c + 8, a + 8);
           }
           if (there && w == 0) p.prefix_ml[slot * p.prefix_rows + row] = make_float2(top, l * mine + x.y * theirs);
         }
         tc_fence_before();
         asm volatile("bar.sync 1, 256;" ::: "memory");  // O and ml are free for the next unit
       }
-      at += nt;
     }
   }
   tc_fence_before();
@@ -435,8 +510,9 @@ static int launch_prefix_of(const PagedParams& p, const CUtensorMap& mk, const C
   constexpr int smem = (int)sizeof(PrefixSmem<D, kE4M3, kWide>);
   static_assert(smem <= 227 * 1024, "shared memory of one CTA");
   static_assert(PrefixSmem<D, kE4M3, kWide>::kRing >= 3, "two tiles under way and one on its way");
-  FA4B_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  FA4B_CUDA(launch_overlapped(kernel, p.prefix_ctas, kE4M3 ? 448 : 320, smem, st, p, mk, mv));
+  static std::atomic<uint64_t> allowed{0};
+  if (int s = allow_smem(kernel, smem, allowed)) return s;
+  FA4B_CUDA(launch_overlapped(kernel, p.prefix_workers, prefix_threads(kE4M3), smem, st, p, mk, mv));
   return FA4B_OK;
 }
 

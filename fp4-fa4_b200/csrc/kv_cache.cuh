@@ -3,6 +3,7 @@
 #include "common.cuh"
 
 #include <algorithm>
+#include <atomic>
 #include <utility>
 
 namespace fa4b {
@@ -46,6 +47,19 @@ cudaError_t launch_overlapped(void (*kernel)(P...), dim3 grid, dim3 block, size_
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(std::forward<A>(args))...);
+}
+
+// Dynamic shared memory above 48 KB is allowed once per kernel and device; one `done` for each kernel.
+template <typename K>
+int allow_smem(K kernel, int bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  FA4B_CUDA(cudaGetDevice(&dev));
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (done.load(std::memory_order_acquire) & bit) return FA4B_OK;
+  FA4B_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  FA4B_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));  // CTAs of two launches share an SM
+  done.fetch_or(bit, std::memory_order_release);
+  return FA4B_OK;
 }
 
 }  // namespace fa4b

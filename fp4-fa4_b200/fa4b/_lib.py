@@ -183,26 +183,3 @@ def current_stream() -> int:
     import torch
 
     return torch.cuda.current_stream().cuda_stream
-
-
-class on_device:
-    """The device of a call's tensors as the current one, and its current stream's handle."""
-
-    __slots__ = ("index", "before")
-
-    def __init__(self, device):
-        self.index = device.index
-
-    def __enter__(self) -> int:
-        import torch
-
-        self.before = torch.cuda.current_device()
-        if self.before != self.index:
-            torch.cuda.set_device(self.index)
-        return torch.cuda.current_stream(self.index).cuda_stream
-
-    def __exit__(self, *_):
-        import torch
-
-        if self.before != self.index:
-            torch.cuda.set_device(self.before)

@@ -9,11 +9,17 @@ cache have to be ordered on the device, as they change it."""
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 import torch
 
 from . import _lib
-from ._lib import check, lib, on_device, ptr
+from ._lib import check, lib, ptr
+
+# A decoding step makes several calls of a few microseconds: what one costs on the host counts.  Arguments are packed in one
+# go (native alignment: the layout of the C structs), and a call of the current device takes no device guard.
+_WRITE = struct.Struct("@PP3q3q4iPP")
+_ATTEND = struct.Struct("@P3qP3qP5ifPiPPP")
 
 KV_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float8_e4m3fn: 2}
 
@@ -71,14 +77,28 @@ class PagedKVCache:
         self.k, self.v, self.page_table, self.seq_lens, self.ref_counts = k, v, page_table, seq_lens, ref_counts
         self.k_scale, self.v_scale = k_scale, v_scale
         self.device = k.device
+        self._index = k.device.index
         self._c = _lib.KvCache(ptr(k), ptr(v), k.stride(0), k.stride(1), v.stride(0), v.stride(1), layers, pages, heads, tokens, d,
                                KV_DTYPES[k.dtype], ptr(k_scale), ptr(v_scale), ptr(page_table), page_table.stride(0), page_table.shape[0],
                                page_table.shape[1], ptr(seq_lens), ptr(ref_counts), 0)
-        with on_device(self.device):
-            self._work = torch.zeros((lib().fa4b_kv_workspace_bytes(C.byref(self._c)) + 3) // 4, dtype=torch.int32, device=self.device)
-            self._c.work = ptr(self._work)
-            self._at = C.addressof(self._c)
-            check(lib().fa4b_kv_free(self._at, 0, 0, 0), "PagedKVCache")  # an empty list: the checks of the C side
+        self._at = C.addressof(self._c)
+        self._lib = lib()
+        self._heads, self._d, self._takes = heads, d, (torch.bfloat16, torch.float16) if e4m3 else (k.dtype,)
+        self._ws_bytes: dict = {}
+        self._work = torch.zeros((self._lib.fa4b_kv_workspace_bytes(self._at) + 3) // 4, dtype=torch.int32, device=self.device)
+        self._c.work = ptr(self._work)
+        self._call("fa4b_kv_free", 0, 0)  # an empty list: the checks of the C side
+
+    def _call(self, name: str, *args) -> None:
+        """One C call on the cache's device and that device's current stream."""
+        index = self._index
+        if torch._C._cuda_getDevice() == index:
+            status = getattr(self._lib, name)(self._at, *args, torch._C._cuda_getCurrentRawStream(index))
+        else:
+            with torch.cuda.device(index):
+                status = getattr(self._lib, name)(self._at, *args, torch._C._cuda_getCurrentRawStream(index))
+        if status:
+            check(status, name)
 
     @classmethod
     def empty(cls, num_pages: int, page_tokens: int, n_kv_heads: int, head_dim: int, max_seqs: int, max_pages_per_seq: int, *, n_layers: int = 1,
@@ -96,66 +116,59 @@ class PagedKVCache:
                    k_scale=k_scale, v_scale=v_scale)
 
     # ------------------------------------------------------------------------------------------------ pages
-    def _list(self, t, name: str, like: torch.Tensor | None = None) -> int:
-        _ints(t, name, 1, self.device)
-        if like is not None and t.shape[0] != like.shape[0]:
-            raise ValueError(f"{name} has {t.shape[0]} entries, expected {like.shape[0]}")
+    def _list(self, t, name: str, n: int = -1) -> int:
+        if type(t) is not torch.Tensor or t.dtype is not torch.int32 or t.dim() != 1 or t.get_device() != self._index or not t.is_contiguous():
+            _ints(t, name, 1, self.device)
+        if n >= 0 and t.shape[0] != n:
+            raise ValueError(f"{name} has {t.shape[0]} entries, expected {n}")
         return t.data_ptr()
 
     def free(self, seqs: torch.Tensor) -> None:
         """The slots ``seqs`` give their pages back and are empty then.  Empty slots and repeated ones do no harm."""
-        a = self._list(seqs, "seqs")
-        with on_device(self.device) as stream:
-            check(lib().fa4b_kv_free(self._at, a, seqs.shape[0], stream), "fa4b_kv_free")
+        self._call("fa4b_kv_free", self._list(seqs, "seqs"), seqs.shape[0])
 
     def extend(self, seqs: torch.Tensor, n_new: torch.Tensor) -> None:
         """Slot ``seqs[i]`` grows by ``n_new[i]`` tokens (:meth:`write` fills them) and claims pages for them: the lowest
         free ones, in the order of the list.  All or nothing; :meth:`check_status` tells."""
-        a, b = self._list(seqs, "seqs"), self._list(n_new, "n_new", seqs)
-        with on_device(self.device) as stream:
-            check(lib().fa4b_kv_extend(self._at, a, b, seqs.shape[0], stream), "fa4b_kv_extend")
+        a, n = self._list(seqs, "seqs"), seqs.shape[0]
+        self._call("fa4b_kv_extend", a, self._list(n_new, "n_new", n), n)
 
     def write(self, k: torch.Tensor, v: torch.Tensor, seqs: torch.Tensor, *, n_new: torch.Tensor | None = None, layer: int = 0) -> None:
         """Keys and values ``[n, Hkv, T, D]`` (any batch / head / token strides) of the newest tokens: token ``t < n_new[i]``
         goes to position ``seq_lens[seqs[i]] - n_new[i] + t`` (``n_new`` None: T for every row).  A 16-bit cache takes its
         own type, an E4M3 cache bf16 or f16, divided by the scale, clamped to +-448 and rounded."""
-        c = self._c
-        a = self._list(seqs, "seqs")
-        b = 0 if n_new is None else self._list(n_new, "n_new", seqs)
+        a, n = self._list(seqs, "seqs"), seqs.shape[0]
+        b = 0 if n_new is None else self._list(n_new, "n_new", n)
         for t, name in ((k, "k"), (v, "v")):
-            if not isinstance(t, torch.Tensor) or t.ndim != 4 or t.shape[0] != seqs.shape[0] or t.shape[1] != c.Hkv or t.shape[3] != c.D:
-                raise ValueError(f"{name} must be a [{seqs.shape[0]}, {c.Hkv}, T, {c.D}] tensor")
-            if t.dtype not in (torch.bfloat16, torch.float16) or (c.dtype != 2 and t.dtype != self.k.dtype):
+            if not isinstance(t, torch.Tensor) or t.dim() != 4 or t.shape[0] != n or t.shape[1] != self._heads or t.shape[3] != self._d:
+                raise ValueError(f"{name} must be a [{n}, {self._heads}, T, {self._d}] tensor")
+            if t.dtype not in self._takes:
                 raise TypeError(f"{name} is {t.dtype}, the cache {self.k.dtype}")
-            if t.device != self.device:
+            if t.get_device() != self._index:
                 raise RuntimeError(f"{name} must live on {self.device}, got {t.device}")
             if t.stride(3) != 1:
                 raise ValueError(f"{name} must have a contiguous head dimension")
         if k.shape != v.shape or k.dtype != v.dtype:
             raise ValueError("k and v must be alike")
-        w = _lib.KvWriteArgs(k.data_ptr(), v.data_ptr(), _strides(k), _strides(v), k.shape[2], KV_DTYPES[k.dtype], layer, seqs.shape[0], a, b)
-        with on_device(self.device) as stream:
-            check(lib().fa4b_kv_write(self._at, C.addressof(w), stream), "fa4b_kv_write")
+        args = _WRITE.pack(k.data_ptr(), v.data_ptr(), *_strides(k), *_strides(v), k.shape[2], KV_DTYPES[k.dtype], layer, n, a, b)
+        self._call("fa4b_kv_write", args)
 
     def fork(self, parents: torch.Tensor, children: torch.Tensor) -> None:
         """Slot ``children[i]``, which is empty, becomes a copy of ``parents[i]``: full pages are shared, the page that is
         still being filled is copied.  All or nothing; :meth:`check_status` tells."""
-        a, b = self._list(parents, "parents"), self._list(children, "children", parents)
-        with on_device(self.device) as stream:
-            check(lib().fa4b_kv_fork(self._at, a, b, parents.shape[0], stream), "fa4b_kv_fork")
+        a, n = self._list(parents, "parents"), parents.shape[0]
+        self._call("fa4b_kv_fork", a, self._list(children, "children", n), n)
 
     def copy_pages(self, src: torch.Tensor, dst: torch.Tensor) -> None:
         """Pages ``src[i]`` to pages ``dst[i]`` in every layer; tables and counts stay.  A pair with a negative entry is
         skipped, and one whose pages another pair writes, or whose destination another reads, is left out and reported."""
-        a, b = self._list(src, "src"), self._list(dst, "dst", src)
-        with on_device(self.device) as stream:
-            check(lib().fa4b_kv_copy_pages(self._at, a, b, src.shape[0], stream), "fa4b_kv_copy_pages")
+        a, n = self._list(src, "src"), src.shape[0]
+        self._call("fa4b_kv_copy_pages", a, self._list(dst, "dst", n), n)
 
     def compact(self) -> None:
         """Moves the used pages behind the first ``n`` (``n``: pages in use) to the free ones among them, in order, so
         that the pages in use are ``0..n-1``; tables and counts follow."""
-        with on_device(self.device) as stream:
-            check(lib().fa4b_kv_compact(self._at, stream), "fa4b_kv_compact")
+        self._call("fa4b_kv_compact")
 
     # ------------------------------------------------------------------------------------------------ attention
     def attend(self, q: torch.Tensor, seqs: torch.Tensor | None = None, *, layer: int = 0, group_offsets: torch.Tensor | None = None,
@@ -167,48 +180,51 @@ class PagedKVCache:
         ``group_offsets [groups + 1]``, ``shared_lens [groups]``: rows ``group_offsets[g]`` up to ``group_offsets[g + 1]`` hold
         the same pages for their first ``shared_lens[g]`` tokens (as :meth:`fork` leaves them), which are read once for
         the group; rows in no group are left as they were.  ``out`` receives O when given (any strides)."""
-        c = self._c
-        if not isinstance(q, torch.Tensor) or q.ndim != 4 or q.shape[3] != c.D:
-            raise ValueError(f"q must be a [n, Hq, T, {c.D}] tensor")
-        if q.dtype not in (torch.bfloat16, torch.float16) or (c.dtype != 2 and q.dtype != self.k.dtype):
+        if not isinstance(q, torch.Tensor) or q.dim() != 4 or q.shape[3] != self._d:
+            raise ValueError(f"q must be a [n, Hq, T, {self._d}] tensor")
+        if q.dtype not in self._takes:
             raise TypeError(f"q is {q.dtype}, the cache {self.k.dtype}")
-        if q.device != self.device:
+        if q.get_device() != self._index:
             raise RuntimeError(f"q must live on {self.device}, got {q.device}")
-        n, hq, t, d = q.shape
+        shape = q.shape
+        n, hq, t, _ = shape
         if q.stride(3) != 1:
             raise ValueError("q must have a contiguous head dimension")
         if (group_offsets is None) != (shared_lens is None):
             raise ValueError("group_offsets and shared_lens go together")
-        slots = 0 if seqs is None else self._list(seqs, "seqs")
-        if seqs is not None and seqs.shape[0] != n:
-            raise ValueError(f"seqs has {seqs.shape[0]} entries, q {n} rows")
+        slots = 0 if seqs is None else self._list(seqs, "seqs", n)
         groups = offsets = shared = 0
         if group_offsets is not None:
-            offsets, shared, groups = self._list(group_offsets, "group_offsets"), self._list(shared_lens, "shared_lens"), shared_lens.shape[0]
+            shared, groups = self._list(shared_lens, "shared_lens"), shared_lens.shape[0]
             if group_offsets.shape[0] != groups + 1:
                 raise ValueError(f"group_offsets must have {groups + 1} entries, got {group_offsets.shape[0]}")
-        with on_device(self.device) as stream:
-            if out is None:
-                out = torch.empty(n, hq, t, d, dtype=q.dtype, device=self.device)
-            elif tuple(out.shape) != (n, hq, t, d) or out.dtype != q.dtype or out.device != self.device or out.stride(3) != 1:
-                raise ValueError(f"out must be a {tuple(q.shape)} tensor like q with a contiguous head dimension")
-            lse = torch.empty(n, hq, t, dtype=torch.float32, device=self.device)
-            a = _lib.AttnPagedArgs(q.data_ptr(), _strides(q), out.data_ptr(), _strides(out), lse.data_ptr(), n, t, hq, layer, KV_DTYPES[q.dtype],
-                                   softmax_scale or 0.0, slots, groups, offsets, shared, 0)
-            at = C.addressof(a)
-            need = lib().fa4b_attn_paged_workspace_bytes(self._at, at)
-            ws = torch.empty(need + 256, dtype=torch.uint8, device=self.device)
-            a.ws = (ws.data_ptr() + 255) & ~255
-            check(lib().fa4b_attn_paged_fwd(self._at, at, stream), "fa4b_attn_paged_fwd")
+            offsets = self._list(group_offsets, "group_offsets")
+        if out is None:
+            out = torch.empty(shape, dtype=q.dtype, device=self.device)
+        elif out.shape != shape or out.dtype != q.dtype or out.device != self.device or out.stride(3) != 1:
+            raise ValueError(f"out must be a {tuple(shape)} tensor like q with a contiguous head dimension")
+        lse = torch.empty((n, hq, t), dtype=torch.float32, device=self.device)
+        code, scale = KV_DTYPES[q.dtype], softmax_scale or 0.0
+        q_strides, o_strides = _strides(q), _strides(out)
+        size = self._ws_bytes.get((n, hq, t, groups))
+        if size is None:
+            args = _ATTEND.pack(q.data_ptr(), *q_strides, out.data_ptr(), *o_strides, lse.data_ptr(), n, t, hq, layer, code, scale, slots, groups, offsets, shared, 0)
+            size = self._lib.fa4b_attn_paged_workspace_bytes(self._at, args)
+            if size:
+                self._ws_bytes[n, hq, t, groups] = size
+        ws = torch.empty(size, dtype=torch.uint8, device=self.device)
+        args = _ATTEND.pack(q.data_ptr(), *q_strides, out.data_ptr(), *o_strides, lse.data_ptr(), n, t, hq, layer, code, scale, slots, groups, offsets, shared,
+                            ws.data_ptr())
+        self._call("fa4b_attn_paged_fwd", args)
         return out, lse
 
     def check_status(self) -> None:
         """Synchronise and raise on what the calls since the last check found wrong on the device (slots out of range, too
         few free pages, ...)."""
-        with on_device(self.device) as stream:
-            check(lib().fa4b_kv_check_status(self._at, stream), "fa4b_kv_check_status")
+        self._call("fa4b_kv_check_status")
 
 
-def _strides(t: torch.Tensor) -> _lib.Strides:
-    # a dimension of one entry carries no stride of its own
-    return _lib.Strides(*(s if n > 1 else 0 for n, s in zip(t.shape[:3], t.stride()[:3])))
+def _strides(t: torch.Tensor) -> tuple:
+    a, b, c, _ = t.shape
+    x, y, z, _ = t.stride()
+    return x if a > 1 else 0, y if b > 1 else 0, z if c > 1 else 0  # a dimension of one entry carries no stride of its own

@@ -108,3 +108,18 @@ def test_attention_over_the_cache_is_refused_before_a_launch():
     got, size, error = call(cache=good(table_width=1 << 18, table_stride=1 << 18, page_tokens=128, k_page_stride=1 << 17, v_page_stride=1 << 17, max_seqs=5000), n=4096)
     assert got == 1 and size == 0 and b"too many" in error
     assert call(cache=good(D=96))[0] == 1
+
+
+def test_packed_arguments_have_the_layout_of_the_structs():
+    from fa4b import kv_cache
+
+    for packed, struct in ((kv_cache._WRITE, _lib.KvWriteArgs), (kv_cache._ATTEND, _lib.AttnPagedArgs)):
+        assert packed.size == C.sizeof(struct)
+        count = len(packed.unpack(bytes(packed.size)))
+        values = tuple(float(i) if i == 14 and struct is _lib.AttnPagedArgs else i + 1 for i in range(count))
+        got = struct.from_buffer_copy(packed.pack(*values))
+        flat = []
+        for name, kind in struct._fields_:
+            x = getattr(got, name)
+            flat += [x.batch, x.head, x.seq] if kind is _lib.Strides else [x]
+        assert tuple(flat) == values
