@@ -4,21 +4,23 @@
 // second product from there.
 //
 // One CTA per SM.  Warps 0-3 and 4-7: softmax, one thread per row, no exchange between threads (kWide: rows 0-127 and
-// 128-255 of the unit, both over every tile; else the same 128 rows, even and odd tiles, joined in TMEM at the end).  While
-// one half exponentiates, the tensor core works for the other.  Warp 8 asks for pages by TMA, warp 9 issues the
-// products.  An E4M3 cache arrives as codes; warps 10-13 turn each tile into f16 (exact) in the operand ring.
+// 128-255 of the unit, both over every key; else the same 128 rows, the first and the last 64 keys of a tile, joined in
+// TMEM at the end).  Either half works in steps of 64 keys on two score buffers of its own: while it exponentiates one,
+// the tensor core fills the other, so that it hardly ever waits (with one buffer of 128 keys per half a step spent as long
+// waiting for P V and the next Q K^T as exponentiating: 282 us instead of @@).  Warp 8 asks for pages by TMA, warps 9 and
+// 10 issue the products of the halves.  An E4M3 cache arrives as codes; warps 11-14 turn each tile into f16 (exact) in the operand ring.
 //
 // A shared part ends on a multiple of 16 keys (the plan sees to it): the last tile's products take N = its keys and K = its
 // keys, so nothing behind them is read and no row needs a mask.
 //
-// TMEM columns: S 0 and 128, O 256 and 384.
+// TMEM columns: S 0 and 64 of the first half, 128 and 192 of the second (P in the lower 32 of each), O 256 and 384.
 #include "attn_paged.cuh"
 
 #include <type_traits>
 
 namespace fa4b {
 
-constexpr int kPrefixTile = 128;
+constexpr int kPrefixTile = 128, kStep = 64;
 
 __device__ __forceinline__ void mma_f16_ss(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
   asm volatile("{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }" ::"r"(d_tmem), "l"(adesc),
@@ -53,32 +55,30 @@ struct PrefixSmem {
   uint8_t ring[kRing][kTile];
   uint8_t raw[kRaw ? kRaw : 1][kRaw ? kRawTile : 16];
   float2 ml[kWide ? 1 : 128];
-  uint64_t q_full, q_free, full[kRing], empty[kRing], raw_full[kRaw ? kRaw : 1], raw_empty[kRaw ? kRaw : 1], s_full[2], p_ready[2], o_done[2], drained;
+  uint64_t q_full, q_free, full[kRing], empty[kRing], raw_full[kRaw ? kRaw : 1], raw_empty[kRaw ? kRaw : 1], s_full[2][2], p_ready[2][2], o_done[2][2], drained;  // [half][score buffer]
   uint32_t tmem_base;
   volatile uint32_t abort_flag;
 };
 
-// Where K and V of tile t of a piece of nt tiles stand in the order of loads, which is the order of use: kWide
-// K0 V0 K1 V1 ..., else (two tiles under way) K0 K1 V0 K2 V1 K3 ... .
+// Keys of step `step` of a half of a piece whose keys end at `keys`, counted from its first tile; 0 behind the last.
 template <bool kWide>
-__device__ __forceinline__ int k_at(int t) {
-  return kWide ? 2 * t : (t == 0 ? 0 : 2 * t - 1);
-}
-template <bool kWide>
-__device__ __forceinline__ int v_at(int t, int nt) {
-  return kWide ? 2 * t + 1 : (t == nt - 1 ? 2 * nt - 1 : 2 * t + 2);
+__device__ __forceinline__ int step_keys(int keys, int half, int step) {
+  const int first = kWide ? step * kStep : step * kPrefixTile + half * kStep;
+  return max(0, min(kStep, keys - first));
 }
 
-// Threads of a CTA: eight warps of softmax, one for pages, one for products, four that turn E4M3 codes.  A narrow 16-bit CTA
+// Threads of a CTA: eight warps of softmax, one for pages, two for products, four that turn E4M3 codes.  A narrow 16-bit CTA
 // is held to 96 registers (the bound of 576 threads), so that a CTA of own units with up to 224 fits beside it in
 // each quarter of the SM (3 x 96 + 224 = 512).
-__host__ __device__ constexpr int prefix_threads(bool e4m3) { return e4m3 ? 448 : 320; }
+__host__ __device__ constexpr int prefix_threads(bool e4m3) { return e4m3 ? 480 : 352; }
 __host__ __device__ constexpr int prefix_bound(bool e4m3, bool wide) { return e4m3 || wide ? prefix_threads(e4m3) : 576; }
 
-// The accumulator of a row scaled where it lies, behind the product that last added to it.
+// The accumulator of a row scaled where it lies, behind the product of the step before (`done`, `parity`).  A barrier of its
+// own for each score buffer: a step's scores are only there when the product of the step before last is, so that a
+// wait is never two phases behind.
 template <int D, typename Smem>
-__device__ __forceinline__ void rescale_o(uint32_t to, float f, Smem& s, int w, int steps, uint32_t* status) {
-  mbar_wait_warp(&s.o_done[w], (uint32_t)(steps - 1) & 1u, &s.abort_flag, status, 19);
+__device__ __forceinline__ void rescale_o(uint32_t to, float f, Smem& s, uint64_t* done, uint32_t parity, uint32_t* status) {
+  mbar_wait_warp(done, parity, &s.abort_flag, status, 19);
   tc_fence_after();
 #pragma unroll 1
   for (int c = 0; c < D; c += 32) {
@@ -92,48 +92,70 @@ __device__ __forceinline__ void rescale_o(uint32_t to, float f, Smem& s, int w, 
   tmem_st_wait();
 }
 
-// A tile of 128 keys that are all there.  Two passes over the scores in TMEM, 32 columns at a time, the next 32 on their way
-// while these are worked on (all 128 in registers at once do not fit beside the rest of the row's state).
-template <int D, typename Mma, typename Smem>
-__device__ __forceinline__ void softmax_tile(uint32_t ts, uint32_t to, float scale, float& m, float& l, bool first, Smem& s, int w, int steps,
-                                             uint32_t* status) {
-  uint32_t a[2][32];
-  tmem_ld32(ts, a[0]);
-  float t0 = -INFINITY, t1 = -INFINITY;
+// One step of a row: scores out of TMEM, probabilities back in as 16-bit.  keys: 16 to 64 in sixteens.  kLean: 32 scores in
+// registers at a time, read once for their maximum and once more to be used.
+template <int D, typename Mma, bool kLean, typename Smem>
+__device__ __forceinline__ void softmax_step(uint32_t ts, uint32_t to, int keys, float scale, float& m, float& l, Smem& s, uint64_t* before,
+                                             uint32_t parity_before, bool first, uint32_t* status) {
+  constexpr int kHeld = kLean ? 1 : 2;
+  uint32_t a[kHeld][32];
+  auto absent = [&](int c, uint32_t (&x)[32]) {  // the rest of the buffer is what an earlier step left
 #pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    tmem_ld_wait(a[c & 1]);
-    tmem_ld32(ts + ((c + 1) & 3) * 32, a[(c + 1) & 1]);  // the last one: the first of the second pass
+    for (int j = 0; j < 32; j += 16)
+      if (keys <= c * 32 + j)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[j + e] = 0xff800000u;
+  };
+  float t0 = -INFINITY, t1 = -INFINITY;
+  if constexpr (!kLean) {
+    tmem_ld32(ts, a[0]);
+    tmem_ld32(ts + 32, a[1]);
+    tmem_ld_wait(a[0]);
+    tmem_ld_wait(a[1]);
+  }
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    uint32_t(&x)[32] = a[kLean ? 0 : c];
+    if constexpr (kLean) {
+      tmem_ld32(ts + c * 32, x);
+      tmem_ld_wait(x);
+    }
+    if (keys < kStep) absent(c, x);
 #pragma unroll
     for (int j = 0; j < 32; j += 4) {
-      t0 = max3(t0, __uint_as_float(a[c & 1][j]), __uint_as_float(a[c & 1][j + 1]));
-      t1 = max3(t1, __uint_as_float(a[c & 1][j + 2]), __uint_as_float(a[c & 1][j + 3]));
+      t0 = max3(t0, __uint_as_float(x[j]), __uint_as_float(x[j + 1]));
+      t1 = max3(t1, __uint_as_float(x[j + 2]), __uint_as_float(x[j + 3]));
     }
   }
   const float top = fmaxf(t0, t1) * scale;
+  // the reference point moves when it has to (see the own units); the accumulator is then scaled where it lies
   if (__any_sync(0xffffffffu, top > m + 8.f)) {
     const float next = fmaxf(m, top), f = next == -INFINITY ? 1.f : paged_ex2(m - next);
     m = next;
     l *= f;
-    if (!first) rescale_o<D>(to, f, s, w, steps, status);
+    if (!first) rescale_o<D>(to, f, s, before, parity_before, status);
   }
   const float shift = m == -INFINITY ? 0.f : -m;
   const uint64_t scale2 = pack2(scale, scale), shift2 = pack2(shift, shift);
   uint64_t sum0 = pack2(0.f, 0.f), sum1 = sum0;
 #pragma unroll
-  for (int c = 0; c < 4; ++c) {
+  for (int c = 0; c < 2; ++c) {
+    uint32_t(&x)[32] = a[kLean ? 0 : c];
+    if constexpr (kLean) {
+      tmem_ld32(ts + c * 32, x);
+      tmem_ld_wait(x);
+    }
     uint32_t out[16];
-    tmem_ld_wait(a[c & 1]);
-    if (c < 3) tmem_ld32(ts + (c + 1) * 32, a[(c + 1) & 1]);
 #pragma unroll
     for (int j = 0; j < 32; j += 2) {
       float e0, e1;
-      unpack2(fma2(pack2u(a[c & 1][j], a[c & 1][j + 1]), scale2, shift2), e0, e1);
+      unpack2(fma2(pack2u(x[j], x[j + 1]), scale2, shift2), e0, e1);
       e0 = paged_ex2(e0), e1 = paged_ex2(e1);
+      if (c * 32 + j >= 16 && keys <= (c * 32 + j) / 16 * 16) e0 = e1 = 0.f;  // not there
       if (j & 2) sum1 = add2(sum1, pack2(e0, e1)); else sum0 = add2(sum0, pack2(e0, e1));
       out[j / 2] = pack16(e0, e1, Mma{});
     }
-    tmem_st16(ts + c * 16, out);  // over scores that have been read: chunk c lies at or below column 16 (c + 1)
+    tmem_st16(ts + c * 16, out);
   }
   tmem_st_wait();
   float s0, s1;
@@ -156,11 +178,13 @@ __global__ void __launch_bounds__(prefix_bound(kE4M3, kWide), 1) attn_prefix_ker
   if (warp == 9) tmem_alloc(&s.tmem_base, 512);
   if (threadIdx.x == 0) {
     mbar_init(&s.q_full, kWide ? 8 : 4);
-    mbar_init(&s.q_free, 1);
-    for (int i = 0; i < kRing; ++i) mbar_init(&s.full[i], kE4M3 ? 4 : 1), mbar_init(&s.empty[i], 1);
+    mbar_init(&s.q_free, 2);
+    for (int i = 0; i < kRing; ++i) mbar_init(&s.full[i], kE4M3 ? 4 : 1), mbar_init(&s.empty[i], 2);
     for (int i = 0; i < kRaw; ++i) mbar_init(&s.raw_full[i], 1), mbar_init(&s.raw_empty[i], 4);
-    for (int i = 0; i < 2; ++i) mbar_init(&s.s_full[i], 1), mbar_init(&s.p_ready[i], 4), mbar_init(&s.o_done[i], 1);
-    mbar_init(&s.drained, 1);
+    for (int i = 0; i < 2; ++i) {
+      for (int j = 0; j < 2; ++j) mbar_init(&s.s_full[i][j], 1), mbar_init(&s.p_ready[i][j], 4), mbar_init(&s.o_done[i][j], 1);
+    }
+    mbar_init(&s.drained, 2);
     s.abort_flag = 0u;
     fence_barrier_init();
     fence_async_smem();
@@ -194,6 +218,8 @@ __global__ void __launch_bounds__(prefix_bound(kE4M3, kWide), 1) attn_prefix_ker
       for (int x = 0; x < 2 * nt; ++x) {
         bool is_v;
         int t;
+        // the order of use: kWide (a tile is two steps, both score buffers) K0 V0 K1 V1 ..., else (a tile is one step, the
+        // buffers hold two tiles) K0 K1 V0 K2 V1 ...
         if constexpr (kWide) is_v = x & 1, t = x >> 1;
         else if (x == 2 * nt - 1) is_v = true, t = nt - 1;
         else if (x == 0) is_v = false, t = 0;
@@ -219,83 +245,111 @@ __global__ void __launch_bounds__(prefix_bound(kE4M3, kWide), 1) attn_prefix_ker
     }
     if (s.abort_flag)  // copies in flight land before the CTA leaves
       for (int k = max(0, issued - kSlots); k < issued; ++k) mbar_wait_teardown(&full[k % kSlots], (uint32_t)(k / kSlots) & 1u);
-  } else if (warp == 9) {  // ---- products
-    if (lane == 0) {
-      int base = 0, units = 0, steps[2] = {0, 0};
-      bool ok = true;
-      auto wait_full = [&](int x) { ok = mbar_wait(&s.full[(base + x) % kRing], (uint32_t)((base + x) / kRing) & 1u, &s.abort_flag, p.status, 12) && ok; };
-      while (!walk.done()) {
-        const PagedUnit u = walk.next(p);
-        const int nt = u.tile_end - u.tile;
-        if (nt == 0) continue;
-        const int halves = kWide ? (u.rows > 128 ? 2 : 1) : (nt > 1 ? 2 : 1);
-        auto keys_of = [&](int t) { return min(kPrefixTile, u.key_hi - (u.tile + t) * kPrefixTile); };
-        auto scores = [&](int w, int t) {  // S of half w = Q . K(t)
-          if (ok) {
-            const uint32_t idesc = idesc_f16(keys_of(t), kIsBf16, 0), qa = smem_u32(s.q[kWide ? w : 0]), ka = smem_u32(s.ring[(base + k_at<kWide>(t)) % kRing]);
+  } else if (warp == 9 || warp == 10) {  // ---- products of the first and of the second half
+    // The warp walks together and one lane issues: what a product takes (descriptors, columns) is then the same in all lanes and
+    // costs an addition each (in a branch of one lane: 60 to 120 cycles an instruction).  One warp for both halves would
+    // spend as long between its products as the tensor core on them.
+    const int w = warp - 9;
+    const bool leader = elect_one();
+    const uint64_t q_desc = make_tile_desc(smem_u32(s.q[kWide ? w : 0]), 128), k_desc = make_tile_desc(smem_u32(s.ring[0]), 128),
+                   v_desc = make_sdesc(smem_u32(s.ring[0]), kSub, 1024, kSwz128);
+    constexpr uint32_t kIdescV = idesc_f16(D, kIsBf16, 1);
+    const uint32_t scol = tmem + w * 128, ocol = tmem + kColO + w * 128;
+    int slot = 0, units = 0;
+    uint32_t parity = 0u, phases = 0u;  // of the ring; of the probabilities that are awaited next, a bit per buffer
+    bool ok = true;
+    auto take = [&]() {  // the next tile of the ring: tiles are used in the order of their loads
+      ok = mbar_wait_warp(&s.full[slot], parity, &s.abort_flag, p.status, 12) && ok;
+      const int got = slot;
+      if (++slot == kRing) slot = 0, parity ^= 1u;
+      return got;
+    };
+    auto commit = [&](uint64_t* bar) {
+      if (leader) mma_commit(bar);
+    };
+    auto scores = [&](int buf, int n, int tile, int row) {  // S = Q . K, n keys from row `row` of a tile
+      const uint32_t idesc = idesc_f16(n, kIsBf16, 0);
+      const uint64_t kd = k_desc + tile * (Smem::kTile >> 4) + row * 8;
+      if (leader) {
+        if (ok)
 #pragma unroll
-            for (int k = 0; k < D / 16; ++k)
-              mma_f16_ss(tmem + w * 128, make_tile_desc(qa + (k >> 2) * kSub + (k & 3) * 32, 128), make_tile_desc(ka + (k >> 2) * kSub + (k & 3) * 32, 128), idesc, k > 0);
-          }
-          mma_commit(&s.s_full[w]);
-        };
-        auto values = [&](int w, int t, bool first) {  // O of half w += P . V(t)
-          ok = mbar_wait(&s.p_ready[w], (uint32_t)steps[w] & 1u, &s.abort_flag, p.status, 13) && ok;
-          ++steps[w];
-          tc_fence_after();
-          if (ok) {
-            const uint32_t idesc = idesc_f16(D, kIsBf16, 1), va = smem_u32(s.ring[(base + v_at<kWide>(t, nt)) % kRing]);
-            const int ks = keys_of(t) / 16;
-            for (int k = 0; k < ks; ++k)
-              mma_f16_ts(tmem + kColO + w * 128, tmem + w * 128 + k * 8, make_sdesc(va + k * 2048, kSub, 1024, kSwz128), idesc, !(first && k == 0));
-          }
-          mma_commit(&s.o_done[w]);
-        };
-        auto release = [&](int x) { mma_commit(&s.empty[(base + x) % kRing]); };
-        ok = mbar_wait(&s.q_full, (uint32_t)units & 1u, &s.abort_flag, p.status, 14) && ok;
-        ++units;
-        if constexpr (kWide) {
-          wait_full(0);
-          for (int w = 0; w < halves; ++w) scores(w, 0);
-          release(0);
-          for (int t = 0; t < nt; ++t) {
-            wait_full(v_at<true>(t, nt));
-            if (t + 1 < nt) wait_full(k_at<true>(t + 1));
-            for (int w = 0; w < halves; ++w) {
-              values(w, t, t == 0);
-              if (t + 1 < nt) scores(w, t + 1);
-            }
-            release(v_at<true>(t, nt));
-            if (t + 1 < nt) release(k_at<true>(t + 1));
-            if (t == max(nt - 2, 0)) mma_commit(&s.q_free);  // the last scores of the unit have been issued
-          }
-        } else {
-          for (int t = 0; t < halves; ++t) {
-            wait_full(k_at<false>(t));
-            scores(t, t);
-            release(k_at<false>(t));
-          }
-          if (nt <= 2) mma_commit(&s.q_free);
-          for (int t = 0; t < nt; ++t) {
-            wait_full(v_at<false>(t, nt));
-            values(t & 1, t, t < 2);
-            release(v_at<false>(t, nt));
-            if (t + 2 < nt) {
-              wait_full(k_at<false>(t + 2));
-              scores(t & 1, t + 2);
-              release(k_at<false>(t + 2));
-              if (t + 3 == nt) mma_commit(&s.q_free);
-            }
+          for (int k = 0; k < D / 16; ++k)
+            mma_f16_ss(scol + buf * kStep, q_desc + ((k >> 2) * kSub + (k & 3) * 32) / 16, kd + ((k >> 2) * kSub + (k & 3) * 32) / 16, idesc, k > 0);
+        mma_commit(&s.s_full[w][buf]);
+      }
+    };
+    auto values = [&](int buf, int n, int tile, int row, bool first) {  // O += P . V
+      const uint64_t vd = v_desc + tile * (Smem::kTile >> 4) + row * 8;
+      const uint32_t pcol = scol + buf * kStep;
+      ok = mbar_wait_warp(&s.p_ready[w][buf], phases >> buf & 1u, &s.abort_flag, p.status, 13) && ok;
+      phases ^= 1u << buf;
+      tc_fence_after();
+      if (leader) {
+        if (ok) {
+          mma_f16_ts(ocol, pcol, vd, kIdescV, !first);
+          if (n == kStep) {
+#pragma unroll
+            for (int k = 1; k < kStep / 16; ++k) mma_f16_ts(ocol, pcol + k * 8, vd + k * 128, kIdescV, 1);
+          } else {
+            for (int k = 1; k < n / 16; ++k) mma_f16_ts(ocol, pcol + k * 8, vd + k * 128, kIdescV, 1);
           }
         }
-        base += 2 * nt;
+        mma_commit(&s.o_done[w][buf]);
       }
-      mma_commit(&s.drained);
-      mbar_wait_teardown(&s.drained, 0u);
+    };
+    while (!walk.done()) {
+      const PagedUnit u = walk.next(p);
+      const int nt = u.tile_end - u.tile;
+      if (nt == 0) continue;
+      const int piece = kWide && w * 128 >= u.rows ? 0 : min(u.key_hi - u.tile * kPrefixTile, nt * kPrefixTile);  // keys; a half without rows takes none
+      ok = mbar_wait_warp(&s.q_full, (uint32_t)units & 1u, &s.abort_flag, p.status, 14) && ok;
+      ++units;
+      if constexpr (kWide) {
+        auto keys = [&](int step) { return min(kStep, piece - step * kStep); };
+        int tile = take();
+        if (keys(0) > 0) scores(0, keys(0), tile, 0);
+        if (keys(1) > 0) scores(1, keys(1), tile, kStep);
+        commit(&s.empty[tile]);
+        if (nt == 1) commit(&s.q_free);
+        for (int t = 0; t < nt; ++t) {
+          const int v = take();
+          const bool more = t + 1 < nt;
+          if (keys(2 * t) > 0) values(0, keys(2 * t), v, 0, t == 0);
+          if (more) tile = take();
+          if (more && keys(2 * t + 2) > 0) scores(0, keys(2 * t + 2), tile, 0);
+          if (keys(2 * t + 1) > 0) values(1, keys(2 * t + 1), v, kStep, false);
+          commit(&s.empty[v]);
+          if (more) {
+            if (keys(2 * t + 3) > 0) scores(1, keys(2 * t + 3), tile, kStep);
+            commit(&s.empty[tile]);
+            if (t + 2 == nt) commit(&s.q_free);  // the last scores of the unit have been issued
+          }
+        }
+      } else {
+        auto keys = [&](int t) { return min(kStep, piece - t * kPrefixTile - w * kStep); };
+        for (int t = 0; t < min(nt, 2); ++t) {
+          const int tile = take();
+          if (keys(t) > 0) scores(t, keys(t), tile, w * kStep);
+          commit(&s.empty[tile]);
+        }
+        if (nt <= 2) commit(&s.q_free);
+        for (int t = 0; t < nt; ++t) {
+          const int v = take();
+          if (keys(t) > 0) values(t & 1, keys(t), v, w * kStep, t == 0);
+          commit(&s.empty[v]);
+          if (t + 2 < nt) {
+            const int tile = take();
+            if (keys(t + 2) > 0) scores(t & 1, keys(t + 2), tile, w * kStep);
+            commit(&s.empty[tile]);
+            if (t + 3 == nt) commit(&s.q_free);
+          }
+        }
+      }
     }
-    __syncwarp();
-  } else if (kE4M3 && warp >= 10) {  // ---- codes to f16
-    const int w = warp - 10, tid = w * 32 + lane;
+    commit(&s.drained);
+    mbar_wait_teardown(&s.drained, 0u);
+  } else if (kE4M3 && warp >= 11) {  // ---- codes to f16
+    const int w = warp - 11, tid = w * 32 + lane;
     constexpr int kChunks = D / 16, kRawRow = D;  // 16 codes each
     int n = 0;
     while (!walk.done()) {
@@ -333,26 +387,40 @@ __global__ void __launch_bounds__(prefix_bound(kE4M3, kWide), 1) attn_prefix_ker
     const int w = warp >> 2, r = threadIdx.x & 127;
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // this warp's quarter of the lanes
     const uint32_t ts = tmem + lanes + w * 128, to = tmem + lanes + kColO + w * 128;
-    int units = 0, steps = 0, other_steps = 0;  // tiles that this half, and the other, have done
+    int units = 0;
+    uint32_t phases = 0u, other_phases = 0u;  // a bit per buffer, of this half and of the other
     while (!walk.done()) {
       const PagedUnit u = walk.next(p);
       const int nt = u.tile_end - u.tile;
       if (nt == 0) continue;
       const int row = (kWide ? w * 128 : 0) + r;
       const bool there = row < u.rows, active = (kWide ? w * 128 : 0) + (warp & 3) * 32 < u.rows;
-      const bool half_there = kWide ? w * 128 < u.rows : w < nt;
+      const int piece = min(u.key_hi - u.tile * kPrefixTile, nt * kPrefixTile);
+      const int n_steps = kWide ? (w * 128 < u.rows ? (piece + kStep - 1) / kStep : 0) : (piece - w * kStep + kPrefixTile - 1) / kPrefixTile;
       if (units > 0) mbar_wait_warp(&s.q_free, (uint32_t)(units - 1) & 1u, &s.abort_flag, p.status, 17);
       float scale = p.scale_log2;
       if (active) {  // the query row, swizzled into shared memory
         const PagedRow pr = paged_row(p, u, there ? row : 0);
         const uint4* src = reinterpret_cast<const uint4*>(p.q + 2 * (pr.i * p.q_sb + pr.h * p.q_sh + pr.t * p.q_st));
-        uint4 x[D / 8];
+        uint8_t* dst = s.q[kWide ? w : 0];
+        if constexpr (kE4M3) {
+          uint4 x[D / 8];
 #pragma unroll
-        for (int c = 0; c < D / 8; ++c) x[c] = src[c];
-        if constexpr (kE4M3) scale = e4m3_query_row<QT, D / 8>(x, scale * p.k_scale[u.head]);
-        if (kWide || w == 0) {
+          for (int c = 0; c < D / 8; ++c) x[c] = src[c];
+          scale = e4m3_query_row<QT, D / 8>(x, scale * p.k_scale[u.head]);
+          if (kWide || w == 0) {
 #pragma unroll
-          for (int c = 0; c < D / 8; ++c) *reinterpret_cast<uint4*>(s.q[kWide ? w : 0] + (c >> 3) * kSub + swizzled_offset(r, (c & 7) * 16, 128)) = x[c];
+            for (int c = 0; c < D / 8; ++c) *reinterpret_cast<uint4*>(dst + (c >> 3) * kSub + swizzled_offset(r, (c & 7) * 16, 128)) = x[c];
+          }
+        } else if (kWide || w == 0) {
+#pragma unroll 1
+          for (int c0 = 0; c0 < D / 8; c0 += 8) {
+            uint4 x[8];
+#pragma unroll
+            for (int c = 0; c < 8; ++c) x[c] = src[c0 + c];
+#pragma unroll
+            for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(dst + (c0 >> 3) * kSub + swizzled_offset(r, c * 16, 128)) = x[c];
+          }
         }
       }
       if (kWide || w == 0) {
@@ -361,92 +429,23 @@ __global__ void __launch_bounds__(prefix_bound(kE4M3, kWide), 1) attn_prefix_ker
       }
       ++units;
       float m = -INFINITY, l = 0.f;
-      if (half_there)
-        for (int t = kWide ? 0 : w; t < nt; t += kWide ? 1 : 2) {
-          const int keys = min(kPrefixTile, u.key_hi - (u.tile + t) * kPrefixTile);
-          mbar_wait_warp(&s.s_full[w], (uint32_t)steps & 1u, &s.abort_flag, p.status, 18);
-          tc_fence_after();
-          if (active) {
-            if (keys == kPrefixTile) {
-              softmax_tile<D, Mma>(ts, to, scale, m, l, t < (kWide ? 1 : 2), s, w, steps, p.status);
-              tc_fence_before();
-              mbar_arrive_warp(&s.p_ready[w]);
-              ++steps;
-              continue;
-            }
-            float top = -INFINITY;
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              if (c * 64 >= keys) break;
-              uint32_t a[32], b[32];
-              tmem_ld32(ts + c * 64, a);
-              tmem_ld32(ts + c * 64 + 32, b);
-              tmem_ld_wait(a);
-              tmem_ld_wait(b);
-              if (keys >= c * 64 + 64) {
-                float t0 = -INFINITY, t1 = -INFINITY;
-#pragma unroll
-                for (int j = 0; j < 32; j += 2) {
-                  t0 = max3(t0, __uint_as_float(a[j]), __uint_as_float(a[j + 1]));
-                  t1 = max3(t1, __uint_as_float(b[j]), __uint_as_float(b[j + 1]));
-                }
-                top = max3(top, t0, t1);
-              } else {
-#pragma unroll
-                for (int j = 0; j < 32; ++j) {
-                  if (c * 64 + j < keys) top = fmaxf(top, __uint_as_float(a[j]));
-                  if (c * 64 + 32 + j < keys) top = fmaxf(top, __uint_as_float(b[j]));
-                }
-              }
-            }
-            top *= scale;
-            // the reference point moves when it has to (see the own units); the accumulator is then scaled where it lies
-            if (__any_sync(0xffffffffu, top > m + 8.f)) {
-              const float next = fmaxf(m, top), f = next == -INFINITY ? 1.f : paged_ex2(m - next);
-              const bool first = t < (kWide ? 1 : 2);
-              m = next;
-              l *= f;
-              if (!first) rescale_o<D>(to, f, s, w, steps, p.status);
-            }
-            const float shift = m == -INFINITY ? 0.f : -m;
-            const uint64_t scale2 = pack2(scale, scale), shift2 = pack2(shift, shift);
-            uint64_t sum2 = pack2(0.f, 0.f);
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              if (c * 32 >= keys) break;
-              uint32_t a[32], out[16];
-              tmem_ld32(ts + c * 32, a);
-              tmem_ld_wait(a);
-              if (keys < c * 32 + 32) {
-#pragma unroll
-                for (int j = 16; j < 32; ++j) a[j] = 0xff800000u;  // only 16 of these keys are there
-              }
-#pragma unroll
-              for (int j = 0; j < 32; j += 2) {
-                float e0, e1;
-                unpack2(fma2(pack2u(a[j], a[j + 1]), scale2, shift2), e0, e1);
-                e0 = paged_ex2(e0), e1 = paged_ex2(e1);
-                if (j >= 16 && keys < c * 32 + 32) e0 = e1 = 0.f;
-                sum2 = add2(sum2, pack2(e0, e1));
-                out[j / 2] = pack16(e0, e1, Mma{});
-              }
-              tmem_st16(ts + c * 16, out);
-            }
-            tmem_st_wait();
-            float s0, s1;
-            unpack2(sum2, s0, s1);
-            l += s0 + s1;
-          }
-          tc_fence_before();
-          mbar_arrive_warp(&s.p_ready[w]);
-          ++steps;
-        }
+      for (int step = 0; step < n_steps; ++step) {
+        const int buf = step & 1;
+        mbar_wait_warp(&s.s_full[w][buf], phases >> buf & 1u, &s.abort_flag, p.status, 18);
+        phases ^= 1u << buf;
+        tc_fence_after();
+        if (active) softmax_step<D, Mma, !kWide && !kE4M3>(ts + buf * kStep, to, step_keys<kWide>(piece, w, step), scale, m, l, s, &s.o_done[w][buf ^ 1],
+                                                                 (phases >> (buf ^ 1) & 1u) ^ 1u, step == 0, p.status);
+        tc_fence_before();
+        mbar_arrive_warp(&s.p_ready[w][buf]);
+      }
       // ---- the piece goes to its slot
       const int64_t slot = (int64_t)u.index + blockIdx.x;
       float* out = p.prefix_acc + (slot * p.prefix_rows + row) * D;
       if constexpr (kWide) {
-        if (half_there) {
-          mbar_wait_warp(&s.o_done[w], (uint32_t)(steps - 1) & 1u, &s.abort_flag, p.status, 20);
+        if (n_steps > 0) {
+          const int last = (n_steps - 1) & 1;
+          mbar_wait_warp(&s.o_done[w][last], (phases >> last & 1u) ^ 1u, &s.abort_flag, p.status, 20);
           tc_fence_after();
           if (active) {
 #pragma unroll 1
@@ -464,16 +463,18 @@ __global__ void __launch_bounds__(prefix_bound(kE4M3, kWide), 1) attn_prefix_ker
         }
       } else {
         // both halves hold sums of the same rows: each joins one half of the columns
-        other_steps += w == 0 ? nt / 2 : (nt + 1) / 2;
+        const int other = (piece - (w ^ 1) * kStep + kPrefixTile - 1) / kPrefixTile;
+        other_phases ^= (uint32_t)((other + 1) / 2 & 1) | (uint32_t)(other / 2 & 1) << 1;
         if (w == 0) s.ml[r] = make_float2(m, l);
         asm volatile("bar.sync 1, 256;" ::: "memory");
         float2 x;
         if (w == 1) x = s.ml[r], s.ml[r] = make_float2(m, l);
         asm volatile("bar.sync 1, 256;" ::: "memory");
         if (w == 0) x = s.ml[r];
-        const bool both = nt > 1;
-        if (w < nt) mbar_wait_warp(&s.o_done[w], (uint32_t)(steps - 1) & 1u, &s.abort_flag, p.status, 21);
-        if (w != 0 || both) mbar_wait_warp(&s.o_done[w ^ 1], (uint32_t)(other_steps - 1) & 1u, &s.abort_flag, p.status, 22);
+        const bool both = w == 0 ? other > 0 : n_steps > 0;  // the second half has keys of the piece
+        const int last = (n_steps - 1) & 1, other_last = (other - 1) & 1;
+        if (n_steps > 0) mbar_wait_warp(&s.o_done[w][last], (phases >> last & 1u) ^ 1u, &s.abort_flag, p.status, 21);
+        if (other > 0) mbar_wait_warp(&s.o_done[w ^ 1][other_last], (other_phases >> other_last & 1u) ^ 1u, &s.abort_flag, p.status, 22);
         tc_fence_after();
         const float top = fmaxf(m, x.x);
         const float mine = m == -INFINITY ? 0.f : paged_ex2(m - top), theirs = x.x == -INFINITY ? 0.f : paged_ex2(x.x - top);
