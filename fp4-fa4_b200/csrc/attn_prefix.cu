@@ -92,9 +92,10 @@ __device__ __forceinline__ void rescale_o(uint32_t to, float f, Smem& s, uint64_
   tmem_st_wait();
 }
 
-// One step of a row: scores out of TMEM, probabilities back in as 16-bit.  keys: 16 to 64 in sixteens.  kLean: 32 scores in
+// One step of a row: scores out of TMEM, probabilities back in as 16-bit.  keys: 16 to 64 in sixteens; kFull: 64 (with
+// the other case in the same code every exponential hangs on a branch: 36 cycles a pair).  kLean: 32 scores in
 // registers at a time, read once for their maximum and once more to be used.
-template <int D, typename Mma, bool kLean, typename Smem>
+template <int D, typename Mma, bool kLean, bool kFull, typename Smem>
 __device__ __forceinline__ void softmax_step(uint32_t ts, uint32_t to, int keys, float scale, float& m, float& l, Smem& s, uint64_t* before,
                                              uint32_t parity_before, bool first, uint32_t* status) {
   constexpr int kHeld = kLean ? 1 : 2;
@@ -120,7 +121,7 @@ __device__ __forceinline__ void softmax_step(uint32_t ts, uint32_t to, int keys,
       tmem_ld32(ts + c * 32, x);
       tmem_ld_wait(x);
     }
-    if (keys < kStep) absent(c, x);
+    if constexpr (!kFull) absent(c, x);
 #pragma unroll
     for (int j = 0; j < 32; j += 4) {
       t0 = max3(t0, __uint_as_float(x[j]), __uint_as_float(x[j + 1]));
@@ -136,8 +137,7 @@ __device__ __forceinline__ void softmax_step(uint32_t ts, uint32_t to, int keys,
     if (!first) rescale_o<D>(to, f, s, before, parity_before, status);
   }
   const float shift = m == -INFINITY ? 0.f : -m;
-  const uint64_t scale2 = pack2(scale, scale), shift2 = pack2(shift, shift);
-  uint64_t sum0 = pack2(0.f, 0.f), sum1 = sum0;
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
     uint32_t(&x)[32] = a[kLean ? 0 : c];
@@ -147,20 +147,21 @@ __device__ __forceinline__ void softmax_step(uint32_t ts, uint32_t to, int keys,
     }
     uint32_t out[16];
 #pragma unroll
-    for (int j = 0; j < 32; j += 2) {
-      float e0, e1;
-      unpack2(fma2(pack2u(x[j], x[j + 1]), scale2, shift2), e0, e1);
-      e0 = paged_ex2(e0), e1 = paged_ex2(e1);
-      if (c * 32 + j >= 16 && keys <= (c * 32 + j) / 16 * 16) e0 = e1 = 0.f;  // not there
-      if (j & 2) sum1 = add2(sum1, pack2(e0, e1)); else sum0 = add2(sum0, pack2(e0, e1));
-      out[j / 2] = pack16(e0, e1, Mma{});
+    for (int j = 0; j < 32; j += 4) {
+      float e[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        e[i] = paged_ex2(fmaf(__uint_as_float(x[j + i]), scale, shift));
+        if constexpr (!kFull)
+          if (c * 32 + j >= 16 && keys <= (c * 32 + j) / 16 * 16) e[i] = 0.f;  // not there
+        sum[i] += e[i];
+      }
+      out[j / 2] = pack16(e[0], e[1], Mma{}), out[j / 2 + 1] = pack16(e[2], e[3], Mma{});
     }
     tmem_st16(ts + c * 16, out);
   }
   tmem_st_wait();
-  float s0, s1;
-  unpack2(add2(sum0, sum1), s0, s1);
-  l += s0 + s1;
+  l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
 }
 
 template <int D, bool kE4M3, typename QT, bool kWide>
@@ -434,8 +435,15 @@ __global__ void __launch_bounds__(prefix_bound(kE4M3, kWide), 1) attn_prefix_ker
         mbar_wait_warp(&s.s_full[w][buf], phases >> buf & 1u, &s.abort_flag, p.status, 18);
         phases ^= 1u << buf;
         tc_fence_after();
-        if (active) softmax_step<D, Mma, !kWide && !kE4M3>(ts + buf * kStep, to, step_keys<kWide>(piece, w, step), scale, m, l, s, &s.o_done[w][buf ^ 1],
-                                                                 (phases >> (buf ^ 1) & 1u) ^ 1u, step == 0, p.status);
+        if (active) {
+          const int keys = step_keys<kWide>(piece, w, step);
+          uint64_t* before = &s.o_done[w][buf ^ 1];
+          const uint32_t parity_before = (phases >> (buf ^ 1) & 1u) ^ 1u;
+          if (keys == kStep)
+            softmax_step<D, Mma, !kWide && !kE4M3, true>(ts + buf * kStep, to, keys, scale, m, l, s, before, parity_before, step == 0, p.status);
+          else
+            softmax_step<D, Mma, !kWide && !kE4M3, false>(ts + buf * kStep, to, keys, scale, m, l, s, before, parity_before, step == 0, p.status);
+        }
         tc_fence_before();
         mbar_arrive_warp(&s.p_ready[w][buf]);
       }

@@ -189,19 +189,50 @@ struct WriteParams {
   int T, D, tile_tokens;
 };
 
+// The head's scale with its reciprocal, for the quotients of div2_exact: correctly rounded ones for a scale of ordinary size
+// whose significand is not all ones (r = 0: divide).
+struct QuantScale {
+  float s, r;
+  __device__ __forceinline__ explicit QuantScale(float scale) : s(scale) {
+    const float a = fabsf(scale);
+    r = a >= 5.4e-20f && a <= 1.8e19f && !significand_all_ones(scale) ? __frcp_rn(scale) : 0.f;
+  }
+};
 template <typename Src>
-__device__ __forceinline__ uint2 quantise8(uint4 x, float scale) {
+__device__ __forceinline__ uint2 quantise8(uint4 x, QuantScale scale) {
   const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-  float f[8];
+  uint64_t f[4], q[4];
+  uint32_t top = 0u;  // largest magnitudes of the even and of the odd values
+  const uint64_t r2 = pack2(scale.r, scale.r), neg2 = pack2(-scale.s, -scale.s);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    float2 p;
-    if constexpr (sizeof(Src) == 2 && std::is_same<Src, __half>::value) p = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-    else p = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[i]));
-    f[2 * i] = __fdiv_rn(p.x, scale);  // the definition's quotient: one rounding to 32 bits, one to E4M3
-    f[2 * i + 1] = __fdiv_rn(p.y, scale);
+    if constexpr (std::is_same<Src, __half>::value) {
+      const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      f[i] = pack2(p.x, p.y);
+    } else {
+      f[i] = bf16x2_to_f32x2(w[i]);
+      top = absmax_bf16x2(top, w[i]);
+    }
+    q[i] = div2_exact(f[i], r2, neg2);
   }
-  return make_uint2(cvt_e4m3x4(f[0], f[1], f[2], f[3]), cvt_e4m3x4(f[4], f[5], f[6], f[7]));
+  float a[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) unpack2(q[i], a[2 * i], a[2 * i + 1]);
+  // an odd scale, or a quotient that may overflow on the way (f16: infinity alone, whose quotient is one as well)
+  const float most = std::is_same<Src, __half>::value ? 0.f : fmaxf(__uint_as_float(top << 16), __uint_as_float(top & 0xffff0000u));
+  bool divide = scale.r == 0.f || !(most * fabsf(scale.r) < 1.0e30f);
+  if constexpr (std::is_same<Src, __half>::value) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) divide |= (w[i] & 0x7fffu) == 0x7c00u || (w[i] & 0x7fff0000u) == 0x7c000000u;
+  }
+  if (divide) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      unpack2(f[i], a[2 * i], a[2 * i + 1]);
+      a[2 * i] = __fdiv_rn(a[2 * i], scale.s), a[2 * i + 1] = __fdiv_rn(a[2 * i + 1], scale.s);
+    }
+  }
+  return make_uint2(cvt_e4m3x4(a[0], a[1], a[2], a[3]), cvt_e4m3x4(a[4], a[5], a[6], a[7]));
 }
 
 // grid (row of the batch x kv head, tile of tokens); a thread takes 16 bytes of K and of V of one token at a time, so a
@@ -210,36 +241,54 @@ template <bool kE4M3, typename Src>
 __global__ void __launch_bounds__(256) kv_write_kernel(const KvView c, const WriteParams w) {
   pdl_trigger();
   pdl_wait();
-  const int i = blockIdx.x / c.heads, h = blockIdx.x % c.heads;
-  const int slot = w.seqs[i];
+  const int i = blockIdx.x / c.heads, h = blockIdx.x - i * c.heads;
+  const int slot = w.seqs[i], n_new = w.n_new ? w.n_new[i] : w.T;
+  const int tile0 = blockIdx.y * w.tile_tokens, t_end = min(min(n_new, w.T), tile0 + w.tile_tokens);
   if (slot < 0 || slot >= c.max_seqs) {
     if (threadIdx.x == 0 && h == 0 && blockIdx.y == 0) kv_report(c, kBadSlot, i, slot);
     return;
   }
-  const int add = w.n_new ? min(w.n_new[i], w.T) : w.T;
-  const int64_t start = (int64_t)c.lens[slot] - (w.n_new ? w.n_new[i] : w.T);
+  if (tile0 >= t_end) return;
+  const int64_t start = (int64_t)c.lens[slot] - n_new;
   const int chunks = w.D / 8, chunk = threadIdx.x & (chunks - 1), step = 256 / chunks;
   const int32_t* row = c.table + slot * c.table_stride;
-  const float sk = kE4M3 ? w.scale[0][h] : 1.f, sv = kE4M3 ? w.scale[1][h] : 1.f;
-  const int t_end = min(add, (int)(blockIdx.y + 1) * w.tile_tokens);
-#pragma unroll 4
-  for (int t = blockIdx.y * w.tile_tokens + (int)(threadIdx.x / chunks); t < t_end; t += step) {
-    const int64_t pos = start + t;
-    if (pos < 0 || (pos >> c.page_shift) >= c.width) continue;
-    const int p = row[pos >> c.page_shift];
-    if (p < 0 || p >= c.pages) continue;
-    const uint4 xk = __ldcs(reinterpret_cast<const uint4*>(w.src[0] + i * w.sb[0] + h * w.sh[0] + t * w.st[0]) + chunk);
-    const uint4 xv = __ldcs(reinterpret_cast<const uint4*>(w.src[1] + i * w.sb[1] + h * w.sh[1] + t * w.st[1]) + chunk);
-    const int64_t in_page = ((int64_t)h * c.page_tokens + (pos & (c.page_tokens - 1))) * c.row_bytes;
-    uint8_t* dk = w.dst[0] + p * c.k_page + in_page;
-    uint8_t* dv = w.dst[1] + p * c.v_page + in_page;
-    if constexpr (kE4M3) {
-      reinterpret_cast<uint2*>(dk)[chunk] = quantise8<Src>(xk, sk);
-      reinterpret_cast<uint2*>(dv)[chunk] = quantise8<Src>(xv, sv);
-    } else {
-      reinterpret_cast<uint4*>(dk)[chunk] = xk;
-      reinterpret_cast<uint4*>(dv)[chunk] = xv;
+  const QuantScale sk(kE4M3 ? w.scale[0][h] : 1.f), sv(kE4M3 ? w.scale[1][h] : 1.f);
+  constexpr int kOut = kE4M3 ? 8 : 16;
+  const uint8_t* k_src = w.src[0] + i * w.sb[0] + h * w.sh[0] + chunk * 16;
+  const uint8_t* v_src = w.src[1] + i * w.sb[1] + h * w.sh[1] + chunk * 16;
+  uint8_t* k_dst = w.dst[0] + (int64_t)h * c.page_tokens * c.row_bytes + chunk * kOut;
+  uint8_t* v_dst = w.dst[1] + (int64_t)h * c.page_tokens * c.row_bytes + chunk * kOut;
+  // four tokens per thread at a time: their pages, then all their loads, then the stores
+#pragma unroll 1
+  for (int t0 = tile0 + (int)(threadIdx.x / chunks); t0 < t_end; t0 += 4 * step) {
+    int page[4], at[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t pos = start + t0 + j * step;
+      const bool there = t0 + j * step < t_end && pos >= 0 && (pos >> c.page_shift) < c.width;
+      page[j] = there ? row[(int)(pos >> c.page_shift)] : -1;
+      at[j] = ((int)pos & (c.page_tokens - 1)) * c.row_bytes;
     }
+    uint4 xk[4], xv[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if ((uint32_t)page[j] < (uint32_t)c.pages) {
+        xk[j] = __ldcs(reinterpret_cast<const uint4*>(k_src + (t0 + j * step) * w.st[0]));
+        xv[j] = __ldcs(reinterpret_cast<const uint4*>(v_src + (t0 + j * step) * w.st[1]));
+      }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if ((uint32_t)page[j] < (uint32_t)c.pages) {
+        uint8_t* dk = k_dst + page[j] * c.k_page + at[j];
+        uint8_t* dv = v_dst + page[j] * c.v_page + at[j];
+        if constexpr (kE4M3) {
+          *reinterpret_cast<uint2*>(dk) = quantise8<Src>(xk[j], sk);
+          *reinterpret_cast<uint2*>(dv) = quantise8<Src>(xv[j], sv);
+        } else {
+          *reinterpret_cast<uint4*>(dk) = xk[j];
+          *reinterpret_cast<uint4*>(dv) = xv[j];
+        }
+      }
   }
 }
 
@@ -649,7 +698,9 @@ int fa4b_kv_write(const fa4b_kv_cache* c, const fa4b_kv_write_args* a, void* str
   if (c->dtype == FA4B_KV_E4M3) w.scale[0] = c->k_scale + (int64_t)a->layer * c->Hkv, w.scale[1] = c->v_scale + (int64_t)a->layer * c->Hkv;
   w.dst[0] = v.k + a->layer * v.k_layer, w.dst[1] = v.v + a->layer * v.v_layer;
   w.seqs = a->seqs, w.n_new = a->n_new, w.T = a->T, w.D = c->D;
-  w.tile_tokens = 4 * (256 / (c->D / 8));  // four tokens of K and V in flight per thread
+  // four tokens of K and V in flight per thread; twice over where there are CTAs enough without
+  w.tile_tokens = 4 * (256 / (c->D / 8));
+  if ((int64_t)a->n * c->Hkv * a->T > 16ll * w.tile_tokens * std::max(sm_count(), 1)) w.tile_tokens *= 2;
   const int64_t tiles = ((int64_t)a->T + w.tile_tokens - 1) / w.tile_tokens;
   FA4B_REQUIRE(tiles <= 65535, FA4B_BAD_SHAPE, "T=%d: at most %d tokens in one call", a->T, 65535 * w.tile_tokens);
   const dim3 grid((unsigned)(a->n * c->Hkv), (unsigned)tiles);

@@ -21,6 +21,8 @@ from ._lib import check, lib, ptr
 _WRITE = struct.Struct("@PP3q3q4iPP")
 _ATTEND = struct.Struct("@P3qP3qP5ifPiPPP")
 
+_current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+
 KV_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float8_e4m3fn: 2}
 
 
@@ -92,11 +94,11 @@ class PagedKVCache:
     def _call(self, name: str, *args) -> None:
         """One C call on the cache's device and that device's current stream."""
         index = self._index
-        if torch._C._cuda_getDevice() == index:
-            status = getattr(self._lib, name)(self._at, *args, torch._C._cuda_getCurrentRawStream(index))
+        if _current_device() == index:
+            status = getattr(self._lib, name)(self._at, *args, _raw_stream(index))
         else:
             with torch.cuda.device(index):
-                status = getattr(self._lib, name)(self._at, *args, torch._C._cuda_getCurrentRawStream(index))
+                status = getattr(self._lib, name)(self._at, *args, _raw_stream(index))
         if status:
             check(status, name)
 
@@ -200,10 +202,10 @@ class PagedKVCache:
                 raise ValueError(f"group_offsets must have {groups + 1} entries, got {group_offsets.shape[0]}")
             offsets = self._list(group_offsets, "group_offsets")
         if out is None:
-            out = torch.empty(shape, dtype=q.dtype, device=self.device)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
         elif out.shape != shape or out.dtype != q.dtype or out.device != self.device or out.stride(3) != 1:
             raise ValueError(f"out must be a {tuple(shape)} tensor like q with a contiguous head dimension")
-        lse = torch.empty((n, hq, t), dtype=torch.float32, device=self.device)
+        lse = q.new_empty((n, hq, t), dtype=torch.float32)
         code, scale = KV_DTYPES[q.dtype], softmax_scale or 0.0
         q_strides, o_strides = _strides(q), _strides(out)
         size = self._ws_bytes.get((n, hq, t, groups))
@@ -212,7 +214,7 @@ class PagedKVCache:
             size = self._lib.fa4b_attn_paged_workspace_bytes(self._at, args)
             if size:
                 self._ws_bytes[n, hq, t, groups] = size
-        ws = torch.empty(size, dtype=torch.uint8, device=self.device)
+        ws = self._work.new_empty(size >> 2)  # of this call alone: calls on two streams, or of two captured graphs, may overlap
         args = _ATTEND.pack(q.data_ptr(), *q_strides, out.data_ptr(), *o_strides, lse.data_ptr(), n, t, hq, layer, code, scale, slots, groups, offsets, shared,
                             ws.data_ptr())
         self._call("fa4b_attn_paged_fwd", args)

@@ -56,7 +56,9 @@ class ModelCache:
         """What the pool holds for values [Hkv, D] of one token."""
         if self.scale is None:
             return x
-        return (x.float() / self.scale[which][layer][:, None]).clamp(-448, 448).to(torch.float8_e4m3fn)
+        q = x.float() / self.scale[which][layer][:, None]
+        codes = q.clamp(-448, 448).to(torch.float8_e4m3fn).view(torch.uint8)
+        return codes.masked_fill(q.isnan(), 0x7f).view(torch.float8_e4m3fn)  # NaN has two codes: the one without a sign
 
     def write(self, k, v, seqs, n_new, layer):
         for i, s in enumerate(seqs):

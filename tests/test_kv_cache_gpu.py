@@ -201,6 +201,22 @@ def test_a_list_of_thousands():
         c.free(ints(list(range(4097))))
 
 
+@pytest.mark.parametrize("scale", [2.0 ** -70, 1e-30, 1.9999998807907104, 2.0 ** 70, -0.037])
+def test_an_e4m3_cache_with_an_odd_scale_stores_the_divisions_codes(scale):
+    """Scales that the quotient by reciprocal does not cover, and values over the whole range: the 32-bit division's codes."""
+    c = make(pages=30, heads=2, d=64, layers=1, dtype=torch.float8_e4m3fn)
+    c.k_scale.fill_(scale), c.v_scale.fill_(0.0123)
+    gen = torch.Generator().manual_seed(9)
+    k, v = [(torch.randn(1, 2, 40, 64, generator=gen) * 10.0 ** torch.randint(-36, 36, (1, 2, 40, 64), generator=gen)).to(torch.bfloat16).to(DEV) for _ in range(2)]
+    k[0, 0, 0, :4] = torch.tensor([float("inf"), -float("inf"), float("nan"), 0.0])
+    v[0, 0, 0, :4] = k[0, 0, 0, :4]
+    c.extend(ints([3]), ints([40]))
+    m = ModelCache(c)
+    c.write(k, v, ints([3]))
+    m.write(k, v, [3], None, 0)
+    m.check(c)
+
+
 @pytest.mark.parametrize("src", [torch.bfloat16, torch.float16])
 def test_what_an_e4m3_cache_stores(src):
     """Against the quotient in 64 bits: the 32-bit quotient is off by at most half a step (2^-24 relative), the code by half
