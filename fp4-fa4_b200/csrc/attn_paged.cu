@@ -6,42 +6,55 @@
 // be empty for the most part, and the 16-row form already computes a tile in a quarter of the time its bytes take.
 #include "attn_paged.cuh"
 
+#include <cstddef>
 #include <type_traits>
 
 namespace fa4b {
 
 // ---- plan -------------------------------------------------------------------------------------------------------------
-__device__ __forceinline__ int paged_scan(int v, int* warp_sums, int& total) {  // exclusive, 1024 threads
+// One CTA runs this once, so what it costs is the fetching of its instructions: a line of eight that nobody has run yet takes
+// longer than the eight.  Hence one copy of what is used twice, no unrolling, shifts for divisions.
+__device__ __noinline__ uint32_t paged_div(uint32_t a, uint32_t b) { return a / b; }
+
+// Exclusive prefix sums of a[0..n) in shared memory, in place, by a block of 1024 threads; returns the total.
+__device__ __noinline__ int paged_scan(int* a, int n, int* warp_sums) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int x = v;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, x, o);
-    if (lane >= o) x += y;
-  }
-  if (lane == 31) warp_sums[warp] = x;
+  int total = 0;
   __syncthreads();
-  int w = warp_sums[lane];
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, w, o);
-    if (lane >= o) w += y;
+#pragma unroll 1
+  for (int base = 0; base < n; base += 1024) {
+    const int i = base + threadIdx.x, v = i < n ? a[i] : 0;
+    int x = v;
+#pragma unroll 1
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    if (n > 32) {  // the sums of the warps
+      if (lane == 31) warp_sums[warp] = x;
+      __syncthreads();
+      const int w = warp_sums[lane];
+      x += __reduce_add_sync(0xffffffffu, lane < warp ? w : 0);
+      if (i < n) a[i] = total + x - v;
+      total += __reduce_add_sync(0xffffffffu, w);
+    } else {
+      if (warp == 0 && i < n) a[i] = x - v;
+      if (threadIdx.x == 31) warp_sums[0] = x;
+      __syncthreads();
+      total = warp_sums[0];
+    }
+    __syncthreads();
   }
-  total = __shfl_sync(0xffffffffu, w, 31);
-  const int before = __shfl_sync(0xffffffffu, w, (warp + 31) & 31);
-  __syncthreads();
-  return x - v + (warp ? before : 0);
+  return total;
 }
 
-// One CTA: lengths, groups, and the lines of tiles.  The shared part of a group is what the caller says, cut to what every
-// query row of every member sees (so that no row of a prefix unit needs a mask) and to whole 16 keys; a group of one
-// member has none.
-// The last i in [0, n) whose part of the line begins at or before x; cum counts one `factor`-th of it.
-__device__ __forceinline__ int paged_find(const int* cum, int n, int64_t x, int64_t factor) {
+// The last i in [0, n) with cum[i] <= x.
+__device__ __noinline__ int paged_find(const int* cum, int n, uint32_t x) {
   int lo = 0, hi = n - 1;
+#pragma unroll 1
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (cum[mid] * factor <= x) lo = mid; else hi = mid - 1;
+    if ((uint32_t)cum[mid] <= x) lo = mid; else hi = mid - 1;
   }
   return lo;
 }
@@ -49,8 +62,10 @@ __device__ __forceinline__ int paged_find(const int* cum, int n, int64_t x, int6
 // dynamic shared memory of the plan, in words
 __host__ __device__ inline size_t paged_plan_words(int n, int groups) { return 4 * (size_t)n + 6 * (size_t)groups + 1; }
 
+// Lengths, groups, and the lines of tiles.  The shared part of a group is what the caller says, cut to what every query row
+// of every member sees (so that no row of a prefix unit needs a mask) and to whole 16 keys; a group of one member has none.
 __global__ void __launch_bounds__(1024) paged_plan_kernel(const PagedParams p) {
-  __shared__ int warp_sums[32];
+  __shared__ int warp_sums[32], bad;
   extern __shared__ int dyn[];
   int* own_cum = dyn;                  // [n]
   int* s_slot = own_cum + p.n;         // [n]
@@ -62,120 +77,116 @@ __global__ void __launch_bounds__(1024) paged_plan_kernel(const PagedParams p) {
   int* g_count = g_first + p.groups;   // [groups] members with keys, then whether a shared page is missing
   int* g_cum = g_count + p.groups;     // [groups]
   int* g_unit = g_cum + p.groups;      // [groups]
+  const int tid = threadIdx.x;
   pdl_trigger();
+  if (tid == 0) bad = 0;
+#pragma unroll 1
+  for (int g = tid; g < p.groups; g += 1024) g_shared[g] = INT_MAX, g_first[g] = INT_MAX, g_count[g] = 0;
   pdl_wait();
-  for (int g = threadIdx.x; g < p.groups; g += 1024) offsets[g] = p.offsets[g], g_shared[g] = INT_MAX, g_first[g] = INT_MAX, g_count[g] = 0;
-  if (threadIdx.x == 0 && p.groups > 0) offsets[p.groups] = p.offsets[p.groups];
-  for (int i = threadIdx.x; i < p.n; i += 1024) {
+#pragma unroll 1
+  for (int g = tid; g <= p.groups && p.groups > 0; g += 1024) offsets[g] = p.offsets[g];
+#pragma unroll 1
+  for (int i = tid; i < p.n; i += 1024) {
     const int slot = p.seqs ? p.seqs[i] : i;
-    int len = 0;
-    if (slot >= 0 && slot < p.c.max_seqs) len = (int)min((int64_t)max(p.c.lens[slot], 0), (int64_t)p.c.width << p.c.page_shift);
-    s_slot[i] = slot, s_len[i] = len, s_group[i] = p.groups > 0 ? -1 : 0;
+    s_slot[i] = slot, s_group[i] = p.groups > 0 ? -1 : 0;
+    s_len[i] = (uint32_t)slot < (uint32_t)p.c.max_seqs ? min(max(p.c.lens[slot], 0), p.c.width << p.c.page_shift) : 0;
   }
   __syncthreads();
-  int prefix_total = 0;
   if (p.groups > 0) {
-    bool bad = false;  // groups have to lie behind one another: the slots of their units are counted on it
-    for (int g = threadIdx.x; g < p.groups; g += 1024) bad |= offsets[g] < 0 || offsets[g + 1] < offsets[g] || offsets[g + 1] > p.n;
-    bad = __syncthreads_or(bad);
-    if (bad && threadIdx.x == 0 && atomicCAS(p.status, 0u, 2u) == 0u) p.status[1] = (uint32_t)p.groups;
-    if (!bad)
-      for (int i = threadIdx.x; i < p.n; i += 1024) {
-        int lo = 0, hi = p.groups - 1;  // the last group that begins at or before i
-        while (lo < hi) {
-          const int mid = (lo + hi + 1) >> 1;
-          if (offsets[mid] <= i) lo = mid; else hi = mid - 1;
-        }
-        if (i < offsets[lo] || i >= offsets[lo + 1]) continue;
-        s_group[i] = lo;
-        if (s_len[i] > 0) {
-          atomicMin(g_shared + lo, max(s_len[i] - p.T, 0));
-          atomicMin(g_first + lo, i);
-          atomicAdd(g_count + lo, 1);
-        }
+    // groups have to lie behind one another: the slots of their units are counted on it
+#pragma unroll 1
+    for (int g = tid; g < p.groups; g += 1024)
+      if (offsets[g] < 0 || offsets[g + 1] < offsets[g] || offsets[g + 1] > p.n) bad = 1;
+#pragma unroll 1
+    for (int i = tid; i < p.n; i += 1024) {
+      const int g = paged_find(offsets, p.groups, (uint32_t)i);  // the last group that begins at or before i
+      if (i < offsets[g] || i >= offsets[g + 1]) continue;
+      s_group[i] = g;
+      if (s_len[i] > 0) {
+        atomicMin(g_shared + g, max(s_len[i] - p.T, 0));
+        atomicMin(g_first + g, i);
+        atomicAdd(g_count + g, 1);
       }
+    }
     __syncthreads();
-    for (int g = threadIdx.x; g < p.groups; g += 1024) {
-      g_shared[g] = g_count[g] > 1 ? min(max(p.shared[g], 0), g_shared[g]) / kPagedAlign * kPagedAlign : 0;
+    if (bad != 0) {
+      if (tid == 0 && atomicCAS(p.status, 0u, 2u) == 0u) p.status[1] = (uint32_t)p.groups;
+#pragma unroll 1
+      for (int i = tid; i < p.n; i += 1024) s_group[i] = -1;
+    }
+#pragma unroll 1
+    for (int g = tid; g < p.groups; g += 1024) {
+      g_shared[g] = g_count[g] > 1 && bad == 0 ? min(max(p.shared[g], 0), g_shared[g]) & ~(kPagedAlign - 1) : 0;
       g_count[g] = 0;
     }
     __syncthreads();
     // A shared page that the table does not name: the group goes without, the own units know how to leave such a page out.
-    const int per_group = 1024 >> (32 - __clz(min(p.groups, 32) - 1));  // threads: a warp at least
-    for (int g = threadIdx.x / per_group; g < p.groups; g += 1024 / per_group) {
+    const int shift = p.groups >= 32 ? 5 : 10 - (31 - __clz(2 * p.groups - 1));  // 2^shift threads for a group: a warp at least
+#pragma unroll 1
+    for (int g = tid >> shift; g < p.groups; g += 1024 >> shift) {
       const int pages = (g_shared[g] + p.c.page_tokens - 1) >> p.c.page_shift;
       const int32_t* row = p.c.table + (pages ? (int64_t)s_slot[g_first[g]] * p.c.table_stride : 0);
-      bool missing = false;
-#pragma unroll 4
-      for (int j = threadIdx.x % per_group; j < pages; j += per_group) missing |= (uint32_t)row[j] >= (uint32_t)p.c.pages;
-      if (missing) g_count[g] = 1;
+#pragma unroll 2
+      for (int j = tid & ((1 << shift) - 1); j < pages; j += 1 << shift)
+        if ((uint32_t)row[j] >= (uint32_t)p.c.pages) g_count[g] = 1;
     }
     __syncthreads();
-    int units = 0;
-    for (int base = 0; base < p.groups; base += 1024) {
-      const int g = base + threadIdx.x;
-      int length = 0, own_u = 0;
-      PagedGroup r{};
-      if (g < p.groups) {
-        r.shared = g_count[g] ? 0 : g_shared[g];
-        g_shared[g] = r.shared;
-        if (r.shared > 0) {
-          r.row = offsets[g], r.rows = (offsets[g + 1] - r.row) * p.R;
-          r.slot = s_slot[g_first[g]];
-          r.blocks = ceil_div(r.rows, p.prefix_rows);
-          own_u = p.c.heads * r.blocks;
-          length = own_u * (ceil_div(r.shared, p.prefix_tile) + p.prefix_extra);
-        }
-      }
-      int t_total, u_total;
-      r.cum = prefix_total + paged_scan(length, warp_sums, t_total), r.unit = units + paged_scan(own_u, warp_sums, u_total);
-      if (g < p.groups) p.group[g] = r, g_cum[g] = r.cum, g_unit[g] = r.unit;
-      prefix_total += t_total, units += u_total;
+#pragma unroll 1
+    for (int g = tid; g < p.groups; g += 1024) {
+      const int shared = g_count[g] ? 0 : g_shared[g];
+      const int units = shared ? p.c.heads * (((offsets[g + 1] - offsets[g]) * p.R + p.prefix_rows - 1) >> p.prefix_shift) : 0;
+      g_shared[g] = shared;
+      g_unit[g] = units;
+      g_cum[g] = units * ((shared + kPagedPrefixTile - 1) / kPagedPrefixTile + p.prefix_extra);
     }
-    __syncthreads();
   }
-  int own_total = 0;
-  for (int base = 0; base < p.n; base += 1024) {
-    const int i = base + threadIdx.x;
-    int length = 0;
-    PagedSeq s{};
-    if (i < p.n) {
-      const int g = s_group[i];
-      s.slot = s_slot[i], s.len = s_len[i], s.left_alone = g < 0;
-      if (g >= 0) {
-        if (p.groups > 0 && g_shared[g] > 0 && s.len > 0)
-          s.first = g_shared[g], s.g_row = offsets[g], s.g_blocks = ceil_div((offsets[g + 1] - offsets[g]) * p.R, p.prefix_rows), s.g_unit = g_unit[g], s.g_cum = g_cum[g];
-        length = own_tiles(p, s.first, s.len);
-        length += length ? p.own_extra : 0;
-      }
-    }
-    int total;
-    s.cum = own_total + paged_scan(length, warp_sums, total);
-    if (i < p.n) p.seq[i] = s, own_cum[i] = s.cum;
-    own_total += total;
+  const int prefix_total = paged_scan(g_cum, p.groups, warp_sums);
+  paged_scan(g_unit, p.groups, warp_sums);
+#pragma unroll 1
+  for (int i = tid; i < p.n; i += 1024) {
+    const int g = s_group[i];
+    const int tiles = g < 0 ? 0 : own_tiles(p, p.groups > 0 && s_len[i] > 0 ? g_shared[g] : 0, s_len[i]);
+    own_cum[i] = tiles + (tiles ? p.own_extra : 0);
   }
-  __syncthreads();
-  const int per = p.c.heads * p.own_blocks;
-  const int64_t line = (int64_t)own_total * per;
-  const int64_t own_per = max((line + p.own_workers - 1) / p.own_workers, (int64_t)p.own_min);
-  const int64_t prefix_per = max((prefix_total + p.prefix_workers - 1) / p.prefix_workers, 1);
-  if (threadIdx.x == 0) *p.head = {line, own_per, prefix_total, prefix_per};
-  for (int w = threadIdx.x; w < p.own_workers; w += 1024) {
-    const int64_t at = w * own_per;
-    if (at >= line) break;
-    const int i = paged_find(own_cum, p.n, at, per);
-    const int length = (i + 1 < p.n ? own_cum[i + 1] : own_total) - own_cum[i];
-    const int64_t off = at - (int64_t)own_cum[i] * per;
-    const int which = (int)(off / length);
-    p.own_start[w] = {i, which, (int)(off - (int64_t)which * length), 0};
+  const int own_total = paged_scan(own_cum, p.n, warp_sums);
+  // the line of the own units has p.own_units of each entry of own_cum
+  uint32_t line = (uint32_t)own_total * p.own_units;
+  if ((uint64_t)own_total * p.own_units >= INT_MAX) {  // beyond what positions count: nothing is computed
+    if (tid == 0 && atomicCAS(p.status, 0u, 3u) == 0u) p.status[1] = (uint32_t)own_total;
+    line = 0u;
   }
-  if (prefix_total == 0) return;
-  for (int w = threadIdx.x; w < p.prefix_workers; w += 1024) {
-    const int64_t at = w * prefix_per;
-    if (at >= prefix_total) break;
-    const int g = paged_find(g_cum, p.groups, at, 1);
-    const int length = ceil_div(g_shared[g], p.prefix_tile) + p.prefix_extra, off = (int)at - g_cum[g];
-    p.prefix_start[w] = {g, off / length, off % length, 0};
+  const uint32_t own_per = max(paged_div(line + p.own_workers - 1, p.own_workers), (uint32_t)p.own_min);
+  const uint32_t prefix_per = max(paged_div(prefix_total + p.prefix_workers - 1, p.prefix_workers), 1u);
+  if (tid == 0) *p.head = {line, own_per, (uint32_t)prefix_total, prefix_per};
+  // all is known: the records
+#pragma unroll 1
+  for (int i = tid; i < p.n; i += 1024) {
+    const int g = max(s_group[i], 0), first = p.groups > 0 && s_len[i] > 0 ? g_shared[g] : 0;
+    int4* r = reinterpret_cast<int4*>(p.seq + i);
+    r[0] = make_int4(s_slot[i], s_len[i], first, own_cum[i]);
+    r[2] = make_int4(s_group[i] < 0 || line == 0u && own_total > 0, 0, 0, 0);
+    if (first > 0) r[1] = make_int4(offsets[g], ((offsets[g + 1] - offsets[g]) * p.R + p.prefix_rows - 1) >> p.prefix_shift, g_unit[g], g_cum[g]);
+  }
+#pragma unroll 1
+  for (int w = tid; w < p.own_workers && w * own_per < line; w += 1024) {
+    const uint32_t at = w * own_per;
+    const int i = paged_find(own_cum, p.n, paged_div(at, p.own_units));
+    const uint32_t length = (i + 1 < p.n ? own_cum[i + 1] : own_total) - own_cum[i], off = at - own_cum[i] * p.own_units, which = paged_div(off, length);
+    p.own_start[w] = {i, (int)which, (int)(off - which * length), 0};
+  }
+#pragma unroll 1
+  for (int g = tid; g < p.groups; g += 1024) {
+    int4* r = reinterpret_cast<int4*>(p.group + g);
+    const int shared = g_shared[g], rows = (offsets[g + 1] - offsets[g]) * p.R;
+    r[0] = make_int4(shared, shared ? s_slot[g_first[g]] : 0, offsets[g], rows);
+    r[1] = make_int4(g_cum[g], g_unit[g], (rows + p.prefix_rows - 1) >> p.prefix_shift, 0);
+  }
+#pragma unroll 1
+  for (int w = tid; w < p.prefix_workers && w * prefix_per < (uint32_t)prefix_total; w += 1024) {
+    const uint32_t at = w * prefix_per;
+    const int g = paged_find(g_cum, p.groups, at);
+    const uint32_t length = (g_shared[g] + kPagedPrefixTile - 1) / kPagedPrefixTile + p.prefix_extra, off = at - g_cum[g], which = paged_div(off, length);
+    p.prefix_start[w] = {g, (int)which, (int)(off - which * length), 0};
   }
 }
 
@@ -452,6 +463,7 @@ struct SoloSmem {
   alignas(1024) uint8_t ring[4][kStages][2][kTileBytes];
   uint64_t full[4][kStages];
   volatile uint32_t abort_flag;
+  static constexpr int kUsed = 4 * kStages * (2 * kTileBytes + 8) + 16;  // the struct without what its alignment adds
 };
 
 template <int D, bool kE4M3, typename QT>
@@ -572,6 +584,7 @@ struct TeamSmem {
   uint64_t full[kStages], empty[kStages];
   uint32_t valid[kStages];  // a bit per 16 keys: the table names a page of the pool
   volatile uint32_t abort_flag;
+  static constexpr int kUsed = kStages * (2 * kTileBytes + 16 + 4) + 2 * 16 * D * 4 + 4 * 16 * 8 + 16;
 };
 
 template <int D, bool kE4M3, typename QT, int kWM>
@@ -714,18 +727,18 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PagedParams p) {
   int64_t prefix_slot = 0, own_slot = 0;
   if (len - (p.T - 1 - (int)t) > 0) {
     if (s.first > 0) {
-      const int row = ((int)i - s.g_row) * p.R + r, block = row / p.prefix_rows, which = head * s.g_blocks + block;
-      const int tiles = ceil_div(s.first, p.prefix_tile);
-      const uint32_t per = (uint32_t)line.prefix_per, from = (uint32_t)(s.g_cum + which * (tiles + p.prefix_extra) + p.prefix_extra), worker = from / per;
-      n_prefix = (int)((from + tiles - 1) / per - worker) + 1;
+      const int row = ((int)i - s.g_row) * p.R + r, block = row >> p.prefix_shift, which = head * s.g_blocks + block;
+      const int tiles = (s.first + kPagedPrefixTile - 1) / kPagedPrefixTile;
+      const uint32_t from = (uint32_t)(s.g_cum + which * (tiles + p.prefix_extra) + p.prefix_extra), worker = from / line.prefix_per;
+      n_prefix = (int)((from + tiles - 1) / line.prefix_per - worker) + 1;
       prefix_slot = s.g_unit + which + (int64_t)worker;
-      prefix_row = row - block * p.prefix_rows;
+      prefix_row = row & (p.prefix_rows - 1);
     }
-    const int per = p.c.heads * p.own_blocks, block = r / p.own_rows, which = head * p.own_blocks + block, tiles = own_tiles(p, s.first, len);
-    const int64_t from = (int64_t)s.cum * per + (int64_t)which * (tiles + p.own_extra) + p.own_extra, worker = from / line.own_per;
-    own_slot = (int64_t)i * per + which + worker;
+    const int block = r >> p.own_rows_shift, which = head * p.own_blocks + block, tiles = own_tiles(p, s.first, len);
+    const uint32_t from = (uint32_t)(s.cum * p.own_units + which * (tiles + p.own_extra) + p.own_extra), worker = from / line.own_per;
+    own_slot = (int64_t)i * p.own_units + which + worker;
     n_own = (int)((from + tiles - 1) / line.own_per - worker) + 1;
-    own_row = r - block * p.own_rows;
+    own_row = r & (p.own_rows - 1);
   }
   pdl_wait();
   if (!there || s.left_alone) return;  // or behind the last group
@@ -795,8 +808,8 @@ struct PagedMaps {
 template <typename Smem, typename K>
 static int launch_units(K kernel, const PagedParams& p, const CUtensorMap& mk, const CUtensorMap& mv, int ctas, int threads, cudaStream_t st,
                         std::atomic<uint64_t>& allowed) {
-  constexpr int smem = (int)sizeof(Smem);
-  static_assert(smem <= 113 * 1024, "two CTAs per SM");
+  constexpr int smem = Smem::kUsed;
+  static_assert(smem >= (int)offsetof(Smem, abort_flag) + 4 && smem <= 113 * 1024, "two CTAs per SM");
   if (int s = allow_smem(kernel, smem, allowed)) return s;
   FA4B_CUDA(launch_overlapped(kernel, ctas, threads, smem, st, p, mk, mv));
   return FA4B_OK;
@@ -853,18 +866,19 @@ static int paged_params(const fa4b_kv_cache* c, const fa4b_attn_paged_args* a, P
   p.own_blocks = (p.R + p.own_rows - 1) / p.own_rows;
   const bool solo = p.own_rows == 16, short_rows = c->D * (c->dtype == FA4B_KV_E4M3 ? 1 : 2) < 256;
   p.own_tile = !solo ? TeamSmem<64, true>::kKeys : short_rows ? 32 : 16;
+  p.own_shift = __builtin_ctz((unsigned)p.own_tile), p.own_rows_shift = __builtin_ctz((unsigned)p.own_rows), p.own_units = c->Hkv * p.own_blocks;
   p.own_workers = (solo ? 8 : 2) * n_sm;
   p.own_extra = solo ? 2 : 1;
   p.own_min = p.own_extra + (solo ? 64 / p.own_tile : 1);  // a piece shorter than 64 keys is mostly its beginning
   // two blocks of 128 rows over the same keys where the groups have the rows for it: each tile then comes from memory half
   // as often; otherwise the two halves of a CTA take the keys in turn
   p.prefix_rows = p.groups > 0 && (int64_t)p.n * p.R > 128ll * p.groups ? 256 : 128;
-  p.prefix_tile = 128, p.prefix_workers = n_sm, p.prefix_extra = 1;
+  p.prefix_shift = __builtin_ctz((unsigned)p.prefix_rows), p.prefix_workers = n_sm, p.prefix_extra = 1;
   const int64_t keys = (int64_t)c->table_width * c->page_tokens, own_length = keys / p.own_tile + 2 + p.own_extra;
   const int64_t prefix_units = p.groups ? (int64_t)c->Hkv * (((int64_t)p.n * p.R + p.prefix_rows - 1) / p.prefix_rows + p.groups) : 0;
   const int64_t own_slots = (int64_t)p.n * c->Hkv * p.own_blocks + p.own_workers, prefix_slots = p.groups ? prefix_units + p.prefix_workers : 0;
   // positions on the lines (of one head and row block, and of all) are counted in 32 bits
-  FA4B_REQUIRE(p.n * own_length < INT32_MAX && prefix_units * (keys / p.prefix_tile + 2 + p.prefix_extra) < INT32_MAX && own_slots < INT32_MAX, FA4B_BAD_SHAPE,
+  FA4B_REQUIRE(p.n * own_length < INT32_MAX && prefix_units * (keys / kPagedPrefixTile + 2 + p.prefix_extra) < INT32_MAX && own_slots < INT32_MAX, FA4B_BAD_SHAPE,
                "%d rows over tables of %d pages of %d tokens are too many for one call", p.n, c->table_width, c->page_tokens);
   size_t off = 0;
   uint8_t* ws = static_cast<uint8_t*>(a->ws);

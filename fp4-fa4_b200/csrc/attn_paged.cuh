@@ -16,6 +16,7 @@
 namespace fa4b {
 
 constexpr int kPagedBox = 64;         // tokens of a page that one copy brings at most
+constexpr int kPagedPrefixTile = 128; // keys of a tile of the prefix units
 constexpr int kPagedAlign = 16;       // the shared part of a group ends on a multiple of this
 constexpr int kPagedMaxRows = 4096;   // sequences of one call
 constexpr int kPagedMaxT = 16;
@@ -34,7 +35,7 @@ struct PagedStart {  // where a worker begins
   int item, which, off, pad;             // sequence or group, its unit, position in the unit
 };
 struct PagedHead {
-  int64_t own_total, own_per, prefix_total, prefix_per;  // lengths of the lines and of their pieces
+  uint32_t own_total, own_per, prefix_total, prefix_per;  // lengths of the lines and of their pieces
 };
 
 struct PagedParams {
@@ -64,13 +65,14 @@ struct PagedParams {
   float2* prefix_ml;
   int own_rows, own_blocks, own_tile, own_extra, own_min, own_workers;  // rows of a unit, units per (sequence, kv head), keys of
                          // a tile, what a unit costs beside its tiles, the shortest piece, pieces
-  int prefix_rows, prefix_tile, prefix_extra, prefix_workers;
+  int own_shift, own_rows_shift, own_units;             // log2 of own_tile and own_rows; units of a sequence
+  int prefix_rows, prefix_shift, prefix_extra, prefix_workers;  // prefix_shift: log2 of prefix_rows
   uint32_t* status;
 };
 
 __device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
 __device__ __forceinline__ int own_tiles(const PagedParams& p, int first, int len) {
-  return len > first ? ceil_div(len, p.own_tile) - first / p.own_tile : 0;
+  return len > first ? ((len + p.own_tile - 1) >> p.own_shift) - (first >> p.own_shift) : 0;
 }
 
 // ---- numbers ----------------------------------------------------------------------------------------------------------
@@ -186,9 +188,9 @@ struct PagedUnit {
 
 template <bool kPrefix>
 struct PagedWalk {
-  int64_t left;     // positions of the line to go
+  int left;             // positions of the line to go
   int item, which, off;
-  int a0, a1, a2, a3, b0, b1, b2;  // the item's record
+  int a0, a1, a2, a3, b1, b2;  // the item's record
 
   __device__ __forceinline__ void load(const PagedParams& p) {
     const int4* r = kPrefix ? reinterpret_cast<const int4*>(p.group + item) : reinterpret_cast<const int4*>(p.seq + item);
@@ -196,24 +198,27 @@ struct PagedWalk {
     a0 = a.x, a1 = a.y, a2 = a.z, a3 = a.w;
     if constexpr (kPrefix) {
       const int4 b = r[1];
-      b0 = b.x, b1 = b.y, b2 = b.z;
+      b1 = b.y, b2 = b.z;
     }
   }
   __device__ __forceinline__ void start(const PagedParams& p, int worker) {
-    const int64_t total = kPrefix ? p.head->prefix_total : p.head->own_total, per = kPrefix ? p.head->prefix_per : p.head->own_per;
+    const PagedHead h = *p.head;
+    const uint32_t total = kPrefix ? h.prefix_total : h.own_total, per = kPrefix ? h.prefix_per : h.own_per;
     const int4 s = *reinterpret_cast<const int4*>((kPrefix ? p.prefix_start : p.own_start) + worker);
-    left = min(per, total - worker * per);
+    const uint64_t at = (uint64_t)worker * per;
+    left = at < total ? (int)min(per, total - (uint32_t)at) : 0;
     item = s.x, which = s.y, off = s.z;
     if (left > 0) load(p);
   }
-  __device__ __forceinline__ int tiles(const PagedParams& p) const { return kPrefix ? ceil_div(a0, p.prefix_tile) : own_tiles(p, a2, a1); }
+  __device__ __forceinline__ int tiles(const PagedParams& p) const {
+    return kPrefix ? (a0 + kPagedPrefixTile - 1) / kPagedPrefixTile : own_tiles(p, a2, a1);
+  }
   __device__ __forceinline__ bool done() const { return left <= 0; }
 
   // the unit at hand; then the walk stands at the next one
   __device__ __forceinline__ PagedUnit next(const PagedParams& p) {
     PagedUnit u;
-    const int n_tiles = tiles(p), extra = kPrefix ? p.prefix_extra : p.own_extra, length = n_tiles + extra;
-    const int upto = (int)min((int64_t)length, off + left);
+    const int extra = kPrefix ? p.prefix_extra : p.own_extra, length = tiles(p) + extra, upto = min(length, off + left);
     u.tile = max(off - extra, 0);
     u.tile_end = max(upto - extra, 0);
     int units;
@@ -221,20 +226,20 @@ struct PagedWalk {
       units = p.c.heads * b2;
       u.key_lo = 0, u.key_hi = u.key_all = a0;
       u.index = b1 + which;
-      u.head = which / b2;
-      u.row0 = (which - u.head * b2) * p.prefix_rows;
+      u.head = b2 == 1 ? which : which / b2;
+      u.row0 = (which - u.head * b2) << p.prefix_shift;
       u.rows = min(p.prefix_rows, a3 - u.row0);
       u.first_row = a2;
       u.table_slot = a1;
     } else {
-      units = p.c.heads * p.own_blocks;
+      units = p.own_units;
       u.key_lo = a2, u.key_hi = a1;
       u.key_all = max(a2, a1 - (p.T - 1));
-      const int skip = a2 / p.own_tile;
+      const int skip = a2 >> p.own_shift;
       u.tile += skip, u.tile_end += skip;
       u.index = item * units + which;
-      u.head = which / p.own_blocks;
-      u.row0 = (which - u.head * p.own_blocks) * p.own_rows;
+      u.head = p.own_blocks == 1 ? which : which / p.own_blocks;
+      u.row0 = (which - u.head * p.own_blocks) << p.own_rows_shift;
       u.rows = min(p.own_rows, p.R - u.row0);
       u.first_row = item;
       u.table_slot = a0;

@@ -16,11 +16,12 @@
 // TMEM columns: S 0 and 64 of the first half, 128 and 192 of the second (P in the lower 32 of each), O 256 and 384.
 #include "attn_paged.cuh"
 
+#include <cstddef>
 #include <type_traits>
 
 namespace fa4b {
 
-constexpr int kPrefixTile = 128, kStep = 64;
+constexpr int kPrefixTile = kPagedPrefixTile, kStep = 64;
 
 __device__ __forceinline__ void mma_f16_ss(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
   asm volatile("{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }" ::"r"(d_tmem), "l"(adesc),
@@ -58,6 +59,9 @@ struct PrefixSmem {
   uint64_t q_full, q_free, full[kRing], empty[kRing], raw_full[kRaw ? kRaw : 1], raw_empty[kRaw ? kRaw : 1], s_full[2][2], p_ready[2][2], o_done[2][2], drained;  // [half][score buffer]
   uint32_t tmem_base;
   volatile uint32_t abort_flag;
+  // the struct without what its alignment adds: beside a CTA of the own units each kilobyte counts
+  static constexpr int kUsed = ((kWide ? 2 : 1) + kRing) * kTile + (kRaw ? kRaw * kRawTile : 16) + (kWide ? 1 : 128) * 8 +
+                               8 * (2 + 2 * kRing + 2 * (kRaw ? kRaw : 1) + 13) + 16;
 };
 
 // Keys of step `step` of a half of a piece whose keys end at `keys`, counted from its first tile; 0 behind the last.
@@ -516,8 +520,9 @@ __global__ void __launch_bounds__(prefix_bound(kE4M3, kWide), 1) attn_prefix_ker
 template <int D, bool kE4M3, typename QT, bool kWide>
 static int launch_prefix_of(const PagedParams& p, const CUtensorMap& mk, const CUtensorMap& mv, cudaStream_t st) {
   auto kernel = attn_prefix_kernel<D, kE4M3, QT, kWide>;
-  constexpr int smem = (int)sizeof(PrefixSmem<D, kE4M3, kWide>);
-  static_assert(smem <= 227 * 1024, "shared memory of one CTA");
+  using Smem = PrefixSmem<D, kE4M3, kWide>;
+  constexpr int smem = PrefixSmem<D, kE4M3, kWide>::kUsed;
+  static_assert(smem >= (int)offsetof(Smem, abort_flag) + 4 && smem <= 227 * 1024, "shared memory of one CTA");
   static_assert(PrefixSmem<D, kE4M3, kWide>::kRing >= 3, "two tiles under way and one on its way");
   static std::atomic<uint64_t> allowed{0};
   if (int s = allow_smem(kernel, smem, allowed)) return s;

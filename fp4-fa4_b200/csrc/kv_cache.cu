@@ -764,6 +764,10 @@ int fa4b_kv_check_status(const fa4b_kv_cache* c, void* stream) {
   FA4B_CUDA(cudaMemsetAsync(v.work + kWorkStatus, 0, sizeof(host), st));
   const int32_t* attn = host + kKvAttnStatus;
   FA4B_REQUIRE(attn[0] != 1, FA4B_TIMEOUT, "a device-side wait of the attention over the cache ran out (site %d, block %d)", attn[1], attn[2]);
+  if (host[0] == kOk && attn[0] == 3) {
+    set_error("the batch's keys are too many for one call (%d tiles per kv head)", attn[1]);
+    return FA4B_BAD_ARG;
+  }
   if (host[0] == kOk) {
     set_error("the offsets of %d groups do not rise from 0 to at most the number of rows", attn[1]);
     return FA4B_BAD_ARG;
