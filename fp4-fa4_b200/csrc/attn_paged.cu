@@ -12,20 +12,20 @@
 namespace fa4b {
 
 // ---- plan -------------------------------------------------------------------------------------------------------------
-// One CTA runs this once, so what it costs is the fetching of its instructions: a line of eight that nobody has run yet takes
-// longer than the eight.  Hence one copy of what is used twice, no unrolling, shifts for divisions.
+// One CTA, and every other launch of the call waits for it.  Its warps mostly walk the same instructions, so that more of
+// them cost more than they help: 256 threads unless the batch is long (1024 took 7.1 us for 32 sequences, 256 take @@).
 __device__ __noinline__ uint32_t paged_div(uint32_t a, uint32_t b) { return a / b; }
 
-// Exclusive prefix sums of a[0..n) in shared memory, in place, by a block of 1024 threads; returns the total.
+// Exclusive prefix sums of a[0..n) in shared memory, in place, by the block; returns the total.
 __device__ __noinline__ int paged_scan(int* a, int n, int* warp_sums) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   int total = 0;
   __syncthreads();
 #pragma unroll 1
-  for (int base = 0; base < n; base += 1024) {
+  for (int base = 0; base < n; base += blockDim.x) {
     const int i = base + threadIdx.x, v = i < n ? a[i] : 0;
     int x = v;
-#pragma unroll 1
+#pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int y = __shfl_up_sync(0xffffffffu, x, o);
       if (lane >= o) x += y;
@@ -33,7 +33,7 @@ __device__ __noinline__ int paged_scan(int* a, int n, int* warp_sums) {
     if (n > 32) {  // the sums of the warps
       if (lane == 31) warp_sums[warp] = x;
       __syncthreads();
-      const int w = warp_sums[lane];
+      const int w = lane < warps ? warp_sums[lane] : 0;
       x += __reduce_add_sync(0xffffffffu, lane < warp ? w : 0);
       if (i < n) a[i] = total + x - v;
       total += __reduce_add_sync(0xffffffffu, w);
@@ -46,6 +46,43 @@ __device__ __noinline__ int paged_scan(int* a, int n, int* warp_sums) {
     __syncthreads();
   }
   return total;
+}
+
+// Sum over the block of what the threads give; everyone gets it.
+__device__ __noinline__ uint32_t paged_sum(uint32_t v, uint32_t* word) {
+  __syncthreads();
+  if (threadIdx.x == 0) *word = 0u;
+  __syncthreads();
+  v = __reduce_add_sync(0xffffffffu, v);
+  if ((threadIdx.x & 31) == 0 && v != 0u) atomicAdd(word, v);
+  __syncthreads();
+  return *word;
+}
+
+// How a line is cut.  Items i < n have units[i] (or `each`) units of tiles[i] tiles.  A piece that ends one unit and begins
+// another pays for the beginning of both (about `extra` tiles), so pieces that keep to one unit are best where they are no
+// longer for it: the shortest such length for which the pieces of all units are no more than the workers.  Otherwise the line
+// with `extra` tiles put before each unit is cut at equal distances.
+__device__ __noinline__ PagedCut paged_cut(const int* tiles, const int* units, int n, uint32_t each, uint32_t workers, uint32_t extra, uint32_t least,
+                                           uint32_t* word) {
+  uint32_t all = 0u, all_units = 0u;
+#pragma unroll 1
+  for (int i = threadIdx.x; i < n; i += blockDim.x) {
+    const uint32_t u = tiles[i] ? (units ? (uint32_t)units[i] : each) : 0u;
+    all += u * tiles[i], all_units += u;
+  }
+  all = paged_sum(all, word), all_units = paged_sum(all_units, word);
+  const uint32_t line = max(paged_div(all + all_units * extra + workers - 1, workers), least + extra);
+  uint32_t per = max(paged_div(all + workers - 1, workers), least);
+  if (all_units <= workers)
+#pragma unroll 1
+    for (int tries = 0; tries < 8 && per <= line; ++tries, ++per) {
+      uint32_t pieces = 0u;
+#pragma unroll 1
+      for (int i = threadIdx.x; i < n; i += blockDim.x) pieces += (units ? (uint32_t)units[i] : each) * paged_div(tiles[i] + per - 1, per);
+      if (paged_sum(pieces, word) <= workers) return {per, 0u, 1u};
+    }
+  return {line, extra, 0u};
 }
 
 // The last i in [0, n) with cum[i] <= x.
@@ -66,6 +103,7 @@ __host__ __device__ inline size_t paged_plan_words(int n, int groups) { return 4
 // of every member sees (so that no row of a prefix unit needs a mask) and to whole 16 keys; a group of one member has none.
 __global__ void __launch_bounds__(1024) paged_plan_kernel(const PagedParams p) {
   __shared__ int warp_sums[32], bad;
+  __shared__ uint32_t word;
   extern __shared__ int dyn[];
   int* own_cum = dyn;                  // [n]
   int* s_slot = own_cum + p.n;         // [n]
@@ -77,28 +115,30 @@ __global__ void __launch_bounds__(1024) paged_plan_kernel(const PagedParams p) {
   int* g_count = g_first + p.groups;   // [groups] members with keys, then whether a shared page is missing
   int* g_cum = g_count + p.groups;     // [groups]
   int* g_unit = g_cum + p.groups;      // [groups]
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, nt = blockDim.x;
   pdl_trigger();
   if (tid == 0) bad = 0;
 #pragma unroll 1
-  for (int g = tid; g < p.groups; g += 1024) g_shared[g] = INT_MAX, g_first[g] = INT_MAX, g_count[g] = 0;
+  for (int g = tid; g < p.groups; g += nt) g_shared[g] = INT_MAX, g_first[g] = INT_MAX, g_count[g] = 0;
   pdl_wait();
 #pragma unroll 1
-  for (int g = tid; g <= p.groups && p.groups > 0; g += 1024) offsets[g] = p.offsets[g];
+  for (int g = tid; g <= p.groups && p.groups > 0; g += nt) offsets[g] = p.offsets[g];
 #pragma unroll 1
-  for (int i = tid; i < p.n; i += 1024) {
+  for (int i = tid; i < p.n; i += nt) {
     const int slot = p.seqs ? p.seqs[i] : i;
     s_slot[i] = slot, s_group[i] = p.groups > 0 ? -1 : 0;
     s_len[i] = (uint32_t)slot < (uint32_t)p.c.max_seqs ? min(max(p.c.lens[slot], 0), p.c.width << p.c.page_shift) : 0;
   }
   __syncthreads();
+  int prefix_total = 0;
+  PagedCut prefix{1u, 0u, 0u};
   if (p.groups > 0) {
     // groups have to lie behind one another: the slots of their units are counted on it
 #pragma unroll 1
-    for (int g = tid; g < p.groups; g += 1024)
+    for (int g = tid; g < p.groups; g += nt)
       if (offsets[g] < 0 || offsets[g + 1] < offsets[g] || offsets[g + 1] > p.n) bad = 1;
 #pragma unroll 1
-    for (int i = tid; i < p.n; i += 1024) {
+    for (int i = tid; i < p.n; i += nt) {
       const int g = paged_find(offsets, p.groups, (uint32_t)i);  // the last group that begins at or before i
       if (i < offsets[g] || i >= offsets[g + 1]) continue;
       s_group[i] = g;
@@ -112,42 +152,56 @@ __global__ void __launch_bounds__(1024) paged_plan_kernel(const PagedParams p) {
     if (bad != 0) {
       if (tid == 0 && atomicCAS(p.status, 0u, 2u) == 0u) p.status[1] = (uint32_t)p.groups;
 #pragma unroll 1
-      for (int i = tid; i < p.n; i += 1024) s_group[i] = -1;
+      for (int i = tid; i < p.n; i += nt) s_group[i] = -1;
     }
 #pragma unroll 1
-    for (int g = tid; g < p.groups; g += 1024) {
+    for (int g = tid; g < p.groups; g += nt) {
       g_shared[g] = g_count[g] > 1 && bad == 0 ? min(max(p.shared[g], 0), g_shared[g]) & ~(kPagedAlign - 1) : 0;
       g_count[g] = 0;
     }
     __syncthreads();
     // A shared page that the table does not name: the group goes without, the own units know how to leave such a page out.
-    const int shift = p.groups >= 32 ? 5 : 10 - (31 - __clz(2 * p.groups - 1));  // 2^shift threads for a group: a warp at least
+    const int shift = max(5, 31 - __clz(nt) - (31 - __clz(2 * p.groups - 1)));  // 2^shift threads for a group: a warp at least
 #pragma unroll 1
-    for (int g = tid >> shift; g < p.groups; g += 1024 >> shift) {
+    for (int g = tid >> shift; g < p.groups; g += nt >> shift) {
       const int pages = (g_shared[g] + p.c.page_tokens - 1) >> p.c.page_shift;
       const int32_t* row = p.c.table + (pages ? (int64_t)s_slot[g_first[g]] * p.c.table_stride : 0);
-#pragma unroll 2
-      for (int j = tid & ((1 << shift) - 1); j < pages; j += 1 << shift)
-        if ((uint32_t)row[j] >= (uint32_t)p.c.pages) g_count[g] = 1;
+      bool missing = false;
+#pragma unroll 1
+      for (int j = tid & ((1 << shift) - 1); j < pages; j += 8 << shift) {
+        int e[8];  // all on their way at once
+#pragma unroll
+        for (int k = 0; k < 8; ++k) e[k] = j + (k << shift) < pages ? row[j + (k << shift)] : 0;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) missing |= (uint32_t)e[k] >= (uint32_t)p.c.pages;
+      }
+      if (missing) g_count[g] = 1;
     }
     __syncthreads();
 #pragma unroll 1
-    for (int g = tid; g < p.groups; g += 1024) {
+    for (int g = tid; g < p.groups; g += nt) {
       const int shared = g_count[g] ? 0 : g_shared[g];
       const int units = shared ? p.c.heads * (((offsets[g + 1] - offsets[g]) * p.R + p.prefix_rows - 1) >> p.prefix_shift) : 0;
       g_shared[g] = shared;
       g_unit[g] = units;
-      g_cum[g] = units * ((shared + kPagedPrefixTile - 1) / kPagedPrefixTile + p.prefix_extra);
+      g_cum[g] = (shared + kPagedPrefixTile - 1) / kPagedPrefixTile;
     }
-  }
-  const int prefix_total = paged_scan(g_cum, p.groups, warp_sums);
-  paged_scan(g_unit, p.groups, warp_sums);
+    __syncthreads();
+    prefix = paged_cut(g_cum, g_unit, p.groups, 0u, p.prefix_workers, p.prefix_extra, 1u, &word);
 #pragma unroll 1
-  for (int i = tid; i < p.n; i += 1024) {
-    const int g = s_group[i];
-    const int tiles = g < 0 ? 0 : own_tiles(p, p.groups > 0 && s_len[i] > 0 ? g_shared[g] : 0, s_len[i]);
-    own_cum[i] = tiles + (tiles ? p.own_extra : 0);
+    for (int g = tid; g < p.groups; g += nt) g_cum[g] = g_unit[g] * (int)prefix.length(g_cum[g]);
+    prefix_total = paged_scan(g_cum, p.groups, warp_sums);
+    paged_scan(g_unit, p.groups, warp_sums);
   }
+#pragma unroll 1
+  for (int i = tid; i < p.n; i += nt) {
+    const int g = s_group[i];
+    own_cum[i] = g < 0 ? 0 : own_tiles(p, p.groups > 0 && s_len[i] > 0 ? g_shared[g] : 0, s_len[i]);
+  }
+  __syncthreads();
+  const PagedCut own = paged_cut(own_cum, nullptr, p.n, p.own_units, p.own_workers, p.own_extra, p.own_min, &word);
+#pragma unroll 1
+  for (int i = tid; i < p.n; i += nt) own_cum[i] = own.length(own_cum[i]);
   const int own_total = paged_scan(own_cum, p.n, warp_sums);
   // the line of the own units has p.own_units of each entry of own_cum
   uint32_t line = (uint32_t)own_total * p.own_units;
@@ -155,38 +209,24 @@ __global__ void __launch_bounds__(1024) paged_plan_kernel(const PagedParams p) {
     if (tid == 0 && atomicCAS(p.status, 0u, 3u) == 0u) p.status[1] = (uint32_t)own_total;
     line = 0u;
   }
-  const uint32_t own_per = max(paged_div(line + p.own_workers - 1, p.own_workers), (uint32_t)p.own_min);
-  const uint32_t prefix_per = max(paged_div(prefix_total + p.prefix_workers - 1, p.prefix_workers), 1u);
-  if (tid == 0) *p.head = {line, own_per, (uint32_t)prefix_total, prefix_per};
+  if (tid == 0) *p.head = {{line, own}, {(uint32_t)prefix_total, prefix}};
   // all is known: the records
 #pragma unroll 1
-  for (int i = tid; i < p.n; i += 1024) {
+  for (int i = tid; i < p.n; i += nt) {
     const int g = max(s_group[i], 0), first = p.groups > 0 && s_len[i] > 0 ? g_shared[g] : 0;
     int4* r = reinterpret_cast<int4*>(p.seq + i);
     r[0] = make_int4(s_slot[i], s_len[i], first, own_cum[i]);
+    p.own_cum[i] = own_cum[i];
     r[2] = make_int4(s_group[i] < 0 || line == 0u && own_total > 0, 0, 0, 0);
     if (first > 0) r[1] = make_int4(offsets[g], ((offsets[g + 1] - offsets[g]) * p.R + p.prefix_rows - 1) >> p.prefix_shift, g_unit[g], g_cum[g]);
   }
 #pragma unroll 1
-  for (int w = tid; w < p.own_workers && w * own_per < line; w += 1024) {
-    const uint32_t at = w * own_per;
-    const int i = paged_find(own_cum, p.n, paged_div(at, p.own_units));
-    const uint32_t length = (i + 1 < p.n ? own_cum[i + 1] : own_total) - own_cum[i], off = at - own_cum[i] * p.own_units, which = paged_div(off, length);
-    p.own_start[w] = {i, (int)which, (int)(off - which * length), 0};
-  }
-#pragma unroll 1
-  for (int g = tid; g < p.groups; g += 1024) {
+  for (int g = tid; g < p.groups; g += nt) {
     int4* r = reinterpret_cast<int4*>(p.group + g);
     const int shared = g_shared[g], rows = (offsets[g + 1] - offsets[g]) * p.R;
     r[0] = make_int4(shared, shared ? s_slot[g_first[g]] : 0, offsets[g], rows);
+    p.g_cum[g] = g_cum[g];
     r[1] = make_int4(g_cum[g], g_unit[g], (rows + p.prefix_rows - 1) >> p.prefix_shift, 0);
-  }
-#pragma unroll 1
-  for (int w = tid; w < p.prefix_workers && w * prefix_per < (uint32_t)prefix_total; w += 1024) {
-    const uint32_t at = w * prefix_per;
-    const int g = paged_find(g_cum, p.groups, at);
-    const uint32_t length = (g_shared[g] + kPagedPrefixTile - 1) / kPagedPrefixTile + p.prefix_extra, off = at - g_cum[g], which = paged_div(off, length);
-    p.prefix_start[w] = {g, (int)which, (int)(off - which * length), 0};
   }
 }
 
@@ -729,15 +769,17 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PagedParams p) {
     if (s.first > 0) {
       const int row = ((int)i - s.g_row) * p.R + r, block = row >> p.prefix_shift, which = head * s.g_blocks + block;
       const int tiles = (s.first + kPagedPrefixTile - 1) / kPagedPrefixTile;
-      const uint32_t from = (uint32_t)(s.g_cum + which * (tiles + p.prefix_extra) + p.prefix_extra), worker = from / line.prefix_per;
-      n_prefix = (int)((from + tiles - 1) / line.prefix_per - worker) + 1;
+      const PagedCut cut = line.prefix.cut;
+      const uint32_t from = s.g_cum + which * cut.length(tiles) + cut.extra, worker = from / cut.per;
+      n_prefix = (int)((from + tiles - 1) / cut.per - worker) + 1;
       prefix_slot = s.g_unit + which + (int64_t)worker;
       prefix_row = row & (p.prefix_rows - 1);
     }
     const int block = r >> p.own_rows_shift, which = head * p.own_blocks + block, tiles = own_tiles(p, s.first, len);
-    const uint32_t from = (uint32_t)(s.cum * p.own_units + which * (tiles + p.own_extra) + p.own_extra), worker = from / line.own_per;
+    const PagedCut cut = line.own.cut;
+    const uint32_t from = s.cum * p.own_units + which * cut.length(tiles) + cut.extra, worker = from / cut.per;
     own_slot = (int64_t)i * p.own_units + which + worker;
-    n_own = (int)((from + tiles - 1) / line.own_per - worker) + 1;
+    n_own = (int)((from + tiles - 1) / cut.per - worker) + 1;
     own_row = r & (p.own_rows - 1);
   }
   pdl_wait();
@@ -821,7 +863,7 @@ static int launch_paged(const PagedParams& p, const PagedMaps& m, cudaStream_t s
   static std::atomic<uint64_t> allowed[4];
   if (smem > 48 * 1024)
     if (int s = allow_smem(paged_plan_kernel, 4 * (int)paged_plan_words(kPagedMaxRows, kPagedMaxRows), allowed[3])) return s;
-  FA4B_CUDA(launch_overlapped(paged_plan_kernel, 1, 1024, smem, st, p));
+  FA4B_CUDA(launch_overlapped(paged_plan_kernel, 1, p.n <= 512 ? 256 : 1024, smem, st, p));
   if (p.groups > 0)
     if (int s = launch_prefix(p, D, kE4M3, std::is_same<QT, TagF16>::value, m.prefix_k, m.prefix_v, st)) return s;
   const int s = p.own_rows == 16   ? launch_units<SoloSmem<D, kE4M3>>(attn_solo_kernel<D, kE4M3, QT>, p, m.own_k, m.own_v, p.own_workers / 4, 128, st, allowed[0])
@@ -869,16 +911,16 @@ static int paged_params(const fa4b_kv_cache* c, const fa4b_attn_paged_args* a, P
   p.own_shift = __builtin_ctz((unsigned)p.own_tile), p.own_rows_shift = __builtin_ctz((unsigned)p.own_rows), p.own_units = c->Hkv * p.own_blocks;
   p.own_workers = (solo ? 8 : 2) * n_sm;
   p.own_extra = solo ? 2 : 1;
-  p.own_min = p.own_extra + (solo ? 64 / p.own_tile : 1);  // a piece shorter than 64 keys is mostly its beginning
+  p.own_min = solo ? 64 / p.own_tile : 1;  // a piece shorter than 64 keys is mostly its beginning
   // two blocks of 128 rows over the same keys where the groups have the rows for it: each tile then comes from memory half
   // as often; otherwise the two halves of a CTA take the keys in turn
   p.prefix_rows = p.groups > 0 && (int64_t)p.n * p.R > 128ll * p.groups ? 256 : 128;
-  p.prefix_shift = __builtin_ctz((unsigned)p.prefix_rows), p.prefix_workers = n_sm, p.prefix_extra = 1;
-  const int64_t keys = (int64_t)c->table_width * c->page_tokens, own_length = keys / p.own_tile + 2 + p.own_extra;
+  p.prefix_shift = __builtin_ctz((unsigned)p.prefix_rows), p.prefix_workers = n_sm, p.prefix_extra = 3;
+  const int64_t keys = (int64_t)c->table_width * c->page_tokens, own_length = 2 * (keys / p.own_tile) + 2 + p.own_extra;
   const int64_t prefix_units = p.groups ? (int64_t)c->Hkv * (((int64_t)p.n * p.R + p.prefix_rows - 1) / p.prefix_rows + p.groups) : 0;
   const int64_t own_slots = (int64_t)p.n * c->Hkv * p.own_blocks + p.own_workers, prefix_slots = p.groups ? prefix_units + p.prefix_workers : 0;
   // positions on the lines (of one head and row block, and of all) are counted in 32 bits
-  FA4B_REQUIRE(p.n * own_length < INT32_MAX && prefix_units * (keys / kPagedPrefixTile + 2 + p.prefix_extra) < INT32_MAX && own_slots < INT32_MAX, FA4B_BAD_SHAPE,
+  FA4B_REQUIRE(p.n * own_length < INT32_MAX && prefix_units * (2 * (keys / kPagedPrefixTile) + 2 + p.prefix_extra) < INT32_MAX && own_slots < INT32_MAX, FA4B_BAD_SHAPE,
                "%d rows over tables of %d pages of %d tokens are too many for one call", p.n, c->table_width, c->page_tokens);
   size_t off = 0;
   uint8_t* ws = static_cast<uint8_t*>(a->ws);
@@ -891,8 +933,8 @@ static int paged_params(const fa4b_kv_cache* c, const fa4b_attn_paged_args* a, P
   p.head = reinterpret_cast<PagedHead*>(take(sizeof(PagedHead)));
   p.seq = reinterpret_cast<PagedSeq*>(take(sizeof(PagedSeq) * n));
   p.group = reinterpret_cast<PagedGroup*>(take(sizeof(PagedGroup) * g));
-  p.own_start = reinterpret_cast<PagedStart*>(take(sizeof(PagedStart) * p.own_workers));
-  p.prefix_start = reinterpret_cast<PagedStart*>(take(sizeof(PagedStart) * p.prefix_workers));
+  p.own_cum = reinterpret_cast<int*>(take(4 * n));
+  p.g_cum = reinterpret_cast<int*>(take(4 * g));
   p.own_ml = reinterpret_cast<float2*>(take((size_t)own_slots * p.own_rows * 8));
   p.prefix_ml = reinterpret_cast<float2*>(take((size_t)prefix_slots * p.prefix_rows * 8));
   p.own_acc = reinterpret_cast<float*>(take((size_t)own_slots * p.own_rows * c->D * 4));

@@ -3,8 +3,8 @@
 // A call has two kinds of work.  "Own" units: one sequence, one kv head, up to own_rows of its T x (Hq / Hkv) query rows,
 // over the keys that are the sequence's own.  "Prefix" units: one group, one kv head, up to prefix_rows of the group's
 // rows, over the keys that its members share, so that those are read once for all of them.  Either kind's units are
-// laid end to end as one line, each as long as its tiles of keys plus what starting a unit costs, and the line is cut into
-// equal pieces, one per worker (a warp, or a CTA): long and short sequences load every SM alike.  What a worker has of a
+// laid end to end as one line of tiles of keys, and the line is cut into pieces of equal length, one per worker (a warp, or a
+// CTA): long and short sequences load every SM alike.  What a worker has of a
 // unit goes to a slot of its own (unit + worker: either grows along the line, so the sum names the pair).  The last launch
 // joins the slots of a row: out = sum 2^(m_i - M) acc_i / sum 2^(m_i - M) l_i.
 #pragma once
@@ -21,7 +21,8 @@ constexpr int kPagedAlign = 16;       // the shared part of a group ends on a mu
 constexpr int kPagedMaxRows = 4096;   // sequences of one call
 constexpr int kPagedMaxT = 16;
 
-// What the plan writes down, so that a worker knows all about its first unit after one round of loads.
+// What the plan writes down: a worker finds its first unit in one round of loads for up to 32 sequences (two for 1024), and
+// has its record in one more.
 struct PagedSeq {    // one row of the batch
   int slot, len, first, cum;             // first key that is its own; length of the line before it, of one (kv head, row block)
   int g_row, g_blocks, g_unit, g_cum;  // its group's first row, row blocks, first unit, length of the line before it
@@ -31,11 +32,20 @@ struct PagedGroup {
   int shared, slot, row, rows;           // keys; whose row of the table names the pages; first row of the batch, query rows per kv head
   int cum, unit, blocks, pad;
 };
-struct PagedStart {  // where a worker begins
-  int item, which, off, pad;             // sequence or group, its unit, position in the unit
+// How a line is cut: at multiples of `per`.  Either every unit begins at one (`whole`: a unit's length is rounded up to pieces,
+// and no piece has parts of two), or units follow one another with `extra` positions before the tiles of each.
+struct PagedCut {
+  uint32_t per, extra, whole;
+  __device__ __forceinline__ uint32_t length(uint32_t tiles) const {  // of a unit on the line
+    return tiles == 0u ? 0u : whole ? (tiles + per - 1u) / per * per : tiles + extra;
+  }
+};
+struct PagedLine {
+  uint32_t total;
+  PagedCut cut;
 };
 struct PagedHead {
-  uint32_t own_total, own_per, prefix_total, prefix_per;  // lengths of the lines and of their pieces
+  PagedLine own, prefix;
 };
 
 struct PagedParams {
@@ -57,8 +67,8 @@ struct PagedParams {
   PagedHead* head;       // the plan
   PagedSeq* seq;         // [n]
   PagedGroup* group;     // [groups]
-  PagedStart* own_start; // [own_workers]
-  PagedStart* prefix_start;
+  int* own_cum;          // [n] the line before each sequence, of one unit of each
+  int* g_cum;            // [groups] the line before each group
   float* own_acc;        // [slots][own_rows][D]
   float2* own_ml;        // [slots][own_rows]: running maximum (log2 domain), sum
   float* prefix_acc;
@@ -190,6 +200,7 @@ template <bool kPrefix>
 struct PagedWalk {
   int left;             // positions of the line to go
   int item, which, off;
+  PagedCut cut;
   int a0, a1, a2, a3, b1, b2;  // the item's record
 
   __device__ __forceinline__ void load(const PagedParams& p) {
@@ -201,14 +212,34 @@ struct PagedWalk {
       b1 = b.y, b2 = b.z;
     }
   }
-  __device__ __forceinline__ void start(const PagedParams& p, int worker) {
-    const PagedHead h = *p.head;
-    const uint32_t total = kPrefix ? h.prefix_total : h.own_total, per = kPrefix ? h.prefix_per : h.own_per;
-    const int4 s = *reinterpret_cast<const int4*>((kPrefix ? p.prefix_start : p.own_start) + worker);
-    const uint64_t at = (uint64_t)worker * per;
-    left = at < total ? (int)min(per, total - (uint32_t)at) : 0;
-    item = s.x, which = s.y, off = s.z;
-    if (left > 0) load(p);
+  __device__ __forceinline__ void start(const PagedParams& p, int worker) {  // whole warps
+    const int* cum = kPrefix ? p.g_cum : p.own_cum;
+    const int n = kPrefix ? p.groups : p.n, lane = threadIdx.x & 31;
+    // the first round does not wait for the head of the plan: 32 places at equal distances
+    int step = (n + 31) >> 5, first = lane * step < n ? cum[lane * step] : INT_MAX;
+    const int4 h = *reinterpret_cast<const int4*>(kPrefix ? &p.head->prefix : &p.head->own);
+    const uint32_t total = h.x;
+    cut = {(uint32_t)h.y, (uint32_t)h.z, (uint32_t)h.w};
+    const uint64_t from = (uint64_t)worker * cut.per;
+    left = from < total ? (int)min(cut.per, total - (uint32_t)from) : 0;
+    item = which = off = 0;
+    if (left == 0) return;
+    const uint32_t at = (uint32_t)from, x = kPrefix ? at : at / (uint32_t)p.own_units;
+    int base = 0, cum_base = 0, range = n;
+    for (;;) {  // the last item that begins at or before x
+      const int k = 31 - __clz(__ballot_sync(0xffffffffu, (uint32_t)first <= x));
+      cum_base = __shfl_sync(0xffffffffu, first, k);
+      base += k * step;
+      range = min(step, range - k * step);
+      if (step == 1) break;
+      step = (range + 31) >> 5;
+      first = lane * step < range ? cum[base + lane * step] : INT_MAX;
+    }
+    item = base;
+    load(p);
+    const uint32_t length = cut.length(tiles(p)), rest = at - (uint32_t)cum_base * (kPrefix ? 1u : (uint32_t)p.own_units);
+    which = (int)(rest / length);
+    off = (int)(rest - which * length);
   }
   __device__ __forceinline__ int tiles(const PagedParams& p) const {
     return kPrefix ? (a0 + kPagedPrefixTile - 1) / kPagedPrefixTile : own_tiles(p, a2, a1);
@@ -218,9 +249,9 @@ struct PagedWalk {
   // the unit at hand; then the walk stands at the next one
   __device__ __forceinline__ PagedUnit next(const PagedParams& p) {
     PagedUnit u;
-    const int extra = kPrefix ? p.prefix_extra : p.own_extra, length = tiles(p) + extra, upto = min(length, off + left);
+    const int n_tiles = tiles(p), extra = (int)cut.extra, length = (int)cut.length(n_tiles), upto = min(length, off + left);
     u.tile = max(off - extra, 0);
-    u.tile_end = max(upto - extra, 0);
+    u.tile_end = max(min(upto - extra, n_tiles), u.tile);
     int units;
     if constexpr (kPrefix) {
       units = p.c.heads * b2;

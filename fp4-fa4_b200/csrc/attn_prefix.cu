@@ -48,8 +48,7 @@ struct PrefixSmem {
   static constexpr int kSub = 128 * 128;                 // 128 rows of 64 values
   static constexpr int kTile = D / 64 * kSub;            // K or V of 128 keys, or 128 query rows
   static constexpr int kRawTile = 128 * D;
-  // without E4M3 tiles to turn, a narrow CTA leaves room for one of the own units beside it
-  static constexpr int kRoom = (kWide || kE4M3 ? 224 : 128) * 1024 - (kWide ? 2 : 1) * kTile;
+  static constexpr int kRoom = 224 * 1024 - (kWide ? 2 : 1) * kTile;
   static constexpr int kRaw = kE4M3 ? 4 : 0;
   static constexpr int kRing = (kRoom - kRaw * kRawTile) / kTile > 8 ? 8 : (kRoom - kRaw * kRawTile) / kTile;
   alignas(1024) uint8_t q[kWide ? 2 : 1][kTile];
@@ -59,7 +58,7 @@ struct PrefixSmem {
   uint64_t q_full, q_free, full[kRing], empty[kRing], raw_full[kRaw ? kRaw : 1], raw_empty[kRaw ? kRaw : 1], s_full[2][2], p_ready[2][2], o_done[2][2], drained;  // [half][score buffer]
   uint32_t tmem_base;
   volatile uint32_t abort_flag;
-  // the struct without what its alignment adds: beside a CTA of the own units each kilobyte counts
+  // the struct without what its alignment adds
   static constexpr int kUsed = ((kWide ? 2 : 1) + kRing) * kTile + (kRaw ? kRaw * kRawTile : 16) + (kWide ? 1 : 128) * 8 +
                                8 * (2 + 2 * kRing + 2 * (kRaw ? kRaw : 1) + 13) + 16;
 };
@@ -71,11 +70,8 @@ __device__ __forceinline__ int step_keys(int keys, int half, int step) {
   return max(0, min(kStep, keys - first));
 }
 
-// Threads of a CTA: eight warps of softmax, one for pages, two for products, four that turn E4M3 codes.  A narrow 16-bit CTA
-// is held to 96 registers (the bound of 576 threads), so that a CTA of own units with up to 224 fits beside it in
-// each quarter of the SM (3 x 96 + 224 = 512).
+// eight warps of softmax, one for pages, two for products, four that turn E4M3 codes
 __host__ __device__ constexpr int prefix_threads(bool e4m3) { return e4m3 ? 480 : 352; }
-__host__ __device__ constexpr int prefix_bound(bool e4m3, bool wide) { return e4m3 || wide ? prefix_threads(e4m3) : 576; }
 
 // The accumulator of a row scaled where it lies, behind the product of the step before (`done`, `parity`).  A barrier of its
 // own for each score buffer: a step's scores are only there when the product of the step before last is, so that a
@@ -97,35 +93,26 @@ __device__ __forceinline__ void rescale_o(uint32_t to, float f, Smem& s, uint64_
 }
 
 // One step of a row: scores out of TMEM, probabilities back in as 16-bit.  keys: 16 to 64 in sixteens; kFull: 64 (with
-// the other case in the same code every exponential hangs on a branch: 36 cycles a pair).  kLean: 32 scores in
-// registers at a time, read once for their maximum and once more to be used.
-template <int D, typename Mma, bool kLean, bool kFull, typename Smem>
+// the other case in the same code every exponential hangs on a branch).
+template <int D, typename Mma, bool kFull, typename Smem>
 __device__ __forceinline__ void softmax_step(uint32_t ts, uint32_t to, int keys, float scale, float& m, float& l, Smem& s, uint64_t* before,
                                              uint32_t parity_before, bool first, uint32_t* status) {
-  constexpr int kHeld = kLean ? 1 : 2;
-  uint32_t a[kHeld][32];
-  auto absent = [&](int c, uint32_t (&x)[32]) {  // the rest of the buffer is what an earlier step left
-#pragma unroll
-    for (int j = 0; j < 32; j += 16)
-      if (keys <= c * 32 + j)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) x[j + e] = 0xff800000u;
-  };
+  uint32_t a[2][32];
+  tmem_ld32(ts, a[0]);
+  tmem_ld32(ts + 32, a[1]);
+  tmem_ld_wait(a[0]);
+  tmem_ld_wait(a[1]);
   float t0 = -INFINITY, t1 = -INFINITY;
-  if constexpr (!kLean) {
-    tmem_ld32(ts, a[0]);
-    tmem_ld32(ts + 32, a[1]);
-    tmem_ld_wait(a[0]);
-    tmem_ld_wait(a[1]);
-  }
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
-    uint32_t(&x)[32] = a[kLean ? 0 : c];
-    if constexpr (kLean) {
-      tmem_ld32(ts + c * 32, x);
-      tmem_ld_wait(x);
+    uint32_t(&x)[32] = a[c];
+    if constexpr (!kFull) {  // the rest of the buffer is what an earlier step left
+#pragma unroll
+      for (int j = 0; j < 32; j += 16)
+        if (keys <= c * 32 + j)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) x[j + e] = 0xff800000u;
     }
-    if constexpr (!kFull) absent(c, x);
 #pragma unroll
     for (int j = 0; j < 32; j += 4) {
       t0 = max3(t0, __uint_as_float(x[j]), __uint_as_float(x[j + 1]));
@@ -144,11 +131,7 @@ __device__ __forceinline__ void softmax_step(uint32_t ts, uint32_t to, int keys,
   float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
-    uint32_t(&x)[32] = a[kLean ? 0 : c];
-    if constexpr (kLean) {
-      tmem_ld32(ts + c * 32, x);
-      tmem_ld_wait(x);
-    }
+    uint32_t(&x)[32] = a[c];
     uint32_t out[16];
 #pragma unroll
     for (int j = 0; j < 32; j += 4) {
@@ -169,7 +152,7 @@ __device__ __forceinline__ void softmax_step(uint32_t ts, uint32_t to, int keys,
 }
 
 template <int D, bool kE4M3, typename QT, bool kWide>
-__global__ void __launch_bounds__(prefix_bound(kE4M3, kWide), 1) attn_prefix_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_k,
+__global__ void __launch_bounds__(prefix_threads(kE4M3), 1) attn_prefix_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_k,
                                                                            const __grid_constant__ CUtensorMap map_v) {
   using Smem = PrefixSmem<D, kE4M3, kWide>;
   using Mma = typename std::conditional<kE4M3, TagF16, QT>::type;
@@ -444,9 +427,9 @@ __global__ void __launch_bounds__(prefix_bound(kE4M3, kWide), 1) attn_prefix_ker
           uint64_t* before = &s.o_done[w][buf ^ 1];
           const uint32_t parity_before = (phases >> (buf ^ 1) & 1u) ^ 1u;
           if (keys == kStep)
-            softmax_step<D, Mma, !kWide && !kE4M3, true>(ts + buf * kStep, to, keys, scale, m, l, s, before, parity_before, step == 0, p.status);
+            softmax_step<D, Mma, true>(ts + buf * kStep, to, keys, scale, m, l, s, before, parity_before, step == 0, p.status);
           else
-            softmax_step<D, Mma, !kWide && !kE4M3, false>(ts + buf * kStep, to, keys, scale, m, l, s, before, parity_before, step == 0, p.status);
+            softmax_step<D, Mma, false>(ts + buf * kStep, to, keys, scale, m, l, s, before, parity_before, step == 0, p.status);
         }
         tc_fence_before();
         mbar_arrive_warp(&s.p_ready[w][buf]);
