@@ -12,66 +12,45 @@
 namespace fa4b {
 
 // ---- plan -------------------------------------------------------------------------------------------------------------
-// One CTA, and every other launch of the call waits for it.  Its warps mostly walk the same instructions, so that more of
-// them cost more than they help: 256 threads unless the batch is long (1024 took 7.1 us for 32 sequences, 256 take @@).
+// One CTA, and every other launch of the call waits for it.  More warps would walk the same instructions and cost more than
+// they help (1024 threads took 7.1 us for 32 sequences), and what is sums over items a warp does alone: three of them at once
+// for the three lines of sums, without a barrier.
+constexpr int kPlanThreads = 256;
+
 __device__ __noinline__ uint32_t paged_div(uint32_t a, uint32_t b) { return a / b; }
 
-// Exclusive prefix sums of a[0..n) in shared memory, in place, by the block; returns the total.
-__device__ __noinline__ int paged_scan(int* a, int n, int* warp_sums) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+// Exclusive prefix sums of a[0..n) in shared memory, in place, by one warp; returns the total.
+__device__ __noinline__ int warp_scan(int* a, int n) {
+  const int lane = threadIdx.x & 31;
   int total = 0;
-  __syncthreads();
 #pragma unroll 1
-  for (int base = 0; base < n; base += blockDim.x) {
-    const int i = base + threadIdx.x, v = i < n ? a[i] : 0;
+  for (int base = 0; base < n; base += 32) {
+    const int i = base + lane, v = i < n ? a[i] : 0;
     int x = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int y = __shfl_up_sync(0xffffffffu, x, o);
       if (lane >= o) x += y;
     }
-    if (n > 32) {  // the sums of the warps
-      if (lane == 31) warp_sums[warp] = x;
-      __syncthreads();
-      const int w = lane < warps ? warp_sums[lane] : 0;
-      x += __reduce_add_sync(0xffffffffu, lane < warp ? w : 0);
-      if (i < n) a[i] = total + x - v;
-      total += __reduce_add_sync(0xffffffffu, w);
-    } else {
-      if (warp == 0 && i < n) a[i] = x - v;
-      if (threadIdx.x == 31) warp_sums[0] = x;
-      __syncthreads();
-      total = warp_sums[0];
-    }
-    __syncthreads();
+    if (i < n) a[i] = total + x - v;
+    total += __shfl_sync(0xffffffffu, x, 31);
   }
   return total;
 }
 
-// Sum over the block of what the threads give; everyone gets it.
-__device__ __noinline__ uint32_t paged_sum(uint32_t v, uint32_t* word) {
-  __syncthreads();
-  if (threadIdx.x == 0) *word = 0u;
-  __syncthreads();
-  v = __reduce_add_sync(0xffffffffu, v);
-  if ((threadIdx.x & 31) == 0 && v != 0u) atomicAdd(word, v);
-  __syncthreads();
-  return *word;
-}
-
-// How a line is cut.  Items i < n have units[i] (or `each`) units of tiles[i] tiles.  A piece that ends one unit and begins
-// another pays for the beginning of both (about `extra` tiles), so pieces that keep to one unit are best where they are no
+// How a line is cut, by one warp.  Items i < n have units[i] (or `each`) units of tiles[i] tiles.  A piece that ends one unit
+// and begins another pays for the beginning of both (about `extra` tiles), so pieces that keep to one unit are best where they are no
 // longer for it: the shortest such length for which the pieces of all units are no more than the workers.  Otherwise the line
 // with `extra` tiles put before each unit is cut at equal distances.
-__device__ __noinline__ PagedCut paged_cut(const int* tiles, const int* units, int n, uint32_t each, uint32_t workers, uint32_t extra, uint32_t least,
-                                           uint32_t* word) {
+__device__ __noinline__ PagedCut warp_cut(const int* tiles, const int* units, int n, uint32_t each, uint32_t workers, uint32_t extra, uint32_t least) {
+  const int lane = threadIdx.x & 31;
   uint32_t all = 0u, all_units = 0u;
 #pragma unroll 1
-  for (int i = threadIdx.x; i < n; i += blockDim.x) {
+  for (int i = lane; i < n; i += 32) {
     const uint32_t u = tiles[i] ? (units ? (uint32_t)units[i] : each) : 0u;
     all += u * tiles[i], all_units += u;
   }
-  all = paged_sum(all, word), all_units = paged_sum(all_units, word);
+  all = __reduce_add_sync(0xffffffffu, all), all_units = __reduce_add_sync(0xffffffffu, all_units);
   const uint32_t line = max(paged_div(all + all_units * extra + workers - 1, workers), least + extra);
   uint32_t per = max(paged_div(all + workers - 1, workers), least);
   if (all_units <= workers)
@@ -79,8 +58,8 @@ __device__ __noinline__ PagedCut paged_cut(const int* tiles, const int* units, i
     for (int tries = 0; tries < 8 && per <= line; ++tries, ++per) {
       uint32_t pieces = 0u;
 #pragma unroll 1
-      for (int i = threadIdx.x; i < n; i += blockDim.x) pieces += (units ? (uint32_t)units[i] : each) * paged_div(tiles[i] + per - 1, per);
-      if (paged_sum(pieces, word) <= workers) return {per, 0u, 1u};
+      for (int i = lane; i < n; i += 32) pieces += (units ? (uint32_t)units[i] : each) * paged_div(tiles[i] + per - 1, per);
+      if (__reduce_add_sync(0xffffffffu, pieces) <= workers) return {per, 0u, 1u};
     }
   return {line, extra, 0u};
 }
@@ -101,9 +80,9 @@ __host__ __device__ inline size_t paged_plan_words(int n, int groups) { return 4
 
 // Lengths, groups, and the lines of tiles.  The shared part of a group is what the caller says, cut to what every query row
 // of every member sees (so that no row of a prefix unit needs a mask) and to whole 16 keys; a group of one member has none.
-__global__ void __launch_bounds__(1024) paged_plan_kernel(const PagedParams p) {
-  __shared__ int warp_sums[32], bad;
-  __shared__ uint32_t word;
+__global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PagedParams p) {
+  __shared__ int bad;
+  __shared__ PagedLine s_own, s_prefix;
   extern __shared__ int dyn[];
   int* own_cum = dyn;                  // [n]
   int* s_slot = own_cum + p.n;         // [n]
@@ -115,7 +94,8 @@ __global__ void __launch_bounds__(1024) paged_plan_kernel(const PagedParams p) {
   int* g_count = g_first + p.groups;   // [groups] members with keys, then whether a shared page is missing
   int* g_cum = g_count + p.groups;     // [groups]
   int* g_unit = g_cum + p.groups;      // [groups]
-  const int tid = threadIdx.x, nt = blockDim.x;
+  constexpr int nt = kPlanThreads;
+  const int tid = threadIdx.x, warp = tid >> 5;
   pdl_trigger();
   if (tid == 0) bad = 0;
 #pragma unroll 1
@@ -130,8 +110,6 @@ __global__ void __launch_bounds__(1024) paged_plan_kernel(const PagedParams p) {
     s_len[i] = (uint32_t)slot < (uint32_t)p.c.max_seqs ? min(max(p.c.lens[slot], 0), p.c.width << p.c.page_shift) : 0;
   }
   __syncthreads();
-  int prefix_total = 0;
-  PagedCut prefix{1u, 0u, 0u};
   if (p.groups > 0) {
     // groups have to lie behind one another: the slots of their units are counted on it
 #pragma unroll 1
@@ -161,7 +139,7 @@ __global__ void __launch_bounds__(1024) paged_plan_kernel(const PagedParams p) {
     }
     __syncthreads();
     // A shared page that the table does not name: the group goes without, the own units know how to leave such a page out.
-    const int shift = max(5, 31 - __clz(nt) - (31 - __clz(2 * p.groups - 1)));  // 2^shift threads for a group: a warp at least
+    const int shift = max(5, 8 - (31 - __clz(2 * p.groups - 1)));  // 2^shift threads for a group: a warp at least
 #pragma unroll 1
     for (int g = tid >> shift; g < p.groups; g += nt >> shift) {
       const int pages = (g_shared[g] + p.c.page_tokens - 1) >> p.c.page_shift;
@@ -186,12 +164,6 @@ __global__ void __launch_bounds__(1024) paged_plan_kernel(const PagedParams p) {
       g_unit[g] = units;
       g_cum[g] = (shared + kPagedPrefixTile - 1) / kPagedPrefixTile;
     }
-    __syncthreads();
-    prefix = paged_cut(g_cum, g_unit, p.groups, 0u, p.prefix_workers, p.prefix_extra, 1u, &word);
-#pragma unroll 1
-    for (int g = tid; g < p.groups; g += nt) g_cum[g] = g_unit[g] * (int)prefix.length(g_cum[g]);
-    prefix_total = paged_scan(g_cum, p.groups, warp_sums);
-    paged_scan(g_unit, p.groups, warp_sums);
   }
 #pragma unroll 1
   for (int i = tid; i < p.n; i += nt) {
@@ -199,17 +171,30 @@ __global__ void __launch_bounds__(1024) paged_plan_kernel(const PagedParams p) {
     own_cum[i] = g < 0 ? 0 : own_tiles(p, p.groups > 0 && s_len[i] > 0 ? g_shared[g] : 0, s_len[i]);
   }
   __syncthreads();
-  const PagedCut own = paged_cut(own_cum, nullptr, p.n, p.own_units, p.own_workers, p.own_extra, p.own_min, &word);
+  // warps 0, 1: the cuts and lines; warp 2: the numbers of units
+  if (warp < 2) {
+    const bool own = warp == 0;
+    int* tiles = own ? own_cum : g_cum;
+    const int* units = own ? nullptr : g_unit;
+    const int n = own ? p.n : p.groups;
+    const PagedCut cut = warp_cut(tiles, units, n, p.own_units, own ? p.own_workers : p.prefix_workers, own ? p.own_extra : p.prefix_extra, own ? p.own_min : 1);
 #pragma unroll 1
-  for (int i = tid; i < p.n; i += nt) own_cum[i] = own.length(own_cum[i]);
-  const int own_total = paged_scan(own_cum, p.n, warp_sums);
+    for (int i = tid & 31; i < n; i += 32) tiles[i] = (own ? 1 : units[i]) * (int)cut.length(tiles[i]);
+    __syncwarp();
+    const int total = warp_scan(tiles, n);
+    if ((tid & 31) == 0) (own ? s_own : s_prefix) = {(uint32_t)total, cut};
+  }
+  __syncthreads();
+  if (warp == 2) warp_scan(g_unit, p.groups);
+  const int own_total = s_own.total;
   // the line of the own units has p.own_units of each entry of own_cum
   uint32_t line = (uint32_t)own_total * p.own_units;
   if ((uint64_t)own_total * p.own_units >= INT_MAX) {  // beyond what positions count: nothing is computed
     if (tid == 0 && atomicCAS(p.status, 0u, 3u) == 0u) p.status[1] = (uint32_t)own_total;
     line = 0u;
   }
-  if (tid == 0) *p.head = {{line, own}, {(uint32_t)prefix_total, prefix}};
+  if (tid == 0) *p.head = {{line, s_own.cut}, s_prefix};
+  __syncthreads();
   // all is known: the records
 #pragma unroll 1
   for (int i = tid; i < p.n; i += nt) {
@@ -278,8 +263,7 @@ struct PagedRows {
         for (int k = 0; k < D / 16; ++k)
 #pragma unroll
           for (int x = 0; x < 4; x += 2) {
-            const float2 f = unpack16(q[k][half + x], TagBf16{});
-            q[k][half + x] = pack16(f.x * to_f16.a * to_f16.b, f.y * to_f16.a * to_f16.b, TagF16{});
+            q[k][half + x] = bf16x2_shifted(q[k][half + x], to_f16);
           }
         scale[half] = scale[half] / to_f16.a / to_f16.b;
       }
@@ -863,7 +847,7 @@ static int launch_paged(const PagedParams& p, const PagedMaps& m, cudaStream_t s
   static std::atomic<uint64_t> allowed[4];
   if (smem > 48 * 1024)
     if (int s = allow_smem(paged_plan_kernel, 4 * (int)paged_plan_words(kPagedMaxRows, kPagedMaxRows), allowed[3])) return s;
-  FA4B_CUDA(launch_overlapped(paged_plan_kernel, 1, p.n <= 512 ? 256 : 1024, smem, st, p));
+  FA4B_CUDA(launch_overlapped(paged_plan_kernel, 1, kPlanThreads, smem, st, p));
   if (p.groups > 0)
     if (int s = launch_prefix(p, D, kE4M3, std::is_same<QT, TagF16>::value, m.prefix_k, m.prefix_v, st)) return s;
   const int s = p.own_rows == 16   ? launch_units<SoloSmem<D, kE4M3>>(attn_solo_kernel<D, kE4M3, QT>, p, m.own_k, m.own_v, p.own_workers / 4, 128, st, allowed[0])

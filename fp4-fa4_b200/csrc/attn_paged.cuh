@@ -136,8 +136,7 @@ __device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map
 
 
 // A query row against E4M3 keys in f16: bf16 values are brought into f16's range by a power of two (the largest becomes
-// 2^14..2^15; a row of zeros, subnormals or infinities stays as it is), and the sign of the factor moves into the row.
-// Returns the factor, no longer negative, that undoes both.
+// 2^14..2^15; a row of zeros, subnormals or infinities stays as it is).
 struct RowShift {
   float a, b;  // the power of two in two steps: it may be beyond the range of one float
 };
@@ -146,35 +145,9 @@ __device__ __forceinline__ RowShift row_shift(float top) {
   const int shift = (e == 0 || e == 255) ? 0 : 127 + 14 - e;
   return {__uint_as_float((uint32_t)(127 + shift / 2) << 23), __uint_as_float((uint32_t)(127 + shift - shift / 2) << 23)};
 }
-template <typename QT, int kVecs>
-__device__ __forceinline__ float e4m3_query_row(uint4 (&x)[kVecs], float scale) {
-  const uint32_t sign = scale < 0.f ? 0x80008000u : 0u;
-  scale = fabsf(scale);
-  uint32_t(*w)[4] = reinterpret_cast<uint32_t(*)[4]>(x);
-  if constexpr (std::is_same<QT, TagBf16>::value) {
-    float top = 0.f;
-#pragma unroll
-    for (int i = 0; i < kVecs; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 f = unpack16(w[i][j], TagBf16{});
-        top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
-      }
-    const RowShift s = row_shift(top);
-#pragma unroll
-    for (int i = 0; i < kVecs; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 f = unpack16(w[i][j], TagBf16{});
-        w[i][j] = pack16(f.x * s.a * s.b, f.y * s.a * s.b, TagF16{});
-      }
-    scale = scale / s.a / s.b;
-  }
-#pragma unroll
-  for (int i = 0; i < kVecs; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) w[i][j] ^= sign;
-  return scale;
+__device__ __forceinline__ uint32_t bf16x2_shifted(uint32_t x, RowShift s) {  // two values of such a row
+  const float2 f = unpack16(x, TagBf16{});
+  return pack16(f.x * s.a * s.b, f.y * s.a * s.b, TagF16{});
 }
 
 // eight neighbours in one 32-byte store

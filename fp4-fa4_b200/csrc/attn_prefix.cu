@@ -93,19 +93,26 @@ __device__ __forceinline__ void rescale_o(uint32_t to, float f, Smem& s, uint64_
 }
 
 // One step of a row: scores out of TMEM, probabilities back in as 16-bit.  keys: 16 to 64 in sixteens; kFull: 64 (with
-// the other case in the same code every exponential hangs on a branch).
-template <int D, typename Mma, bool kFull, typename Smem>
+// the other case in the same code every exponential hangs on a branch).  kLean: 32 scores in registers at a time, read once
+// for their maximum and once more to be used (with the threads that turn codes there are 128 registers for each).
+template <int D, typename Mma, bool kLean, bool kFull, typename Smem>
 __device__ __forceinline__ void softmax_step(uint32_t ts, uint32_t to, int keys, float scale, float& m, float& l, Smem& s, uint64_t* before,
                                              uint32_t parity_before, bool first, uint32_t* status) {
-  uint32_t a[2][32];
-  tmem_ld32(ts, a[0]);
-  tmem_ld32(ts + 32, a[1]);
-  tmem_ld_wait(a[0]);
-  tmem_ld_wait(a[1]);
+  uint32_t a[kLean ? 1 : 2][32];
+  if constexpr (!kLean) {
+    tmem_ld32(ts, a[0]);
+    tmem_ld32(ts + 32, a[1]);
+    tmem_ld_wait(a[0]);
+    tmem_ld_wait(a[1]);
+  }
   float t0 = -INFINITY, t1 = -INFINITY;
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
-    uint32_t(&x)[32] = a[c];
+    uint32_t(&x)[32] = a[kLean ? 0 : c];
+    if constexpr (kLean) {
+      tmem_ld32(ts + c * 32, x);
+      tmem_ld_wait(x);
+    }
     if constexpr (!kFull) {  // the rest of the buffer is what an earlier step left
 #pragma unroll
       for (int j = 0; j < 32; j += 16)
@@ -131,7 +138,11 @@ __device__ __forceinline__ void softmax_step(uint32_t ts, uint32_t to, int keys,
   float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
-    uint32_t(&x)[32] = a[c];
+    uint32_t(&x)[32] = a[kLean ? 0 : c];
+    if constexpr (kLean) {
+      tmem_ld32(ts + c * 32, x);
+      tmem_ld_wait(x);
+    }
     uint32_t out[16];
 #pragma unroll
     for (int j = 0; j < 32; j += 4) {
@@ -391,14 +402,41 @@ __global__ void __launch_bounds__(prefix_threads(kE4M3), 1) attn_prefix_kernel(c
         const PagedRow pr = paged_row(p, u, there ? row : 0);
         const uint4* src = reinterpret_cast<const uint4*>(p.q + 2 * (pr.i * p.q_sb + pr.h * p.q_sh + pr.t * p.q_st));
         uint8_t* dst = s.q[kWide ? w : 0];
-        if constexpr (kE4M3) {
-          uint4 x[D / 8];
+        if constexpr (kE4M3) {  // in f16; the factor's sign moves into the row
+          RowShift to_f16{1.f, 1.f};
+          if constexpr (std::is_same<QT, TagBf16>::value) {
+            float top = 0.f;
+#pragma unroll 1
+            for (int c0 = 0; c0 < D / 8; c0 += 8) {
+              uint4 x[8];
 #pragma unroll
-          for (int c = 0; c < D / 8; ++c) x[c] = src[c];
-          scale = e4m3_query_row<QT, D / 8>(x, scale * p.k_scale[u.head]);
+              for (int c = 0; c < 8; ++c) x[c] = src[c0 + c];
+#pragma unroll
+              for (int c = 0; c < 8; ++c) {
+                const uint32_t m01 = absmax_bf16x2(absmax_bf16x2(0u, x[c].x), x[c].y), m = absmax_bf16x2(absmax_bf16x2(m01, x[c].z), x[c].w);
+                top = fmaxf(top, fmaxf(__uint_as_float(m << 16), __uint_as_float(m & 0xffff0000u)));
+              }
+            }
+            to_f16 = row_shift(top);
+          }
+          const float factor = scale * p.k_scale[u.head];
+          const uint32_t sign = factor < 0.f ? 0x80008000u : 0u;
+          scale = fabsf(factor) / to_f16.a / to_f16.b;
           if (kWide || w == 0) {
+#pragma unroll 1
+            for (int c0 = 0; c0 < D / 8; c0 += 4) {
+              uint4 x[4];
 #pragma unroll
-            for (int c = 0; c < D / 8; ++c) *reinterpret_cast<uint4*>(dst + (c >> 3) * kSub + swizzled_offset(r, (c & 7) * 16, 128)) = x[c];
+              for (int c = 0; c < 4; ++c) x[c] = src[c0 + c];
+#pragma unroll
+              for (int c = 0; c < 4; ++c) {
+                uint4 y = x[c];
+                if constexpr (std::is_same<QT, TagBf16>::value)
+                  y = make_uint4(bf16x2_shifted(y.x, to_f16), bf16x2_shifted(y.y, to_f16), bf16x2_shifted(y.z, to_f16), bf16x2_shifted(y.w, to_f16));
+                y.x ^= sign, y.y ^= sign, y.z ^= sign, y.w ^= sign;
+                *reinterpret_cast<uint4*>(dst + ((c0 + c) >> 3) * kSub + swizzled_offset(r, ((c0 + c) & 7) * 16, 128)) = y;
+              }
+            }
           }
         } else if (kWide || w == 0) {
 #pragma unroll 1
@@ -427,9 +465,9 @@ __global__ void __launch_bounds__(prefix_threads(kE4M3), 1) attn_prefix_kernel(c
           uint64_t* before = &s.o_done[w][buf ^ 1];
           const uint32_t parity_before = (phases >> (buf ^ 1) & 1u) ^ 1u;
           if (keys == kStep)
-            softmax_step<D, Mma, true>(ts + buf * kStep, to, keys, scale, m, l, s, before, parity_before, step == 0, p.status);
+            softmax_step<D, Mma, kE4M3, true>(ts + buf * kStep, to, keys, scale, m, l, s, before, parity_before, step == 0, p.status);
           else
-            softmax_step<D, Mma, false>(ts + buf * kStep, to, keys, scale, m, l, s, before, parity_before, step == 0, p.status);
+            softmax_step<D, Mma, kE4M3, false>(ts + buf * kStep, to, keys, scale, m, l, s, before, parity_before, step == 0, p.status);
         }
         tc_fence_before();
         mbar_arrive_warp(&s.p_ready[w][buf]);
