@@ -223,6 +223,7 @@ template <int D, bool kE4M3, typename QT>
 struct PagedRows {
   using Mma = typename std::conditional<kE4M3, TagF16, QT>::type;
   static constexpr int kBoxBytes = D * (kE4M3 ? 1 : 2) < 128 ? D : 128;  // of a row, side by side in one box of shared memory
+  static constexpr int kRows = 16;
   uint32_t q[D / 16][4];
   float acc[D / 8][4], scale[2], m[2], l[2];
   int limit[2];  // the row sees keys below
@@ -450,6 +451,235 @@ struct PagedRows {
   }
 };
 
+// Up to eight query rows (a single token of up to eight query heads per kv head), the other way round: keys and values are the
+// 16-row operand of the products, S^T = K Q^T and O^T += V^T P^T, and the query rows their eight columns, so that no half of
+// a product is empty and a thread holds half as many scores, accumulators and query values.  A thread has two rows (2c and
+// 2c + 1), and of a tile of sixteen keys the keys quad and quad + 8 of both.
+template <int D, bool kE4M3, typename QT>
+struct PagedRows8 {
+  using Mma = typename std::conditional<kE4M3, TagF16, QT>::type;
+  static constexpr int kBoxBytes = D * (kE4M3 ? 1 : 2) < 128 ? D : 128;
+  static constexpr int kRows = 8;
+  uint32_t q[D / 16][2];
+  float acc[D / 16][4], scale[2], m[2], l[2];
+  int limit[2];
+
+  __device__ __forceinline__ void start(const PagedParams& p, const PagedUnit& u, int) {
+    const int lane = threadIdx.x & 31, quad = lane >> 2, c4 = lane & 3;
+    const bool there = quad < u.rows;
+    {
+      const PagedRow r = paged_row(p, u, there ? quad : 0);
+      const uint8_t* src = p.q + 2 * (r.i * p.q_sb + r.h * p.q_sh + r.t * p.q_st);
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) {
+        if constexpr (kE4M3) {  // four neighbours, as in a thread's codes of K
+          const uint2 x = there ? *reinterpret_cast<const uint2*>(src + 2 * (k * 16 + c4 * 4)) : make_uint2(0u, 0u);
+          q[k][0] = x.x, q[k][1] = x.y;
+        } else {
+          q[k][0] = there ? *reinterpret_cast<const uint32_t*>(src + 2 * (k * 16 + c4 * 2)) : 0u;
+          q[k][1] = there ? *reinterpret_cast<const uint32_t*>(src + 2 * (k * 16 + 8 + c4 * 2)) : 0u;
+        }
+      }
+    }
+    float factor = p.scale_log2 * (kE4M3 ? p.k_scale[u.head] : 1.f);
+    if constexpr (kE4M3 && std::is_same<QT, TagBf16>::value) {
+      uint32_t top2 = 0u;
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) top2 = absmax_bf16x2(absmax_bf16x2(top2, q[k][0]), q[k][1]);
+      float top = fmaxf(__uint_as_float(top2 << 16), __uint_as_float(top2 & 0xffff0000u));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const RowShift to_f16 = row_shift(top);
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) q[k][0] = bf16x2_shifted(q[k][0], to_f16), q[k][1] = bf16x2_shifted(q[k][1], to_f16);
+      factor = factor / to_f16.a / to_f16.b;
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {  // of rows 2c and 2c + 1: their lanes are 4 rows on
+      const int row = 2 * c4 + e;
+      scale[e] = __shfl_sync(0xffffffffu, factor, row * 4);
+      limit[e] = u.key_hi - (p.T - 1 - (u.row0 + (row < u.rows ? row : 0)) / p.G);
+      m[e] = -INFINITY, l[e] = 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
+  }
+
+  template <int kKeys, int kTileRows>
+  __device__ __forceinline__ void tile(const PagedUnit& u, const uint8_t* ktile, const uint8_t* vtile, int at, int key0, uint32_t valid) {
+    const int lane = threadIdx.x & 31, quad = lane >> 2, c4 = lane & 3;
+    const uint32_t kbase = smem_u32(ktile), vbase = smem_u32(vtile);
+    constexpr uint32_t kAllValid = (1u << (kKeys / 16)) - 1u;
+    const bool special = key0 < u.key_lo || key0 + kKeys > u.key_all || (valid & kAllValid) != kAllValid;
+    // matrices of ldmatrix: keys 0-7 and 8-15 of a block, then of the next sixteen bytes of the row
+    const uint32_t krow = at + ((lane >> 3) & 1) * 8 + (lane & 7);
+    float sc[kKeys / 16][4];
+#pragma unroll
+    for (int j = 0; j < kKeys / 16; ++j) {
+      float other[4] = {0.f, 0.f, 0.f, 0.f};  // two chains of products
+      sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.f;
+      if constexpr (kE4M3) {
+#pragma unroll
+        for (int x = 0; x < D / 32; ++x) {
+          uint32_t b[4];
+          ldmatrix4(b, kbase + swizzled_offset(krow + j * 16, x * 32 + (lane >> 4) * 16, kBoxBytes));
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const uint32_t a[4] = {e4m3x2_to_f16x2(b[2 * e]), e4m3x2_to_f16x2(b[2 * e + 1]), e4m3x2_to_f16x2(b[2 * e] >> 16), e4m3x2_to_f16x2(b[2 * e + 1] >> 16)};
+            mma16816(e ? other : sc[j], a, q[2 * x + e][0], q[2 * x + e][1], Mma{});
+          }
+        }
+      } else {
+#pragma unroll
+        for (int x = 0; x < D / 16; ++x) {
+          uint32_t a[4];
+          const uint32_t col = x * 32 + (lane >> 4) * 16;
+          ldmatrix4(a, kbase + (col >> 7) * (kTileRows * 128) + swizzled_offset(krow + j * 16, col & 127u, 128));
+          mma16816(x & 1 ? other : sc[j], a, q[x][0], q[x][1], Mma{});
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sc[j][e] += other[e];
+    }
+    float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int j = 0; j < kKeys / 16; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {  // row 2c + (e & 1), key quad or quad + 8
+        float x = sc[j][e] * scale[e & 1];
+        if (special) {
+          const int key = key0 + j * 16 + (e >> 1) * 8 + quad;
+          if (key < u.key_lo || key >= limit[e & 1] || !(valid >> j & 1u)) x = -INFINITY;
+        }
+        sc[j][e] = x;
+        top[e & 1] = fmaxf(top[e & 1], x);
+      }
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) {
+      top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], o));
+      top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], o));
+    }
+    if (__any_sync(0xffffffffu, top[0] > m[0] + 8.f || top[1] > m[1] + 8.f)) {  // as for sixteen rows
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float next = fmaxf(m[e], top[e]);
+        const float f = next == -INFINITY ? 1.f : paged_ex2(m[e] - next);
+        m[e] = next;
+        l[e] *= f;
+#pragma unroll
+        for (int j = 0; j < D / 16; ++j) acc[j][e] *= f, acc[j][e + 2] *= f;
+      }
+    }
+    const float m0 = m[0] == -INFINITY ? 0.f : m[0], m1 = m[1] == -INFINITY ? 0.f : m[1];
+#pragma unroll
+    for (int j = 0; j < kKeys / 16; ++j) {
+      sc[j][0] = paged_ex2(sc[j][0] - m0), sc[j][2] = paged_ex2(sc[j][2] - m0);
+      sc[j][1] = paged_ex2(sc[j][1] - m1), sc[j][3] = paged_ex2(sc[j][3] - m1);
+      l[0] += sc[j][0] + sc[j][2], l[1] += sc[j][1] + sc[j][3];
+    }
+    // values: as for sixteen rows, keys that are not there for every row are taken out of the product on both sides
+#pragma unroll
+    for (int kk = 0; kk < kKeys / 16; ++kk) {
+      uint32_t b0 = transposed(pack16(sc[kk][0], sc[kk][1], Mma{})), b1 = transposed(pack16(sc[kk][2], sc[kk][3], Mma{}));
+      uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
+      if (special) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int key = key0 + kk * 16 + h * 8 + c4 * 2;
+          const bool ok = valid >> kk & 1u;
+          keep[h] = (ok && key >= u.key_lo && key < u.key_all ? 0x0000ffffu : 0u) | (ok && key + 1 >= u.key_lo && key + 1 < u.key_all ? 0xffff0000u : 0u);
+        }
+        b0 &= keep[0], b1 &= keep[1];
+      }
+      if constexpr (kE4M3) {
+#pragma unroll
+        for (int x = 0; x < D / 32; ++x) {  // matrices: keys 0-7 and 8-15 of 16 codes, then of the next 16
+          uint32_t b[4];
+          ldmatrix4_trans(b, vbase + swizzled_offset(krow + kk * 16, x * 32 + (lane >> 4) * 16, kBoxBytes));
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {  // (key, key + 1) x (d, d + 1) in a register: even d are rows 0-7 of the product, odd d rows 8-15
+            uint32_t a[4] = {e4m3x2_to_f16x2(__byte_perm(b[2 * e], 0, 0x4420)), e4m3x2_to_f16x2(__byte_perm(b[2 * e], 0, 0x4431)),
+                             e4m3x2_to_f16x2(__byte_perm(b[2 * e + 1], 0, 0x4420)), e4m3x2_to_f16x2(__byte_perm(b[2 * e + 1], 0, 0x4431))};
+            if (special) a[0] &= keep[0], a[1] &= keep[0], a[2] &= keep[1], a[3] &= keep[1];
+            mma16816(acc[2 * x + e], a, b0, b1, Mma{});
+          }
+        }
+      } else {
+        const uint32_t vrow = at + kk * 16 + (lane >> 4) * 8 + (lane & 7);
+#pragma unroll
+        for (int x = 0; x < D / 16; ++x) {  // matrices: d 0-7 and 8-15 of keys 0-7, then of keys 8-15
+          uint32_t a[4];
+          const uint32_t col = x * 32 + ((lane >> 3) & 1) * 16;
+          ldmatrix4_trans(a, vbase + (col >> 7) * (kTileRows * 128) + swizzled_offset(vrow, col & 127u, 128));
+          if (special) a[0] &= keep[0], a[1] &= keep[0], a[2] &= keep[1], a[3] &= keep[1];
+          mma16816(acc[x], a, b0, b1, Mma{});
+        }
+      }
+    }
+    if (key0 + kKeys > u.key_all) {  // the newest keys, which some rows see
+#pragma unroll 1
+      for (int kk = max(0, u.key_all - key0); kk < min(kKeys, u.key_hi - key0); ++kk) {
+        if (!(valid >> (kk >> 4) & 1u)) continue;
+        float mine[2] = {0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < kKeys / 16; ++j)
+          if (j == kk >> 4) mine[0] = kk & 8 ? sc[j][2] : sc[j][0], mine[1] = kk & 8 ? sc[j][3] : sc[j][1];
+        const int from = (kk & 7) * 4 + c4;
+        const float p0 = __shfl_sync(0xffffffffu, mine[0], from), p1 = __shfl_sync(0xffffffffu, mine[1], from);
+        const bool see0 = key0 + kk < limit[0], see1 = key0 + kk < limit[1];
+        const uint32_t row = at + kk;
+#pragma unroll
+        for (int j = 0; j < D / 16; ++j) {
+          float2 f;  // the d of this thread's two rows of the product
+          if constexpr (kE4M3) {
+            const uint32_t two = *reinterpret_cast<const uint16_t*>(vtile + swizzled_offset(row, j * 16 + quad * 2, kBoxBytes));
+            f = unpack16(e4m3x2_to_f16x2(two), TagF16{});
+          } else {
+            const uint32_t c0 = j * 32 + quad * 2, c1 = c0 + 16;
+            const uint32_t lo = *reinterpret_cast<const uint16_t*>(vtile + (c0 >> 7) * (kTileRows * 128) + swizzled_offset(row, c0 & 127u, 128));
+            const uint32_t hi = *reinterpret_cast<const uint16_t*>(vtile + (c1 >> 7) * (kTileRows * 128) + swizzled_offset(row, c1 & 127u, 128));
+            f = unpack16(lo | hi << 16, Mma{});
+          }
+          if (see0) acc[j][0] = fmaf(p0, f.x, acc[j][0]), acc[j][2] = fmaf(p0, f.y, acc[j][2]);
+          if (see1) acc[j][1] = fmaf(p1, f.x, acc[j][1]), acc[j][3] = fmaf(p1, f.y, acc[j][3]);
+        }
+      }
+    }
+  }
+
+  __device__ __forceinline__ void sum_up() {  // the eight lanes of a row meet
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) {
+      l[0] += __shfl_xor_sync(0xffffffffu, l[0], o);
+      l[1] += __shfl_xor_sync(0xffffffffu, l[1], o);
+    }
+  }
+
+  __device__ __forceinline__ void store(const PagedParams& p, const PagedUnit& u, int, int worker) const {
+    const int lane = threadIdx.x & 31, quad = lane >> 2, c4 = lane & 3;
+    const int64_t slot = (int64_t)u.index + worker;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int row = 2 * c4 + e;
+      if (row >= u.rows) continue;
+      float* out = p.own_acc + (slot * p.own_rows + row) * D;
+      if (quad == 0) p.own_ml[slot * p.own_rows + row] = make_float2(m[e], l[e]);
+#pragma unroll
+      for (int j = 0; j < D / 16; ++j) {
+        if constexpr (kE4M3) *reinterpret_cast<float2*>(out + j * 16 + quad * 2) = make_float2(acc[j][e], acc[j][e + 2]);
+        else out[j * 16 + quad] = acc[j][e], out[j * 16 + 8 + quad] = acc[j][e + 2];
+      }
+    }
+  }
+
+  // an 8 x 8 matrix of pairs (row quad, columns 2c and 2c + 1) -> its transpose in the same places
+  static __device__ __forceinline__ uint32_t transposed(uint32_t x) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+    return r;
+  }
+};
+
 // One box of tokens as a producing lane sees it: which of them a copy is asked for, and what the consumers may look at.
 struct PagedBoxes {
   int tokens, per_tile;  // of a box; boxes of a tile
@@ -478,22 +708,24 @@ struct OwnOrder {
 
 // Up to sixteen query rows per unit (a single token, or a few drafted ones, of a group of query heads): every warp is a worker
 // with a line piece, a ring of tiles and copies of its own, and nothing in the loop waits for another warp.
-template <int D, bool kE4M3>
+template <int D, bool kE4M3, int kRows>
 struct SoloSmem {
   static constexpr int kRowBytes = D * (kE4M3 ? 1 : 2);
   static constexpr int kKeys = kRowBytes == 256 ? 16 : 32;            // of a tile
   static constexpr int kTileBytes = kKeys * kRowBytes;               // K or V: 4 KB, 2 KB for E4M3 with D = 64
-  static constexpr int kStages = 24 * 1024 / (2 * kTileBytes);       // 24 KB in flight per warp, 192 KB per SM
+  static constexpr int kCtas = kRows == 8 ? 3 : 2;                   // per SM: what the registers of a row's state allow
+  static constexpr int kStages = 48 * 1024 / kCtas / (2 * kTileBytes);  // 192 KB in flight per SM
   alignas(1024) uint8_t ring[4][kStages][2][kTileBytes];
   uint64_t full[4][kStages];
   volatile uint32_t abort_flag;
   static constexpr int kUsed = 4 * kStages * (2 * kTileBytes + 8) + 16;  // the struct without what its alignment adds
 };
 
-template <int D, bool kE4M3, typename QT>
-__global__ void __launch_bounds__(128, 2) attn_solo_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_k,
+template <int D, bool kE4M3, typename QT, int kRows>
+__global__ void __launch_bounds__(128, kRows == 8 ? 3 : 2) attn_solo_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_k,
                                                            const __grid_constant__ CUtensorMap map_v) {
-  using Smem = SoloSmem<D, kE4M3>;
+  using Smem = SoloSmem<D, kE4M3, kRows>;
+  using Rows = typename std::conditional<kRows == 8, PagedRows8<D, kE4M3, QT>, PagedRows<D, kE4M3, QT>>::type;
   constexpr int kBytes = kE4M3 ? 1 : 2, kRowBytes = Smem::kRowBytes, kBoxBytes = kRowBytes < 128 ? kRowBytes : 128, kSubs = kRowBytes / kBoxBytes;
   constexpr int kKeys = Smem::kKeys, kStages = Smem::kStages;
   extern __shared__ __align__(1024) uint8_t raw[];
@@ -572,7 +804,7 @@ __global__ void __launch_bounds__(128, 2) attn_solo_kernel(const PagedParams p, 
   for (int i = 0; i < kStages; ++i) issue();
 
   int done = 0;
-  PagedRows<D, kE4M3, QT> rows;
+  Rows rows;
   while (!walk.done()) {
     const PagedUnit u = walk.next(p);
     if (u.tile == u.tile_end) continue;
@@ -844,13 +1076,14 @@ static int launch_units(K kernel, const PagedParams& p, const CUtensorMap& mk, c
 template <int D, bool kE4M3, typename QT>
 static int launch_paged(const PagedParams& p, const PagedMaps& m, cudaStream_t st) {
   const size_t smem = 4 * paged_plan_words(p.n, p.groups);
-  static std::atomic<uint64_t> allowed[4];
+  static std::atomic<uint64_t> allowed[5];
   if (smem > 48 * 1024)
     if (int s = allow_smem(paged_plan_kernel, 4 * (int)paged_plan_words(kPagedMaxRows, kPagedMaxRows), allowed[3])) return s;
   FA4B_CUDA(launch_overlapped(paged_plan_kernel, 1, kPlanThreads, smem, st, p));
   if (p.groups > 0)
     if (int s = launch_prefix(p, D, kE4M3, std::is_same<QT, TagF16>::value, m.prefix_k, m.prefix_v, st)) return s;
-  const int s = p.own_rows == 16   ? launch_units<SoloSmem<D, kE4M3>>(attn_solo_kernel<D, kE4M3, QT>, p, m.own_k, m.own_v, p.own_workers / 4, 128, st, allowed[0])
+  const int s = p.own_rows == 8    ? launch_units<SoloSmem<D, kE4M3, 8>>(attn_solo_kernel<D, kE4M3, QT, 8>, p, m.own_k, m.own_v, p.own_workers / 4, 128, st, allowed[4])
+                : p.own_rows == 16 ? launch_units<SoloSmem<D, kE4M3, 16>>(attn_solo_kernel<D, kE4M3, QT, 16>, p, m.own_k, m.own_v, p.own_workers / 4, 128, st, allowed[0])
                 : p.own_rows == 32 ? launch_units<TeamSmem<D, kE4M3>>(attn_team_kernel<D, kE4M3, QT, 2>, p, m.own_k, m.own_v, p.own_workers, 160, st, allowed[1])
                                    : launch_units<TeamSmem<D, kE4M3>>(attn_team_kernel<D, kE4M3, QT, 4>, p, m.own_k, m.own_v, p.own_workers, 160, st, allowed[2]);
   if (s) return s;
@@ -888,12 +1121,12 @@ static int paged_params(const fa4b_kv_cache* c, const fa4b_attn_paged_args* a, P
   p.scale_log2 = (a->softmax_scale > 0.f ? a->softmax_scale : 1.0f / sqrtf((float)c->D)) * kLog2e;
   if (c->dtype == FA4B_KV_E4M3) p.k_scale = c->k_scale + (int64_t)a->layer * c->Hkv, p.v_scale = c->v_scale + (int64_t)a->layer * c->Hkv;
   const int n_sm = sm_count() > 0 ? sm_count() : 148;
-  p.own_rows = p.R <= 16 ? 16 : p.R <= 32 ? 32 : 64;
+  p.own_rows = p.R <= 8 ? 8 : p.R <= 16 ? 16 : p.R <= 32 ? 32 : 64;
   p.own_blocks = (p.R + p.own_rows - 1) / p.own_rows;
-  const bool solo = p.own_rows == 16, short_rows = c->D * (c->dtype == FA4B_KV_E4M3 ? 1 : 2) < 256;
+  const bool solo = p.own_rows <= 16, short_rows = c->D * (c->dtype == FA4B_KV_E4M3 ? 1 : 2) < 256;
   p.own_tile = !solo ? TeamSmem<64, true>::kKeys : short_rows ? 32 : 16;
   p.own_shift = __builtin_ctz((unsigned)p.own_tile), p.own_rows_shift = __builtin_ctz((unsigned)p.own_rows), p.own_units = c->Hkv * p.own_blocks;
-  p.own_workers = (solo ? 8 : 2) * n_sm;
+  p.own_workers = (p.own_rows == 8 ? 12 : solo ? 8 : 2) * n_sm;
   p.own_extra = solo ? 2 : 1;
   p.own_min = solo ? 64 / p.own_tile : 1;  // a piece shorter than 64 keys is mostly its beginning
   // two blocks of 128 rows over the same keys where the groups have the rows for it: each tile then comes from memory half
