@@ -202,7 +202,7 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PagedPar
     int4* r = reinterpret_cast<int4*>(p.seq + i);
     r[0] = make_int4(s_slot[i], s_len[i], first, own_cum[i]);
     p.own_cum[i] = own_cum[i];
-    r[2] = make_int4(s_group[i] < 0 || line == 0u && own_total > 0, 0, 0, 0);
+    r[2] = make_int4(s_group[i] < 0 || line == 0u && own_total > 0, first > 0 ? (offsets[g + 1] - offsets[g]) * p.R : 0, 0, 0);
     if (first > 0) r[1] = make_int4(offsets[g], ((offsets[g + 1] - offsets[g]) * p.R + p.prefix_rows - 1) >> p.prefix_shift, g_unit[g], g_cum[g]);
   }
 #pragma unroll 1
@@ -960,26 +960,28 @@ __global__ void __launch_bounds__(160, 2) attn_team_kernel(const PagedParams p, 
 }
 
 // ---- join -------------------------------------------------------------------------------------------------------------
-// One warp per output row.  The pieces' statistics come to the lanes at once, so that what is left to wait for is one
-// round of loads: a lane holds D / 32 neighbours of eight pieces at a time.  Which pieces there are follows from the
-// plan, which is complete when this launch comes up (the own units trigger behind it), so it is looked up before the wait.
-template <int D, typename QT>
+// One warp per output row, or (kSplit) four, each with a quarter of the pieces, where the rows are few.  The pieces' statistics
+// come to the lanes at once, so that what is left to wait for is one round of loads: a lane holds D / 32 neighbours of eight
+// pieces at a time.  Which pieces there are follows from the plan, which is complete when this launch comes up (the own units
+// trigger behind it), so it is looked up before the wait.
+template <int D, typename QT, bool kSplit>
 __global__ void __launch_bounds__(128) paged_join_kernel(const PagedParams p) {
   constexpr int kPer = D / 32;
-  const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
+  __shared__ float parts[kSplit ? 3 : 1][D];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = kSplit ? warp : 0;
+  const uint32_t w = kSplit ? blockIdx.x : blockIdx.x * 4 + warp;
   pdl_trigger();
-  const bool there = w < (int64_t)p.n * p.Hq * p.T;
-  const uint32_t row_id = there ? (uint32_t)w : 0u;
-  const uint32_t t = row_id % (uint32_t)p.T, ih = row_id / (uint32_t)p.T, h = ih % (uint32_t)p.Hq, i = ih / (uint32_t)p.Hq;
+  const bool there = w < (uint32_t)(p.n * p.Hq * p.T);
+  const uint32_t row_id = there ? w : 0u;
+  const uint32_t t = p.T == 1 ? 0u : row_id % (uint32_t)p.T, ih = p.T == 1 ? row_id : row_id / (uint32_t)p.T, i = ih / (uint32_t)p.Hq, h = ih - i * (uint32_t)p.Hq;
   const PagedSeq s = p.seq[i];
   const PagedHead line = *p.head;
-  const int head = h / p.G, r = t * p.G + h % p.G, len = s.len;
+  const int head = h / (uint32_t)p.G, r = t * p.G + (h - head * p.G), len = s.len;
   float acc[kPer], m = -INFINITY, l = 0.f;
 #pragma unroll
   for (int e = 0; e < kPer; ++e) acc[e] = 0.f;
   // the workers that have a part of the unit's tiles: from the one where the first tile lies to the one where the last does
-  int n_prefix = 0, prefix_row = 0, n_own = 0, own_row = 0;
+  int n_prefix = 0, prefix_row = 0, n_own = 0, own_row = 0, two = 0;
   int64_t prefix_slot = 0, own_slot = 0;
   if (len - (p.T - 1 - (int)t) > 0) {
     if (s.first > 0) {
@@ -987,7 +989,8 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PagedParams p) {
       const int tiles = (s.first + kPagedPrefixTile - 1) / kPagedPrefixTile;
       const PagedCut cut = line.prefix.cut;
       const uint32_t from = s.g_cum + which * cut.length(tiles) + cut.extra, worker = from / cut.per;
-      n_prefix = (int)((from + tiles - 1) / cut.per - worker) + 1;
+      two = prefix_in_two(p, s.g_rows - (block << p.prefix_shift));
+      n_prefix = (int)((from + tiles - 1) / cut.per - worker + 1) << two;
       prefix_slot = s.g_unit + which + (int64_t)worker;
       prefix_row = row & (p.prefix_rows - 1);
     }
@@ -999,53 +1002,61 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PagedParams p) {
     own_row = r & (p.own_rows - 1);
   }
   pdl_wait();
-  if (!there || s.left_alone) return;  // or behind the last group
-  {
-    for (int base = 0; base < n_prefix + n_own; base += 32) {
-      const int k = base + lane;
-      const bool is_prefix = k < n_prefix;
-      const int64_t row = is_prefix ? (prefix_slot + k) * p.prefix_rows + prefix_row : (own_slot + (k - n_prefix)) * p.own_rows + own_row;
-      float2 x = make_float2(-INFINITY, 0.f);
-      if (k < n_prefix + n_own) x = is_prefix ? p.prefix_ml[row] : p.own_ml[row];
-      float top = x.x;
+  if (!there || s.left_alone) return;  // or behind the last group; the same for all warps of a row
+  for (int base = 0; base < n_prefix + n_own; base += 32) {
+    const int k = base + lane;
+    const bool is_prefix = k < n_prefix;
+    const int64_t row = is_prefix ? (prefix_slot + (k >> two)) * p.prefix_rows + (k & two) * 64 + prefix_row : (own_slot + (k - n_prefix)) * p.own_rows + own_row;
+    float2 x = make_float2(-INFINITY, 0.f);
+    if (k < n_prefix + n_own) x = is_prefix ? p.prefix_ml[row] : p.own_ml[row];
+    float top = x.x;
 #pragma unroll
-      for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      const float next = fmaxf(m, top), f = m == -INFINITY ? 0.f : paged_ex2(m - next);
-      const float y = x.x == -INFINITY ? 0.f : paged_ex2(x.x - next);
-      float sum = x.y * y;
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float next = fmaxf(m, top), f = m == -INFINITY ? 0.f : paged_ex2(m - next);
+    const float y = x.x == -INFINITY ? 0.f : paged_ex2(x.x - next);
+    float sum = x.y * y;
 #pragma unroll
-      for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      m = next, l = l * f + sum;
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    m = next, l = l * f + sum;
 #pragma unroll
-      for (int e = 0; e < kPer; ++e) acc[e] *= f;
-      const float* at = (is_prefix ? p.prefix_acc : p.own_acc) + row * D;
-      const int count = min(32, n_prefix + n_own - base);
-      for (int k0 = 0; k0 < count; k0 += 8) {
-        float v[8][kPer], weight[8];
+    for (int e = 0; e < kPer; ++e) acc[e] *= f;
+    const float* at = (is_prefix ? p.prefix_acc : p.own_acc) + row * D;
+    const int count = min(32, n_prefix + n_own - base), each = kSplit ? (count + 3) / 4 : count, end = min(count, (part + 1) * each);
+    for (int k0 = part * each; k0 < end; k0 += 8) {
+      float v[8][kPer], weight[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          weight[j] = __shfl_sync(0xffffffffu, y, (k0 + j) & 31);
-          const float* from_row = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, (unsigned long long)at, (k0 + j) & 31));
+      for (int j = 0; j < 8; ++j) {
+        weight[j] = __shfl_sync(0xffffffffu, y, (k0 + j) & 31);
+        const float* from_row = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, (unsigned long long)at, (k0 + j) & 31));
 #pragma unroll
-          for (int e = 0; e < kPer; ++e) v[j][e] = 0.f;
-          if (k0 + j < count) {
-            if constexpr (kPer == 4) {
-              const float4 q = __ldcg(reinterpret_cast<const float4*>(from_row) + lane);
-              v[j][0] = q.x, v[j][1] = q.y, v[j][2] = q.z, v[j][3] = q.w;
-            } else {
-              const float2 q = __ldcg(reinterpret_cast<const float2*>(from_row) + lane);
-              v[j][0] = q.x, v[j][1] = q.y;
-            }
+        for (int e = 0; e < kPer; ++e) v[j][e] = 0.f;
+        if (k0 + j < end) {
+          if constexpr (kPer == 4) {
+            const float4 q = __ldcg(reinterpret_cast<const float4*>(from_row) + lane);
+            v[j][0] = q.x, v[j][1] = q.y, v[j][2] = q.z, v[j][3] = q.w;
           } else {
-            weight[j] = 0.f;
+            const float2 q = __ldcg(reinterpret_cast<const float2*>(from_row) + lane);
+            v[j][0] = q.x, v[j][1] = q.y;
           }
+        } else {
+          weight[j] = 0.f;
         }
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-#pragma unroll
-          for (int e = 0; e < kPer; ++e) acc[e] = fmaf(v[j][e], weight[j], acc[e]);
       }
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) acc[e] = fmaf(v[j][e], weight[j], acc[e]);
     }
+  }
+  if constexpr (kSplit) {
+    if (warp > 0) {
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) parts[warp - 1][lane * kPer + e] = acc[e];
+    }
+    __syncthreads();
+    if (warp > 0) return;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) acc[e] += (parts[0][lane * kPer + e] + parts[1][lane * kPer + e]) + parts[2][lane * kPer + e];
   }
   const float inv = l == 0.f ? 0.f : (p.v_scale ? p.v_scale[head] : 1.f) / l;  // a row that sees nothing: zeros, -inf
   uint8_t* out = p.o + 2 * ((int64_t)i * p.o_sb + (int64_t)h * p.o_sh + (int64_t)t * p.o_st + lane * kPer);
@@ -1088,7 +1099,9 @@ static int launch_paged(const PagedParams& p, const PagedMaps& m, cudaStream_t s
                                    : launch_units<TeamSmem<D, kE4M3>>(attn_team_kernel<D, kE4M3, QT, 4>, p, m.own_k, m.own_v, p.own_workers, 160, st, allowed[2]);
   if (s) return s;
   const int64_t rows = (int64_t)p.n * p.Hq * p.T;
-  FA4B_CUDA(launch_overlapped(paged_join_kernel<D, QT>, (unsigned)((rows + 3) / 4), 128, 0, st, p));
+  // four warps a row up to where the rows alone fill the SMs with warps (8 CTAs of four each; 5.7 against 7.0 us of a 34 us call with 1024 rows, but 5.8 against 3.5 us with 1536)
+  if (rows <= 8ll * p.prefix_workers) FA4B_CUDA(launch_overlapped(paged_join_kernel<D, QT, true>, (unsigned)rows, 128, 0, st, p));
+  else FA4B_CUDA(launch_overlapped(paged_join_kernel<D, QT, false>, (unsigned)((rows + 3) / 4), 128, 0, st, p));
   return FA4B_OK;
 }
 

@@ -26,7 +26,7 @@ constexpr int kPagedMaxT = 16;
 struct PagedSeq {    // one row of the batch
   int slot, len, first, cum;             // first key that is its own; length of the line before it, of one (kv head, row block)
   int g_row, g_blocks, g_unit, g_cum;  // its group's first row, row blocks, first unit, length of the line before it
-  int left_alone, pad[3];               // 1: in no group
+  int left_alone, g_rows, pad[2];       // 1: in no group; query rows of its group, per kv head
 };
 struct PagedGroup {
   int shared, slot, row, rows;           // keys; whose row of the table names the pages; first row of the batch, query rows per kv head
@@ -260,6 +260,10 @@ struct PagedWalk {
     return u;
   }
 };
+
+// A prefix unit of up to 64 rows in a CTA whose halves share 128: rows 0-63 take the first half's keys and rows 64-127, the same
+// rows again, the second half's, so that the warps at work sit in different quarters of the SM.
+__device__ __forceinline__ int prefix_in_two(const PagedParams& p, int rows) { return p.prefix_rows == 128 && rows <= 64; }
 
 // a row of a unit: batch row, token and query head
 struct PagedRow {

@@ -54,12 +54,12 @@ struct PrefixSmem {
   alignas(1024) uint8_t q[kWide ? 2 : 1][kTile];
   uint8_t ring[kRing][kTile];
   uint8_t raw[kRaw ? kRaw : 1][kRaw ? kRawTile : 16];
-  float2 ml[kWide ? 1 : 128];
+  float2 ml[2][kWide ? 1 : 128];
   uint64_t q_full, q_free, full[kRing], empty[kRing], raw_full[kRaw ? kRaw : 1], raw_empty[kRaw ? kRaw : 1], s_full[2][2], p_ready[2][2], o_done[2][2], drained;  // [half][score buffer]
   uint32_t tmem_base;
   volatile uint32_t abort_flag;
   // the struct without what its alignment adds
-  static constexpr int kUsed = ((kWide ? 2 : 1) + kRing) * kTile + (kRaw ? kRaw * kRawTile : 16) + (kWide ? 1 : 128) * 8 +
+  static constexpr int kUsed = ((kWide ? 2 : 1) + kRing) * kTile + (kRaw ? kRaw * kRawTile : 16) + (kWide ? 1 : 128) * 16 +
                                8 * (2 + 2 * kRing + 2 * (kRaw ? kRaw : 1) + 13) + 16;
 };
 
@@ -392,14 +392,16 @@ __global__ void __launch_bounds__(prefix_threads(kE4M3), 1) attn_prefix_kernel(c
       const PagedUnit u = walk.next(p);
       const int nt = u.tile_end - u.tile;
       if (nt == 0) continue;
-      const int row = (kWide ? w * 128 : 0) + r;
-      const bool there = row < u.rows, active = (kWide ? w * 128 : 0) + (warp & 3) * 32 < u.rows;
+      const bool two = !kWide && prefix_in_two(p, u.rows);
+      const int row = kWide ? w * 128 + r : two ? r & 63 : r;
+      const bool mine = !two || r >> 6 == w;                          // of this half
+      const bool loads = (row & ~31) < u.rows, active = loads && mine, there = row < u.rows && mine;
       const int piece = min(u.key_hi - u.tile * kPrefixTile, nt * kPrefixTile);
       const int n_steps = kWide ? (w * 128 < u.rows ? (piece + kStep - 1) / kStep : 0) : (piece - w * kStep + kPrefixTile - 1) / kPrefixTile;
       if (units > 0) mbar_wait_warp(&s.q_free, (uint32_t)(units - 1) & 1u, &s.abort_flag, p.status, 17);
       float scale = p.scale_log2;
-      if (active) {  // the query row, swizzled into shared memory
-        const PagedRow pr = paged_row(p, u, there ? row : 0);
+      if (loads) {  // the query row, swizzled into shared memory
+        const PagedRow pr = paged_row(p, u, row < u.rows ? row : 0);
         const uint4* src = reinterpret_cast<const uint4*>(p.q + 2 * (pr.i * p.q_sb + pr.h * p.q_sh + pr.t * p.q_st));
         uint8_t* dst = s.q[kWide ? w : 0];
         if constexpr (kE4M3) {  // in f16; the factor's sign moves into the row
@@ -439,14 +441,11 @@ __global__ void __launch_bounds__(prefix_threads(kE4M3), 1) attn_prefix_kernel(c
             }
           }
         } else if (kWide || w == 0) {
-#pragma unroll 1
-          for (int c0 = 0; c0 < D / 8; c0 += 8) {
-            uint4 x[8];
+          uint4 x[D / 8];
 #pragma unroll
-            for (int c = 0; c < 8; ++c) x[c] = src[c0 + c];
+          for (int c = 0; c < D / 8; ++c) x[c] = src[c];
 #pragma unroll
-            for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(dst + (c0 >> 3) * kSub + swizzled_offset(r, c * 16, 128)) = x[c];
-          }
+          for (int c = 0; c < D / 8; ++c) *reinterpret_cast<uint4*>(dst + (c >> 3) * kSub + swizzled_offset(r, (c & 7) * 16, 128)) = x[c];
         }
       }
       if (kWide || w == 0) {
@@ -474,36 +473,35 @@ __global__ void __launch_bounds__(prefix_threads(kE4M3), 1) attn_prefix_kernel(c
       }
       // ---- the piece goes to its slot
       const int64_t slot = (int64_t)u.index + blockIdx.x;
-      float* out = p.prefix_acc + (slot * p.prefix_rows + row) * D;
-      if constexpr (kWide) {
-        if (n_steps > 0) {
-          const int last = (n_steps - 1) & 1;
-          mbar_wait_warp(&s.o_done[w][last], (phases >> last & 1u) ^ 1u, &s.abort_flag, p.status, 20);
-          tc_fence_after();
-          if (active) {
+      const int64_t at = slot * p.prefix_rows + (kWide ? row : r);
+      float* out = p.prefix_acc + at * D;
+      const int other = kWide ? 0 : (piece - (w ^ 1) * kStep + kPrefixTile - 1) / kPrefixTile;
+      other_phases ^= (uint32_t)((other + 1) / 2 & 1) | (uint32_t)(other / 2 & 1) << 1;
+      if (kWide || two) {
+        const int last = (n_steps - 1) & 1;
+        if (n_steps > 0) mbar_wait_warp(&s.o_done[w][last], (phases >> last & 1u) ^ 1u, &s.abort_flag, p.status, 20);
+        tc_fence_after();
+        if (active) {
 #pragma unroll 1
-            for (int c = 0; c < D; c += 32) {
-              uint32_t o[32];
-              tmem_ld32(to + c, o);
-              tmem_ld_wait(o);
-              if (there)
+          for (int c = 0; c < D; c += 32) {
+            uint32_t o[32];
+            tmem_ld32(to + c, o);
+            tmem_ld_wait(o);
+            if (n_steps == 0)  // a piece without keys for this half
 #pragma unroll
-                for (int j = 0; j < 32; j += 8) store8(out + c + j, o + j);
-            }
-            if (there) p.prefix_ml[slot * p.prefix_rows + row] = make_float2(m, l);
+              for (int j = 0; j < 32; ++j) o[j] = 0u;
+            if (there)
+#pragma unroll
+              for (int j = 0; j < 32; j += 8) store8(out + c + j, o + j);
           }
-          tc_fence_before();
+          if (there) p.prefix_ml[at] = make_float2(m, l);
         }
+        tc_fence_before();
       } else {
         // both halves hold sums of the same rows: each joins one half of the columns
-        const int other = (piece - (w ^ 1) * kStep + kPrefixTile - 1) / kPrefixTile;
-        other_phases ^= (uint32_t)((other + 1) / 2 & 1) | (uint32_t)(other / 2 & 1) << 1;
-        if (w == 0) s.ml[r] = make_float2(m, l);
+        s.ml[w][r] = make_float2(m, l);
         asm volatile("bar.sync 1, 256;" ::: "memory");
-        float2 x;
-        if (w == 1) x = s.ml[r], s.ml[r] = make_float2(m, l);
-        asm volatile("bar.sync 1, 256;" ::: "memory");
-        if (w == 0) x = s.ml[r];
+        const float2 x = s.ml[w ^ 1][r];
         const bool both = w == 0 ? other > 0 : n_steps > 0;  // the second half has keys of the piece
         const int last = (n_steps - 1) & 1, other_last = (other - 1) & 1;
         if (n_steps > 0) mbar_wait_warp(&s.o_done[w][last], (phases >> last & 1u) ^ 1u, &s.abort_flag, p.status, 21);
@@ -525,7 +523,7 @@ __global__ void __launch_bounds__(prefix_threads(kE4M3), 1) attn_prefix_kernel(c
             for (int j = 0; j < 16; ++j) a[j] = __float_as_uint(__uint_as_float(a[j]) * f0 + (both ? __uint_as_float(b[j]) * f1 : 0.f));
             if (there) store8(out + c, a), store8(out + c + 8, a + 8);
           }
-          if (there && w == 0) p.prefix_ml[slot * p.prefix_rows + row] = make_float2(top, l * mine + x.y * theirs);
+          if (there && w == 0) p.prefix_ml[at] = make_float2(top, l * mine + x.y * theirs);
         }
         tc_fence_before();
         asm volatile("bar.sync 1, 256;" ::: "memory");  // O and ml are free for the next unit
