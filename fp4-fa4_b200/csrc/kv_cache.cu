@@ -10,7 +10,7 @@ namespace fa4b {
 // of a compaction: used pages of each block of kBlockPages, holes, movers by the used pages before them, and those per page
 constexpr int kWorkStatus = kKvStatus, kWorkHead = kKvHead, kWorkFresh = 16, kWorkFlags = kWorkFresh + FA4B_KV_MAX_LIST,
               kWorkLists = kWorkFlags + FA4B_KV_MAX_LIST;
-constexpr int kBlockPages = 4096;
+constexpr int kBlockPages = 4096;  // of a compaction: 1024 threads x 4
 constexpr int kPieceBytes = 32768;  // what one CTA of the copy kernels moves: 256 threads x 8 x 16 bytes, all loads in flight at once
 constexpr int kWarpBytes = 4096;    // the same per warp
 constexpr int kCheckInline = 512;   // copy lists up to this length are checked for collisions by the copying CTAs themselves
@@ -53,8 +53,8 @@ __device__ __forceinline__ int block_scan1024(int v, int* warp_sums, int& total)
   return before;
 }
 
-// sixteen counts from page `p` on as a mask of the pages in use (or, with `want_free`, of the free ones)
-__device__ __forceinline__ uint32_t page_mask16(const KvView& c, int64_t p, bool want_free) {
+// sixteen counts from page `p` on as a mask of the free pages
+__device__ __forceinline__ uint32_t free_mask16(const KvView& c, int64_t p) {
   int r[16];
   if (p + 16 <= c.pages) {
     const int4* q = reinterpret_cast<const int4*>(c.refs + p);
@@ -65,12 +65,25 @@ __device__ __forceinline__ uint32_t page_mask16(const KvView& c, int64_t p, bool
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) r[i] = p + i < c.pages ? __ldcg(c.refs + p + i) : (want_free ? 1 : 0);
+    for (int i = 0; i < 16; ++i) r[i] = p + i < c.pages ? __ldcg(c.refs + p + i) : 1;
   }
   uint32_t m = 0;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) m |= (uint32_t)((r[i] > 0) != want_free) << i;
+  for (int i = 0; i < 16; ++i) m |= (uint32_t)(r[i] <= 0) << i;
   return m;
+}
+
+// the same for the four pages in use from `p` on
+__device__ __forceinline__ uint32_t used_mask4(const KvView& c, int64_t p) {
+  int4 r = make_int4(0, 0, 0, 0);
+  if (p + 4 <= c.pages) {
+    r = __ldcg(reinterpret_cast<const int4*>(c.refs + p));
+  } else {
+    if (p < c.pages) r.x = __ldcg(c.refs + p);
+    if (p + 1 < c.pages) r.y = __ldcg(c.refs + p + 1);
+    if (p + 2 < c.pages) r.z = __ldcg(c.refs + p + 2);
+  }
+  return (uint32_t)(r.x > 0) | (uint32_t)(r.y > 0) << 1 | (uint32_t)(r.z > 0) << 2 | (uint32_t)(r.w > 0) << 3;
 }
 
 // The first `want` free pages in ascending order into out[]; a block of 1024 threads looks at 16384 pages per step and
@@ -79,7 +92,7 @@ __device__ int find_free(const KvView& c, int want, int32_t* out, int* warp_sums
   int have = 0;
   for (int64_t base = 0; base < c.pages && have < want; base += 16384) {
     const int64_t p = base + threadIdx.x * 16;
-    uint32_t m = p < c.pages ? page_mask16(c, p, true) : 0u;
+    uint32_t m = p < c.pages ? free_mask16(c, p) : 0u;
     int total;
     int rank = have + block_scan1024(__popc(m), warp_sums, total);
     while (m != 0u && rank < want) {
@@ -238,7 +251,7 @@ __device__ __forceinline__ uint2 quantise8(uint4 x, QuantScale scale) {
 // grid (row of the batch x kv head, tile of tokens); a thread takes 16 bytes of K and of V of one token at a time, so a
 // warp reads 512 contiguous bytes and writes whole rows.  Bound by memory: 2 x 2 bytes read, 2 x (1 or 2) written a value.
 template <bool kE4M3, typename Src>
-__global__ void __launch_bounds__(256) kv_write_kernel(const KvView c, const WriteParams w) {
+__global__ void __launch_bounds__(256, 3) kv_write_kernel(const KvView c, const WriteParams w) {
   pdl_trigger();
   pdl_wait();
   const int i = blockIdx.x / c.heads, h = blockIdx.x - i * c.heads;
@@ -489,55 +502,44 @@ __device__ __forceinline__ CompactLists compact_lists(const KvView& c) {
   return l;
 }
 
-// used pages of each block of 4096
-__global__ void __launch_bounds__(256) kv_compact_count_kernel(const KvView c) {
+// used pages of each block, where there is more than one
+__global__ void __launch_bounds__(1024) kv_compact_count_kernel(const KvView c) {
   pdl_trigger();
   pdl_wait();
-  const int64_t p = (int64_t)blockIdx.x * kBlockPages + threadIdx.x * 16;
-  int v = p < c.pages ? __popc(page_mask16(c, p, false)) : 0;
-  __shared__ int sum;
-  if (threadIdx.x == 0) sum = 0;
-  __syncthreads();
-  v = __reduce_add_sync(0xffffffffu, v);
-  if ((threadIdx.x & 31) == 0) atomicAdd(&sum, v);
-  __syncthreads();
-  if (threadIdx.x == 0) compact_lists(c).counts[blockIdx.x] = sum;
+  __shared__ int warp_sums[32];
+  int total;
+  block_scan1024(__popc(used_mask4(c, (int64_t)blockIdx.x * kBlockPages + threadIdx.x * 4)), warp_sums, total);
+  if (threadIdx.x == 0) compact_lists(c).counts[blockIdx.x] = total;
 }
 
 // With U used pages in all and b(p) used pages below p: a free page p < U is hole p - b(p); a used page p >= U is the
 // mover after the b(p) - b(U) movers before it.  Movers are kept at b(p); head = {U, b(U)} lets the last launch pair them.
-__global__ void __launch_bounds__(256) kv_compact_plan_kernel(const KvView c) {
+__global__ void __launch_bounds__(1024) kv_compact_plan_kernel(const KvView c) {
   pdl_trigger();
   pdl_wait();
   const CompactLists l = compact_lists(c);
-  __shared__ int warp_sums[8], all_before, all_used;
-  if (threadIdx.x == 0) all_before = all_used = 0;
-  __syncthreads();
-  int before = 0, used = 0;
-  for (int j = threadIdx.x; j < (int)gridDim.x; j += 256) {
-    const int v = l.counts[j];
-    used += v;
-    before += j < (int)blockIdx.x ? v : 0;
+  __shared__ int warp_sums[32], sums[2];
+  if (threadIdx.x < 2) sums[threadIdx.x] = 0;
+  const int64_t p0 = (int64_t)blockIdx.x * kBlockPages + threadIdx.x * 4;
+  const uint32_t m = used_mask4(c, p0);
+  int n_used;
+  int b = block_scan1024(__popc(m), warp_sums, n_used);
+  if (gridDim.x > 1) {
+    int before = 0, used = 0;
+    for (int j = threadIdx.x; j < (int)gridDim.x; j += 1024) {
+      const int v = l.counts[j];
+      used += v;
+      before += j < (int)blockIdx.x ? v : 0;
+    }
+    used = __reduce_add_sync(0xffffffffu, used);
+    before = __reduce_add_sync(0xffffffffu, before);
+    if ((threadIdx.x & 31) == 0) atomicAdd(&sums[0], used), atomicAdd(&sums[1], before);
+    __syncthreads();
+    n_used = sums[0];
+    b += sums[1];
   }
-  used = __reduce_add_sync(0xffffffffu, used);
-  before = __reduce_add_sync(0xffffffffu, before);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  if (lane == 0) atomicAdd(&all_used, used), atomicAdd(&all_before, before);
-  const int64_t p0 = (int64_t)blockIdx.x * kBlockPages + threadIdx.x * 16;
-  const uint32_t m = p0 < c.pages ? page_mask16(c, p0, false) : 0u;
-  int x = __popc(m);
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, x, o);
-    if (lane >= o) x += y;
-  }
-  if (lane == 31) warp_sums[warp] = x;
-  __syncthreads();
-  int b = all_before + x - __popc(m);
-  for (int w = 0; w < warp; ++w) b += warp_sums[w];
-  const int n_used = all_used;
-#pragma unroll
-  for (int j = 0; j < 16; ++j) {
+  for (int j = 0; j < 4; ++j) {
     const int64_t p = p0 + j;
     if (p >= c.pages) break;
     if (p == n_used) c.work[kWorkHead] = n_used, c.work[kWorkHead + 1] = b;
@@ -745,8 +747,9 @@ int fa4b_kv_compact(const fa4b_kv_cache* c, void* stream) {
   if (int s = kv_view(c, &v)) return s;
   const int pieces = (v.block_bytes + kPieceBytes - 1) / kPieceBytes;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  FA4B_CUDA(launch_overlapped(kv_compact_count_kernel, compact_blocks(v.pages), 256, 0, st, v));
-  FA4B_CUDA(launch_overlapped(kv_compact_plan_kernel, compact_blocks(v.pages), 256, 0, st, v));
+  const int blocks = compact_blocks(v.pages);
+  if (blocks > 1) FA4B_CUDA(launch_overlapped(kv_compact_count_kernel, blocks, 1024, 0, st, v));
+  FA4B_CUDA(launch_overlapped(kv_compact_plan_kernel, blocks, 1024, 0, st, v));
   const int64_t most = std::max<int64_t>((int64_t)(v.pages / 2) * v.layers * 2 * pieces, (v.max_seqs + 7) / 8);
   const unsigned grid = (unsigned)std::min<int64_t>(std::max<int64_t>(most, 1), (int64_t)std::max(sm_count(), 1) * 6);
   FA4B_CUDA(launch_overlapped(kv_compact_move_kernel, grid, 256, 0, st, v, pieces));
