@@ -446,3 +446,144 @@ def test_a_generation_from_the_prompt_to_compaction():
     c.compact()
     assert int(c.ref_counts.sum()) == 0 and int(c.seq_lens.sum()) == 0 and (c.page_table == -1).all()
     c.check_status()
+
+
+def test_pools_and_tables_that_are_views():
+    """K and V as views of one tensor with layers between them, a table whose rows are part of a wider tensor."""
+    layers, pages, page, hkv, d = 3, 30, 32, 2, 128
+    gen = torch.Generator().manual_seed(40)
+    both = torch.randn(layers, pages, 2, hkv, page, d, generator=gen).to(BF).to(DEV)
+    wide = torch.full((4, 40), 7777, dtype=torch.int32, device=DEV)
+    table = wide[:, 5:17]
+    c = PagedKVCache(both[:, :, 0], both[:, :, 1], table, torch.zeros(4, dtype=torch.int32, device=DEV), torch.zeros(pages, dtype=torch.int32, device=DEV))
+    table.fill_(-1)
+    slots = [2, 0, 3]
+    c.extend(ints(slots), ints([300, 33, 200]))
+    c.fork(ints([2]), ints([1]))
+    assert (wide[:, :5] == 7777).all() and (wide[:, 17:] == 7777).all()
+    q = queries(4, 6, 2, d, BF, 41)
+    for layer in range(layers):
+        out, lse = c.attend(q, ints([2, 1, 0, 3]), layer=layer, group_offsets=ints([0, 2, 4]), shared_lens=ints([288, 0]))
+        compare(c, q, out, lse, [2, 1, 0, 3], layer=layer)
+    c.check_status()
+
+
+def test_a_pool_beyond_32_bit_offsets():
+    """Pages whose elements lie beyond 2^32: written, copied, forked, attended to (both kinds of units)."""
+    page, hkv, d, pages = 128, 8, 128, 33500  # 4.4e9 elements a pool
+    k, v = [torch.empty(1, pages, hkv, page, d, dtype=BF, device=DEV) for _ in range(2)]
+    refs = torch.ones(pages, dtype=torch.int32, device=DEV)
+    refs[pages - 40:] = 0
+    refs[3] = 0
+    c = PagedKVCache(k, v, torch.full((8, 20), -1, dtype=torch.int32, device=DEV), torch.zeros(8, dtype=torch.int32, device=DEV), refs)
+    c.extend(ints([0, 1]), ints([300, 700]))
+    for s, n in ((0, 300), (1, 700)):
+        gen = torch.Generator().manual_seed(s)
+        c.write(*[torch.randn(1, hkv, n, d, generator=gen).to(BF).to(DEV) for _ in range(2)], ints([s]))
+    c.fork(ints([1, 1, 1]), ints([2, 3, 4]))
+    assert int(c.page_table[1, 0]) == pages - 38 and int(c.page_table[0, 0]) == 3
+    q = queries(5, 16, 1, d, BF, 42)
+    for args in ({}, dict(group_offsets=ints([0, 1, 5]), shared_lens=ints([0, 640]))):
+        out, lse = c.attend(q, ints([0, 1, 2, 3, 4]), **args)
+        compare(c, q, out, lse, [0, 1, 2, 3, 4])
+    last = int(c.page_table[1, 1])
+    c.copy_pages(ints([last]), ints([pages - 1]))
+    assert torch.equal(c.k[0, pages - 1], c.k[0, last]) and torch.equal(c.v[0, pages - 1], c.v[0, last])
+    c.free(ints([0]))
+    c.compact()  # the last of the used pages moves into the hole
+    out2, lse2 = c.attend(q[1:], ints([1, 2, 3, 4]))
+    assert torch.equal(out2, c.attend(q[1:], ints([1, 2, 3, 4]))[0])
+    compare(c, q[1:], out2, lse2, [1, 2, 3, 4])
+    c.check_status()
+
+
+@pytest.mark.parametrize("hq,hkv,t", [(128, 1, 16), (64, 2, 16), (40, 8, 3)])
+def test_many_rows_of_one_sequence(hq, hkv, t):
+    lens = [500, 17, 260]
+    c, slots, _ = build(lens, [], [], hkv=hkv, d=64, seed=43)
+    q = queries(3, hq, t, 64, BF, 44)
+    out, lse = c.attend(q, ints(slots))
+    compare(c, q, out, lse, slots)
+    lens = [400, 300, 271 + t]
+    c, slots, offsets = build(lens, [256], [3], hkv=hkv, d=64, seed=45)
+    out, lse = c.attend(q, ints(slots), group_offsets=ints(offsets), shared_lens=ints([256]))
+    compare(c, q, out, lse, slots)
+    c.check_status()
+
+
+def test_thousands_of_groups():
+    n = 4096
+    lens = [40 + i % 30 for i in range(n)]
+    members = [2] * (n // 2)
+    c, slots, offsets = build(lens, [32] * len(members), members, hkv=1, d=64, seed=46)
+    q = queries(n, 4, 1, 64, BF, 47)
+    out, lse = c.attend(q, ints(slots), group_offsets=ints(offsets), shared_lens=ints([32] * len(members)))
+    c.check_status()
+    compare(c, q, out, lse, slots, rows=list(range(0, n, 61)) + [n - 1])
+    ones = ints(list(range(n + 1)))
+    out, lse = c.attend(q, ints(slots), group_offsets=ones, shared_lens=ints([32] * n))
+    compare(c, q, out, lse, slots, rows=range(0, n, 97))
+
+
+@pytest.mark.parametrize("qt", [BF, HF])
+def test_scales_of_either_sign_and_zero(qt):
+    lens = [200 + 16, 200 + 33, 200 + 7]
+    c, slots, offsets = build(lens, [192], [3], hkv=3, d=128, dtype=E4, seed=48)
+    c.k_scale[0] = torch.tensor([0.1, -0.13, 0.0], device=DEV)
+    c.v_scale[0] = torch.tensor([-0.2, 0.1, 0.3], device=DEV)
+    q = queries(3, 12, 1, 128, qt, 49)
+    for args in ({}, dict(group_offsets=ints(offsets), shared_lens=ints([192]))):
+        out, lse = c.attend(q, ints(slots), **args)
+        compare(c, q, out, lse, slots)
+
+
+def test_what_is_no_number_shows_in_its_row_alone():
+    lens = [300, 280, 290]
+    c, slots, offsets = build(lens, [256], [3], hkv=2, d=128, seed=50)
+    q = queries(3, 8, 1, 128, BF, 51)
+    args = dict(group_offsets=ints(offsets), shared_lens=ints([256]))
+    clean, clean_lse = c.attend(q, ints(slots), **args)
+    bad = q.clone()
+    bad[1, 2, 0, 5] = float("nan")
+    out, lse = c.attend(bad, ints(slots), **args)
+    assert out[1, 2].isnan().all() and lse[1, 2].isnan().all()
+    keep = torch.ones(3, 8, dtype=torch.bool)
+    keep[1, 2] = False
+    assert torch.equal(out[keep.to(DEV)], clean[keep.to(DEV)]) and torch.equal(lse[keep.to(DEV)], clean_lse[keep.to(DEV)])
+    # a shared key that is no number: every row of its kv head, and none of the other's
+    p = int(c.page_table[slots[0], 3])
+    c.k[0, p, 1, 7] = float("nan")
+    out, lse = c.attend(q, ints(slots), **args)
+    assert out[:, 4:].isnan().all() and torch.equal(out[:, :4], clean[:, :4])
+
+
+def test_calls_on_two_streams_at_once():
+    lens = [900 + 40 * i for i in range(12)]
+    c, slots, offsets = build(lens, [800], [12], hkv=2, d=128, seed=52)
+    qs = [queries(12, 8, t, 128, BF, 53 + t) for t in (1, 2)]
+    args = dict(group_offsets=ints(offsets), shared_lens=ints([800]))
+    s = ints(slots)
+    want = [c.attend(q, s, **args) for q in qs]
+    streams = [torch.cuda.Stream() for _ in qs]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for turn in range(10):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(c.attend(qs[i], s, **args))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for out, lse in got[i]:
+            assert torch.equal(out, want[i][0]) and torch.equal(lse, want[i][1])
+    c.check_status()
+
+
+@pytest.mark.parametrize("length", [-5, 2 ** 31 - 1])
+def test_lengths_that_cannot_be_are_cut_to_the_table(length):
+    c, slots, _ = build([64, 64], [], [], hkv=1, d=64, width=4, seed=54)
+    q = queries(2, 4, 1, 64, BF, 55)
+    c.seq_lens[slots[1]] = length
+    out, lse = c.attend(q, ints(slots))
+    c.check_status()
+    c.seq_lens[slots[1]] = 64 if length > 0 else 0
+    compare(c, q, out, lse, slots)
