@@ -6,6 +6,7 @@
 // be empty for the most part, and the 16-row form already computes a tile in a quarter of the time its bytes take.
 #include "attn_paged.cuh"
 
+#include <cmath>
 #include <cstddef>
 #include <type_traits>
 
@@ -1131,6 +1132,7 @@ static int paged_params(const fa4b_kv_cache* c, const fa4b_attn_paged_args* a, P
   for (int64_t s : {p.q_sb, p.q_sh, p.q_st, p.o_sb, p.o_sh, p.o_st})
     FA4B_REQUIRE(s % 8 == 0, FA4B_BAD_ALIGN, "strides of q and o must be multiples of 8 elements");
   FA4B_REQUIRE(!off16(p.q) && !off16(p.o), FA4B_BAD_ALIGN, "q and o must be 16-byte aligned");
+  FA4B_REQUIRE(std::isfinite(a->softmax_scale), FA4B_BAD_ARG, "softmax_scale is not a finite number");
   p.scale_log2 = (a->softmax_scale > 0.f ? a->softmax_scale : 1.0f / sqrtf((float)c->D)) * kLog2e;
   if (c->dtype == FA4B_KV_E4M3) p.k_scale = c->k_scale + (int64_t)a->layer * c->Hkv, p.v_scale = c->v_scale + (int64_t)a->layer * c->Hkv;
   const int n_sm = sm_count() > 0 ? sm_count() : 148;

@@ -207,6 +207,8 @@ class PagedKVCache:
             raise ValueError(f"out must be a {tuple(shape)} tensor like q with a contiguous head dimension")
         lse = q.new_empty((n, hq, t), dtype=torch.float32)
         code, scale = KV_DTYPES[q.dtype], softmax_scale or 0.0
+        if not scale >= 0.0:
+            raise ValueError(f"softmax_scale must be positive, got {softmax_scale}")
         q_strides, o_strides = _strides(q), _strides(out)
         size = self._ws_bytes.get((n, hq, t, groups))
         if size is None:

@@ -587,3 +587,10 @@ def test_lengths_that_cannot_be_are_cut_to_the_table(length):
     c.check_status()
     c.seq_lens[slots[1]] = 64 if length > 0 else 0
     compare(c, q, out, lse, slots)
+
+
+@pytest.mark.parametrize("scale", [-0.1, float("nan"), float("inf")])
+def test_a_softmax_scale_that_cannot_be_is_refused(scale):
+    c, slots, _ = build([50, 20], [], [], hkv=2, d=64, seed=20)
+    with pytest.raises(ValueError, match="softmax_scale"):
+        c.attend(queries(2, 4, 1, 64, BF, 0), ints(slots), softmax_scale=scale)

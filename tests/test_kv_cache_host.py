@@ -104,6 +104,9 @@ def test_attention_over_the_cache_is_refused_before_a_launch():
                                  (dict(seqs=0, n=11), 1, b"list of slots"), (dict(q=0x1008), 2, b"16-byte"), (dict(o_strides=_lib.Strides(4, 8, 8)), 2, b"multiples of 8")):
         got, size, error = call(**change)
         assert got == status and size == 0 and text in error, change
+    for scale in (float("nan"), float("inf"), float("-inf")):
+        got, size, error = call(softmax_scale=scale)
+        assert got == 6 and size == 0 and b"finite" in error
     assert call(ws=0)[0] == 6 and call(lse=0)[0] == 6 and call(ws=0x10010)[0] == 2 and call(n=0, q=0, o=0, lse=0, ws=0)[0] == 0
     got, size, error = call(cache=good(table_width=1 << 18, table_stride=1 << 18, page_tokens=128, k_page_stride=1 << 17, v_page_stride=1 << 17, max_seqs=5000), n=4096)
     assert got == 1 and size == 0 and b"too many" in error
