@@ -200,6 +200,8 @@ class PagedKVCache:
             shared, groups = self._list(shared_lens, "shared_lens"), shared_lens.shape[0]
             if group_offsets.shape[0] != groups + 1:
                 raise ValueError(f"group_offsets must have {groups + 1} entries, got {group_offsets.shape[0]}")
+            if groups == 0 and n > 0:
+                raise ValueError("no groups: without group_offsets and shared_lens every row stands by itself")
             offsets = self._list(group_offsets, "group_offsets")
         if out is None:
             out = torch.empty_like(q, memory_format=torch.contiguous_format)

@@ -594,3 +594,12 @@ def test_a_softmax_scale_that_cannot_be_is_refused(scale):
     c, slots, _ = build([50, 20], [], [], hkv=2, d=64, seed=20)
     with pytest.raises(ValueError, match="softmax_scale"):
         c.attend(queries(2, 4, 1, 64, BF, 0), ints(slots), softmax_scale=scale)
+
+
+def test_an_empty_list_of_groups_is_refused():
+    """Rows in no group are left as they were, which with no group at all is every row; a C call with groups == 0 computes all of them."""
+    c, slots, _ = build([50, 20], [], [], hkv=2, d=64, seed=20)
+    with pytest.raises(ValueError, match="no groups"):
+        c.attend(queries(2, 4, 1, 64, BF, 0), ints(slots), group_offsets=ints([0]), shared_lens=ints([]))
+    out, lse = c.attend(queries(0, 4, 1, 64, BF, 0), ints([]), group_offsets=ints([0]), shared_lens=ints([]))
+    assert out.shape == (0, 4, 1, 64) and lse.shape == (0, 4, 1)
