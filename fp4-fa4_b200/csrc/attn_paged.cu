@@ -1131,6 +1131,7 @@ static int paged_params(const fa4b_kv_cache* c, const fa4b_attn_paged_args* a, P
   p.lse = a->lse;
   for (int64_t s : {p.q_sb, p.q_sh, p.q_st, p.o_sb, p.o_sh, p.o_st})
     FA4B_REQUIRE(s % 8 == 0, FA4B_BAD_ALIGN, "strides of q and o must be multiples of 8 elements");
+  FA4B_REQUIRE((p.n <= 1 || p.o_sb != 0) && (p.Hq == 1 || p.o_sh != 0) && (p.T == 1 || p.o_st != 0), FA4B_BAD_SHAPE, "rows of o lie on one another (a stride of 0)");
   FA4B_REQUIRE(!off16(p.q) && !off16(p.o), FA4B_BAD_ALIGN, "q and o must be 16-byte aligned");
   FA4B_REQUIRE(std::isfinite(a->softmax_scale), FA4B_BAD_ARG, "softmax_scale is not a finite number");
   p.scale_log2 = (a->softmax_scale > 0.f ? a->softmax_scale : 1.0f / sqrtf((float)c->D)) * kLog2e;

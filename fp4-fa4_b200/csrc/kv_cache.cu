@@ -622,6 +622,8 @@ int kv_view(const fa4b_kv_cache* c, KvView* out) {
     FA4B_REQUIRE(s >= 0 && s * esz % 16 == 0, FA4B_BAD_ALIGN, "layer and page strides must be multiples of 16 bytes");
   FA4B_REQUIRE(c->num_pages == 1 || (c->k_page_stride >= block && c->v_page_stride >= block), FA4B_BAD_SHAPE, "pages overlap: the page stride is below %lld",
                (long long)block);
+  FA4B_REQUIRE(c->layers == 1 || (c->k_layer_stride >= block && c->v_layer_stride >= block), FA4B_BAD_SHAPE, "layers overlap: the layer stride is below %lld",
+               (long long)block);
   KvView v{};
   v.k = static_cast<uint8_t*>(c->k);
   v.v = static_cast<uint8_t*>(c->v);

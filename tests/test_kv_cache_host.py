@@ -31,6 +31,31 @@ def test_every_call_refuses_a_bad_cache(change, status, text):
         assert got == status and text in h.fa4b_last_error()
 
 
+@pytest.mark.parametrize("which", ["k_layer_stride", "v_layer_stride"])
+def test_layers_that_lie_on_one_another_are_refused(which):
+    h = _lib.lib()
+    block = 8 * 16 * 128
+    for stride, status in ((0, 1), (block - 128, 1), (block, 0)):
+        c = good(**{which: stride})
+        assert h.fa4b_kv_free(C.addressof(c), 0, 0, 0) == status and (status == 0 or b"layers overlap" in h.fa4b_last_error())
+    c = good(layers=1, **{which: 0})  # one layer: the stride says nothing
+    assert h.fa4b_kv_free(C.addressof(c), 0, 0, 0) == 0
+
+
+def test_rows_of_the_result_that_lie_on_one_another_are_refused():
+    h = _lib.lib()
+    c, z = good(), _lib.Strides(1024, 128, 128)
+
+    def call(o_strides, n=2, T=2):
+        a = _lib.AttnPagedArgs(q=0x1000, q_strides=z, o=0x2000, o_strides=o_strides, lse=0x3000, n=n, T=T, Hq=8, layer=0, q_dtype=0, softmax_scale=0.0, seqs=0x4000,
+                               groups=0, group_offsets=0, shared_lens=0, ws=0x10000)
+        return h.fa4b_attn_paged_workspace_bytes(C.addressof(c), C.addressof(a))
+
+    for bad in ((0, 128, 1024), (2048, 0, 1024), (2048, 128, 0)):
+        assert call(_lib.Strides(*bad)) == 0 and b"one another" in h.fa4b_last_error()
+    assert call(_lib.Strides(2048, 128, 1024)) > 0 and call(_lib.Strides(0, 128, 0), n=1, T=1) > 0
+
+
 def test_lists_and_arguments_are_checked():
     h = _lib.lib()
     c = good()
