@@ -1,9 +1,16 @@
 // Attention of the newest tokens of a batch over a paged cache (single tokens, or a few drafted ones), with the keys that
 // a group of sequences shares read once for all of them.
 //
-// Bound by memory: a key and a value are used by the few query rows of one sequence (own units), so the kernel is a
-// stream of pages through shared memory: tiles are asked for by TMA several tiles ahead.  Scores and values go through mma.sync m16n8k16: with 4 to 16 query rows a tcgen05 tile of 128 rows would
-// be empty for the most part, and the 16-row form already computes a tile in a quarter of the time its bytes take.
+// A call is a chain of launches, each of which comes up while the one before still runs: plan (who reads what), prefix units
+// (only with groups: attn_prefix.cu), own units, join.  For 32 sequences of 600 keys behind 8219 shared ones (32 query and 8 kv heads,
+// D 128, bf16) that is 32 us: plan 5, prefix 13.5, own 9 beside and behind it, join 3-5, against 11 us for the bytes; what is left is
+// the latency of the chain.  One sequence of 1000 keys takes 10 us in a graph.
+//
+// Own units are bound by memory: a key and a value are used by the few query rows of one sequence, so the kernel is a
+// stream of pages through shared memory, with tiles asked for by TMA several tiles ahead: 32 sequences of up to 8k keys, 537
+// MB of bf16, take 97 us with all launches (5.5 TB/s), 268 MB of E4M3 60 us.  Scores and values go through mma.sync m16n8k16:
+// with 4 to 16 query rows a tcgen05 tile of 128 rows would be empty for the most part, and up to 16 rows the products of a tile
+// take less time than its bytes.  With 64 rows they do not any more (bf16 237 us).
 #include "attn_paged.cuh"
 
 #include <cmath>
@@ -14,7 +21,7 @@ namespace fa4b {
 
 // ---- plan -------------------------------------------------------------------------------------------------------------
 // One CTA, and every other launch of the call waits for it.  More warps would walk the same instructions and cost more than
-// they help (1024 threads took 7.1 us for 32 sequences), and what is sums over items a warp does alone: three of them at once
+// they help (1024 threads took 7.1 us for 32 sequences, these 5), and what is sums over items a warp does alone: three of them at once
 // for the three lines of sums, without a barrier.
 constexpr int kPlanThreads = 256;
 
@@ -454,7 +461,8 @@ struct PagedRows {
 
 // Up to eight query rows (a single token of up to eight query heads per kv head), the other way round: keys and values are the
 // 16-row operand of the products, S^T = K Q^T and O^T += V^T P^T, and the query rows their eight columns, so that no half of
-// a product is empty and a thread holds half as many scores, accumulators and query values.  A thread has two rows (2c and
+// a product is empty and a thread holds half as many scores, accumulators and query values: three CTAs fit on an SM instead of two
+// (97 against 107 us for 32 sequences of up to 8k bf16 keys, 60 against 74 us for E4M3).  A thread has two rows (2c and
 // 2c + 1), and of a tile of sixteen keys the keys quad and quad + 8 of both.
 template <int D, bool kE4M3, typename QT>
 struct PagedRows8 {
@@ -708,7 +716,8 @@ struct OwnOrder {
 };
 
 // Up to sixteen query rows per unit (a single token, or a few drafted ones, of a group of query heads): every warp is a worker
-// with a line piece, a ring of tiles and copies of its own, and nothing in the loop waits for another warp.
+// with a line piece, a ring of tiles and copies of its own, and nothing in the loop waits for another warp (four warps that shared
+// their tiles, as in the team below, took 25 us where this takes 12.4 and the memory 5).
 template <int D, bool kE4M3, int kRows>
 struct SoloSmem {
   static constexpr int kRowBytes = D * (kE4M3 ? 1 : 2);
@@ -828,7 +837,7 @@ __global__ void __launch_bounds__(128, kRows == 8 ? 3 : 2) attn_solo_kernel(cons
 }
 
 // More rows than that: kWM warps side by side over rows (16 each), 4 / kWM over the keys of a tile of 64; a fifth warp asks for
-// the tiles.
+// the tiles.  Bound by the products (eight warps per SM and mma.sync: 134 us for 32 rows over 537 MB of bf16).
 template <int D, bool kE4M3>
 struct TeamSmem {
   static constexpr int kKeys = 64;
@@ -963,7 +972,8 @@ __global__ void __launch_bounds__(160, 2) attn_team_kernel(const PagedParams p, 
 // ---- join -------------------------------------------------------------------------------------------------------------
 // One warp per output row, or (kSplit) four, each with a quarter of the pieces, where the rows are few.  The pieces' statistics
 // come to the lanes at once, so that what is left to wait for is one round of loads: a lane holds D / 32 neighbours of eight
-// pieces at a time.  Which pieces there are follows from the plan, which is complete when this launch comes up (the own units
+// pieces at a time (one piece behind another took 26 us where this takes 12, and 3 to 5 with four warps).  Latency bounds it, and for
+// many rows the memory (16384 rows of 5 to 7 pieces: 18 us).  Which pieces there are follows from the plan, which is complete when this launch comes up (the own units
 // trigger behind it), so it is looked up before the wait.
 template <int D, typename QT, bool kSplit>
 __global__ void __launch_bounds__(128) paged_join_kernel(const PagedParams p) {
@@ -1094,13 +1104,18 @@ static int launch_paged(const PagedParams& p, const PagedMaps& m, cudaStream_t s
   FA4B_CUDA(launch_overlapped(paged_plan_kernel, 1, kPlanThreads, smem, st, p));
   if (p.groups > 0)
     if (int s = launch_prefix(p, D, kE4M3, std::is_same<QT, TagF16>::value, m.prefix_k, m.prefix_v, st)) return s;
-  const int s = p.own_rows == 8    ? launch_units<SoloSmem<D, kE4M3, 8>>(attn_solo_kernel<D, kE4M3, QT, 8>, p, m.own_k, m.own_v, p.own_workers / 4, 128, st, allowed[4])
-                : p.own_rows == 16 ? launch_units<SoloSmem<D, kE4M3, 16>>(attn_solo_kernel<D, kE4M3, QT, 16>, p, m.own_k, m.own_v, p.own_workers / 4, 128, st, allowed[0])
-                : p.own_rows == 32 ? launch_units<TeamSmem<D, kE4M3>>(attn_team_kernel<D, kE4M3, QT, 2>, p, m.own_k, m.own_v, p.own_workers, 160, st, allowed[1])
-                                   : launch_units<TeamSmem<D, kE4M3>>(attn_team_kernel<D, kE4M3, QT, 4>, p, m.own_k, m.own_v, p.own_workers, 160, st, allowed[2]);
+  // which of these a type takes: see paged_params
+  int s;
+  if (p.own_rows == 8) s = launch_units<SoloSmem<D, kE4M3, 8>>(attn_solo_kernel<D, kE4M3, QT, 8>, p, m.own_k, m.own_v, p.own_workers / 4, 128, st, allowed[4]);
+  else if (p.own_rows == 16) s = launch_units<SoloSmem<D, kE4M3, 16>>(attn_solo_kernel<D, kE4M3, QT, 16>, p, m.own_k, m.own_v, p.own_workers / 4, 128, st, allowed[0]);
+  else if constexpr (kE4M3 && D == 128) s = FA4B_UNSUPPORTED;
+  else if (p.own_rows == 32) s = launch_units<TeamSmem<D, kE4M3>>(attn_team_kernel<D, kE4M3, QT, 2>, p, m.own_k, m.own_v, p.own_workers, 160, st, allowed[1]);
+  else if constexpr (!kE4M3 && D == 64) s = FA4B_UNSUPPORTED;
+  else s = launch_units<TeamSmem<D, kE4M3>>(attn_team_kernel<D, kE4M3, QT, 4>, p, m.own_k, m.own_v, p.own_workers, 160, st, allowed[2]);
   if (s) return s;
   const int64_t rows = (int64_t)p.n * p.Hq * p.T;
-  // four warps a row up to where the rows alone fill the SMs with warps (8 CTAs of four each; 5.7 against 7.0 us of a 34 us call with 1024 rows, but 5.8 against 3.5 us with 1536)
+  // four warps a row up to where the rows alone fill the SMs with warps, 8 CTAs of four each (1024 rows: 5.7 against 7.0 us; 1536 rows:
+  // 5.8 against 3.5 us)
   if (rows <= 8ll * p.prefix_workers) FA4B_CUDA(launch_overlapped(paged_join_kernel<D, QT, true>, (unsigned)rows, 128, 0, st, p));
   else FA4B_CUDA(launch_overlapped(paged_join_kernel<D, QT, false>, (unsigned)((rows + 3) / 4), 128, 0, st, p));
   return FA4B_OK;
@@ -1137,7 +1152,14 @@ static int paged_params(const fa4b_kv_cache* c, const fa4b_attn_paged_args* a, P
   p.scale_log2 = (a->softmax_scale > 0.f ? a->softmax_scale : 1.0f / sqrtf((float)c->D)) * kLog2e;
   if (c->dtype == FA4B_KV_E4M3) p.k_scale = c->k_scale + (int64_t)a->layer * c->Hkv, p.v_scale = c->v_scale + (int64_t)a->layer * c->Hkv;
   const int n_sm = sm_count() > 0 ? sm_count() : 148;
-  p.own_rows = p.R <= 8 ? 8 : p.R <= 16 ? 16 : p.R <= 32 ? 32 : 64;
+  // Rows of an own unit.  32 sequences of up to 8k keys, 8 kv heads (us; rows of a sequence and kv head on the left):
+  //   bf16 D 128   8: 8 rows 97, 16 rows 107, 32 rows 120     16: 16 rows 109, 32 rows 124      32: 16 rows 187, 32 rows 134, 64 rows 212
+  //   56 (4 kv heads): 16 rows 162, 32 rows 123, 64 rows 120
+  //   E4M3 D 128   8: 8 rows 60, 16 rows 74     16: 16 rows 78, 32 rows 151     32: 16 rows 145, 32 rows 161     56: 16 rows 141, 64 rows 146
+  //   bf16 D 64   32: 16 rows 104, 32 rows 87      56: 32 rows 86, 64 rows 90       E4M3 D 64   32: 16 rows 110, 32 rows 94      56: 32 rows 92, 64 rows 82
+  // With E4M3 and D = 128 a warp spends as long on turning codes as on products, and the warps of a team all turn the same ones.
+  const bool wide_codes = c->dtype == FA4B_KV_E4M3 && c->D == 128, short_16 = c->dtype != FA4B_KV_E4M3 && c->D == 64;
+  p.own_rows = p.R <= 8 ? 8 : p.R <= 16 || wide_codes ? 16 : p.R <= 32 || short_16 ? 32 : 64;
   p.own_blocks = (p.R + p.own_rows - 1) / p.own_rows;
   const bool solo = p.own_rows <= 16, short_rows = c->D * (c->dtype == FA4B_KV_E4M3 ? 1 : 2) < 256;
   p.own_tile = !solo ? TeamSmem<64, true>::kKeys : short_rows ? 32 : 16;
@@ -1145,9 +1167,12 @@ static int paged_params(const fa4b_kv_cache* c, const fa4b_attn_paged_args* a, P
   p.own_workers = (p.own_rows == 8 ? 12 : solo ? 8 : 2) * n_sm;
   p.own_extra = solo ? 2 : 1;
   p.own_min = solo ? 64 / p.own_tile : 1;  // a piece shorter than 64 keys is mostly its beginning
-  // two blocks of 128 rows over the same keys where the groups have the rows for it: each tile then comes from memory half
-  // as often; otherwise the two halves of a CTA take the keys in turn
-  p.prefix_rows = p.groups > 0 && (int64_t)p.n * p.R > 128ll * p.groups ? 256 : 128;
+  // Two blocks of 128 rows over the same keys where the groups have the rows for it: each tile then comes from memory half as
+  // often (8 groups of 160 rows over 8k keys: bf16 D 128 99 against 135 us, E4M3 108 against 125, D 64 83 against 91 and 94
+  // against 97).  With fewer rows the two halves of a CTA take the keys in turn (8 groups of 128 rows: E4M3 83 against 86 us,
+  // D 64 61 against 67; 8 groups of 16 rows over 32k keys: 172 against 197 and 99 against 155); but bf16 with D = 128 is bound by the
+  // tensor core's 64-key products either way and better off without the join of the halves (83 against 87 us; 207 against 215).
+  p.prefix_rows = p.groups > 0 && ((int64_t)p.n * p.R > 128ll * p.groups || paged_prefix_wide(c->D, c->dtype == FA4B_KV_E4M3)) ? 256 : 128;
   p.prefix_shift = __builtin_ctz((unsigned)p.prefix_rows), p.prefix_workers = n_sm, p.prefix_extra = 3;
   const int64_t keys = (int64_t)c->table_width * c->page_tokens, own_length = 2 * (keys / p.own_tile) + 2 + p.own_extra;
   const int64_t prefix_units = p.groups ? (int64_t)c->Hkv * (((int64_t)p.n * p.R + p.prefix_rows - 1) / p.prefix_rows + p.groups) : 0;

@@ -261,6 +261,9 @@ struct PagedWalk {
   }
 };
 
+// Caches whose prefix units always have two blocks of 128 rows.
+__host__ __device__ constexpr bool paged_prefix_wide(int D, bool e4m3) { return D == 128 && !e4m3; }
+
 // A prefix unit of up to 64 rows in a CTA whose halves share 128: rows 0-63 take the first half's keys and rows 64-127, the same
 // rows again, the second half's, so that the warps at work sit in different quarters of the SM.
 __device__ __forceinline__ int prefix_in_two(const PagedParams& p, int rows) { return p.prefix_rows == 128 && rows <= 64; }

@@ -7,8 +7,14 @@
 // 128-255 of the unit, both over every key; else the same 128 rows, the first and the last 64 keys of a tile, joined in
 // TMEM at the end).  Either half works in steps of 64 keys on two score buffers of its own: while it exponentiates one,
 // the tensor core fills the other, so that it hardly ever waits (with one buffer of 128 keys per half a step spent as long
-// waiting for P V and the next Q K^T as exponentiating: 282 us instead of @@).  Warp 8 asks for pages by TMA, warps 9 and
-// 10 issue the products of the halves.  An E4M3 cache arrives as codes; warps 11-14 turn each tile into f16 (exact) in the operand ring.
+// waiting for P V and the next Q K^T as exponentiating).  Warp 8 asks for pages by TMA, warps 9 and 10 issue the products of the
+// halves.  An E4M3 cache arrives as codes; warps 11-14 turn each tile into f16 (exact) in the operand ring.
+//
+// 2048 rows (128 sequences of 4 tokens and 4 query heads) over 32768 keys and 8 kv heads, D 128, bf16: 255 us (275 GFLOP: 0.66 of
+// the rate measured for a library's product of large matrices; one buffer 281 us, one issuing warp 482).  The tensor core bounds it: a
+// product of 64 keys takes it about 85 cycles, as long as one of 128, so a step of 64 keys costs more than its share; scores of 128
+// keys at once would leave no second buffer and were slower (382 against 333 us for the call).  With 128 rows and 8k keys it is 13.5
+// us: 7 of them are the beginning (plan, query rows, first pages) and the end (the sums out of TMEM).
 //
 // A shared part ends on a multiple of 16 keys (the plan sees to it): the last tile's products take N = its keys and K = its
 // keys, so nothing behind them is read and no row needs a mask.
@@ -551,7 +557,8 @@ static int launch_prefix_of(const PagedParams& p, const CUtensorMap& mk, const C
 
 template <int D, bool kE4M3, typename QT>
 static int launch_prefix_wide(const PagedParams& p, const CUtensorMap& mk, const CUtensorMap& mv, cudaStream_t st) {
-  return p.prefix_rows == 256 ? launch_prefix_of<D, kE4M3, QT, true>(p, mk, mv, st) : launch_prefix_of<D, kE4M3, QT, false>(p, mk, mv, st);
+  if constexpr (paged_prefix_wide(D, kE4M3)) return launch_prefix_of<D, kE4M3, QT, true>(p, mk, mv, st);
+  else return p.prefix_rows == 256 ? launch_prefix_of<D, kE4M3, QT, true>(p, mk, mv, st) : launch_prefix_of<D, kE4M3, QT, false>(p, mk, mv, st);
 }
 
 int launch_prefix(const PagedParams& p, int D, bool e4m3, bool q_f16, const CUtensorMap& mk, const CUtensorMap& mv, cudaStream_t st) {
