@@ -87,6 +87,7 @@ class PagedKVCache:
         self._lib = lib()
         self._heads, self._d, self._takes = heads, d, (torch.bfloat16, torch.float16) if e4m3 else (k.dtype,)
         self._ws_bytes: dict = {}
+        self._floats = torch.empty(0, dtype=torch.float32, device=self.device)
         self._work = torch.zeros((self._lib.fa4b_kv_workspace_bytes(self._at) + 3) // 4, dtype=torch.int32, device=self.device)
         self._c.work = ptr(self._work)
         self._call("fa4b_kv_free", 0, 0)  # an empty list: the checks of the C side
@@ -121,26 +122,37 @@ class PagedKVCache:
     def _list(self, t, name: str, n: int = -1) -> int:
         if type(t) is not torch.Tensor or t.dtype is not torch.int32 or t.dim() != 1 or t.get_device() != self._index or not t.is_contiguous():
             _ints(t, name, 1, self.device)
-        if n >= 0 and t.shape[0] != n:
-            raise ValueError(f"{name} has {t.shape[0]} entries, expected {n}")
+        if n >= 0 and t.numel() != n:
+            raise ValueError(f"{name} has {t.numel()} entries, expected {n}")
         return t.data_ptr()
 
     def free(self, seqs: torch.Tensor) -> None:
         """The slots ``seqs`` give their pages back and are empty then.  Empty slots and repeated ones do no harm."""
-        self._call("fa4b_kv_free", self._list(seqs, "seqs"), seqs.shape[0])
+        self._call("fa4b_kv_free", self._list(seqs, "seqs"), seqs.numel())
 
     def extend(self, seqs: torch.Tensor, n_new: torch.Tensor) -> None:
         """Slot ``seqs[i]`` grows by ``n_new[i]`` tokens (:meth:`write` fills them) and claims pages for them: the lowest
         free ones, in the order of the list.  All or nothing; :meth:`check_status` tells."""
-        a, n = self._list(seqs, "seqs"), seqs.shape[0]
+        a, n = self._list(seqs, "seqs"), seqs.numel()
         self._call("fa4b_kv_extend", a, self._list(n_new, "n_new", n), n)
 
     def write(self, k: torch.Tensor, v: torch.Tensor, seqs: torch.Tensor, *, n_new: torch.Tensor | None = None, layer: int = 0) -> None:
         """Keys and values ``[n, Hkv, T, D]`` (any batch / head / token strides) of the newest tokens: token ``t < n_new[i]``
         goes to position ``seq_lens[seqs[i]] - n_new[i] + t`` (``n_new`` None: T for every row).  A 16-bit cache takes its
-        own type, an E4M3 cache bf16 or f16, divided by the scale, clamped to +-448 and rounded."""
-        a, n = self._list(seqs, "seqs"), seqs.shape[0]
+        own type, an E4M3 cache bf16 or f16, divided by the scale, clamped to +-448 and rounded.  Tokens from before a
+        :meth:`fork` lie in pages that the samples share: write those before it.  A slot named twice gets either row's values."""
+        a, n = self._list(seqs, "seqs"), seqs.numel()
         b = 0 if n_new is None else self._list(n_new, "n_new", n)
+        if type(k) is not torch.Tensor or type(v) is not torch.Tensor:
+            self._check_new(k, v, n)
+        dtype, index, (k_shape, k_strides), (v_shape, v_strides) = k.dtype, self._index, (k.shape, k.stride()), (v.shape, v.stride())
+        if (len(k_shape) != 4 or k_shape != v_shape or k_shape[0] != n or k_shape[1] != self._heads or k_shape[3] != self._d or dtype is not v.dtype or
+                dtype not in self._takes or k.get_device() != index or v.get_device() != index or k_strides[3] != 1 or v_strides[3] != 1):
+            self._check_new(k, v, n)
+        args = _WRITE.pack(k.data_ptr(), v.data_ptr(), *_strides(k_shape, k_strides), *_strides(v_shape, v_strides), k_shape[2], KV_DTYPES[dtype], layer, n, a, b)
+        self._call("fa4b_kv_write", args)
+
+    def _check_new(self, k, v, n: int) -> None:
         for t, name in ((k, "k"), (v, "v")):
             if not isinstance(t, torch.Tensor) or t.dim() != 4 or t.shape[0] != n or t.shape[1] != self._heads or t.shape[3] != self._d:
                 raise ValueError(f"{name} must be a [{n}, {self._heads}, T, {self._d}] tensor")
@@ -152,19 +164,17 @@ class PagedKVCache:
                 raise ValueError(f"{name} must have a contiguous head dimension")
         if k.shape != v.shape or k.dtype != v.dtype:
             raise ValueError("k and v must be alike")
-        args = _WRITE.pack(k.data_ptr(), v.data_ptr(), *_strides(k), *_strides(v), k.shape[2], KV_DTYPES[k.dtype], layer, n, a, b)
-        self._call("fa4b_kv_write", args)
 
     def fork(self, parents: torch.Tensor, children: torch.Tensor) -> None:
         """Slot ``children[i]``, which is empty, becomes a copy of ``parents[i]``: full pages are shared, the page that is
         still being filled is copied.  All or nothing; :meth:`check_status` tells."""
-        a, n = self._list(parents, "parents"), parents.shape[0]
+        a, n = self._list(parents, "parents"), parents.numel()
         self._call("fa4b_kv_fork", a, self._list(children, "children", n), n)
 
     def copy_pages(self, src: torch.Tensor, dst: torch.Tensor) -> None:
         """Pages ``src[i]`` to pages ``dst[i]`` in every layer; tables and counts stay.  A pair with a negative entry is
         skipped, and one whose pages another pair writes, or whose destination another reads, is left out and reported."""
-        a, n = self._list(src, "src"), src.shape[0]
+        a, n = self._list(src, "src"), src.numel()
         self._call("fa4b_kv_copy_pages", a, self._list(dst, "dst", n), n)
 
     def compact(self) -> None:
@@ -181,44 +191,47 @@ class PagedKVCache:
 
         ``group_offsets [groups + 1]``, ``shared_lens [groups]``: rows ``group_offsets[g]`` up to ``group_offsets[g + 1]`` hold
         the same pages for their first ``shared_lens[g]`` tokens (as :meth:`fork` leaves them), which are read once for
-        the group; rows in no group are left as they were.  ``out`` receives O when given (any strides)."""
-        if not isinstance(q, torch.Tensor) or q.dim() != 4 or q.shape[3] != self._d:
+        the group; rows in no group are left as they were.  ``out`` receives O when given (any strides but 0).  There is no
+        gradient."""
+        if not isinstance(q, torch.Tensor) or len(shape := q.shape) != 4 or shape[3] != self._d:
             raise ValueError(f"q must be a [n, Hq, T, {self._d}] tensor")
-        if q.dtype not in self._takes:
-            raise TypeError(f"q is {q.dtype}, the cache {self.k.dtype}")
+        dtype, strides = q.dtype, q.stride()
+        if dtype not in self._takes:
+            raise TypeError(f"q is {dtype}, the cache {self.k.dtype}")
         if q.get_device() != self._index:
             raise RuntimeError(f"q must live on {self.device}, got {q.device}")
-        shape = q.shape
-        n, hq, t, _ = shape
-        if q.stride(3) != 1:
+        n, hq, t, d = shape
+        if strides[3] != 1:
             raise ValueError("q must have a contiguous head dimension")
         if (group_offsets is None) != (shared_lens is None):
             raise ValueError("group_offsets and shared_lens go together")
         slots = 0 if seqs is None else self._list(seqs, "seqs", n)
         groups = offsets = shared = 0
         if group_offsets is not None:
-            shared, groups = self._list(shared_lens, "shared_lens"), shared_lens.shape[0]
-            if group_offsets.shape[0] != groups + 1:
-                raise ValueError(f"group_offsets must have {groups + 1} entries, got {group_offsets.shape[0]}")
+            shared, groups = self._list(shared_lens, "shared_lens"), shared_lens.numel()
+            if group_offsets.numel() != groups + 1:
+                raise ValueError(f"group_offsets must have {groups + 1} entries, got {group_offsets.numel()}")
             if groups == 0 and n > 0:
                 raise ValueError("no groups: without group_offsets and shared_lens every row stands by itself")
             offsets = self._list(group_offsets, "group_offsets")
         if out is None:
-            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+            out, o_strides = q.new_empty(shape), (hq * t * d, t * d, d)
         elif out.shape != shape or out.dtype != q.dtype or out.device != self.device or out.stride(3) != 1:
             raise ValueError(f"out must be a {tuple(shape)} tensor like q with a contiguous head dimension")
-        lse = q.new_empty((n, hq, t), dtype=torch.float32)
-        code, scale = KV_DTYPES[q.dtype], softmax_scale or 0.0
+        else:
+            o_strides = _strides(shape, out.stride())
+        lse = self._floats.new_empty((n, hq, t))
+        code, scale = KV_DTYPES[dtype], softmax_scale or 0.0
         if not scale >= 0.0:
             raise ValueError(f"softmax_scale must be positive, got {softmax_scale}")
-        q_strides, o_strides = _strides(q), _strides(out)
+        q_strides = _strides(shape, strides)
         size = self._ws_bytes.get((n, hq, t, groups))
         if size is None:
             args = _ATTEND.pack(q.data_ptr(), *q_strides, out.data_ptr(), *o_strides, lse.data_ptr(), n, t, hq, layer, code, scale, slots, groups, offsets, shared, 0)
             size = self._lib.fa4b_attn_paged_workspace_bytes(self._at, args)
             if size:
                 self._ws_bytes[n, hq, t, groups] = size
-        ws = self._work.new_empty(size >> 2)  # of this call alone: calls on two streams, or of two captured graphs, may overlap
+        ws = self._floats.new_empty(size >> 2)  # of this call alone: calls on two streams, or of two captured graphs, may overlap
         args = _ATTEND.pack(q.data_ptr(), *q_strides, out.data_ptr(), *o_strides, lse.data_ptr(), n, t, hq, layer, code, scale, slots, groups, offsets, shared,
                             ws.data_ptr())
         self._call("fa4b_attn_paged_fwd", args)
@@ -230,7 +243,7 @@ class PagedKVCache:
         self._call("fa4b_kv_check_status")
 
 
-def _strides(t: torch.Tensor) -> tuple:
-    a, b, c, _ = t.shape
-    x, y, z, _ = t.stride()
+def _strides(shape, strides) -> tuple:
+    a, b, c, _ = shape
+    x, y, z, _ = strides
     return x if a > 1 else 0, y if b > 1 else 0, z if c > 1 else 0  # a dimension of one entry carries no stride of its own
