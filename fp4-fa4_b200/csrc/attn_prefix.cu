@@ -11,8 +11,9 @@
 // halves.  An E4M3 cache arrives as codes; warps 11-14 turn each tile into f16 (exact) in the operand ring.
 //
 // 2048 rows (128 sequences of 4 tokens and 4 query heads) over 32768 keys and 8 kv heads, D 128, bf16: 255 us (275 GFLOP: 0.66 of
-// the rate measured for a library's product of large matrices; one buffer 281 us, one issuing warp 482).  The tensor core bounds it: a
-// product of 64 keys takes it about 85 cycles, as long as one of 128, so a step of 64 keys costs more than its share; scores of 128
+// the rate measured for a library's product of large matrices; one buffer 281 us, one issuing warp 482).  The products bound it: one of
+// 64 keys takes about 85 cycles, as long as one of 128, because the query operand comes from shared memory for each (TMEM is full),
+// so a step of both halves, 16 products of scores and 8 of values, is 1900 of the 2130 cycles that it takes.  Scores of 128
 // keys at once would leave no second buffer and were slower (382 against 333 us for the call).  With 128 rows and 8k keys it is 13.5
 // us: 7 of them are the beginning (plan, query rows, first pages) and the end (the sums out of TMEM).
 //

@@ -528,7 +528,8 @@ int fa4b_kv_extend(const fa4b_kv_cache* c, const int32_t* seqs, const int32_t* n
 /* fa4b_kv_write: token t < n_new[i] of row i goes to position seq_lens[seqs[i]] - n_new[i] + t (n_new NULL: T for every
  * row).  k_new, v_new: [n, Hkv, T, D] bf16 or f16, batch / head / token strides in elements (multiples of 8), pointers
  * 16-byte aligned.  A 16-bit cache takes values of its own type; an E4M3 cache stores RN(clamp(x / scale, +-448)),
- * NaN kept.  Positions below 0 and rows whose slot is out of range are left out. */
+ * NaN kept.  Positions below 0 and rows whose slot is out of range are left out.  Tokens from before a fork lie in pages that
+ * the samples share (write those before it); a slot named twice gets either row's values. */
 typedef struct fa4b_kv_write_args {
   const void* k_new;
   const void* v_new;
@@ -566,7 +567,7 @@ int fa4b_kv_compact(const fa4b_kv_cache* c, void* stream);
  * rise from 0 or more to n or less; rows in no group are left as they were.  groups == 0: every row by itself. */
 typedef struct fa4b_attn_paged_args {
   const void* q; fa4b_strides q_strides;  /* [n, Hq, T, D] bf16 or f16 (16-bit caches: the cache's type); any strides, multiples of 8 */
-  void* o; fa4b_strides o_strides;        /* [n, Hq, T, D], q's type */
+  void* o; fa4b_strides o_strides;        /* [n, Hq, T, D], q's type; no stride of 0 over more than one row */
   float* lse;                             /* [n, Hq, T] dense */
   int32_t n, T, Hq, layer;                /* n <= 4096, T <= 16 */
   int32_t q_dtype;                        /* FA4B_KV_BF16 or FA4B_KV_F16 */
