@@ -1,10 +1,10 @@
 // Attention of the newest tokens of a batch over a paged cache (single tokens, or a few drafted ones), with the keys that
 // a group of sequences shares read once for all of them.
 //
-// A call is a chain of launches, each of which comes up while the one before still runs: plan (who reads what), prefix units
+// A call is a chain of launches, each of which comes up while the one before still runs: plan (who reads what; not for few rows), prefix units
 // (only with groups: attn_prefix.cu), own units, join.  For 32 sequences of 600 keys behind 8219 shared ones (32 query and 8 kv heads,
 // D 128, bf16) that is 32 us: plan 5, prefix 13.5, own 9 beside and behind it, join 3-5, against 11 us for the bytes; what is left is
-// the latency of the chain.  One sequence of 1000 keys takes 10 us in a graph.
+// the latency of the chain.  One sequence of 1000 keys takes 8.7 us in a graph.
 //
 // Own units are bound by memory: a key and a value are used by the few query rows of one sequence, so the kernel is a
 // stream of pages through shared memory, with tiles asked for by TMA several tiles ahead: 32 sequences of up to 8k keys, 537
@@ -221,6 +221,36 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PagedPar
     p.g_cum[g] = g_cum[g];
     r[1] = make_int4(g_cum[g], g_unit[g], (rows + p.prefix_rows - 1) >> p.prefix_shift, 0);
   }
+}
+
+// The plan of a call of up to 32 rows without groups, a row to a lane: two rounds of loads and two sums, which a warp that needs it
+// works out sooner than a launch before it does (8 rows of up to 1000 bf16 keys 11.9 against 13.1 us with all launches in a graph, of 8192
+// keys 18.6 against 20.3; 32 rows the same either way: the join's many warps then do it over and over).  `cum`: 32 words of shared memory of this warp's.
+constexpr int kSmallRows = 32;
+struct PagedSmall {
+  int slot, len, cum, left_alone;  // of row `lane`
+  PagedLine line;
+};
+__device__ __forceinline__ PagedSmall paged_small(const PagedParams& p, int* cum) {
+  const int lane = threadIdx.x & 31;
+  PagedSmall s;
+  s.slot = lane < p.n ? (p.seqs ? p.seqs[lane] : lane) : -1;
+  s.len = (uint32_t)s.slot < (uint32_t)p.c.max_seqs ? min(max(p.c.lens[s.slot], 0), p.c.width << p.c.page_shift) : 0;
+  const int tiles = own_tiles(p, 0, s.len);
+  cum[lane] = tiles;
+  __syncwarp();
+  const PagedCut cut = warp_cut(cum, nullptr, p.n, p.own_units, p.own_workers, p.own_extra, p.own_min);
+  __syncwarp();
+  cum[lane] = (int)cut.length(tiles);
+  __syncwarp();
+  const int total = warp_scan(cum, p.n);
+  __syncwarp();
+  s.cum = cum[lane];
+  const bool fits = (uint64_t)total * p.own_units < INT_MAX;  // positions are counted in 32 bits
+  s.line = {fits ? (uint32_t)total * p.own_units : 0u, cut};
+  s.left_alone = !fits;
+  if (!fits && blockIdx.x == 0 && lane == 0 && atomicCAS(p.status, 0u, 3u) == 0u) p.status[1] = (uint32_t)total;
+  return s;
 }
 
 // ---- the units over keys of one sequence ------------------------------------------------------------------------------
@@ -726,9 +756,13 @@ struct SoloSmem {
   static constexpr int kCtas = kRows == 8 ? 3 : 2;                   // per SM: what the registers of a row's state allow
   static constexpr int kStages = 48 * 1024 / kCtas / (2 * kTileBytes);  // 192 KB in flight per SM
   alignas(1024) uint8_t ring[4][kStages][2][kTileBytes];
+  PagedSeq seq[kSmallRows];  // the plan of a small call
+  int cum[kSmallRows];
+  PagedLine line;
   uint64_t full[4][kStages];
   volatile uint32_t abort_flag;
-  static constexpr int kUsed = 4 * kStages * (2 * kTileBytes + 8) + 16;  // the struct without what its alignment adds
+  // the struct without what its alignment adds
+  static constexpr int kUsed = 4 * kStages * (2 * kTileBytes + 8) + kSmallRows * ((int)sizeof(PagedSeq) + 4) + (int)sizeof(PagedLine) + 16;
 };
 
 template <int D, bool kE4M3, typename QT, int kRows>
@@ -757,8 +791,16 @@ __global__ void __launch_bounds__(128, kRows == 8 ? 3 : 2) attn_solo_kernel(cons
     if (threadIdx.x == 0) p.status[1] = 99u, p.status[0] = 1u;
     return;
   }
+  if (p.small) {
+    if (warp == 0) {
+      const PagedSmall x = paged_small(p, s.cum);
+      *reinterpret_cast<int4*>(s.seq + lane) = make_int4(x.slot, x.len, 0, x.cum);
+      if (lane == 0) s.line = x.line;
+    }
+    __syncthreads();
+  }
   PagedWalk<false> ahead, walk;  // of the copies, and of the products
-  ahead.start(p, worker);
+  ahead.start(p, worker, p.small ? PagedTables{&s.line, s.seq, s.cum} : PagedTables{&p.head->own, p.seq, p.own_cum});
   walk = ahead;
   if (walk.done()) return;
 
@@ -879,7 +921,7 @@ __global__ void __launch_bounds__(160, 2) attn_team_kernel(const PagedParams p, 
     return;
   }
   PagedWalk<false> walk;
-  walk.start(p, blockIdx.x);
+  walk.start(p, blockIdx.x, {&p.head->own, p.seq, p.own_cum});
 
   if (warp == 4) {  // ---- producer: lane b of a tile's boxes asks for its own part of the pages
     const PagedBoxes box{min(p.c.page_tokens, kTile), kTile / min(p.c.page_tokens, kTile)};
@@ -985,8 +1027,18 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PagedParams p) {
   const bool there = w < (uint32_t)(p.n * p.Hq * p.T);
   const uint32_t row_id = there ? w : 0u;
   const uint32_t t = p.T == 1 ? 0u : row_id % (uint32_t)p.T, ih = p.T == 1 ? row_id : row_id / (uint32_t)p.T, i = ih / (uint32_t)p.Hq, h = ih - i * (uint32_t)p.Hq;
-  const PagedSeq s = p.seq[i];
-  const PagedHead line = *p.head;
+  PagedSeq s;
+  PagedHead line;
+  if (p.small) {
+    __shared__ int cum[4][kSmallRows];
+    const PagedSmall x = paged_small(p, cum[warp]);
+    s.len = __shfl_sync(0xffffffffu, x.len, i), s.cum = __shfl_sync(0xffffffffu, x.cum, i);
+    s.first = 0, s.left_alone = x.left_alone;
+    line.own = x.line;
+  } else {
+    s = p.seq[i];
+    line = *p.head;
+  }
   const int head = h / (uint32_t)p.G, r = t * p.G + (h - head * p.G), len = s.len;
   float acc[kPer], m = -INFINITY, l = 0.f;
 #pragma unroll
@@ -1101,7 +1153,7 @@ static int launch_paged(const PagedParams& p, const PagedMaps& m, cudaStream_t s
   static std::atomic<uint64_t> allowed[5];
   if (smem > 48 * 1024)
     if (int s = allow_smem(paged_plan_kernel, 4 * (int)paged_plan_words(kPagedMaxRows, kPagedMaxRows), allowed[3])) return s;
-  FA4B_CUDA(launch_overlapped(paged_plan_kernel, 1, kPlanThreads, smem, st, p));
+  if (!p.small) FA4B_CUDA(launch_overlapped(paged_plan_kernel, 1, kPlanThreads, smem, st, p));
   if (p.groups > 0)
     if (int s = launch_prefix(p, D, kE4M3, std::is_same<QT, TagF16>::value, m.prefix_k, m.prefix_v, st)) return s;
   // which of these a type takes: see paged_params
@@ -1174,6 +1226,7 @@ static int paged_params(const fa4b_kv_cache* c, const fa4b_attn_paged_args* a, P
   // tensor core's 64-key products either way and better off without the join of the halves (83 against 87 us; 207 against 215).
   p.prefix_rows = p.groups > 0 && ((int64_t)p.n * p.R > 128ll * p.groups || paged_prefix_wide(c->D, c->dtype == FA4B_KV_E4M3)) ? 256 : 128;
   p.prefix_shift = __builtin_ctz((unsigned)p.prefix_rows), p.prefix_workers = n_sm, p.prefix_extra = 3;
+  p.small = p.groups == 0 && p.n <= kSmallRows && solo;
   const int64_t keys = (int64_t)c->table_width * c->page_tokens, own_length = 2 * (keys / p.own_tile) + 2 + p.own_extra;
   const int64_t prefix_units = p.groups ? (int64_t)c->Hkv * (((int64_t)p.n * p.R + p.prefix_rows - 1) / p.prefix_rows + p.groups) : 0;
   const int64_t own_slots = (int64_t)p.n * c->Hkv * p.own_blocks + p.own_workers, prefix_slots = p.groups ? prefix_units + p.prefix_workers : 0;

@@ -64,6 +64,7 @@ struct PagedParams {
   float scale_log2;
   const float* k_scale;  // this layer's [Hkv], or NULL
   const float* v_scale;
+  int small;             // 1: few rows and no groups, no plan is written down: who needs it works it out
   PagedHead* head;       // the plan
   PagedSeq* seq;         // [n]
   PagedGroup* group;     // [groups]
@@ -169,15 +170,23 @@ struct PagedUnit {
   int tile, tile_end;     // tiles (counted from key 0) that this worker takes; none, when its piece only has the unit's beginning
 };
 
+// Where the own units' part of the plan lies.
+struct PagedTables {
+  const PagedLine* line;
+  const PagedSeq* seq;
+  const int* cum;
+};
+
 template <bool kPrefix>
 struct PagedWalk {
+  const PagedSeq* seq;  // own units
   int left;             // positions of the line to go
   int item, which, off;
   PagedCut cut;
   int a0, a1, a2, a3, b1, b2;  // the item's record
 
   __device__ __forceinline__ void load(const PagedParams& p) {
-    const int4* r = kPrefix ? reinterpret_cast<const int4*>(p.group + item) : reinterpret_cast<const int4*>(p.seq + item);
+    const int4* r = kPrefix ? reinterpret_cast<const int4*>(p.group + item) : reinterpret_cast<const int4*>(seq + item);
     const int4 a = r[0];
     a0 = a.x, a1 = a.y, a2 = a.z, a3 = a.w;
     if constexpr (kPrefix) {
@@ -185,12 +194,13 @@ struct PagedWalk {
       b1 = b.y, b2 = b.z;
     }
   }
-  __device__ __forceinline__ void start(const PagedParams& p, int worker) {  // whole warps
-    const int* cum = kPrefix ? p.g_cum : p.own_cum;
+  __device__ __forceinline__ void start(const PagedParams& p, int worker, PagedTables t) {  // whole warps
+    seq = t.seq;
+    const int* cum = t.cum;
     const int n = kPrefix ? p.groups : p.n, lane = threadIdx.x & 31;
     // the first round does not wait for the head of the plan: 32 places at equal distances
     int step = (n + 31) >> 5, first = lane * step < n ? cum[lane * step] : INT_MAX;
-    const int4 h = *reinterpret_cast<const int4*>(kPrefix ? &p.head->prefix : &p.head->own);
+    const int4 h = *reinterpret_cast<const int4*>(t.line);
     const uint32_t total = h.x;
     cut = {(uint32_t)h.y, (uint32_t)h.z, (uint32_t)h.w};
     const uint64_t from = (uint64_t)worker * cut.per;

@@ -204,7 +204,7 @@ __global__ void __launch_bounds__(prefix_threads(kE4M3), 1) attn_prefix_kernel(c
   pdl_wait();
   pdl_trigger();
   PagedWalk<true> walk;
-  walk.start(p, blockIdx.x);
+  walk.start(p, blockIdx.x, {&p.head->prefix, nullptr, p.g_cum});
   if (!aligned) walk.left = 0;
   if (!aligned && threadIdx.x == 0) p.status[1] = 98u, p.status[0] = 1u;
 

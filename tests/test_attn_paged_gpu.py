@@ -603,3 +603,24 @@ def test_an_empty_list_of_groups_is_refused():
         c.attend(queries(2, 4, 1, 64, BF, 0), ints(slots), group_offsets=ints([0]), shared_lens=ints([]))
     out, lse = c.attend(queries(0, 4, 1, 64, BF, 0), ints([]), group_offsets=ints([0]), shared_lens=ints([]))
     assert out.shape == (0, 4, 1, 64) and lse.shape == (0, 4, 1)
+
+
+@pytest.mark.parametrize("d,page,dtype", [(128, 16, BF), (64, 128, E4)])
+@pytest.mark.parametrize("n,t", [(1, 1), (2, 4), (31, 1), (32, 2), (32, 4), (33, 2), (64, 1)])
+def test_rows_without_groups_around_the_size_that_needs_no_plan(n, t, d, page, dtype):
+    """One row, several, and both sides of 32 rows; lengths of zero, one and many, padding in the middle, a long row beside short ones."""
+    rng = random.Random(n * 10 + t)
+    lens = [rng.choice([0, 1, t, 15, 16, 17, 130, 700]) for _ in range(n)]
+    lens[n // 2] = 5000
+    c, slots, _ = build(lens, [], [], hkv=2, d=d, page=page, dtype=dtype, seed=n)
+    named = list(slots)
+    if n > 2:
+        named[1], named[n - 1] = -1, 10 ** 9
+        named[0] = named[n // 2]  # the same sequence twice
+    q = queries(n, 8, t, d, BF, n)
+    out, lse = c.attend(q, ints(named))
+    c.check_status()
+    compare(c, q, out, lse, named)
+    for _ in range(3):  # cold or warm, early or late: the same bits
+        again, lse2 = c.attend(q, ints(named))
+        assert torch.equal(again, out) and torch.equal(lse2, lse)
