@@ -1012,15 +1012,18 @@ __global__ void __launch_bounds__(160, 2) attn_team_kernel(const PagedParams p, 
 }
 
 // ---- join -------------------------------------------------------------------------------------------------------------
-// One warp per output row, or (kSplit) four, each with a quarter of the pieces, where the rows are few.  The pieces' statistics
-// come to the lanes at once, so that what is left to wait for is one round of loads: a lane holds D / 32 neighbours of eight
-// pieces at a time (one piece behind another took 26 us where this takes 12, and 3 to 5 with four warps).  Latency bounds it, and for
-// many rows the memory (16384 rows of 5 to 7 pieces: 18 us).  Which pieces there are follows from the plan, which is complete when this launch comes up (the own units
-// trigger behind it), so it is looked up before the wait.
+// One warp per output row, or (kSplit) four, each with a quarter of the pieces and sums of its own, where the rows are few (one
+// sequence of 8k keys has 128 pieces a row: 16.2 us for the call against 17.9 when the four went through them together, 32
+// at a time).  The statistics of 32 pieces come to the lanes at once, so that what is left to wait for is one round of loads: a
+// lane holds D / 32 neighbours of eight pieces at a time (one piece behind another took 26 us where this takes 12, and 3 to 5 with
+// four warps).  Latency bounds it, and for many rows the memory (16384 rows of 5 to 7 pieces: 18 us).  Which pieces there are
+// follows from the plan, which is complete when this launch comes up (the own units trigger behind it), or from the lengths,
+// so it is looked up before the wait.
 template <int D, typename QT, bool kSplit>
 __global__ void __launch_bounds__(128) paged_join_kernel(const PagedParams p) {
   constexpr int kPer = D / 32;
   __shared__ float parts[kSplit ? 3 : 1][D];
+  __shared__ float2 part_ml[4];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = kSplit ? warp : 0;
   const uint32_t w = kSplit ? blockIdx.x : blockIdx.x * 4 + warp;
   pdl_trigger();
@@ -1066,12 +1069,13 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PagedParams p) {
   }
   pdl_wait();
   if (!there || s.left_alone) return;  // or behind the last group; the same for all warps of a row
-  for (int base = 0; base < n_prefix + n_own; base += 32) {
+  const int total = n_prefix + n_own, each = kSplit ? (total + 3) / 4 : total, end = min(total, (part + 1) * each);
+  for (int base = part * each; base < end; base += 32) {
     const int k = base + lane;
     const bool is_prefix = k < n_prefix;
     const int64_t row = is_prefix ? (prefix_slot + (k >> two)) * p.prefix_rows + (k & two) * 64 + prefix_row : (own_slot + (k - n_prefix)) * p.own_rows + own_row;
     float2 x = make_float2(-INFINITY, 0.f);
-    if (k < n_prefix + n_own) x = is_prefix ? p.prefix_ml[row] : p.own_ml[row];
+    if (k < end) x = is_prefix ? p.prefix_ml[row] : p.own_ml[row];
     float top = x.x;
 #pragma unroll
     for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -1084,8 +1088,8 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PagedParams p) {
 #pragma unroll
     for (int e = 0; e < kPer; ++e) acc[e] *= f;
     const float* at = (is_prefix ? p.prefix_acc : p.own_acc) + row * D;
-    const int count = min(32, n_prefix + n_own - base), each = kSplit ? (count + 3) / 4 : count, end = min(count, (part + 1) * each);
-    for (int k0 = part * each; k0 < end; k0 += 8) {
+    const int count = min(32, end - base);
+    for (int k0 = 0; k0 < count; k0 += 8) {
       float v[8][kPer], weight[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
@@ -1093,7 +1097,7 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PagedParams p) {
         const float* from_row = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, (unsigned long long)at, (k0 + j) & 31));
 #pragma unroll
         for (int e = 0; e < kPer; ++e) v[j][e] = 0.f;
-        if (k0 + j < end) {
+        if (k0 + j < count) {
           if constexpr (kPer == 4) {
             const float4 q = __ldcg(reinterpret_cast<const float4*>(from_row) + lane);
             v[j][0] = q.x, v[j][1] = q.y, v[j][2] = q.z, v[j][3] = q.w;
@@ -1116,10 +1120,21 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PagedParams p) {
 #pragma unroll
       for (int e = 0; e < kPer; ++e) parts[warp - 1][lane * kPer + e] = acc[e];
     }
+    if (lane == 0) part_ml[warp] = make_float2(m, l);
     __syncthreads();
     if (warp > 0) return;
+    const float top = fmaxf(fmaxf(m, part_ml[1].x), fmaxf(part_ml[2].x, part_ml[3].x)), f = m == -INFINITY ? 0.f : paged_ex2(m - top);
+    m = top, l *= f;
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) acc[e] += (parts[0][lane * kPer + e] + parts[1][lane * kPer + e]) + parts[2][lane * kPer + e];
+    for (int e = 0; e < kPer; ++e) acc[e] *= f;
+#pragma unroll
+    for (int w = 1; w < 4; ++w) {
+      const float2 x = part_ml[w];
+      const float g = x.x == -INFINITY ? 0.f : paged_ex2(x.x - top);
+      l = fmaf(x.y, g, l);
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) acc[e] = fmaf(parts[w - 1][lane * kPer + e], g, acc[e]);
+    }
   }
   const float inv = l == 0.f ? 0.f : (p.v_scale ? p.v_scale[head] : 1.f) / l;  // a row that sees nothing: zeros, -inf
   uint8_t* out = p.o + 2 * ((int64_t)i * p.o_sb + (int64_t)h * p.o_sh + (int64_t)t * p.o_st + lane * kPer);
