@@ -223,9 +223,8 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PagedPar
   }
 }
 
-// The plan of a call of up to 32 rows without groups, a row to a lane: two rounds of loads and two sums, which a warp that needs it
-// works out sooner than a launch before it does (8 rows of up to 1000 bf16 keys 11.9 against 13.1 us with all launches in a graph, of 8192
-// keys 18.6 against 20.3; 32 rows the same either way: the join's many warps then do it over and over).  `cum`: 32 words of shared memory of this warp's.
+// The plan of a call of up to 32 rows without groups, a row to a lane: two rounds of loads and two sums, which a CTA of the own units
+// works out sooner than a launch before it does; the first of them writes it down for the join.  `cum`: 32 words of shared memory of this warp's.
 constexpr int kSmallRows = 32;
 struct PagedSmall {
   int slot, len, cum, left_alone;  // of row `lane`
@@ -731,20 +730,6 @@ struct PagedBoxes {
   }
 };
 
-// How a launch of own units stands to the ones before it.  Behind a plan it waits for it.  Behind prefix units it comes up
-// once all of those have seen the plan end (they trigger behind their own wait) and needs nothing of what they compute: it
-// runs beside them, and waits for them when it is done, so that the join, which waits for this launch, finds both.
-struct OwnOrder {
-  const bool beside;
-  __device__ __forceinline__ explicit OwnOrder(const PagedParams& p) : beside(p.groups > 0) {
-    if (!beside) pdl_wait();
-    pdl_trigger();
-  }
-  __device__ __forceinline__ ~OwnOrder() {
-    if (beside) pdl_wait();
-  }
-};
-
 // Up to sixteen query rows per unit (a single token, or a few drafted ones, of a group of query heads): every warp is a worker
 // with a line piece, a ring of tiles and copies of its own, and nothing in the loop waits for another warp (four warps that shared
 // their tiles, as in the team below, took 25 us where this takes 12.4 and the memory 5).
@@ -786,18 +771,26 @@ __global__ void __launch_bounds__(128, kRows == 8 ? 3 : 2) attn_solo_kernel(cons
     tma_prefetch_desc(&map_v);
   }
   __syncthreads();
-  OwnOrder order(p);
-  if (!aligned) {
-    if (threadIdx.x == 0) p.status[1] = 99u, p.status[0] = 1u;
-    return;
-  }
+  pdl_wait();
+  pdl_trigger();
   if (p.small) {
     if (warp == 0) {
       const PagedSmall x = paged_small(p, s.cum);
       *reinterpret_cast<int4*>(s.seq + lane) = make_int4(x.slot, x.len, 0, x.cum);
       if (lane == 0) s.line = x.line;
+      if (blockIdx.x == 0) {  // for the join
+        if (lane < p.n) {
+          int4* r = reinterpret_cast<int4*>(p.seq + lane);
+          r[0] = make_int4(x.slot, x.len, 0, x.cum), r[2] = make_int4(x.left_alone, 0, 0, 0);
+        }
+        if (lane == 0) p.head->own = x.line;
+      }
     }
     __syncthreads();
+  }
+  if (!aligned) {
+    if (threadIdx.x == 0) p.status[1] = 99u, p.status[0] = 1u;
+    return;
   }
   PagedWalk<false> ahead, walk;  // of the copies, and of the products
   ahead.start(p, worker, p.small ? PagedTables{&s.line, s.seq, s.cum} : PagedTables{&p.head->own, p.seq, p.own_cum});
@@ -915,7 +908,8 @@ __global__ void __launch_bounds__(160, 2) attn_team_kernel(const PagedParams p, 
     tma_prefetch_desc(&map_v);
   }
   __syncthreads();
-  OwnOrder order(p);
+  pdl_wait();
+  pdl_trigger();
   if (!aligned) {
     if (threadIdx.x == 0) p.status[1] = 99u, p.status[0] = 1u;
     return;
@@ -1017,8 +1011,8 @@ __global__ void __launch_bounds__(160, 2) attn_team_kernel(const PagedParams p, 
 // at a time).  The statistics of 32 pieces come to the lanes at once, so that what is left to wait for is one round of loads: a
 // lane holds D / 32 neighbours of eight pieces at a time (one piece behind another took 26 us where this takes 12, and 3 to 5 with
 // four warps).  Latency bounds it, and for many rows the memory (16384 rows of 5 to 7 pieces: 18 us).  Which pieces there are
-// follows from the plan, which is complete when this launch comes up (the own units trigger behind it), or from the lengths,
-// so it is looked up before the wait.
+// follows from the plan, which is read behind this launch's own wait: the plan has ended when the launch comes up, but only the wait
+// makes what earlier launches wrote visible.
 template <int D, typename QT, bool kSplit>
 __global__ void __launch_bounds__(128) paged_join_kernel(const PagedParams p) {
   constexpr int kPer = D / 32;
@@ -1030,18 +1024,9 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PagedParams p) {
   const bool there = w < (uint32_t)(p.n * p.Hq * p.T);
   const uint32_t row_id = there ? w : 0u;
   const uint32_t t = p.T == 1 ? 0u : row_id % (uint32_t)p.T, ih = p.T == 1 ? row_id : row_id / (uint32_t)p.T, i = ih / (uint32_t)p.Hq, h = ih - i * (uint32_t)p.Hq;
-  PagedSeq s;
-  PagedHead line;
-  if (p.small) {
-    __shared__ int cum[4][kSmallRows];
-    const PagedSmall x = paged_small(p, cum[warp]);
-    s.len = __shfl_sync(0xffffffffu, x.len, i), s.cum = __shfl_sync(0xffffffffu, x.cum, i);
-    s.first = 0, s.left_alone = x.left_alone;
-    line.own = x.line;
-  } else {
-    s = p.seq[i];
-    line = *p.head;
-  }
+  pdl_wait();
+  const PagedSeq s = p.seq[i];
+  const PagedHead line = *p.head;
   const int head = h / (uint32_t)p.G, r = t * p.G + (h - head * p.G), len = s.len;
   float acc[kPer], m = -INFINITY, l = 0.f;
 #pragma unroll
@@ -1067,7 +1052,6 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PagedParams p) {
     n_own = (int)((from + tiles - 1) / cut.per - worker) + 1;
     own_row = r & (p.own_rows - 1);
   }
-  pdl_wait();
   if (!there || s.left_alone) return;  // or behind the last group; the same for all warps of a row
   const int total = n_prefix + n_own, each = kSplit ? (total + 3) / 4 : total, end = min(total, (part + 1) * each);
   for (int base = part * each; base < end; base += 32) {

@@ -64,7 +64,7 @@ struct PagedParams {
   float scale_log2;
   const float* k_scale;  // this layer's [Hkv], or NULL
   const float* v_scale;
-  int small;             // 1: few rows and no groups, no plan is written down: who needs it works it out
+  int small;             // 1: few rows and no groups, no launch for the plan: the own units work it out
   PagedHead* head;       // the plan
   PagedSeq* seq;         // [n]
   PagedGroup* group;     // [groups]

@@ -624,3 +624,31 @@ def test_rows_without_groups_around_the_size_that_needs_no_plan(n, t, d, page, d
     for _ in range(3):  # cold or warm, early or late: the same bits
         again, lse2 = c.attend(q, ints(named))
         assert torch.equal(again, out) and torch.equal(lse2, lse)
+
+
+def test_calls_that_differ_follow_one_another_without_a_pause():
+    """Lengths, tables, groups, tokens and the kind of call change from one to the next on one stream, in the same workspace memory: each
+    call sees its own plan, and not what one before it left."""
+    lens = [700, 690, 1500, 333, 1481, 64, 900, 910]
+    c, slots, _ = build(lens, [640, 320], [2, 2], hkv=2, d=128, seed=60)
+    table, seq = c.page_table.clone(), c.seq_lens.clone()
+    c.k.nan_to_num_(nan=0.25), c.v.nan_to_num_(nan=-0.5)
+    turned = table.clone()
+    turned[slots[6]], turned[slots[7]] = table[slots[7]], table[slots[6]]  # as many pages
+    states = [(table, seq), (turned, (seq - 130).clamp(min=0)), (table, (seq // 3)), (turned, (seq - 17).clamp(min=0))]
+    kinds = [dict(group_offsets=ints([0, 2, 4, 8]), shared_lens=ints([640, 320, 0])), {}, dict(group_offsets=ints([0, 2, 8]), shared_lens=ints([208, 0])),
+             dict(group_offsets=ints([0, 1, 2, 8]), shared_lens=ints([640, 640, 0]))]
+    qs = [queries(8, 8, t, 128, BF, 61 + t) for t in (1, 2, 4)]
+    rng = random.Random(6)
+    order = [(rng.randrange(4), rng.randrange(4), rng.randrange(3)) for _ in range(60)]
+    s, results = ints(slots), []
+    torch.cuda.synchronize()
+    for state, kind, which in order:
+        c.page_table.copy_(states[state][0]), c.seq_lens.copy_(states[state][1])
+        results.append(c.attend(qs[which], s, **kinds[kind]))
+        results[-1] += c.attend(qs[which], s, **kinds[kind - 1])
+    c.check_status()
+    for (state, kind, which), (out, lse, out2, lse2) in zip(order, results):
+        c.page_table.copy_(states[state][0]), c.seq_lens.copy_(states[state][1])
+        compare(c, qs[which], out, lse, slots)
+        compare(c, qs[which], out2, lse2, slots)

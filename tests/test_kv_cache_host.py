@@ -151,3 +151,31 @@ def test_packed_arguments_have_the_layout_of_the_structs():
             x = getattr(got, name)
             flat += [x.batch, x.head, x.seq] if kind is _lib.Strides else [x]
         assert tuple(flat) == values
+
+
+def _kernels(name):
+    """Every kernel of a source file: name, parameters, body."""
+    import pathlib
+    import re
+
+    text = (pathlib.Path(_lib.__file__).resolve().parents[1] / "csrc" / name).read_text()
+    text = re.sub(r"//[^\n]*", "", text)
+    for m in re.finditer(r"__global__ void (?:__launch_bounds__\([^\n]*?\) )?(\w+)\(([^{]*?)\) \{\n(.*?)\n\}\n", text, re.S):
+        yield m.groups()
+
+
+def test_kernels_that_come_up_early_wait_before_they_read():
+    """A launch that overlaps the one before sees what earlier launches wrote behind its own wait only, also what an even earlier one has
+    long written: nothing but the arguments is looked at before it."""
+    import re
+
+    memory = re.compile(r"\bp\.(seq|head|group|seqs|offsets|shared|q|k_scale|own_acc|own_ml|own_cum|g_cum|prefix_acc|prefix_ml)\b|\bc\.(lens|table|refs|work(?! \+)|k|v)\b|"
+                        r"\b(seqs|n_new|parents|children|src|dst)\[|paged_small|\.start\(|tma_load")
+    seen = set()
+    for name in ("kv_cache.cu", "attn_paged.cu", "attn_prefix.cu"):
+        for kernel, _, body in _kernels(name):
+            before, wait, _ = body.partition("pdl_wait();")
+            assert wait, kernel
+            assert not memory.search(before), (kernel, memory.search(before))
+            seen.add(kernel)
+    assert {"paged_plan_kernel", "attn_prefix_kernel", "attn_solo_kernel", "attn_team_kernel", "paged_join_kernel", "kv_extend_kernel", "kv_copy_kernel"} <= seen and len(seen) == 15, seen
