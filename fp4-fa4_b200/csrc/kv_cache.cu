@@ -107,7 +107,7 @@ __device__ int find_free(const KvView& c, int want, int32_t* out, int* warp_sums
 
 // ---- free -------------------------------------------------------------------------------------------------------------
 // One CTA per slot.  The exchange of the length decides who frees a slot that the list names twice.
-__global__ void __launch_bounds__(128) kv_free_kernel(const KvView c, const int32_t* __restrict__ seqs) {
+__global__ void __launch_bounds__(128) kv_free_kernel(const KvView c, const int32_t* seqs) {
   pdl_trigger();
   pdl_wait();
   __shared__ int held;
@@ -136,8 +136,8 @@ __device__ __forceinline__ int check_slot(const KvView& c, int slot, uint32_t* s
 
 // One CTA: what is claimed in one call is a few thousand pages at most, and the order of the claims is a prefix sum over
 // requests and one over free pages.  Latency bounds it (a few rounds of loads and two sums: 2 to 6 us).
-__global__ void __launch_bounds__(1024) kv_extend_kernel(const KvView c, const int32_t* __restrict__ seqs, const int32_t* __restrict__ n_new,
-                                                         int n, int32_t* __restrict__ fresh) {
+__global__ void __launch_bounds__(1024) kv_extend_kernel(const KvView c, const int32_t* seqs, const int32_t* n_new,
+                                                         int n, int32_t* fresh) {
   extern __shared__ int dyn[];
   __shared__ int warp_sums[32];
   int* first = dyn;                                          // [n + 1]: claims before request i
@@ -310,8 +310,8 @@ __global__ void __launch_bounds__(256, 3) kv_write_kernel(const KvView c, const 
 // ---- fork -------------------------------------------------------------------------------------------------------------
 // First launch, one CTA: checks the lists, claims the tail pages.  fresh[i]: child i's tail page, -1: none; head[0]: 1
 // when the second launch may go on.
-__global__ void __launch_bounds__(1024) kv_fork_plan_kernel(const KvView c, const int32_t* __restrict__ parents, const int32_t* __restrict__ children,
-                                                            int n, int32_t* __restrict__ list) {
+__global__ void __launch_bounds__(1024) kv_fork_plan_kernel(const KvView c, const int32_t* parents, const int32_t* children,
+                                                            int n, int32_t* list) {
   extern __shared__ uint32_t seen[];  // [max_seqs / 32]
   __shared__ int warp_sums[32];
   int32_t* fresh = c.work + kWorkFresh;
@@ -374,7 +374,7 @@ __global__ void __launch_bounds__(1024) kv_fork_plan_kernel(const KvView c, cons
 // Second launch.  CTAs 0..n-1: the child's row of the table and the counts of the pages it shares.  The others: one warp
 // per 4 KB of a tail page's rows of one kv head, K or V, one layer.  Bound by memory where it is large: 256 forks of 4 layers with
 // frees before them (70 MB) take 17.6 us in a graph, of which the copies take about 11; four forks take 7.9 us, three launches' latency.
-__global__ void __launch_bounds__(256) kv_fork_move_kernel(const KvView c, const int32_t* __restrict__ parents, const int32_t* __restrict__ children,
+__global__ void __launch_bounds__(256) kv_fork_move_kernel(const KvView c, const int32_t* parents, const int32_t* children,
                                                            int n, int pieces, int64_t units) {
   pdl_trigger();
   pdl_wait();
@@ -439,7 +439,7 @@ __device__ __forceinline__ void piece_store(const PieceRegs& x, uint8_t* to, int
 __device__ __forceinline__ bool collides(int i, int j, int s, int d, int sj, int dj) { return (j != i && dj == d) || sj == d || dj == s; }
 
 // one warp per pair
-__global__ void __launch_bounds__(256) kv_copy_check_kernel(const KvView c, const int32_t* __restrict__ src, const int32_t* __restrict__ dst, int n) {
+__global__ void __launch_bounds__(256) kv_copy_check_kernel(const KvView c, const int32_t* src, const int32_t* dst, int n) {
   pdl_trigger();
   pdl_wait();
   const int i = blockIdx.x * 8 + (threadIdx.x >> 5);
@@ -457,7 +457,7 @@ __global__ void __launch_bounds__(256) kv_copy_check_kernel(const KvView c, cons
 // Up to kCheckInline pairs each CTA checks its own pair (up to eight words per thread while the loads are on their way), above it
 // a launch of its own does, which then costs less than the lists read by every CTA: 1024 pages of 1 KB in one layer take 5.7
 // us this way and 8.5 us with a launch, 4096 of them in eight layers 190 and 141 us.
-__global__ void __launch_bounds__(256) kv_copy_kernel(const KvView c, const int32_t* __restrict__ src, const int32_t* __restrict__ dst, int n,
+__global__ void __launch_bounds__(256) kv_copy_kernel(const KvView c, const int32_t* src, const int32_t* dst, int n,
                                                       int pieces) {
   pdl_trigger();
   pdl_wait();

@@ -30,7 +30,8 @@ int kv_view(const fa4b_kv_cache* c, KvView* out);
 
 // A launch that may begin while the kernel before it on the stream still runs: every kernel launched this way runs
 // pdl_wait() before it touches memory (which returns once the kernel before has ended and its writes are visible), so only
-// the launch itself overlaps.  pdl_trigger() lets the next such launch come up early.
+// the launch itself overlaps.  pdl_trigger() lets the next such launch come up early.  Pointer parameters of such a kernel are not
+// __restrict__: loads through them might move above the wait.
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

@@ -179,3 +179,11 @@ def test_kernels_that_come_up_early_wait_before_they_read():
             assert not memory.search(before), (kernel, memory.search(before))
             seen.add(kernel)
     assert {"paged_plan_kernel", "attn_prefix_kernel", "attn_solo_kernel", "attn_team_kernel", "paged_join_kernel", "kv_extend_kernel", "kv_copy_kernel"} <= seen and len(seen) == 15, seen
+
+
+def test_kernels_that_come_up_early_promise_nothing_about_their_lists():
+    """`const T* __restrict__` tells the compiler that nobody writes the list while the kernel runs, so that its loads may move above the wait;
+    the kernel that writes it may still be running then."""
+    for name in ("kv_cache.cu", "attn_paged.cu", "attn_prefix.cu"):
+        for kernel, parameters, _ in _kernels(name):
+            assert "__restrict__" not in parameters, kernel
