@@ -6,22 +6,31 @@
 
 namespace fa4b {
 
-// `work` behind the status words: header of a fork or compaction, the pages a fork claims, flags of a copy, then the lists
-// of a compaction: used pages of each block of kBlockPages, holes, movers by the used pages before them, and those per page
-constexpr int kWorkStatus = kKvStatus, kWorkHead = kKvHead, kWorkFresh = 16, kWorkFlags = kWorkFresh + FA4B_KV_MAX_LIST,
-              kWorkLists = kWorkFlags + FA4B_KV_MAX_LIST;
+// `work` behind the status words: header of a fork or compaction, a bit per slot whose last extend was refused, then the lists
+// of a compaction: used pages of each block of kBlockPages, holes, movers by the used pages before them, and those per page (at least
+// 3 num_pages words; claims, forks and copies keep their free pages and flags there)
+constexpr int kWorkStatus = kKvStatus, kWorkHead = kKvHead, kWorkRefused = 16, kWorkLists = kWorkRefused + FA4B_KV_MAX_SEQS / 32;
 constexpr int kBlockPages = 4096;  // of a compaction: 1024 threads x 4
 constexpr int kPieceBytes = 32768;  // what one CTA of the copy kernels moves: 256 threads x 8 x 16 bytes, all loads in flight at once
 constexpr int kWarpBytes = 4096;    // the same per warp
 constexpr int kCheckInline = 1024;  // copy lists up to this length are checked for collisions by the copying CTAs themselves
 
-enum KvFinding { kOk = 0, kNoPages = 1, kBadSlot = 2, kSlotTwice = 3, kChildInUse = 4, kRowTooShort = 5, kBadPage = 6, kBadCount = 7, kCollision = 8 };
+enum KvFinding { kOk = 0, kNoPages = 1, kBadSlot = 2, kSlotTwice = 3, kChildInUse = 4, kRowTooShort = 5, kBadPage = 6, kBadCount = 7, kCollision = 8, kRefused = 9 };
 
 __device__ __forceinline__ void kv_report(const KvView& c, int what, int index, int detail) {
   if (atomicCAS(c.work + kWorkStatus, 0, what) == 0) {
     c.work[kWorkStatus + 1] = index;
     c.work[kWorkStatus + 2] = detail;
   }
+}
+
+// A slot whose last extend was refused: the tokens that were to follow have no place, so that a write, which goes by the length, would
+// land on the tokens before them.
+__device__ __forceinline__ uint32_t* refused_word(const KvView& c, int slot) { return reinterpret_cast<uint32_t*>(c.work) + kWorkRefused + (slot >> 5); }
+__device__ __forceinline__ bool is_refused(const KvView& c, int slot) { return *refused_word(c, slot) >> (slot & 31) & 1u; }
+__device__ __forceinline__ void mark_refused(const KvView& c, int slot) { atomicOr(refused_word(c, slot), 1u << (slot & 31)); }
+__device__ __forceinline__ void clear_refused(const KvView& c, int slot) {
+  if (is_refused(c, slot)) atomicAnd(refused_word(c, slot), ~(1u << (slot & 31)));
 }
 
 __device__ __forceinline__ int pages_of(const KvView& c, int len) { return (int)(((int64_t)len + c.page_tokens - 1) >> c.page_shift); }
@@ -116,7 +125,10 @@ __global__ void __launch_bounds__(128) kv_free_kernel(const KvView c, const int3
     if (threadIdx.x == 0) kv_report(c, kBadSlot, blockIdx.x, slot);
     return;
   }
-  if (threadIdx.x == 0) held = min(pages_of(c, max(atomicExch(c.lens + slot, 0), 0)), c.width);
+  if (threadIdx.x == 0) {
+    held = min(pages_of(c, max(atomicExch(c.lens + slot, 0), 0)), c.width);
+    clear_refused(c, slot);
+  }
   __syncthreads();
   int32_t* row = c.table + slot * c.table_stride;
   for (int j = threadIdx.x; j < held; j += 128) {
@@ -171,10 +183,14 @@ __global__ void __launch_bounds__(1024) kv_extend_kernel(const KvView c, const i
     want += total;  // at most 4096 x 2^18
   }
   if (threadIdx.x == 0) first[n] = want;
-  if (__syncthreads_or(bad)) return;
-  const int have = want ? find_free(c, want, fresh, warp_sums) : 0;
-  if (have < want) {
-    if (threadIdx.x == 0) kv_report(c, kNoPages, want, have);
+  bad = __syncthreads_or(bad);
+  const int have = want && !bad ? find_free(c, want, fresh, warp_sums) : 0;
+  if (bad || have < want) {
+    if (threadIdx.x == 0 && !bad) kv_report(c, kNoPages, want, have);
+    for (int i = threadIdx.x; i < n; i += 1024) {
+      const int slot = seqs[i];
+      if (slot >= 0 && slot < c.max_seqs) mark_refused(c, slot);
+    }
     return;
   }
   for (int r = threadIdx.x; r < want; r += 1024) {
@@ -188,7 +204,11 @@ __global__ void __launch_bounds__(1024) kv_extend_kernel(const KvView c, const i
     c.refs[p] = 1;
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < n; i += 1024) c.lens[seqs[i]] += n_new[i];
+  for (int i = threadIdx.x; i < n; i += 1024) {
+    const int slot = seqs[i];
+    c.lens[slot] += n_new[i];
+    clear_refused(c, slot);
+  }
 }
 
 // ---- write ------------------------------------------------------------------------------------------------------------
@@ -265,6 +285,10 @@ __global__ void __launch_bounds__(256, 3) kv_write_kernel(const KvView c, const 
   }
   if (tile0 >= t_end) return;
   const int64_t start = (int64_t)c.lens[slot] - n_new;
+  if (is_refused(c, slot)) {
+    if (threadIdx.x == 0 && h == 0 && blockIdx.y == 0) kv_report(c, kRefused, i, slot);
+    return;
+  }
   const int chunks = w.D / 8, chunk = threadIdx.x & (chunks - 1), step = 256 / chunks;
   const int32_t* row = c.table + slot * c.table_stride;
   const QuantScale sk(kE4M3 ? w.scale[0][h] : 1.f), sv(kE4M3 ? w.scale[1][h] : 1.f);
@@ -308,13 +332,14 @@ __global__ void __launch_bounds__(256, 3) kv_write_kernel(const KvView c, const 
 }
 
 // ---- fork -------------------------------------------------------------------------------------------------------------
-// First launch, one CTA: checks the lists, claims the tail pages.  fresh[i]: child i's tail page, -1: none; head[0]: 1
-// when the second launch may go on.
+// First launch, one CTA: checks the lists, claims the tail pages and puts them into the children's rows; head[0]: 1 when the second
+// launch may go on.
 __global__ void __launch_bounds__(1024) kv_fork_plan_kernel(const KvView c, const int32_t* parents, const int32_t* children,
                                                             int n, int32_t* list) {
   extern __shared__ uint32_t seen[];  // [max_seqs / 32]
   __shared__ int warp_sums[32];
-  int32_t* fresh = c.work + kWorkFresh;
+  constexpr int kEach = FA4B_KV_MAX_LIST / 1024;
+  int rank[kEach];  // of the tail pages of this thread's children among all; -1: none
   pdl_trigger();
   for (int i = threadIdx.x; i < (c.max_seqs + 31) / 32; i += 1024) seen[i] = 0u;
   __syncthreads();
@@ -322,8 +347,11 @@ __global__ void __launch_bounds__(1024) kv_fork_plan_kernel(const KvView c, cons
   if (threadIdx.x == 0) c.work[kWorkHead] = 0;
   bool bad = false;
   int want = 0;
-  for (int base = 0; base < n; base += 1024) {
-    const int i = base + threadIdx.x;
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    const int i = k * 1024 + threadIdx.x;
+    rank[k] = -1;
+    if (k * 1024 >= n) continue;
     int need = 0;
     if (i < n) {
       const int parent = parents[i], child = children[i];
@@ -342,7 +370,7 @@ __global__ void __launch_bounds__(1024) kv_fork_plan_kernel(const KvView c, cons
     }
     int total;
     const int before = block_scan1024(need, warp_sums, total);
-    if (i < n) fresh[i] = need ? want + before : -1;
+    if (need) rank[k] = want + before;
     want += total;
   }
   __syncthreads();
@@ -359,14 +387,18 @@ __global__ void __launch_bounds__(1024) kv_fork_plan_kernel(const KvView c, cons
     if (threadIdx.x == 0) kv_report(c, kNoPages, want, have);
     return;
   }
-  for (int i = threadIdx.x; i < n; i += 1024) {
-    const int rank = fresh[i];
-    if (rank >= 0) {
-      const int p = list[rank];
-      fresh[i] = p;
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    const int i = k * 1024 + threadIdx.x;
+    if (i >= n) break;
+    const int child = children[i], len = c.lens[parents[i]];
+    if (rank[k] >= 0) {
+      const int p = list[rank[k]];
+      c.table[child * c.table_stride + (len >> c.page_shift)] = p;
       c.refs[p] = 1;
     }
-    c.lens[children[i]] = c.lens[parents[i]];
+    c.lens[child] = len;
+    clear_refused(c, child);
   }
   if (threadIdx.x == 0) c.work[kWorkHead] = 1;
 }
@@ -379,7 +411,6 @@ __global__ void __launch_bounds__(256) kv_fork_move_kernel(const KvView c, const
   pdl_trigger();
   pdl_wait();
   if (c.work[kWorkHead] == 0) return;
-  const int32_t* fresh = c.work + kWorkFresh;
   if ((int)blockIdx.x < n) {
     const int i = blockIdx.x, len = c.lens[parents[i]], full = len >> c.page_shift;
     const int32_t* from = c.table + parents[i] * c.table_stride;
@@ -389,7 +420,6 @@ __global__ void __launch_bounds__(256) kv_fork_move_kernel(const KvView c, const
       to[j] = p;
       if (p >= 0 && p < c.pages) atomicAdd(c.refs + p, 1);
     }
-    if (threadIdx.x == 0 && fresh[i] >= 0) to[full] = fresh[i];
     return;
   }
   int64_t u = (int64_t)(blockIdx.x - n) * 8 + (threadIdx.x >> 5);
@@ -401,12 +431,10 @@ __global__ void __launch_bounds__(256) kv_fork_move_kernel(const KvView c, const
   const bool is_v = u & 1;
   u >>= 1;
   const int layer = (int)(u % c.layers), i = (int)(u / c.layers);
-  const int dst = fresh[i];
-  if (dst < 0) return;
   const int len = c.lens[parents[i]];
   const int bytes = (len & (c.page_tokens - 1)) * c.row_bytes - piece * kWarpBytes;  // of this head's rows, from this piece on
   if (bytes <= 0) return;
-  const int src = c.table[parents[i] * c.table_stride + (len >> c.page_shift)];
+  const int src = c.table[parents[i] * c.table_stride + (len >> c.page_shift)], dst = c.table[children[i] * c.table_stride + (len >> c.page_shift)];
   if (src < 0 || src >= c.pages) return;
   uint8_t* base = (is_v ? c.v : c.k) + layer * (is_v ? c.v_layer : c.k_layer) + (int64_t)h * c.page_tokens * c.row_bytes + piece * kWarpBytes;
   const int64_t page = is_v ? c.v_page : c.k_page;
@@ -439,7 +467,7 @@ __device__ __forceinline__ void piece_store(const PieceRegs& x, uint8_t* to, int
 __device__ __forceinline__ bool collides(int i, int j, int s, int d, int sj, int dj) { return (j != i && dj == d) || sj == d || dj == s; }
 
 // one warp per pair
-__global__ void __launch_bounds__(256) kv_copy_check_kernel(const KvView c, const int32_t* src, const int32_t* dst, int n) {
+__global__ void __launch_bounds__(256) kv_copy_check_kernel(const KvView c, const int32_t* src, const int32_t* dst, int n, int32_t* flags) {
   pdl_trigger();
   pdl_wait();
   const int i = blockIdx.x * 8 + (threadIdx.x >> 5);
@@ -449,7 +477,7 @@ __global__ void __launch_bounds__(256) kv_copy_check_kernel(const KvView c, cons
   if (s >= 0 && d >= 0)
     for (int j = threadIdx.x & 31; j < n; j += 32) bad |= collides(i, j, s, d, src[j], dst[j]);
   bad = __any_sync(0xffffffffu, bad);
-  if ((threadIdx.x & 31) == 0) c.work[kWorkFlags + i] = bad;
+  if ((threadIdx.x & 31) == 0) flags[i] = bad;
 }
 
 // One CTA per 32 KB of a page of one layer, K or V: every thread has eight 16-byte loads in flight before its first store.  Bound by
@@ -458,7 +486,7 @@ __global__ void __launch_bounds__(256) kv_copy_check_kernel(const KvView c, cons
 // a launch of its own does, which then costs less than the lists read by every CTA: 1024 pages of 1 KB in one layer take 5.7
 // us this way and 8.5 us with a launch, 4096 of them in eight layers 190 and 141 us.
 __global__ void __launch_bounds__(256) kv_copy_kernel(const KvView c, const int32_t* src, const int32_t* dst, int n,
-                                                      int pieces) {
+                                                      int pieces, const int32_t* flags) {
   pdl_trigger();
   pdl_wait();
   int64_t u = blockIdx.x;
@@ -480,11 +508,11 @@ __global__ void __launch_bounds__(256) kv_copy_kernel(const KvView c, const int3
   PieceRegs x;
   piece_load(x, base + s * page, bytes);
   bool bad = false;
-  if (n <= kCheckInline) {
+  if (flags == nullptr) {
     for (int j = threadIdx.x; j < n; j += 256) bad |= collides(i, j, s, d, src[j], dst[j]);
     bad = __syncthreads_or(bad);
   } else {
-    bad = c.work[kWorkFlags + i] != 0;
+    bad = flags[i] != 0;
   }
   if (bad) {
     if (reports) kv_report(c, kCollision, i, d);
@@ -732,7 +760,7 @@ int fa4b_kv_fork(const fa4b_kv_cache* c, const int32_t* parents, const int32_t* 
   FA4B_REQUIRE(ctas < 1ll << 31, FA4B_BAD_SHAPE, "%d forks over %d layers and %d heads are too many for one call", n, v.layers, v.heads);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const size_t smem = 4 * (size_t)((v.max_seqs + 31) / 32);
-  FA4B_CUDA(launch_overlapped(kv_fork_plan_kernel, 1, 1024, smem, st, v, parents, children, n, v.work + kWorkFlags));
+  FA4B_CUDA(launch_overlapped(kv_fork_plan_kernel, 1, 1024, smem, st, v, parents, children, n, v.work + kWorkLists));
   FA4B_CUDA(launch_overlapped(kv_fork_move_kernel, (unsigned)ctas, 256, 0, st, v, parents, children, n, pieces, units));
   return FA4B_OK;
 }
@@ -746,8 +774,10 @@ int fa4b_kv_copy_pages(const fa4b_kv_cache* c, const int32_t* src, const int32_t
   const int64_t ctas = (int64_t)n * v.layers * 2 * pieces;
   FA4B_REQUIRE(ctas < 1ll << 31, FA4B_BAD_SHAPE, "%d pages of %d layers are too many for one call", n, v.layers);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (n > kCheckInline) FA4B_CUDA(launch_overlapped(kv_copy_check_kernel, (n + 7) / 8, 256, 0, st, v, src, dst, n));
-  FA4B_CUDA(launch_overlapped(kv_copy_kernel, (unsigned)ctas, 256, 0, st, v, src, dst, n, pieces));
+  // more pairs than the work area has room for flags are more than the pool has pages: few of them can be free of collisions
+  int32_t* flags = n > kCheckInline && n <= 3ll * v.pages ? v.work + kWorkLists : nullptr;
+  if (flags) FA4B_CUDA(launch_overlapped(kv_copy_check_kernel, (n + 7) / 8, 256, 0, st, v, src, dst, n, flags));
+  FA4B_CUDA(launch_overlapped(kv_copy_kernel, (unsigned)ctas, 256, 0, st, v, src, dst, n, pieces, flags));
   return FA4B_OK;
 }
 
@@ -792,6 +822,7 @@ int fa4b_kv_check_status(const fa4b_kv_cache* c, void* stream) {
     case kRowTooShort: set_error("entry %d: a row of the page table holds %d pages, too few for slot %d", host[1], v.width, host[2]); break;
     case kBadPage: set_error("pair %d names page %d of %d", host[1], host[2], v.pages); break;
     case kBadCount: set_error("entry %d: negative number of new tokens for slot %d", host[1], host[2]); break;
+    case kRefused: set_error("entry %d writes to slot %d, whose last extend was refused", host[1], host[2]); break;
     case kCollision: set_error("pair %d: page %d is also another pair's destination or source", host[1], host[2]); break;
     default: set_error("finding %d (%d, %d)", host[0], host[1], host[2]); break;
   }

@@ -132,14 +132,16 @@ class PagedKVCache:
 
     def extend(self, seqs: torch.Tensor, n_new: torch.Tensor) -> None:
         """Slot ``seqs[i]`` grows by ``n_new[i]`` tokens (:meth:`write` fills them) and claims pages for them: the lowest
-        free ones, in the order of the list.  All or nothing; :meth:`check_status` tells."""
+        free ones, in the order of the list.  All or nothing; :meth:`check_status` tells.  The slots of a list that was refused take no
+        writes until one of their calls (an ``extend``, by 0 tokens too, or a ``free``, or a ``fork`` into them) succeeds."""
         a, n = self._list(seqs, "seqs"), seqs.numel()
         self._call("fa4b_kv_extend", a, self._list(n_new, "n_new", n), n)
 
     def write(self, k: torch.Tensor, v: torch.Tensor, seqs: torch.Tensor, *, n_new: torch.Tensor | None = None, layer: int = 0) -> None:
         """Keys and values ``[n, Hkv, T, D]`` (any batch / head / token strides) of the newest tokens: token ``t < n_new[i]``
         goes to position ``seq_lens[seqs[i]] - n_new[i] + t`` (``n_new`` None: T for every row).  A 16-bit cache takes its
-        own type, an E4M3 cache bf16 or f16, divided by the scale, clamped to +-448 and rounded.  Tokens from before a
+        own type, an E4M3 cache bf16 or f16, divided by the scale, clamped to +-448 and rounded.  A slot whose last :meth:`extend` was
+        refused is left out and reported.  Tokens from before a
         :meth:`fork` lie in pages that the samples share: write those before it.  A slot named twice gets either row's values."""
         a, n = self._list(seqs, "seqs"), seqs.numel()
         b = 0 if n_new is None else self._list(n_new, "n_new", n)

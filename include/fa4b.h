@@ -522,13 +522,15 @@ int fa4b_kv_free(const fa4b_kv_cache* c, const int32_t* seqs, int32_t n, void* s
 
 /* fa4b_kv_extend: slot seqs[i] grows by n_new[i] >= 0 tokens and claims the pages for them: the lowest free pages, in
  * the order of i.  Nothing changes when a slot is out of range or named twice, a row of the table is too short, or
- * there are too few free pages. */
+ * there are too few free pages; the slots that the list names then take no writes until an extend (by 0 tokens, too), a fork or
+ * a free of theirs succeeds. */
 int fa4b_kv_extend(const fa4b_kv_cache* c, const int32_t* seqs, const int32_t* n_new, int32_t n, void* stream);
 
 /* fa4b_kv_write: token t < n_new[i] of row i goes to position seq_lens[seqs[i]] - n_new[i] + t (n_new NULL: T for every
  * row).  k_new, v_new: [n, Hkv, T, D] bf16 or f16, batch / head / token strides in elements (multiples of 8), pointers
  * 16-byte aligned.  A 16-bit cache takes values of its own type; an E4M3 cache stores RN(clamp(x / scale, +-448)),
- * NaN kept.  Positions below 0 and rows whose slot is out of range are left out.  Tokens from before a fork lie in pages that
+ * NaN kept.  Positions below 0 and rows whose slot is out of range are left out, and so are rows whose slot's last extend was refused (its
+ * length is the old one, and the new tokens would land on the old): reported.  Tokens from before a fork lie in pages that
  * the samples share (write those before it); a slot named twice gets either row's values. */
 typedef struct fa4b_kv_write_args {
   const void* k_new;

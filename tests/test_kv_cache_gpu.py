@@ -313,3 +313,141 @@ def test_calls_follow_the_current_stream():
     m.extend([0, 1], [40, 16])
     m.fork([0], [3])
     m.check(c)
+
+
+def full_pool(dtype=torch.bfloat16, length=48):
+    """Slots 0 (forked into 3 at a page's end) and 1, each with `length` tokens written, and two pages left."""
+    c = make(pages=8, dtype=dtype, layers=2)
+    src = torch.float16 if dtype == torch.float16 else torch.bfloat16
+    c.extend(ints([0, 1]), ints([length, length]))
+    for layer in range(2):
+        c.write(*values(2, 2, length, 64, src, layer), ints([0, 1]), layer=layer)
+    c.fork(ints([0]), ints([3]))
+    c.check_status()
+    return c, src
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("seqs,new,error,text", [
+    ([0, 1, 3], [1, 1, 1], RuntimeError, "3 pages were asked for, 2 are free"),
+    ([3, 12, 1], [1, 1, 1], ValueError, "slot 12 of 12"),
+    ([3, 1, 1], [2, 2, 2], ValueError, "second time"),
+    ([1, 3], [9 * 16, 2], ValueError, "too few"),
+    ([1, 0], [2, -2], ValueError, "negative"),
+])
+def test_a_write_behind_an_extend_that_was_refused_leaves_the_tokens_alone(dtype, seqs, new, error, text):
+    """The step goes on (nothing synchronises): what is written then would land on the newest tokens, shared ones among them."""
+    c, src = full_pool(dtype)
+    m = ModelCache(c)
+    c.extend(ints(seqs), ints(new))
+    for layer in range(2):
+        c.write(*values(len(seqs), 2, 2, 64, src, 7 + layer), ints(seqs), n_new=ints([2] * len(seqs)), layer=layer)
+        c.write(*values(len(seqs), 2, 1, 64, src, 9 + layer), ints(seqs), layer=layer)
+    m.check(c)
+    with pytest.raises(error, match=text):
+        c.check_status()
+    c.write(*values(1, 2, 1, 64, src, 11), ints([seqs[0]]))  # the status says nothing about the slot's length: still no place
+    m.check(c)
+    with pytest.raises(ValueError, match=f"slot {seqs[0]}, whose last extend was refused"):
+        c.check_status()
+    c.check_status()
+
+
+def test_slots_that_a_refused_extend_does_not_name_are_written_and_named_ones_again_after_the_next():
+    c, src = full_pool()
+    m = ModelCache(c)
+
+    def write(seqs, seed, ok):
+        k, v = values(len(seqs), 2, 2, 64, src, seed)
+        c.write(k, v, ints(seqs))
+        if ok:
+            m.write(k, v, seqs, None, 0)
+        m.check(c, str(seed))
+
+    c.extend(ints([0, 3, 1]), ints([1, 1, 1]))  # three pages, two are free
+    write([0, 3], 1, False)
+    c.extend(ints([1]), ints([2]))  # another list, which fits
+    assert m.extend([1], [2])
+    write([1], 2, True)
+    write([3], 3, False)
+    c.extend(ints([3, 5]), ints([2, 0]))  # the last page
+    assert m.extend([3, 5], [2, 0])
+    write([3], 4, True)
+    write([0], 5, False)
+    c.free(ints([1]))  # gives pages back
+    m.free([1])
+    c.extend(ints([0]), ints([3]))
+    assert m.extend([0], [3])
+    write([0], 6, True)
+    # a free and a fork open a slot as well
+    c.extend(ints([7, 8]), ints([99, 99]))
+    c.free(ints([8]))
+    c.fork(ints([0]), ints([7]))
+    m.free([8])
+    assert m.fork([0], [7])
+    write([7], 7, True)
+    c.extend(ints([0]), ints([0]))
+    write([0], 8, True)
+    m.invariants()
+
+
+def test_a_captured_step_is_replayed_through_a_full_pool():
+    """Extend and write in one graph: replays that find too few pages change nothing, and the step works again once pages are there."""
+    c, src = full_pool()
+    seqs, new = ints([0, 1, 3]), ints([1, 1, 1])
+    k, v = values(3, 2, 1, 64, src, 20)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            c.extend(seqs, new)
+            c.write(k, v, seqs)
+    torch.cuda.current_stream().wait_stream(side)
+    m = ModelCache(c)
+    for _ in range(2):
+        k.normal_(), v.normal_()
+        graph.replay()
+        m.check(c)
+    with pytest.raises(RuntimeError, match="3 pages were asked for"):
+        c.check_status()
+    c.free(ints([1]))
+    m.free([1])
+    for _ in range(3):
+        k.normal_(), v.normal_()
+        graph.replay()
+        assert m.extend([0, 1, 3], [1, 1, 1])
+        m.write(k, v, [0, 1, 3], None, 0)
+        m.check(c)
+    m.invariants()
+    c.check_status()
+
+
+@pytest.mark.parametrize("seqs", [12, 33, 4500])
+def test_marks_of_refused_slots_are_a_slots_own(seqs):
+    """First and last slots, neighbours in a word, and the other calls in between, which use the work area too."""
+    c = make(pages=6000, heads=1, layers=1, seqs=seqs, width=1)
+    named = sorted({0, 1, 9, seqs // 2, seqs - 2, seqs - 1})
+    others = [s for s in range(seqs) if s not in named][:5]
+    c.extend(ints(named + others), ints([7] * (len(named) + len(others))))
+    c.extend(ints(named), ints([10] * len(named)))  # 17 tokens, rows of 16
+    order = [s for s in range(seqs) if s not in named + others][: 2 * (seqs // 4)]
+    half = len(order) // 2
+    if half:
+        c.extend(ints(order[:half]), ints([3] * half))
+        c.fork(ints(order[:half]), ints(order[half:2 * half]))
+        c.free(ints(order))
+    c.copy_pages(ints(list(range(1200))), ints(list(range(3000, 4200))))
+    c.compact()
+    m = ModelCache(c)
+    k, v = values(len(named) + len(others), 1, 2, 64, torch.bfloat16, 1)
+    c.write(k, v, ints(named + others))
+    m.write(k[len(named):], v[len(named):], others, None, 0)
+    m.check(c)
+    c.free(ints(named[:3]))
+    m.free(named[:3])
+    c.extend(ints(named), ints([1] * len(named)))
+    assert m.extend(named, [1] * len(named))
+    c.write(k[:len(named)], v[:len(named)], ints(named), n_new=ints([1] * len(named)))
+    m.write(k[:len(named)], v[:len(named)], named, [1] * len(named), 0)
+    m.check(c)
