@@ -15,7 +15,7 @@ constexpr int kPieceBytes = 32768;  // what one CTA of the copy kernels moves: 2
 constexpr int kWarpBytes = 4096;    // the same per warp
 constexpr int kCheckInline = 1024;  // copy lists up to this length are checked for collisions by the copying CTAs themselves
 
-enum KvFinding { kOk = 0, kNoPages = 1, kBadSlot = 2, kSlotTwice = 3, kChildInUse = 4, kRowTooShort = 5, kBadPage = 6, kBadCount = 7, kCollision = 8, kRefused = 9 };
+enum KvFinding { kOk = 0, kNoPages = 1, kBadSlot = 2, kSlotTwice = 3, kChildInUse = 4, kRowTooShort = 5, kBadPage = 6, kBadCount = 7, kCollision = 8, kRefused = 9, kShared = 10 };
 
 __device__ __forceinline__ void kv_report(const KvView& c, int what, int index, int detail) {
   if (atomicCAS(c.work + kWorkStatus, 0, what) == 0) {
@@ -309,12 +309,24 @@ __global__ void __launch_bounds__(256, 3) kv_write_kernel(const KvView c, const 
       at[j] = ((int)pos & (c.page_tokens - 1)) * c.row_bytes;
     }
     uint4 xk[4], xv[4];
+    int held[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if ((uint32_t)page[j] < (uint32_t)c.pages) held[j] = c.refs[page[j]];
 #pragma unroll
     for (int j = 0; j < 4; ++j)
       if ((uint32_t)page[j] < (uint32_t)c.pages) {
         xk[j] = __ldcs(reinterpret_cast<const uint4*>(k_src + (t0 + j * step) * w.st[0]));
         xv[j] = __ldcs(reinterpret_cast<const uint4*>(v_src + (t0 + j * step) * w.st[1]));
       }
+    if (max(max(held[0], held[1]), max(held[2], held[3])) > 1) {  // other slots' tokens as well
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (held[j] > 1) {
+          if (h == 0 && chunk == 0) kv_report(c, kShared, i, page[j]);
+          page[j] = -1;
+        }
+    }
 #pragma unroll
     for (int j = 0; j < 4; ++j)
       if ((uint32_t)page[j] < (uint32_t)c.pages) {
@@ -823,6 +835,7 @@ int fa4b_kv_check_status(const fa4b_kv_cache* c, void* stream) {
     case kBadPage: set_error("pair %d names page %d of %d", host[1], host[2], v.pages); break;
     case kBadCount: set_error("entry %d: negative number of new tokens for slot %d", host[1], host[2]); break;
     case kRefused: set_error("entry %d writes to slot %d, whose last extend was refused", host[1], host[2]); break;
+    case kShared: set_error("entry %d writes to page %d, which several slots hold", host[1], host[2]); break;
     case kCollision: set_error("pair %d: page %d is also another pair's destination or source", host[1], host[2]); break;
     default: set_error("finding %d (%d, %d)", host[0], host[1], host[2]); break;
   }

@@ -141,8 +141,8 @@ class PagedKVCache:
         """Keys and values ``[n, Hkv, T, D]`` (any batch / head / token strides) of the newest tokens: token ``t < n_new[i]``
         goes to position ``seq_lens[seqs[i]] - n_new[i] + t`` (``n_new`` None: T for every row).  A 16-bit cache takes its
         own type, an E4M3 cache bf16 or f16, divided by the scale, clamped to +-448 and rounded.  A slot whose last :meth:`extend` was
-        refused is left out and reported.  Tokens from before a
-        :meth:`fork` lie in pages that the samples share: write those before it.  A slot named twice gets either row's values."""
+        refused is left out and reported, and so are tokens whose page several slots hold: those from before a :meth:`fork` (write them
+        before it).  A slot named twice gets either row's values."""
         a, n = self._list(seqs, "seqs"), seqs.numel()
         b = 0 if n_new is None else self._list(n_new, "n_new", n)
         if type(k) is not torch.Tensor or type(v) is not torch.Tensor:

@@ -489,8 +489,8 @@ int fa4b_attn_check_status(const fa4b_attn_dims* d, const void* ws, void* stream
  * layer and page strides are the caller's (16-byte multiples).  A slot (a sequence) names its pages in its row of
  * page_table; token j of slot s is row j % page_tokens of page page_table[s][j / page_tokens].  Invariants that every
  * call keeps: a slot of length len has exactly ceil(len / page_tokens) entries, the rest of its row is -1;
- * ref_counts[p] is the number of slots that hold page p (0: free); a page that several slots hold is full, so nothing
- * is ever written to a shared page.  All of it is device memory: no call synchronises, all may be captured into a
+ * ref_counts[p] is the number of slots that hold page p (0: free); a page that several slots hold is full, and only
+ * fa4b_kv_copy_pages, which goes by page numbers, ever writes to one.  All of it is device memory: no call synchronises, all may be captured into a
  * graph, and calls on one cache have to be ordered (one stream, or events), as they change it.
  *
  * What a call finds wrong on the device (an index out of range, no free pages, ...) goes to the status words in
@@ -530,8 +530,9 @@ int fa4b_kv_extend(const fa4b_kv_cache* c, const int32_t* seqs, const int32_t* n
  * row).  k_new, v_new: [n, Hkv, T, D] bf16 or f16, batch / head / token strides in elements (multiples of 8), pointers
  * 16-byte aligned.  A 16-bit cache takes values of its own type; an E4M3 cache stores RN(clamp(x / scale, +-448)),
  * NaN kept.  Positions below 0 and rows whose slot is out of range are left out, and so are rows whose slot's last extend was refused (its
- * length is the old one, and the new tokens would land on the old): reported.  Tokens from before a fork lie in pages that
- * the samples share (write those before it); a slot named twice gets either row's values. */
+ * length is the old one, and the new tokens would land on the old): reported.  Tokens whose
+ * page several slots hold are left out and reported as well: those from before a fork lie in pages that the samples share (write them
+ * before it).  A slot named twice gets either row's values. */
 typedef struct fa4b_kv_write_args {
   const void* k_new;
   const void* v_new;

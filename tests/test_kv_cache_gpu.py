@@ -451,3 +451,28 @@ def test_marks_of_refused_slots_are_a_slots_own(seqs):
     c.write(k[:len(named)], v[:len(named)], ints(named), n_new=ints([1] * len(named)))
     m.write(k[:len(named)], v[:len(named)], named, [1] * len(named), 0)
     m.check(c)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("page", [16, 64])
+def test_tokens_in_pages_that_several_slots_hold_are_not_written(dtype, page):
+    """A write that reaches behind a fork: the tail is a slot's own, the pages before it belong to the samples too."""
+    c = make(pages=40, page=page, heads=2, dtype=dtype)
+    src = torch.float16 if dtype == torch.float16 else torch.bfloat16
+    length = 5 * page + 7
+    c.extend(ints([0]), ints([length]))
+    c.fork(ints([0]), ints([4]))
+    m = ModelCache(c)
+    k, v = values(2, 2, length, 64, src, 1)
+    c.write(k, v, ints([4, 0]), layer=1)
+    own = [7, 7]
+    m.write(k[:, :, -7:], v[:, :, -7:], [4, 0], own, 1)
+    m.check(c)
+    with pytest.raises(ValueError, match="entry [01] writes to page [0-4], which several slots hold"):
+        c.check_status()
+    c.free(ints([0]))  # then the pages are slot 4's alone
+    m.free([0])
+    c.write(k, v, ints([4, 4]), n_new=ints([length, 0]), layer=0)
+    m.write(k, v, [4, 4], [length, 0], 0)
+    m.check(c)
+    c.check_status()
