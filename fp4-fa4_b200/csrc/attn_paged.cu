@@ -1150,7 +1150,7 @@ template <int D, bool kE4M3, typename QT>
 static int launch_paged(const PagedParams& p, const PagedMaps& m, cudaStream_t st) {
   const size_t smem = 4 * paged_plan_words(p.n, p.groups);
   static std::atomic<uint64_t> allowed[5];
-  if (smem > 48 * 1024)
+  if (smem > kSmemUnasked)
     if (int s = allow_smem(paged_plan_kernel, 4 * (int)paged_plan_words(kPagedMaxRows, kPagedMaxRows), allowed[3])) return s;
   if (!p.small) FA4B_CUDA(launch_overlapped(paged_plan_kernel, 1, kPlanThreads, smem, st, p));
   if (p.groups > 0)

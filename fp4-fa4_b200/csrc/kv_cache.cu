@@ -719,7 +719,7 @@ int fa4b_kv_extend(const fa4b_kv_cache* c, const int32_t* seqs, const int32_t* n
   if (n == 0) return FA4B_OK;
   const size_t smem = 4 * ((size_t)n + 1 + (v.max_seqs + 31) / 32);
   static std::atomic<uint64_t> allowed{0};
-  if (smem > 48 * 1024)
+  if (smem > kSmemUnasked)
     if (int s = allow_smem(kv_extend_kernel, 4 * (FA4B_KV_MAX_LIST + 1 + FA4B_KV_MAX_SEQS / 32), allowed)) return s;
   int32_t* fresh = v.work + kWorkLists;  // the lists of a compaction are at least num_pages long
   FA4B_CUDA(launch_overlapped(kv_extend_kernel, 1, 1024, smem, static_cast<cudaStream_t>(stream), v, seqs, n_new, n, fresh));

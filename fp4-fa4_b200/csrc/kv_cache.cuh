@@ -50,7 +50,11 @@ cudaError_t launch_overlapped(void (*kernel)(P...), dim3 grid, dim3 block, size_
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(std::forward<A>(args))...);
 }
 
-// Dynamic shared memory above 48 KB is allowed once per kernel and device; one `done` for each kernel.
+// A launch may have 48 KB of shared memory without more ado, of which static variables and the system take their part; more than this
+// much dynamic memory is asked for.
+constexpr size_t kSmemUnasked = 40 * 1024;
+
+// More dynamic shared memory than that is allowed once per kernel and device; one `done` for each kernel.
 template <typename K>
 int allow_smem(K kernel, int bytes, std::atomic<uint64_t>& done) {
   int dev = 0;

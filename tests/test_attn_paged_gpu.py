@@ -652,3 +652,33 @@ def test_calls_that_differ_follow_one_another_without_a_pause():
         c.page_table.copy_(states[state][0]), c.seq_lens.copy_(states[state][1])
         compare(c, qs[which], out, lse, slots)
         compare(c, qs[which], out2, lse2, slots)
+
+
+@pytest.mark.parametrize("n,groups", [(3071, 0), (3008, 0), (2000, 714)])
+def test_calls_whose_plan_takes_just_under_48_kb_of_shared_memory(n, groups):
+    """In a process of their own: a larger call before them would have asked for more."""
+    import pathlib
+    import subprocess
+    import sys
+
+    text = f"""
+import test_attn_paged_gpu as A, test_kv_cache_gpu as K
+n, groups = {n}, {groups}
+lens = [20 + i % 7 for i in range(n)]
+members = [2] * groups
+c, slots, offsets = A.build(lens, [16] * groups, members, hkv=1, d=64, seed=70)
+q = A.queries(n, 2, 1, 64, A.BF, 71)
+more = dict(group_offsets=A.ints(offsets), shared_lens=A.ints([16] * groups)) if groups else {{}}
+out, lse = c.attend(q, A.ints(slots), **more)
+c.check_status()
+A.compare(c, q, out, lse, slots, rows=range(0, 2 * groups or n, 101))
+seqs = list(range(262144 - 4090, 262144))
+c = K.make(pages=4096, heads=1, layers=1, seqs=262144, width=1)
+c.extend(K.ints(seqs), K.ints([3] * 4090))
+c.check_status()
+assert int(c.seq_lens.sum()) == 3 * 4090 and (c.page_table[seqs, 0] == K.ints(list(range(4090)))).all()
+"""
+    root = pathlib.Path(__file__).resolve().parents[1]
+    done = subprocess.run([sys.executable, "-c", text], cwd=root, capture_output=True, text=True, timeout=240,
+                          env={**__import__("os").environ, "PYTHONPATH": f"{root / 'fp4-fa4_b200'}:{root / 'tests'}:{root / 'oracle'}"})
+    assert done.returncode == 0, done.stderr[-2000:]
