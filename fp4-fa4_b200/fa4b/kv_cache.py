@@ -23,6 +23,7 @@ _ATTEND = struct.Struct("@P3qP3qP5ifPiPPP")
 
 _current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
+_LARGEST = torch.finfo(torch.float32).max
 KV_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float8_e4m3fn: 2}
 
 
@@ -194,7 +195,7 @@ class PagedKVCache:
         ``group_offsets [groups + 1]``, ``shared_lens [groups]``: rows ``group_offsets[g]`` up to ``group_offsets[g + 1]`` hold
         the same pages for their first ``shared_lens[g]`` tokens (as :meth:`fork` leaves them), which are read once for
         the group; rows in no group are left as they were.  ``out`` receives O when given (any strides but 0).  There is no
-        gradient."""
+        gradient.  ``softmax_scale`` None: ``1 / sqrt(D)``."""
         if not isinstance(q, torch.Tensor) or len(shape := q.shape) != 4 or shape[3] != self._d:
             raise ValueError(f"q must be a [n, Hq, T, {self._d}] tensor")
         dtype, strides = q.dtype, q.stride()
@@ -223,9 +224,9 @@ class PagedKVCache:
         else:
             o_strides = _strides(shape, out.stride())
         lse = self._floats.new_empty((n, hq, t))
-        code, scale = KV_DTYPES[dtype], softmax_scale or 0.0
-        if not scale >= 0.0:
-            raise ValueError(f"softmax_scale must be positive, got {softmax_scale}")
+        code, scale = KV_DTYPES[dtype], 0.0 if softmax_scale is None else softmax_scale
+        if softmax_scale is not None and not 2.0 ** -149 <= scale <= _LARGEST:
+            raise ValueError(f"softmax_scale must be positive and finite in 32 bits, got {softmax_scale}")
         q_strides = _strides(shape, strides)
         size = self._ws_bytes.get((n, hq, t, groups))
         if size is None:

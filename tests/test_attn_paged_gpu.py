@@ -682,3 +682,19 @@ assert int(c.seq_lens.sum()) == 3 * 4090 and (c.page_table[seqs, 0] == K.ints(li
     done = subprocess.run([sys.executable, "-c", text], cwd=root, capture_output=True, text=True, timeout=240,
                           env={**__import__("os").environ, "PYTHONPATH": f"{root / 'fp4-fa4_b200'}:{root / 'tests'}:{root / 'oracle'}"})
     assert done.returncode == 0, done.stderr[-2000:]
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.0, 0, 1e-46, 1e39, -1e39, -float("inf")])
+def test_a_softmax_scale_that_is_no_positive_number_in_32_bits_is_refused(scale):
+    """Zero is no word for the default: None is."""
+    c, slots, _ = build([50, 20], [], [], hkv=2, d=64, seed=20)
+    with pytest.raises(ValueError, match="softmax_scale"):
+        c.attend(queries(2, 4, 1, 64, BF, 0), ints(slots), softmax_scale=scale)
+
+
+def test_the_softmax_scale_may_be_any_positive_number():
+    c, slots, _ = build([50, 20], [], [], hkv=2, d=64, seed=20)
+    q = queries(2, 4, 1, 64, BF, 0)
+    for scale in (1, 2.0 ** -100, 0.125, None):
+        out, lse = c.attend(q, ints(slots), softmax_scale=scale)
+        compare(c, q, out, lse, slots, scale=scale)
