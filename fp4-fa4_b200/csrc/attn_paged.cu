@@ -1052,7 +1052,17 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PagedParams p) {
     n_own = (int)((from + tiles - 1) / cut.per - worker) + 1;
     own_row = r & (p.own_rows - 1);
   }
-  if (!there || s.left_alone) return;  // or behind the last group; the same for all warps of a row
+  if (!there) return;
+  auto o_at = [&]() { return p.o + 2 * ((int64_t)i * p.o_sb + (int64_t)h * p.o_sh + (int64_t)t * p.o_st + lane * kPer); };
+  auto lse_at = [&]() { return p.lse + ((int64_t)i * p.Hq + h) * p.T + t; };
+  if (s.left_alone) {  // in no group; the same for all warps of a row
+    if (p.flags & FA4B_PAGED_CLEAR_O) {
+      if constexpr (kPer == 4) *reinterpret_cast<uint2*>(o_at()) = make_uint2(0u, 0u);
+      else *reinterpret_cast<uint32_t*>(o_at()) = 0u;
+    }
+    if (lane == 0 && (p.flags & FA4B_PAGED_CLEAR_LSE)) *lse_at() = -INFINITY;
+    return;
+  }
   const int total = n_prefix + n_own, each = kSplit ? (total + 3) / 4 : total, end = min(total, (part + 1) * each);
   for (int base = part * each; base < end; base += 32) {
     const int k = base + lane;
@@ -1121,10 +1131,10 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PagedParams p) {
     }
   }
   const float inv = l == 0.f ? 0.f : (p.v_scale ? p.v_scale[head] : 1.f) / l;  // a row that sees nothing: zeros, -inf
-  uint8_t* out = p.o + 2 * ((int64_t)i * p.o_sb + (int64_t)h * p.o_sh + (int64_t)t * p.o_st + lane * kPer);
+  uint8_t* out = o_at();
   if constexpr (kPer == 4) *reinterpret_cast<uint2*>(out) = make_uint2(pack16(acc[0] * inv, acc[1] * inv, QT{}), pack16(acc[2] * inv, acc[3] * inv, QT{}));
   else *reinterpret_cast<uint32_t*>(out) = pack16(acc[0] * inv, acc[1] * inv, QT{});
-  if (lane == 0) p.lse[((int64_t)i * p.Hq + h) * p.T + t] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+  if (lane == 0) *lse_at() = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
 }  // namespace fa4b
@@ -1189,8 +1199,9 @@ static int paged_params(const fa4b_kv_cache* c, const fa4b_attn_paged_args* a, P
   FA4B_REQUIRE(c->dtype == FA4B_KV_E4M3 || a->q_dtype == c->dtype, FA4B_UNSUPPORTED, "a 16-bit cache takes queries of its own type");
   FA4B_REQUIRE(a->groups >= 0 && a->groups <= std::max(a->n, 1), FA4B_BAD_SHAPE, "groups=%d: at most one for each of %d rows", a->groups, a->n);
   FA4B_REQUIRE(a->groups == 0 || (a->group_offsets && a->shared_lens), FA4B_BAD_ARG, "groups need group_offsets and shared_lens");
+  FA4B_REQUIRE((a->flags & ~(FA4B_PAGED_CLEAR_O | FA4B_PAGED_CLEAR_LSE)) == 0, FA4B_BAD_ARG, "unknown flags 0x%x", a->flags);
   FA4B_REQUIRE(a->seqs || a->n <= c->max_seqs, FA4B_BAD_SHAPE, "n=%d rows without a list of slots, and %d slots", a->n, c->max_seqs);
-  p.layer = a->layer, p.n = a->n, p.T = a->T, p.Hq = a->Hq, p.G = a->Hq / c->Hkv, p.R = p.T * p.G, p.groups = a->groups;
+  p.layer = a->layer, p.n = a->n, p.T = a->T, p.Hq = a->Hq, p.G = a->Hq / c->Hkv, p.R = p.T * p.G, p.groups = a->groups, p.flags = a->flags;
   p.seqs = a->seqs, p.offsets = a->group_offsets, p.shared = a->shared_lens;
   p.q = static_cast<const uint8_t*>(a->q), p.q_sb = a->q_strides.batch, p.q_sh = a->q_strides.head, p.q_st = a->q_strides.seq;
   p.o = static_cast<uint8_t*>(a->o), p.o_sb = a->o_strides.batch, p.o_sh = a->o_strides.head, p.o_st = a->o_strides.seq;

@@ -58,6 +58,7 @@ struct PagedParams {
   float* lse;         // [n, Hq, T]
   int n, T, Hq, G, R; // G = Hq / Hkv, R = T G rows of a sequence and kv head
   int groups;         // 0: no groups, nothing shared
+  int flags;          // FA4B_PAGED_CLEAR_*
   const int32_t* seqs;
   const int32_t* offsets;
   const int32_t* shared;

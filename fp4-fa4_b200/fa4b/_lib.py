@@ -120,7 +120,7 @@ class KvWriteArgs(C.Structure):
 class AttnPagedArgs(C.Structure):
     _fields_ = [("q", C.c_void_p), ("q_strides", Strides), ("o", C.c_void_p), ("o_strides", Strides), ("lse", C.c_void_p),
                 ("n", C.c_int32), ("T", C.c_int32), ("Hq", C.c_int32), ("layer", C.c_int32), ("q_dtype", C.c_int32),
-                ("softmax_scale", C.c_float), ("seqs", C.c_void_p), ("groups", C.c_int32), ("group_offsets", C.c_void_p),
+                ("softmax_scale", C.c_float), ("seqs", C.c_void_p), ("groups", C.c_int32), ("flags", C.c_int32), ("group_offsets", C.c_void_p),
                 ("shared_lens", C.c_void_p), ("ws", C.c_void_p)]
 
 

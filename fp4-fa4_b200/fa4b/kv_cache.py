@@ -19,7 +19,7 @@ from ._lib import check, lib, ptr
 # A decoding step makes several calls of a few microseconds: what one costs on the host counts.  Arguments are packed in one
 # go (native alignment: the layout of the C structs), and a call of the current device takes no device guard.
 _WRITE = struct.Struct("@PP3q3q4iPP")
-_ATTEND = struct.Struct("@P3qP3qP5ifPiPPP")
+_ATTEND = struct.Struct("@P3qP3qP5ifP2iPPP")
 
 _current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
@@ -194,7 +194,7 @@ class PagedKVCache:
 
         ``group_offsets [groups + 1]``, ``shared_lens [groups]``: rows ``group_offsets[g]`` up to ``group_offsets[g + 1]`` hold
         the same pages for their first ``shared_lens[g]`` tokens (as :meth:`fork` leaves them), which are read once for
-        the group; rows in no group are left as they were.  ``out`` receives O when given (any strides but 0).  There is no
+        the group; rows in no group have LSE -inf, and O 0 or what ``out`` held.  ``out`` receives O when given (any strides but 0).  There is no
         gradient.  ``softmax_scale`` None: ``1 / sqrt(D)``."""
         if not isinstance(q, torch.Tensor) or len(shape := q.shape) != 4 or shape[3] != self._d:
             raise ValueError(f"q must be a [n, Hq, T, {self._d}] tensor")
@@ -217,8 +217,9 @@ class PagedKVCache:
             if groups == 0 and n > 0:
                 raise ValueError("no groups: without group_offsets and shared_lens every row stands by itself")
             offsets = self._list(group_offsets, "group_offsets")
+        flags = 2  # of rows in no group the LSE says that nothing was computed, and a new O is 0
         if out is None:
-            out, o_strides = q.new_empty(shape), (hq * t * d, t * d, d)
+            out, o_strides, flags = q.new_empty(shape), (hq * t * d, t * d, d), 3
         elif out.shape != shape or out.dtype != q.dtype or out.device != self.device or out.stride(3) != 1:
             raise ValueError(f"out must be a {tuple(shape)} tensor like q with a contiguous head dimension")
         else:
@@ -230,12 +231,12 @@ class PagedKVCache:
         q_strides = _strides(shape, strides)
         size = self._ws_bytes.get((n, hq, t, groups))
         if size is None:
-            args = _ATTEND.pack(q.data_ptr(), *q_strides, out.data_ptr(), *o_strides, lse.data_ptr(), n, t, hq, layer, code, scale, slots, groups, offsets, shared, 0)
+            args = _ATTEND.pack(q.data_ptr(), *q_strides, out.data_ptr(), *o_strides, lse.data_ptr(), n, t, hq, layer, code, scale, slots, groups, flags, offsets, shared, 0)
             size = self._lib.fa4b_attn_paged_workspace_bytes(self._at, args)
             if size:
                 self._ws_bytes[n, hq, t, groups] = size
         ws = self._floats.new_empty(size >> 2)  # of this call alone: calls on two streams, or of two captured graphs, may overlap
-        args = _ATTEND.pack(q.data_ptr(), *q_strides, out.data_ptr(), *o_strides, lse.data_ptr(), n, t, hq, layer, code, scale, slots, groups, offsets, shared,
+        args = _ATTEND.pack(q.data_ptr(), *q_strides, out.data_ptr(), *o_strides, lse.data_ptr(), n, t, hq, layer, code, scale, slots, groups, flags, offsets, shared,
                             ws.data_ptr())
         self._call("fa4b_attn_paged_fwd", args)
         return out, lse

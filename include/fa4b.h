@@ -567,7 +567,9 @@ int fa4b_kv_compact(const fa4b_kv_cache* c, void* stream);
  * Groups: rows group_offsets[g] .. group_offsets[g + 1] - 1 hold the same pages for their first shared_lens[g] tokens
  * (what fa4b_kv_fork makes); those are then read and multiplied once for the group instead of once per row.  The result is
  * the same whatever is said to be shared, as long as it is; the table row of one member names the shared pages.  Offsets
- * rise from 0 or more to n or less; rows in no group are left as they were.  groups == 0: every row by itself. */
+ * rise from 0 or more to n or less.  groups == 0: every row by itself.  Rows in no group, and all rows of a call that is found wrong on the
+ * device, are left as they were, or with the flags get what a row without keys gets. */
+enum { FA4B_PAGED_CLEAR_O = 1, FA4B_PAGED_CLEAR_LSE = 2 };
 typedef struct fa4b_attn_paged_args {
   const void* q; fa4b_strides q_strides;  /* [n, Hq, T, D] bf16 or f16 (16-bit caches: the cache's type); any strides, multiples of 8 */
   void* o; fa4b_strides o_strides;        /* [n, Hq, T, D], q's type; no stride of 0 over more than one row */
@@ -577,6 +579,7 @@ typedef struct fa4b_attn_paged_args {
   float softmax_scale;                    /* <= 0: 1 / sqrt(D) */
   const int32_t* seqs;                    /* [n] or NULL */
   int32_t groups;
+  int32_t flags;                          /* FA4B_PAGED_CLEAR_O: o = 0 for rows that are not computed; FA4B_PAGED_CLEAR_LSE: lse = -inf */
   const int32_t* group_offsets;           /* [groups + 1] */
   const int32_t* shared_lens;             /* [groups] */
   void* ws;                               /* fa4b_attn_paged_workspace_bytes bytes, 256-byte aligned; not shared by calls that may overlap */

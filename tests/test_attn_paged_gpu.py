@@ -698,3 +698,28 @@ def test_the_softmax_scale_may_be_any_positive_number():
     for scale in (1, 2.0 ** -100, 0.125, None):
         out, lse = c.attend(q, ints(slots), softmax_scale=scale)
         compare(c, q, out, lse, slots, scale=scale)
+
+
+@pytest.mark.parametrize("d,kv", [(64, BF), (128, HF), (128, E4)])
+@pytest.mark.parametrize("t", [1, 3])
+@pytest.mark.parametrize("wrong", [False, True])
+def test_rows_that_are_not_computed_are_no_memory_of_something_else(d, kv, t, wrong):
+    """Rows in no group, and every row where the offsets are none: LSE -inf, and O 0 unless the caller brought it."""
+    lens = [40, 100, 77, 30, 64, 50]
+    c, slots, _ = build(lens, [32, 32], [2, 2], hkv=2, d=d, dtype=kv, seed=80)
+    qt = BF if kv == E4 else kv
+    q = queries(6, 4, t, d, qt, 81)
+    offsets, rest = ([1, 3, 2], range(6)) if wrong else ([1, 2, 4], (0, 4, 5))
+    args = dict(group_offsets=ints(offsets), shared_lens=ints([0, 0]))
+    for mine in (None, torch.full_like(q, 7.0)):
+        junk = [torch.full((6, 4, t, d), float("nan"), dtype=qt, device=DEV), torch.full((6, 4, t), float("nan"), device=DEV)]
+        del junk  # the next tensors of these sizes lie there
+        out, lse = c.attend(q, ints(slots), out=mine, **args)
+        for i in rest:
+            assert (out[i] == (0.0 if mine is None else 7.0)).all() and (lse[i] == -math.inf).all()
+        if not wrong:
+            compare(c, q, out, lse, slots, rows=(1, 2, 3))
+    if wrong:
+        with pytest.raises(ValueError, match="offsets"):
+            c.check_status()
+    c.check_status()

@@ -187,3 +187,15 @@ def test_kernels_that_come_up_early_promise_nothing_about_their_lists():
     for name in ("kv_cache.cu", "attn_paged.cu", "attn_prefix.cu"):
         for kernel, parameters, _ in _kernels(name):
             assert "__restrict__" not in parameters, kernel
+
+
+def test_unknown_flags_of_the_attention_are_refused():
+    h = _lib.lib()
+    z = _lib.Strides(1024, 128, 128)
+    c = good()
+    for flags, ok in ((0, True), (1, True), (2, True), (3, True), (4, False), (-1, False)):
+        a = _lib.AttnPagedArgs(q=0x1000, q_strides=z, o=0x2000, o_strides=z, lse=0x3000, n=2, T=1, Hq=8, layer=0, q_dtype=0, softmax_scale=0.0, seqs=0x4000, groups=0,
+                               flags=flags, group_offsets=0, shared_lens=0, ws=0x10000)
+        assert (h.fa4b_attn_paged_workspace_bytes(C.addressof(c), C.addressof(a)) > 0) == ok
+        assert ok or b"flags" in h.fa4b_last_error()
+    assert C.sizeof(_lib.AttnPagedArgs) == 136 and _lib.AttnPagedArgs.group_offsets.offset == 112  # what stands around the flags is where it was
