@@ -195,7 +195,7 @@ class PagedKVCache:
         ``group_offsets [groups + 1]``, ``shared_lens [groups]``: rows ``group_offsets[g]`` up to ``group_offsets[g + 1]`` hold
         the same pages for their first ``shared_lens[g]`` tokens (as :meth:`fork` leaves them), which are read once for
         the group; rows in no group have LSE -inf, and O 0 or what ``out`` held.  ``out`` receives O when given (any strides but 0).  There is no
-        gradient.  ``softmax_scale`` None: ``1 / sqrt(D)``."""
+        gradient: a backward pass that comes to a ``q`` which requires one is refused.  ``softmax_scale`` None: ``1 / sqrt(D)``."""
         if not isinstance(q, torch.Tensor) or len(shape := q.shape) != 4 or shape[3] != self._d:
             raise ValueError(f"q must be a [n, Hq, T, {self._d}] tensor")
         dtype, strides = q.dtype, q.stride()
@@ -239,12 +239,26 @@ class PagedKVCache:
         args = _ATTEND.pack(q.data_ptr(), *q_strides, out.data_ptr(), *o_strides, lse.data_ptr(), n, t, hq, layer, code, scale, slots, groups, flags, offsets, shared,
                             ws.data_ptr())
         self._call("fa4b_attn_paged_fwd", args)
+        if q.requires_grad and torch.is_grad_enabled():
+            out, lse = _WithoutGradient.apply(q, out, lse)
         return out, lse
 
     def check_status(self) -> None:
         """Synchronise and raise on what the calls since the last check found wrong on the device (slots out of range, too
         few free pages, ...)."""
         self._call("fa4b_kv_check_status")
+
+
+class _WithoutGradient(torch.autograd.Function):
+    """Hands results on, and refuses the backward pass instead of leaving a gradient out."""
+
+    @staticmethod
+    def forward(ctx, q, out, lse):
+        return out, lse
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("attention over a paged cache has no gradient")
 
 
 def _strides(shape, strides) -> tuple:

@@ -723,3 +723,25 @@ def test_rows_that_are_not_computed_are_no_memory_of_something_else(d, kv, t, wr
         with pytest.raises(ValueError, match="offsets"):
             c.check_status()
     c.check_status()
+
+
+def test_a_backward_pass_is_refused_and_not_left_out():
+    lens = [50, 20]
+    c, slots, _ = build(lens, [], [], hkv=2, d=64, seed=20)
+    s = ints(slots)
+    plain = queries(2, 4, 1, 64, BF, 0)
+    want, want_lse = c.attend(plain, s)
+    q = plain.clone().requires_grad_()
+    buf = torch.zeros_like(plain)
+    for given in (None, buf, buf):
+        out, lse = c.attend(q * 1, s, out=given)
+        assert torch.equal(out, want) and torch.equal(lse, want_lse)
+        assert given is None or (out.data_ptr() == buf.data_ptr() and torch.equal(buf, want) and not buf.requires_grad)
+        with pytest.raises(RuntimeError, match="no gradient"):
+            out.float().sum().backward()
+        with pytest.raises(RuntimeError, match="no gradient"):
+            c.attend(q, s)[1].sum().backward()
+    with torch.no_grad():
+        out, lse = c.attend(q, s)
+    assert not out.requires_grad and torch.equal(out, want)
+    assert not want.requires_grad and q.grad is None
