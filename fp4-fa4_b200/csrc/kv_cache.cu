@@ -685,6 +685,26 @@ int kv_view(const fa4b_kv_cache* c, KvView* out) {
   return FA4B_OK;
 }
 
+// Do blocks of `block` elements at l * layer + p * page, l < layers and p < pages, keep off one another?  Both strides are `block` at least.
+static bool blocks_apart(int64_t layer, int64_t page, int64_t layers, int64_t pages, int64_t block) {
+  if (layers == 1 || pages == 1 || layer >= (pages - 1) * page + block || page >= (layers - 1) * layer + block) return true;  // nested either way
+  for (int64_t d = 1; d < layers; ++d) {  // layers d apart: the pages that come nearest
+    const int64_t at = d * layer, p = std::min(at / page, pages - 1);
+    if (at - p * page < block || (p + 1 < pages && (p + 1) * page - at < block)) return false;
+  }
+  return true;
+}
+
+// the same for calls that write pages
+static int kv_pools(const fa4b_kv_cache* c, KvView* out) {
+  if (int s = kv_view(c, out)) return s;
+  const int64_t block = (int64_t)c->Hkv * c->page_tokens * c->D;
+  FA4B_REQUIRE(blocks_apart(c->k_layer_stride, c->k_page_stride, c->layers, c->num_pages, block) &&
+                   blocks_apart(c->v_layer_stride, c->v_page_stride, c->layers, c->num_pages, block),
+               FA4B_BAD_SHAPE, "layers overlap: a page of one lies on a page of another");
+  return FA4B_OK;
+}
+
 static int check_list(const fa4b_kv_cache* c, const void* a, const void* b, int32_t n) {
   FA4B_REQUIRE(n >= 0 && n <= FA4B_KV_MAX_LIST, FA4B_BAD_SHAPE, "lists of 0 to %d entries are built, got %d", (int)FA4B_KV_MAX_LIST, n);
   FA4B_REQUIRE(n == 0 || (a && b), FA4B_BAD_ARG, "NULL list");
@@ -728,7 +748,7 @@ int fa4b_kv_extend(const fa4b_kv_cache* c, const int32_t* seqs, const int32_t* n
 
 int fa4b_kv_write(const fa4b_kv_cache* c, const fa4b_kv_write_args* a, void* stream) {
   KvView v;
-  if (int s = kv_view(c, &v)) return s;
+  if (int s = kv_pools(c, &v)) return s;
   FA4B_REQUIRE(a != nullptr, FA4B_BAD_ARG, "args is NULL");
   if (int s = check_list(c, a->seqs, a->seqs, a->n)) return s;
   FA4B_REQUIRE(a->T >= 0, FA4B_BAD_SHAPE, "T=%d is negative", a->T);
@@ -764,7 +784,7 @@ int fa4b_kv_write(const fa4b_kv_cache* c, const fa4b_kv_write_args* a, void* str
 
 int fa4b_kv_fork(const fa4b_kv_cache* c, const int32_t* parents, const int32_t* children, int32_t n, void* stream) {
   KvView v;
-  if (int s = kv_view(c, &v)) return s;
+  if (int s = kv_pools(c, &v)) return s;
   if (int s = check_list(c, parents, children, n)) return s;
   if (n == 0) return FA4B_OK;
   const int pieces = (v.page_tokens * v.row_bytes + kWarpBytes - 1) / kWarpBytes;
@@ -779,7 +799,7 @@ int fa4b_kv_fork(const fa4b_kv_cache* c, const int32_t* parents, const int32_t* 
 
 int fa4b_kv_copy_pages(const fa4b_kv_cache* c, const int32_t* src, const int32_t* dst, int32_t n, void* stream) {
   KvView v;
-  if (int s = kv_view(c, &v)) return s;
+  if (int s = kv_pools(c, &v)) return s;
   if (int s = check_list(c, src, dst, n)) return s;
   if (n == 0) return FA4B_OK;
   const int pieces = (v.block_bytes + kPieceBytes - 1) / kPieceBytes;
@@ -795,7 +815,7 @@ int fa4b_kv_copy_pages(const fa4b_kv_cache* c, const int32_t* src, const int32_t
 
 int fa4b_kv_compact(const fa4b_kv_cache* c, void* stream) {
   KvView v;
-  if (int s = kv_view(c, &v)) return s;
+  if (int s = kv_pools(c, &v)) return s;
   const int pieces = (v.block_bytes + kPieceBytes - 1) / kPieceBytes;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int blocks = compact_blocks(v.pages);

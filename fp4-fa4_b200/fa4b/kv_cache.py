@@ -91,7 +91,7 @@ class PagedKVCache:
         self._floats = torch.empty(0, dtype=torch.float32, device=self.device)
         self._work = torch.zeros((self._lib.fa4b_kv_workspace_bytes(self._at) + 3) // 4, dtype=torch.int32, device=self.device)
         self._c.work = ptr(self._work)
-        self._call("fa4b_kv_free", 0, 0)  # an empty list: the checks of the C side
+        self._call("fa4b_kv_copy_pages", 0, 0, 0)  # empty lists: the checks of the C side
 
     def _call(self, name: str, *args) -> None:
         """One C call on the cache's device and that device's current stream."""

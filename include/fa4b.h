@@ -501,7 +501,8 @@ enum { FA4B_KV_MAX_LIST = 4096, FA4B_KV_MAX_SEQS = 262144 };
 typedef struct fa4b_kv_cache {
   void* k;                          /* 16-byte aligned */
   void* v;
-  int64_t k_layer_stride, k_page_stride, v_layer_stride, v_page_stride; /* elements */
+  int64_t k_layer_stride, k_page_stride, v_layer_stride, v_page_stride; /* elements; layers around pages, pages around layers, or any other
+                                       order in which no page of a layer lies on another's */
   int32_t layers, num_pages, Hkv;
   int32_t page_tokens;              /* 16, 32, 64 or 128 */
   int32_t D;                        /* 64 or 128 */

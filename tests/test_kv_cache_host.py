@@ -199,3 +199,30 @@ def test_unknown_flags_of_the_attention_are_refused():
         assert (h.fa4b_attn_paged_workspace_bytes(C.addressof(c), C.addressof(a)) > 0) == ok
         assert ok or b"flags" in h.fa4b_last_error()
     assert C.sizeof(_lib.AttnPagedArgs) == 136 and _lib.AttnPagedArgs.group_offsets.offset == 112  # what stands around the flags is where it was
+
+
+def _pages_overlap(layer, page, layers, pages, block):
+    at = sorted(i * layer + j * page for i in range(layers) for j in range(pages))
+    return any(b - a < block for a, b in zip(at, at[1:]))
+
+
+def test_pools_whose_layers_share_pages_are_refused_by_every_call_that_writes_them():
+    """Every layout of a few layers and pages against the list of their places; K and V on their own."""
+    h = _lib.lib()
+    block = 2 * 16 * 64
+    w = _lib.KvWriteArgs(0x1000, 0x1000, _lib.Strides(), _lib.Strides(), 0, 0, 0, 1, 0x1000, 0)
+    seen = set()
+    for layers, pages in ((2, 100), (3, 2), (4, 5), (2, 2), (1, 9), (7, 1)):
+        for layer in (block, block + 64, 2 * block, 3 * block, 5 * block, 5 * block + 64, (pages - 1) * block + block, 100 * block, 3 * pages * block):
+            for page in (block, block + 8, 2 * block, 3 * block + 64, layers * block, (layers - 1) * layer + block):
+                bad = _pages_overlap(layer, page, layers, pages, block)
+                for which in "kv":
+                    c = good(Hkv=2, D=64, layers=layers, num_pages=pages, **{f"{x}_{y}_stride": z for x in "kv" for y, z in (("layer", 1000 * block), ("page", block))}
+                             | {f"{which}_layer_stride": layer, f"{which}_page_stride": page})
+                    at = C.addressof(c)
+                    for got in (h.fa4b_kv_copy_pages(at, 0, 0, 0, 0), h.fa4b_kv_fork(at, 0, 0, 0, 0), h.fa4b_kv_write(at, C.addressof(w), 0)):
+                        assert got == bad and (not bad or b"layers overlap" in h.fa4b_last_error()), (layers, pages, layer, page)
+                    if bad:
+                        assert h.fa4b_kv_compact(at, 0) == 1
+                seen.add(bad)
+    assert seen == {False, True}
