@@ -232,7 +232,8 @@ class PagedKVCache:
         size = self._ws_bytes.get((n, hq, t, groups))
         if size is None:
             args = _ATTEND.pack(q.data_ptr(), *q_strides, out.data_ptr(), *o_strides, lse.data_ptr(), n, t, hq, layer, code, scale, slots, groups, flags, offsets, shared, 0)
-            size = self._lib.fa4b_attn_paged_workspace_bytes(self._at, args)
+            with torch.cuda.device(self._index):  # the size goes by the number of SMs
+                size = self._lib.fa4b_attn_paged_workspace_bytes(self._at, args)
             if size:
                 self._ws_bytes[n, hq, t, groups] = size
         ws = self._floats.new_empty(size >> 2)  # of this call alone: calls on two streams, or of two captured graphs, may overlap

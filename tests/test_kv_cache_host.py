@@ -226,3 +226,34 @@ def test_pools_whose_layers_share_pages_are_refused_by_every_call_that_writes_th
                         assert h.fa4b_kv_compact(at, 0) == 1
                 seen.add(bad)
     assert seen == {False, True}
+
+
+def test_the_workspace_is_sized_for_the_device_of_the_cache(monkeypatch):
+    """Pieces of work, and with them the workspace, are as many as the device has room for: the cache's, not the current one."""
+    import contextlib
+    import types
+
+    from fa4b import kv_cache
+
+    current, asked = [1], []
+
+    @contextlib.contextmanager
+    def device(index):
+        before, current[0] = current[0], index
+        yield
+        current[0] = before
+
+    def answer(*_):
+        asked.append(current[0])
+        return 1024
+
+    c = PagedKVCache.__new__(PagedKVCache)
+    c.device, c._index, c._d, c._takes, c._ws_bytes, c._at = torch.device("cpu"), -1, 64, (torch.bfloat16,), {}, 0
+    c._floats = torch.zeros(0)
+    c._lib = types.SimpleNamespace(fa4b_attn_paged_workspace_bytes=answer, fa4b_attn_paged_fwd=lambda *_: asked.append(current[0]) or 0)
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(kv_cache, "_current_device", lambda: current[0])
+    monkeypatch.setattr(kv_cache, "_raw_stream", lambda index: 0)
+    for _ in range(2):
+        c.attend(torch.zeros(2, 4, 1, 64, dtype=torch.bfloat16))
+    assert asked == [-1, -1, -1] and current == [1]
