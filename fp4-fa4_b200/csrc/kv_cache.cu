@@ -835,8 +835,10 @@ int fa4b_kv_check_status(const fa4b_kv_cache* c, void* stream) {
   FA4B_CUDA(cudaMemcpyAsync(host, v.work + kWorkStatus, sizeof(host), cudaMemcpyDeviceToHost, st));
   FA4B_CUDA(cudaStreamSynchronize(st));
   if (host[0] == kOk && host[kKvAttnStatus] == 0) return FA4B_OK;
-  FA4B_CUDA(cudaMemsetAsync(v.work + kWorkStatus, 0, sizeof(host), st));
+  // what is told now is cleared: of both kinds of findings the other waits for the next check
   const int32_t* attn = host + kKvAttnStatus;
+  const bool of_attn = attn[0] == 1 || host[0] == kOk;
+  FA4B_CUDA(cudaMemsetAsync(v.work + (of_attn ? kKvAttnStatus : kWorkStatus), 0, 4 * (kKvAttnStatus - kKvStatus), st));
   FA4B_REQUIRE(attn[0] != 1, FA4B_TIMEOUT, "a device-side wait of the attention over the cache ran out (site %d, block %d)", attn[1], attn[2]);
   if (host[0] == kOk && attn[0] == 3) {
     set_error("the batch's keys are too many for one call (%d tiles per kv head)", attn[1]);

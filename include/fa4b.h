@@ -589,7 +589,8 @@ size_t fa4b_attn_paged_workspace_bytes(const fa4b_kv_cache* c, const fa4b_attn_p
 int fa4b_attn_paged_fwd(const fa4b_kv_cache* c, const fa4b_attn_paged_args* a, void* stream);
 
 /* fa4b_kv_check_status: synchronises `stream`, returns what the calls since the last check found wrong (FA4B_NO_PAGES,
- * FA4B_BAD_ARG; FA4B_TIMEOUT when a bounded wait of the attention ran out; FA4B_OK when nothing) and clears it. */
+ * FA4B_BAD_ARG; FA4B_TIMEOUT when a bounded wait of the attention ran out; FA4B_OK when nothing) and clears it.  The first finding of the page calls and the first of
+ * the attention are kept apart and told one at a time. */
 int fa4b_kv_check_status(const fa4b_kv_cache* c, void* stream);
 
 /* ---- tensor-core self tests ("microgates") -------------------------------

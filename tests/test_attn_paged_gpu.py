@@ -745,3 +745,15 @@ def test_a_backward_pass_is_refused_and_not_left_out():
         out, lse = c.attend(q, s)
     assert not out.requires_grad and torch.equal(out, want)
     assert not want.requires_grad and q.grad is None
+
+
+def test_findings_of_the_pages_and_of_the_attention_are_both_told():
+    c, slots, _ = build([40, 100], [], [], hkv=2, d=64, seed=10)
+    q = queries(2, 4, 1, 64, BF, 11)
+    for _ in range(2):
+        c.extend(ints(slots), ints([1, -1]))
+        c.attend(q, ints(slots), group_offsets=ints([0, 3]), shared_lens=ints([0]))
+        for text in ("negative", "offsets of 1 groups"):
+            with pytest.raises(ValueError, match=text):
+                c.check_status()
+        c.check_status()
