@@ -476,3 +476,42 @@ def test_tokens_in_pages_that_several_slots_hold_are_not_written(dtype, page):
     m.write(k, v, [4, 4], [length, 0], 0)
     m.check(c)
     c.check_status()
+
+
+@pytest.mark.parametrize("n", [1024, 1025, 1030, 4096])
+def test_collisions_in_long_lists_are_left_out(n):
+    """Up to 1024 pairs are checked by the CTAs that copy, more by a launch before them: collisions and bad pages in its first and last warp."""
+    c = make(pages=2 * n + 9, heads=1, layers=2)
+    m = ModelCache(c)
+    rng = random.Random(n)
+    order = rng.sample(range(2 * n), 2 * n)
+    src, dst = order[:n], order[n:]
+    dst[1] = dst[0]
+    dst[n - 1] = dst[n // 2]
+    src[n - 2] = dst[2]
+    src[3] = 2 * n + 9
+    dst[n - 5] = 2 ** 31 - 1
+    src[9], dst[11] = -1, -(2 ** 31)
+    dst[n - 9] = src[n - 9]
+    c.copy_pages(ints(src), ints(dst))
+    m.copy_pages(src, dst)
+    m.check(c)
+    with pytest.raises(ValueError, match="pair"):
+        c.check_status()
+    c.check_status()
+
+
+def test_more_pairs_than_the_pool_has_pages():
+    c = make(pages=300, heads=1, layers=2)
+    m = ModelCache(c)
+    rng = random.Random(1)
+    src = [rng.randrange(0, 150) for _ in range(4000)]
+    dst = [-1] * 4000
+    for at, d in zip(rng.sample(range(4000), 100), range(150, 250)):
+        dst[at] = d
+    dst[5] = dst[3990] = 299
+    c.copy_pages(ints(src), ints(dst))
+    m.copy_pages(src, dst)
+    m.check(c)
+    with pytest.raises(ValueError, match="page 299 is also"):
+        c.check_status()
