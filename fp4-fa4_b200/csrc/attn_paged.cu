@@ -260,7 +260,6 @@ template <int D, bool kE4M3, typename QT>
 struct PagedRows {
   using Mma = typename std::conditional<kE4M3, TagF16, QT>::type;
   static constexpr int kBoxBytes = D * (kE4M3 ? 1 : 2) < 128 ? D : 128;  // of a row, side by side in one box of shared memory
-  static constexpr int kRows = 16;
   uint32_t q[D / 16][4];
   float acc[D / 8][4], scale[2], m[2], l[2];
   int limit[2];  // the row sees keys below
@@ -497,7 +496,6 @@ template <int D, bool kE4M3, typename QT>
 struct PagedRows8 {
   using Mma = typename std::conditional<kE4M3, TagF16, QT>::type;
   static constexpr int kBoxBytes = D * (kE4M3 ? 1 : 2) < 128 ? D : 128;
-  static constexpr int kRows = 8;
   uint32_t q[D / 16][2];
   float acc[D / 16][4], scale[2], m[2], l[2];
   int limit[2];
@@ -1182,8 +1180,6 @@ static int launch_paged(const PagedParams& p, const PagedMaps& m, cudaStream_t s
   return FA4B_OK;
 }
 
-static bool off16(const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15) != 0; }
-
 // checks a call and lays its workspace out; `ws` may be NULL (a size query)
 static int paged_params(const fa4b_kv_cache* c, const fa4b_attn_paged_args* a, PagedParams* out, size_t* bytes) {
   PagedParams p{};
@@ -1209,7 +1205,7 @@ static int paged_params(const fa4b_kv_cache* c, const fa4b_attn_paged_args* a, P
   for (int64_t s : {p.q_sb, p.q_sh, p.q_st, p.o_sb, p.o_sh, p.o_st})
     FA4B_REQUIRE(s % 8 == 0, FA4B_BAD_ALIGN, "strides of q and o must be multiples of 8 elements");
   FA4B_REQUIRE((p.n <= 1 || p.o_sb != 0) && (p.Hq == 1 || p.o_sh != 0) && (p.T == 1 || p.o_st != 0), FA4B_BAD_SHAPE, "rows of o lie on one another (a stride of 0)");
-  FA4B_REQUIRE(!off16(p.q) && !off16(p.o), FA4B_BAD_ALIGN, "q and o must be 16-byte aligned");
+  FA4B_REQUIRE(!misaligned(p.q, 16) && !misaligned(p.o, 16), FA4B_BAD_ALIGN, "q and o must be 16-byte aligned");
   FA4B_REQUIRE(std::isfinite(a->softmax_scale), FA4B_BAD_ARG, "softmax_scale is not a finite number");
   p.scale_log2 = (a->softmax_scale > 0.f ? a->softmax_scale : 1.0f / sqrtf((float)c->D)) * kLog2e;
   if (c->dtype == FA4B_KV_E4M3) p.k_scale = c->k_scale + (int64_t)a->layer * c->Hkv, p.v_scale = c->v_scale + (int64_t)a->layer * c->Hkv;
@@ -1284,7 +1280,7 @@ int fa4b_attn_paged_fwd(const fa4b_kv_cache* c, const fa4b_attn_paged_args* a, v
   if (int s = paged_params(c, a, &p, &bytes)) return s;
   if (a->n == 0) return FA4B_OK;
   FA4B_REQUIRE(a->q && a->o && a->lse && a->ws, FA4B_BAD_ARG, "q, o, lse or ws is NULL");
-  FA4B_REQUIRE((reinterpret_cast<uintptr_t>(a->ws) & 255) == 0, FA4B_BAD_ALIGN, "ws must be 256-byte aligned");
+  FA4B_REQUIRE(!misaligned(a->ws, 256), FA4B_BAD_ALIGN, "ws must be 256-byte aligned");
   const bool e4m3 = c->dtype == FA4B_KV_E4M3;
   // one map per pool and width of a copy: the units take what a tile of theirs holds of a page
   const int esz = e4m3 ? 1 : 2;

@@ -642,8 +642,6 @@ __global__ void __launch_bounds__(256) kv_compact_move_kernel(const KvView c, in
 }
 
 // ---- host -------------------------------------------------------------------------------------------------------------
-static bool misaligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) != 0; }
-
 int kv_view(const fa4b_kv_cache* c, KvView* out) {
   FA4B_REQUIRE(c != nullptr, FA4B_BAD_ARG, "cache is NULL");
   FA4B_REQUIRE(c->dtype == FA4B_KV_BF16 || c->dtype == FA4B_KV_F16 || c->dtype == FA4B_KV_E4M3, FA4B_UNSUPPORTED, "unknown cache dtype %d", c->dtype);
@@ -705,10 +703,9 @@ static int kv_pools(const fa4b_kv_cache* c, KvView* out) {
   return FA4B_OK;
 }
 
-static int check_list(const fa4b_kv_cache* c, const void* a, const void* b, int32_t n) {
+static int check_list(const void* a, const void* b, int32_t n) {
   FA4B_REQUIRE(n >= 0 && n <= FA4B_KV_MAX_LIST, FA4B_BAD_SHAPE, "lists of 0 to %d entries are built, got %d", (int)FA4B_KV_MAX_LIST, n);
   FA4B_REQUIRE(n == 0 || (a && b), FA4B_BAD_ARG, "NULL list");
-  (void)c;
   return FA4B_OK;
 }
 
@@ -726,7 +723,7 @@ size_t fa4b_kv_workspace_bytes(const fa4b_kv_cache* c) {
 int fa4b_kv_free(const fa4b_kv_cache* c, const int32_t* seqs, int32_t n, void* stream) {
   KvView v;
   if (int s = kv_view(c, &v)) return s;
-  if (int s = check_list(c, seqs, seqs, n)) return s;
+  if (int s = check_list(seqs, seqs, n)) return s;
   if (n == 0) return FA4B_OK;
   FA4B_CUDA(launch_overlapped(kv_free_kernel, n, 128, 0, static_cast<cudaStream_t>(stream), v, seqs));
   return FA4B_OK;
@@ -735,7 +732,7 @@ int fa4b_kv_free(const fa4b_kv_cache* c, const int32_t* seqs, int32_t n, void* s
 int fa4b_kv_extend(const fa4b_kv_cache* c, const int32_t* seqs, const int32_t* n_new, int32_t n, void* stream) {
   KvView v;
   if (int s = kv_view(c, &v)) return s;
-  if (int s = check_list(c, seqs, n_new, n)) return s;
+  if (int s = check_list(seqs, n_new, n)) return s;
   if (n == 0) return FA4B_OK;
   const size_t smem = 4 * ((size_t)n + 1 + (v.max_seqs + 31) / 32);
   static std::atomic<uint64_t> allowed{0};
@@ -750,7 +747,7 @@ int fa4b_kv_write(const fa4b_kv_cache* c, const fa4b_kv_write_args* a, void* str
   KvView v;
   if (int s = kv_pools(c, &v)) return s;
   FA4B_REQUIRE(a != nullptr, FA4B_BAD_ARG, "args is NULL");
-  if (int s = check_list(c, a->seqs, a->seqs, a->n)) return s;
+  if (int s = check_list(a->seqs, a->seqs, a->n)) return s;
   FA4B_REQUIRE(a->T >= 0, FA4B_BAD_SHAPE, "T=%d is negative", a->T);
   FA4B_REQUIRE(a->layer >= 0 && a->layer < c->layers, FA4B_BAD_SHAPE, "layer %d of %d", a->layer, c->layers);
   FA4B_REQUIRE(a->src_dtype == FA4B_KV_BF16 || a->src_dtype == FA4B_KV_F16, FA4B_UNSUPPORTED, "values are written from bf16 or f16");
@@ -785,7 +782,7 @@ int fa4b_kv_write(const fa4b_kv_cache* c, const fa4b_kv_write_args* a, void* str
 int fa4b_kv_fork(const fa4b_kv_cache* c, const int32_t* parents, const int32_t* children, int32_t n, void* stream) {
   KvView v;
   if (int s = kv_pools(c, &v)) return s;
-  if (int s = check_list(c, parents, children, n)) return s;
+  if (int s = check_list(parents, children, n)) return s;
   if (n == 0) return FA4B_OK;
   const int pieces = (v.page_tokens * v.row_bytes + kWarpBytes - 1) / kWarpBytes;
   const int64_t units = (int64_t)n * v.layers * 2 * v.heads * pieces, ctas = n + (units + 7) / 8;
@@ -800,7 +797,7 @@ int fa4b_kv_fork(const fa4b_kv_cache* c, const int32_t* parents, const int32_t* 
 int fa4b_kv_copy_pages(const fa4b_kv_cache* c, const int32_t* src, const int32_t* dst, int32_t n, void* stream) {
   KvView v;
   if (int s = kv_pools(c, &v)) return s;
-  if (int s = check_list(c, src, dst, n)) return s;
+  if (int s = check_list(src, dst, n)) return s;
   if (n == 0) return FA4B_OK;
   const int pieces = (v.block_bytes + kPieceBytes - 1) / kPieceBytes;
   const int64_t ctas = (int64_t)n * v.layers * 2 * pieces;

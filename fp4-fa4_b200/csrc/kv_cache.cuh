@@ -28,6 +28,8 @@ constexpr int kKvStatus = 0, kKvAttnStatus = 4, kKvHead = 8, kKvStatusWords = 8;
 // checks a cache's description and turns it into what the kernels take
 int kv_view(const fa4b_kv_cache* c, KvView* out);
 
+inline bool misaligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) != 0; }
+
 // A launch that may begin while the kernel before it on the stream still runs: every kernel launched this way runs
 // pdl_wait() before it touches memory (which returns once the kernel before has ended and its writes are visible), so only
 // the launch itself overlaps.  pdl_trigger() lets the next such launch come up early.  Pointer parameters of such a kernel are not
