@@ -1,14 +1,16 @@
 // Attention of the newest tokens of a batch over a paged cache (single tokens, or a few drafted ones), with the keys that
 // a group of sequences shares read once for all of them.
 //
-// A call is a chain of launches, each of which comes up while the one before still runs: plan (who reads what; not for few rows), prefix units
-// (only with groups: attn_prefix.cu), own units, join.  For 32 sequences of 600 keys behind 8219 shared ones (32 query and 8 kv heads,
-// D 128, bf16) that is 32 us: plan 5, prefix 13.5, own 9 beside and behind it, join 3-5, against 11 us for the bytes; what is left is
-// the latency of the chain.  One sequence of 1000 keys takes 8.7 us in a graph.
+// A call is a chain of launches: plan (who reads what; not for few rows), prefix units (only with groups: attn_prefix.cu), own units, join.
+// Each comes up while the one before still runs and waits for its end before it reads anything: what the plan wrote two launches ago
+// is visible behind that wait only.  (Own units that began beside the prefix units, and a join that read the plan early, took 2 to 4 us less
+// of a call with groups, 1 us of one without, on an order that nothing promised.)  For 32 sequences of 600 keys behind 8219 shared
+// ones (32 query and 8 kv heads, D 128, bf16) that is 34.6 us in a graph: plan 5, prefix 13.5, own units and join 16, against 11 us for the bytes; what is
+// left is the latency of the chain.  One sequence of 1000 keys (f16, D 64) takes 9.6 us.
 //
 // Own units are bound by memory: a key and a value are used by the few query rows of one sequence, so the kernel is a
 // stream of pages through shared memory, with tiles asked for by TMA several tiles ahead: 32 sequences of up to 8k keys, 537
-// MB of bf16, take 97 us with all launches (5.5 TB/s), 268 MB of E4M3 60 us.  Scores and values go through mma.sync m16n8k16:
+// MB of bf16, take 98 us with all launches (5.5 TB/s), 268 MB of E4M3 60 us.  Scores and values go through mma.sync m16n8k16:
 // with 4 to 16 query rows a tcgen05 tile of 128 rows would be empty for the most part, and up to 16 rows the products of a tile
 // take less time than its bytes.  With 64 rows they do not any more (bf16 237 us).
 #include "attn_paged.cuh"
@@ -1005,7 +1007,7 @@ __global__ void __launch_bounds__(160, 2) attn_team_kernel(const PagedParams p, 
 
 // ---- join -------------------------------------------------------------------------------------------------------------
 // One warp per output row, or (kSplit) four, each with a quarter of the pieces and sums of its own, where the rows are few (one
-// sequence of 8k keys has 128 pieces a row: 16.2 us for the call against 17.9 when the four went through them together, 32
+// sequence of 8k keys has 128 pieces a row: 1.7 us less of a call of 16.7 than when the four went through them together, 32
 // at a time).  The statistics of 32 pieces come to the lanes at once, so that what is left to wait for is one round of loads: a
 // lane holds D / 32 neighbours of eight pieces at a time (one piece behind another took 26 us where this takes 12, and 3 to 5 with
 // four warps).  Latency bounds it, and for many rows the memory (16384 rows of 5 to 7 pieces: 18 us).  Which pieces there are
