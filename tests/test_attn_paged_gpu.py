@@ -757,3 +757,51 @@ def test_findings_of_the_pages_and_of_the_attention_are_both_told():
             with pytest.raises(ValueError, match=text):
                 c.check_status()
         c.check_status()
+
+
+def test_a_first_call_may_be_a_captured_one():
+    """A process whose first extend, write and attend are captured, and replayed with lengths that grow."""
+    import os
+    import pathlib
+    import subprocess
+    import sys
+
+    text = """
+import torch, test_attn_paged_gpu as A
+from fa4b import PagedKVCache
+c, slots, offsets = A.build([150, 170, 160], [128], [3], hkv=2, d=128, seed=21, width=40, spare_pages=60)
+s, one, off, sh = A.ints(slots), A.ints([1, 1, 1]), A.ints(offsets), A.ints([128])
+q, k, v = A.queries(3, 8, 1, 128, A.BF, 30), A.queries(3, 2, 1, 128, A.BF, 31), A.queries(3, 2, 1, 128, A.BF, 32)
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    c.extend(s, one)
+    c.write(k, v, s)
+    grouped = c.attend(q, s, group_offsets=off, shared_lens=sh)
+    alone = c.attend(q, s)
+for _ in range(20):
+    q.normal_(), k.normal_(), v.normal_()
+    g.replay()
+    A.compare(c, q, *grouped, slots)
+    A.compare(c, q, *alone, slots)
+c.check_status()
+assert c.seq_lens[slots].tolist() == [170, 190, 180]
+"""
+    root = pathlib.Path(__file__).resolve().parents[1]
+    done = subprocess.run([sys.executable, "-c", text], cwd=root, capture_output=True, text=True, timeout=240,
+                          env={**os.environ, "PYTHONPATH": f"{root / 'fp4-fa4_b200'}:{root / 'tests'}:{root / 'oracle'}"})
+    assert done.returncode == 0, done.stderr[-2000:]
+
+
+@pytest.mark.parametrize("kv", [BF, E4])
+@pytest.mark.parametrize("page,width", [(16, 33), (128, 5)])
+def test_sequences_that_fill_their_row_of_the_table(kv, page, width):
+    lens = [page * width, page * width - 1, page * (width - 1) + 1]
+    c, slots, offsets = build(lens, [page * (width - 2)], [3], page=page, hkv=2, d=128, dtype=kv, seed=90, width=width)
+    for t in (1, 5):
+        for hq in (8, 64):
+            q = queries(3, hq, t, 128, BF, 91)
+            for args in ({}, dict(group_offsets=ints(offsets), shared_lens=ints([page * (width - 2)]))):
+                out, lse = c.attend(q, ints(slots), **args)
+                compare(c, q, out, lse, slots)
+    c.check_status()

@@ -515,3 +515,57 @@ def test_more_pairs_than_the_pool_has_pages():
     m.check(c)
     with pytest.raises(ValueError, match="page 299 is also"):
         c.check_status()
+
+
+def test_a_fork_into_thousands_of_slots():
+    """As many children as a list holds, tails among them, into slots whose last extend was refused; and one page too few."""
+    c = make(pages=4200, heads=1, layers=1, seqs=4120, width=3)
+    new = [16 * (i % 3) + i % 5 for i in range(20)]  # no tail for every fifth, none at all for some
+    c.extend(ints(list(range(20))), ints(new))
+    m = ModelCache(c)
+    rng = random.Random(2)
+    children = rng.sample(range(20, 4120), 4096)
+    parents = [i % 20 for i in range(4096)]
+    c.extend(ints(children[:50]), ints([99] * 50))
+    c.fork(ints(parents), ints(children))
+    assert m.fork(parents, children)
+    m.check(c)
+    m.invariants()
+    k, v = values(4096, 1, 1, 64, torch.bfloat16, 3)
+    c.write(k, v, ints(children), n_new=ints([1 if new[p] % 16 else 0 for p in parents]))
+    m.write(k, v, children, [1 if new[p] % 16 else 0 for p in parents], 0)
+    m.check(c)
+    with pytest.raises(ValueError, match="too few"):
+        c.check_status()
+    c.free(ints(children))
+    m.free(children)
+    spare = m.refs.count(0)
+    c.extend(ints(children[-40:]), ints([33] * 40))
+    assert m.extend(children[-40:], [33] * 40)
+    tails = [p for p in range(20) if new[p] % 16]
+    parents = [tails[i % len(tails)] for i in range(spare - 120 + 1)]
+    c.fork(ints(parents), ints(children[:len(parents)]))
+    assert not m.fork(parents, children[:len(parents)])
+    m.check(c)
+    with pytest.raises(RuntimeError, match=f"{len(parents)} pages were asked for, {len(parents) - 1} are free"):
+        c.check_status()
+
+
+@pytest.mark.parametrize("page", [16, 128])
+def test_rows_that_are_full_to_the_last_entry(page):
+    c = make(pages=30, page=page, seqs=5, width=4)
+    m = ModelCache(c)
+    k, v = values(2, 2, 4 * page, 64, torch.bfloat16, 4)
+    c.extend(ints([4, 1]), ints([4 * page, 4 * page - 1]))
+    assert m.extend([4, 1], [4 * page, 4 * page - 1])
+    c.write(k, v, ints([4, 1]), n_new=ints([4 * page, 4 * page - 1]))
+    m.write(k, v, [4, 1], [4 * page, 4 * page - 1], 0)
+    c.fork(ints([4, 1]), ints([0, 2]))
+    assert m.fork([4, 1], [0, 2])
+    c.extend(ints([2, 4]), ints([1, 0]))
+    assert m.extend([2, 4], [1, 0])
+    c.compact()
+    m.compact()
+    m.check(c)
+    m.invariants()
+    c.check_status()
